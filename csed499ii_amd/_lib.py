@@ -23,6 +23,7 @@ ERR_LAUNCH = 3
 _vp = ctypes.c_void_p
 _i = ctypes.c_int
 _ll = ctypes.c_longlong
+_f = ctypes.c_float
 
 #: name -> (restype, argtypes); must match include/marlin_hip.h
 SIGNATURES = {
@@ -38,6 +39,11 @@ SIGNATURES = {
     "marlin_hip_native_pack": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "marlin_hip_native_unpack": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "marlin_hip_mul_2_4_native": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i]),
+    "marlin_hip_kv4_tables": (_i, [_vp] * 8 + [_i] * 6 + [_vp]),
+    "marlin_hip_kv4_append": (_i, [_vp] * 4 + [_i] * 3 + [_ll] * 4 + [_i] * 5 + [_vp]),
+    "marlin_hip_kv4_gather": (_i, [_vp] * 4 + [_i] * 8 + [_vp]),
+    "marlin_hip_kv4_attention": (_i, [_vp] * 7 + [_i] * 5 + [_ll] * 2 + [_i] * 6 + [_f, _i, _i, _vp]),
+    "marlin_hip_kv4_plan": (_i, [_i] * 8 + [ctypes.POINTER(_i)]),
     "marlin_hip_last_error": (ctypes.c_char_p, []),
 }
 

@@ -11,6 +11,10 @@ Extensions that the reference keeps in side experiments:
   (kernel_experiments/sparse_marlin/metadata_decode).
 * ``expand3``: 3-bit code stream -> nibbles (kernel_experiments/3bit_encoding).
 * ``mul_2_4_w3`` / ``pack_w3``: 3-bit nonzero values (no reference implementation).
+
+Beside the linear layers, what a decoder needs between qkv and o (no reference
+counterpart): ``kv4_cache``, ``kv4_tables``, ``kv4_append``, ``kv4_gather`` and
+``kv4_attention``, a paged KV cache held in 4 bits (``_kv4.py``).
 """
 from __future__ import annotations
 
@@ -21,6 +25,14 @@ import torch
 import torch.nn as nn
 
 from .. import _lib
+from ._kv4 import (
+    kv4_append,
+    kv4_attention,
+    kv4_cache,
+    kv4_gather,
+    kv4_tables,
+    plan_kv4_attention,
+)
 from ._semi_structured_conversions import (
     mask_creator,
     sparse_semi_structured_from_dense_cutlass,
@@ -49,6 +61,12 @@ __all__ = [
     "mul",
     "Layer",
     "pack_dense",
+    "kv4_cache",
+    "kv4_tables",
+    "kv4_append",
+    "kv4_gather",
+    "kv4_attention",
+    "plan_kv4_attention",
 ]
 
 

@@ -173,6 +173,63 @@ int marlin_hip_mul_2_4_native(const void* A, const void* Bn, const void* metan, 
                               int prob_m, int prob_n, int prob_k, int groupsize, int dev, hipStream_t stream,
                               int sms);
 
+/* ---- KV cache held in 4 bits (no counterpart in the reference) ----
+ *
+ * The cache is [num_pages][kv_heads][page_size * (head_dim + 4 * head_dim / groupsize)]
+ * bytes, 16-byte aligned; layout of a block: csed499ii_amd/csrc/kv4_device.h.  page_size is
+ * 16, 32, 64, 128 or 256 tokens, head_dim 64 or 128, groupsize 32, 64, 128 (dividing
+ * head_dim) or -1 (one scale a row), dtype 0 (fp16) or 1 (bf16).  A slot is page *
+ * page_size + offset; num_pages * page_size is at most 2^31 - 1.  Lengths, tables and slots
+ * are int32 on the device and never read on the host.  Codes as above: 1 for sizes and
+ * strides that are refused, 2 for a geometry without kernels, 3 for a failed launch. */
+
+/* Block tables and slot maps of a step.  Request i of `requests` holds context_lens[i]
+ * tokens and gets new_lens[i] more (below zero: zero).  New tokens are numbered request by
+ * request; each that is the first of its page takes the next of free_pages[num_free], which
+ * goes to block_table[requests][max_pages].  Writes slots[tokens] (-1: past the last new
+ * token, no free page left, or past the table's width), cu_new[requests + 1], kv_lens
+ * [requests] (cut at the table's width) and pages_used[1] (pages wanted, which may exceed
+ * num_free; entries without a page are -1).  Tokens past `tokens` get no slot and no page.
+ * One launch. */
+int marlin_hip_kv4_tables(const void* context_lens, const void* new_lens, const void* free_pages, void* block_table,
+                          void* slots, void* cu_new, void* kv_lens, void* pages_used, int requests, int num_free,
+                          int max_pages, int page_size, int tokens, int dev, hipStream_t stream);
+
+/* Quantizes rows k, v [tokens][kv_heads][head_dim] into the cache's slots[tokens]; strides
+ * in elements, multiples of 8, rows 16-byte aligned.  Slots that are negative or past the
+ * last page are skipped. */
+int marlin_hip_kv4_append(const void* k, const void* v, void* cache, const void* slots, int tokens, int kv_heads,
+                          int head_dim, long long k_token_stride, long long k_head_stride, long long v_token_stride,
+                          long long v_head_stride, int page_size, int num_pages, int groupsize, int dtype, int dev,
+                          hipStream_t stream);
+
+/* The values that the cache holds in slots[tokens], as contiguous k, v [tokens][kv_heads]
+ * [head_dim]; zeros for slots that are negative or past the last page. */
+int marlin_hip_kv4_gather(const void* cache, const void* slots, void* k, void* v, int tokens, int kv_heads,
+                          int head_dim, int page_size, int num_pages, int groupsize, int dtype, int dev,
+                          hipStream_t stream);
+
+/* Causal attention.  q [tokens][q_heads][head_dim] (strides in elements, multiples of 8)
+ * holds request i's new tokens at [cu_q[i], cu_q[i + 1]) (cu_q null: one a request); they
+ * are the last of its kv_lens[i] tokens, in the pages block_table[i][max_pages] (entries
+ * outside [0, num_pages): left out; max_pages * page_size at most 2^30).  out is contiguous
+ * [tokens][q_heads][head_dim]; lse fp32 [tokens][q_heads] or null.  A row that sees no token:
+ * zeros and -inf.  max_q bounds a request's new tokens (later ones are not computed);
+ * max_kv plans the split of the cache's length and does not change what is computed.  A
+ * split call uses the stream's split-K scratch, and runs unsplit where a captured stream has
+ * none yet.  scale is positive and finite. */
+int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block_table, const void* kv_lens,
+                             const void* cu_q, void* out, void* lse, int tokens, int requests, int q_heads,
+                             int kv_heads, int head_dim, long long q_token_stride, long long q_head_stride,
+                             int page_size, int num_pages, int max_pages, int groupsize, int max_q, int max_kv,
+                             float scale, int dtype, int dev, hipStream_t stream);
+
+/* The launch plan of a marlin_hip_kv4_attention call, computed on the host without a GPU
+ * (sms <= 0: 256 compute units): out[0] 0 (the split kernel), out[1] workgroups, out[2]
+ * splits of the cache's length (> 1: the call uses its stream's split-K scratch). */
+int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, int groupsize, int max_q, int max_kv,
+                        int sms, int* out);
+
 /* Message describing the last MARLIN_HIP_ERR_* of the calling thread. */
 const char* marlin_hip_last_error(void);
 
