@@ -2,6 +2,7 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
+#include <stdlib.h>
 
 #include "kv4_host.h"
 #include "kv4_split.h"
@@ -15,21 +16,31 @@ int compute_units(int dev) {
 }
 
 struct Plan {
-  int row_blocks, splits;
-  long long tiles;
+  int workgroups, log_kw;
+  bool split;  // a tile may be divided: the call needs scratch
 };
 
-// Splits of the cache's length: enough workgroups for `cus` compute units four times over,
-// each wave with a step at least.
+// Two workgroups of eight waves fill a compute unit.  Waves of a workgroup that share a
+// head (KW) meet in LDS, pieces of a tile in memory: few tiles take all eight for a head,
+// many tiles fewer.
 Plan plan(int requests, int q_heads, int kv_heads, int max_q, int max_kv, int cus) {
   Plan p;
-  p.row_blocks = (int)(((long long)max_q * (q_heads / kv_heads) + 15) / 16);
-  p.tiles = (long long)requests * kv_heads * p.row_blocks;
-  const long long most = ((long long)max_kv + kStep * kWaves - 1) / (kStep * kWaves);
-  long long s = p.tiles > 0 ? (4ll * cus + p.tiles - 1) / p.tiles : 1;
-  if (s > most) s = most;
-  if (s < 1 || p.tiles * (long long)sizeof(uint32_t) > (long long)sm24::kCounterBytes) s = 1;
-  p.splits = (int)s;
+  const long long rows = (long long)max_q * (q_heads / kv_heads);
+  const long long row_blocks = (rows + 15) / 16;
+  const long long steps = ((long long)max_kv + kStep - 1) / kStep;
+  const long long per_cu = getenv("KV4_PER_CU") ? atoi(getenv("KV4_PER_CU")) : 2;
+  const long long most = per_cu * cus;
+  const long long heads = requests * row_blocks * kv_heads;
+  const long long div = getenv("KV4_DIV") ? atoi(getenv("KV4_DIV")) : 4;
+  p.log_kw = 3;
+  while (p.log_kw > 0 && heads * (1 << p.log_kw) / kWaves > most / div) p.log_kw--;
+  if (getenv("KV4_KW")) p.log_kw = atoi(getenv("KV4_KW"));
+  const int hw = kWaves >> p.log_kw;
+  const long long units = steps < 1 ? 1 : (steps + (1 << p.log_kw) - 1) >> p.log_kw;
+  long long w = requests * row_blocks * ((kv_heads + hw - 1) / hw) * units;
+  if (w > most) w = most;
+  p.workgroups = (int)w;
+  p.split = units > 1;
   return p;
 }
 
@@ -55,8 +66,8 @@ int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, i
   if (err != MARLIN_HIP_OK) return err;
   const kv4::Plan p = kv4::plan(requests, q_heads, kv_heads, max_q, max_kv, sms > 0 ? sms : 256);
   out[0] = 0;
-  out[1] = (int)(p.tiles * p.splits);
-  out[2] = p.splits;
+  out[1] = p.workgroups;
+  out[2] = p.split;
   return MARLIN_HIP_OK;
 }
 
@@ -93,22 +104,21 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
   a.max_pages = max_pages;
   a.log_page = 31 - __builtin_clz((unsigned)page_size);
   a.max_rows = 0x7FFFFFFF;
+  a.log_kw = p.log_kw;
+  a.group = q_heads / kv_heads;
   a.c1 = scale * 1.4426950408889634f;
-  if (p.splits > 1) {
-    err = sm24::get_scratch(dev, stream, (size_t)p.tiles * p.splits * 16 * (head_dim + 2) * sizeof(float),
-                            &a.counters, &a.partial);
+  if (p.split) {
+    const size_t rows = (size_t)p.workgroups * 2 * 16 * (kWaves >> p.log_kw);
+    err = sm24::get_scratch(dev, stream, rows * (head_dim + 2) * sizeof(float), &a.counters, &a.partial);
     if (err != MARLIN_HIP_OK) return err;
-    if (!a.counters) p.splits = 1;  // capturing, and this stream has no scratch yet
+    // (null while the stream is captured and has no scratch yet: tiles stay whole)
+    if (a.partial) a.partial_ml = a.partial + rows * head_dim;
   }
-  a.row_blocks = p.row_blocks;
-  a.splits = p.splits;
-  const long long blocks = p.tiles * p.splits;
-  if (blocks > 0xFFFFFFll) return refuse("kv4_attention: more row blocks than one launch takes");
   dispatch(head_dim, groups(head_dim, groupsize), [&](auto d, auto g) {
     constexpr int D = decltype(d)::value, NG = decltype(g)::value;
-    const dim3 grid((unsigned)blocks), block(64 * kWaves);
-    if (dtype == F16) hipLaunchKernelGGL((kv4_split_kernel<D, NG, F16>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((kv4_split_kernel<D, NG, BF16>), grid, block, 0, stream, a);
+    const dim3 grid((unsigned)p.workgroups), block(64 * kWaves);
+    if (dtype == F16) hipLaunchKernelGGL((kv4_split_kernel<D, NG, F16, 1>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((kv4_split_kernel<D, NG, BF16, 1>), grid, block, 0, stream, a);
   });
   return sm24::launch_error(hipGetLastError());
 }

@@ -9,8 +9,11 @@
 // so that the scales leave both products and the matrix cores multiply small integers,
 // which fp16 holds exactly.
 //
-// A workgroup takes 16 rows (one MFMA's columns) of one head and a range of 32-token
-// steps, its waves every fourth step.  Per step and wave:
+// A tile is 16 NB rows (NB MFMAs' columns) of HW heads over all their tokens.  A workgroup
+// gives each head KW of its eight waves, which take turns at the 32-token steps: a unit is a
+// step for each.  The tiles' units, end to end, are divided evenly over the workgroups,
+// whatever the requests' lengths: a workgroup takes the end of one tile, whole tiles, the
+// beginning of another.  Per step and wave:
 //   S^T = K Q^T  16x16x32 MFMAs, A = codes (rows = 16 tokens), B = Q, held in registers;
 //                lane (c, g) gets row c's sums of tokens 4 g .. 4 g + 3: what the second
 //                product wants as its B operand, if its reduction index counts tokens
@@ -31,16 +34,22 @@
 // entry is not a page, slots never written (their scales may be NaN).  Their p v is set to
 // zero after the product, not multiplied by zero.
 //
-// The waves meet in LDS; with more than one split the partial sums go through the
-// uncached scratch, and the last workgroup to arrive on the tile's counter adds them in
-// split order: one launch, and the same bits from run to run.
+// The waves meet in LDS; the partial sums of a divided tile go through the uncached
+// scratch, and the last of its workgroups to arrive on its counter adds them in order: one
+// launch, and the same bits from run to run.
 #pragma once
 #include "kv4_device.h"
 
 namespace kv4 {
 
-constexpr int kWaves = 4;
-constexpr int kStep = 32;          // tokens per wave and step
+constexpr int kLogWaves = 3, kWaves = 1 << kLogWaves;
+constexpr int kLogStep = 5, kStep = 1 << kLogStep;  // tokens per wave and step
+constexpr int kMaxSplits = 64;     // of one tile
+#ifndef KV4_MIN_SHARE
+#define KV4_MIN_SHARE 4
+#endif
+constexpr int kMinShare = KV4_MIN_SHARE;       // units of a piece
+constexpr int kMaxRequests = 2 * 64 * kWaves;  // of a launch that divides by the requests' lengths
 constexpr float kSlack = 8.f;      // p <= 2^8 of the reference
 constexpr float kVTop = 7.f;       // v 2^shift <= 2^7, so p v <= 2^15 < 65504
 constexpr float kNone = -1.0e30f;  // reference of a row that has seen nothing
@@ -53,13 +62,15 @@ struct AttnArgs {
   const int32_t* cu_q;  // null: request i is token i
   void* out;
   float* lse;           // null: not wanted
-  float* partial;       // [tile][split][16][D + 2]
-  uint32_t* counters;   // [tile], zero between launches
+  float* partial;       // [workgroup][first, last][row][D]; null: no tile is divided
+  float* partial_ml;    // [workgroup][first, last][row][2]: reference and sum
+  uint32_t* counters;   // [workgroup], zero between launches
   long long qt, qh;     // strides of q in elements
   int tokens, requests, q_heads, kv_heads;
   int num_pages, max_pages, log_page;
-  int row_blocks, splits;
   int max_rows;         // rows of a request above this are another kernel's
+  int log_kw;           // KW waves of a workgroup share a head (KW HW = kWaves)
+  int group;            // query heads of a kv head
   float c1;             // softmax scale * log2 e
 };
 
@@ -88,7 +99,49 @@ struct Shape {
   static constexpr int PARTS = 16 / BLOCKS;     // 1, 2 or 4
   static constexpr int OPS = 8 / PARTS;         // MFMAs per scale group
   static constexpr int STEPS = KW / NG;         // k-steps per scale group
+  // A step in LDS: K codes of 32 tokens, V codes, scales [half][K, V][quad][NG][4].
+  static constexpr int V_AT = kStep * D / 2, S_AT = kStep * D, STAGE = S_AT + 128 * NG;
+  static constexpr int LOADS = D / 32 + (NG == 4 ? 2 : 1);  // DMA instructions of a step
+  // 128 registers let two workgroups share a compute unit; with several groups of 128 dims
+  // one has it to itself, and its waves twice the steps in flight.
+  static constexpr bool TWO = NG == 1 || D == 64;
+  static constexpr int RING = TWO ? 2 : 4;  // steps of a wave in flight or in use
 };
+
+// x and its value in the lane 16 (32) places over, in one order or the other.  (In assembly:
+// given one value twice, the compiler takes the builtin's two results for the same.  The
+// wait states are those it puts between a VALU write and this read.)
+struct Pair {
+  float a, b;
+};
+__device__ __forceinline__ Pair across16(float x) {
+  Pair p = {x, x};
+  asm("s_nop 1\n\tv_permlane16_swap_b32 %0, %1" : "+v"(p.a), "+v"(p.b));
+  return p;
+}
+__device__ __forceinline__ Pair across32(float x) {
+  Pair p = {x, x};
+  asm("s_nop 1\n\tv_permlane32_swap_b32 %0, %1" : "+v"(p.a), "+v"(p.b));
+  return p;
+}
+// Over the four lanes of an MFMA column.
+__device__ __forceinline__ float column_max(float x) {
+  const Pair p = across16(x), q = across32(fmaxf(p.a, p.b));
+  return fmaxf(q.a, q.b);
+}
+__device__ __forceinline__ float column_sum(float x) {
+  const Pair p = across16(x), q = across32(p.a + p.b);
+  return q.a + q.b;
+}
+
+// Four bytes per lane from the lane's own address into lds + 4 lane.
+__device__ __forceinline__ void dma4(uint32_t lds, const void* src) {
+  asm volatile(
+      "s_mov_b32 m0, %0\n\ts_nop 0\n\t"
+      "global_load_lds_dword %1, off" ::"s"(lds),
+      "v"(src)
+      : "memory", "m0");
+}
 
 template <int D, int NG>
 struct Codes {
@@ -97,9 +150,27 @@ struct Codes {
   half4_t ks[2][NG], vs[2][NG];
 };
 
+// Constants of the unpacking, kept in registers the compiler cannot see through: with
+// literals it takes v_and_b32 and v_or_b32 where v_and_or_b32 does both.
+struct Magic {
+  uint32_t even, odd, exponent;
+  __device__ __forceinline__ Magic() {
+    asm("s_mov_b32 %0, 0x000f000f" : "=s"(even));
+    asm("s_mov_b32 %0, 0x00f000f0" : "=s"(odd));
+    asm("v_mov_b32 %0, 0x64006400" : "=v"(exponent));
+  }
+  // Nibbles 0 and 4, then 1 and 5 of a word, less 8 (see sm24::dequant4).
+  __device__ __forceinline__ half4_t codes(uint32_t q) const {
+    const half2_t l = __builtin_bit_cast(half2_t, (q & even) | exponent) - (half2_t){(_Float16)1032.f, (_Float16)1032.f};
+    const half2_t h = __builtin_bit_cast(half2_t, (q & odd) | exponent) * (half2_t){(_Float16)0.0625f, (_Float16)0.0625f} +
+                      (half2_t){(_Float16)-72.f, (_Float16)-72.f};
+    return (half4_t){l.x, l.y, h.x, h.y};
+  }
+};
+
 // Codes of a word less 8, in nibble order 0 4 1 5 2 6 3 7.
-__device__ __forceinline__ half8_t k_operand(uint32_t w) {
-  const half4_t a = sm24::dequant4(w), b = sm24::dequant4(w >> 8);
+__device__ __forceinline__ half8_t k_operand(const Magic& m, uint32_t w) {
+  const half4_t a = m.codes(w), b = m.codes(w >> 8);
   return (half8_t){a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 }
 
@@ -110,342 +181,603 @@ __device__ __forceinline__ uint32_t part_selector(int part) {
   else return 0x0C040C00u + 0x00010001u * (uint32_t)part;  // one byte each, zero above
 }
 
-// Operands 0 .. OPS - 1 of a scale group from eight tokens' words: operand i holds dim
-// (8 / PARTS) part + i of the words.
+// Operands of a scale group from eight tokens' words: operand i holds dim (8 / PARTS) part + i
+// of the words.  Where a word is one part, its low and its high half in turn, to spare
+// registers.
 template <int PARTS>
-__device__ __forceinline__ void v_operands(const u32x4& a, const u32x4& b, uint32_t sel, half8_t (&out)[8 / PARTS]) {
+constexpr int kTurns = PARTS == 1 ? 2 : 1;
+template <int PARTS>
+constexpr int kTurnOps = 8 / PARTS / kTurns<PARTS>;
+template <int PARTS>
+__device__ __forceinline__ void v_operands(const Magic& m, const u32x4& a, const u32x4& b, uint32_t sel, int turn,
+                                           half8_t (&out)[kTurnOps<PARTS>]) {
   const uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
   for (int p = 0; p < 4; p++) {
-    const uint32_t x = w[2 * p], y = w[2 * p + 1];
-    // t: a part of x's word in the low half, of y's in the high one; dequant4 pairs their
-    // nibbles 0, then their nibbles 1
-    auto put = [&](int i, uint32_t t) {
-      const half4_t h = sm24::dequant4(t);
+    // a part of the even token's word in the low half, of the odd one's in the high: their
+    // nibbles 0 become one pair, their nibbles 1 the next
+    const uint32_t t = __builtin_amdgcn_perm(w[2 * p + 1], w[2 * p],
+                                             PARTS > 1 ? sel : turn ? 0x07060302u : 0x05040100u);
+#pragma unroll
+    for (int i = 0; i < kTurnOps<PARTS>; i += 2) {
+      const half4_t h = m.codes(i ? t >> 8 : t);
       out[i][2 * p] = h.x, out[i][2 * p + 1] = h.y;
       out[i + 1][2 * p] = h.z, out[i + 1][2 * p + 1] = h.w;
-    };
-    if constexpr (PARTS == 1) {
-      const uint32_t t0 = __builtin_amdgcn_perm(y, x, 0x05040100u), t1 = __builtin_amdgcn_perm(y, x, 0x07060302u);
-      put(0, t0);
-      put(2, t0 >> 8);
-      put(4, t1);
-      put(6, t1 >> 8);
-    } else {
-      const uint32_t t = __builtin_amdgcn_perm(y, x, sel);
-      put(0, t);
-      if constexpr (PARTS == 2) put(2, t >> 8);
     }
   }
 }
 
-template <int D, int NG, int TYPE>
-__global__ __launch_bounds__(64 * kWaves) void kv4_split_kernel(AttnArgs a) {
+template <int D, int NG, int TYPE, int NB>
+__global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)) void kv4_split_kernel(AttnArgs a) {
   using S = Shape<D, NG>;
-  constexpr int RP = D + 4;  // floats per row in LDS
-  __shared__ __align__(16) float red[kWaves][16][RP];
-  __shared__ float red_m[kWaves][16], red_l[kWaves][16];
+  // the waves' rings; later 16 rows of D + 4 floats in each
+  static_assert(S::RING * S::STAGE >= 16 * (D + 4) * 4 && S::RING * S::STAGE >= 16 * (kMaxSplits + 2) * 4, "");
+  __shared__ __align__(16) uint8_t lds[kWaves * S::RING * S::STAGE];
+  __shared__ uint32_t begins[kMaxRequests];
+  __shared__ int few_first[64], few_n[64], few_kv[64];
+  __shared__ long long wave_sum[kWaves];
+  __shared__ int wave_max[kWaves];
   __shared__ uint32_t arrived;
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int c = lane & 15, g = lane >> 4;
-  const int split = blockIdx.x % a.splits;
-  const int tile = blockIdx.x / a.splits;  // (request, head, row block)
-  const int rb = tile % a.row_blocks;
-  const int head = tile / a.row_blocks % a.kv_heads;
-  const int r = tile / a.row_blocks / a.kv_heads;
-  const int G = a.q_heads / a.kv_heads;
+  const int G = a.group;
   const int T = 1 << a.log_page;
+  const int KW = 1 << a.log_kw, HW = kWaves >> a.log_kw;
+  const int kw = wave & (KW - 1), hw = wave >> a.log_kw;
+  const int head_groups = (a.kv_heads + HW - 1) >> (kLogWaves - a.log_kw);
 
-  const Request rq = request_of(a, r);
-  const int rows = rq.n * G;
-  if (rows > a.max_rows || rb * 16 >= rows) return;
-  const int past = rq.kv - rq.n;  // token t sees tokens 0 .. past + t
-  const int t_first = rb * 16 / G, t_last = min((rb * 16 + 15) / G, rq.n - 1);
-  const int end = max(past + t_last + 1, 0);  // tokens that some row of the block sees
-  const int all = min(max(past + t_first + 1, 0), end);  // ... that every row sees
-
-  // this split's steps: at least one a wave, so short requests take fewer splits
-  const int steps = (end + kStep - 1) / kStep;
-  const int per = max((steps + a.splits - 1) / a.splits, kWaves);
-  const int live = max((steps + per - 1) / per, 1);
-  if (split >= live) return;
-  const int s0 = split * per, s1 = min(s0 + per, steps);
-
-  // ---- Q: lane (c, g) holds row c's dims [32 w + 8 g, + 8), slots in the order the
-  // unpacking gives ----
-  const int row = rb * 16 + c;
-  const int t_row = row / G, h_row = head * G + row % G;
-  const int seen = row < rows ? max(past + t_row + 1, 0) : 0;  // tokens the row sees
-  half8_t qf[S::KW];
-  float c1 = a.c1;
-  {
-    float x[S::KW][8];
-    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(rq.first + min(t_row, rq.n - 1)) * a.qt +
-                          (long long)h_row * a.qh + 8 * g;
-    float amax = 0.f;
+  // ---- the division: every request's tiles are as long as its last one; rows that see
+  // nothing take a unit, to write their zeros.  Without scratch, and where the units do
+  // not fit 31 bits, tiles count as one and stay whole ----
+  auto blocks_of = [&](const Request& q) { return q.n * G > a.max_rows ? 0 : (q.n * G + 16 * NB - 1) / (16 * NB); };
+  auto units_of = [&](const Request& q) { return max((q.kv + kStep * KW - 1) >> (kLogStep + a.log_kw), 1); };
+  bool divided = a.partial != nullptr;
+  uint32_t total, share;
+  // Up to 64 requests are one to a lane, in every wave alike, and found by a ballot; more
+  // are two to a thread and searched for.
+  const bool few = a.requests <= 64;
+  Request own{0, 0, 0};
+  if (few && lane < a.requests) own = request_of(a, lane);
+  while (true) {
+    long long mine[2] = {0, 0};
+    int longest = 1;
+    auto cost = [&](const Request& q) {
+      long long n = (long long)blocks_of(q) * head_groups;
+      if (divided) {
+        if (n > 0) longest = max(longest, units_of(q));
+        n *= units_of(q);
+      }
+      return n;
+    };
+    if (few) {
+      mine[0] = cost(own);
+    } else {
 #pragma unroll
-    for (int w = 0; w < S::KW; w++) {
-      unpack8<TYPE>(*reinterpret_cast<const u32x4*>(src + 32 * w), x[w]);
-#pragma unroll
-      for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[w][i]));
+      for (int u = 0; u < 2; u++)
+        if (2 * tid + u < a.requests) mine[u] = cost(request_of(a, 2 * tid + u));
     }
-    if constexpr (TYPE == BF16) {
-      // bf16's range does not fit fp16: rows are brought to [2^7, 2^8) by a power of two
-      amax = fmaxf(amax, __shfl_xor(amax, 16));
-      amax = fmaxf(amax, __shfl_xor(amax, 32));
-      const int e = amax > 0.f && amax < __builtin_inff() ? 8 - __builtin_amdgcn_frexp_expf(amax) : 0;
+    long long sum = mine[0] + mine[1], all, before;
+    if (a.requests > 1) {
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const long long x = __shfl_up(sum, d);
+        if (lane >= d) sum += x;
+        longest = max(longest, __shfl_xor(longest, d));
+      }
+    }
+    before = sum - mine[0] - mine[1];
+    if (few) {
+      const int at = a.requests - 1;
+      all = (long long)(uint32_t)__builtin_amdgcn_readlane((int)(sum >> 32), at) << 32 |
+            (uint32_t)__builtin_amdgcn_readlane((int)sum, at);
+      if (wave == 0) {
+        begins[lane] = (uint32_t)before;
+        few_first[lane] = own.first, few_n[lane] = own.n, few_kv[lane] = own.kv;
+      }
+      __syncthreads();
+    } else {
+      if (lane == 63) {
+        wave_sum[wave] = sum;
+        wave_max[wave] = longest;
+      }
+      __syncthreads();
+      all = 0;
+#pragma unroll
+      for (int w = 0; w < kWaves; w++) {
+        if (w < wave) before += wave_sum[w];
+        all += wave_sum[w];
+        longest = max(longest, wave_max[w]);
+      }
+      begins[2 * tid] = (uint32_t)before;
+      begins[2 * tid + 1] = (uint32_t)(before + mine[0]);
+      __syncthreads();
+    }
+    if (divided && __builtin_amdgcn_readfirstlane((int)(all > 0x7FFFFFFFll))) {
+      divided = false;
+      continue;
+    }
+    total = __builtin_amdgcn_readfirstlane((uint32_t)all);
+    share = (total + gridDim.x - 1) / gridDim.x;
+    // a piece is worth its meeting in memory, and a tile lies in kMaxSplits shares at most
+    longest = __builtin_amdgcn_readfirstlane(longest);
+    if (divided) share = max(share, (uint32_t)max(min(longest, kMinShare), (longest + kMaxSplits - 2) / (kMaxSplits - 1)));
+    share = __builtin_amdgcn_readfirstlane(share);
+    break;
+  }
+
+  // The thread's index as a value of this piece only: what is computed from it is not kept
+  // in registers through the loop.
+  auto per_piece = [](int x) {
+    asm volatile("" : "+v"(x));
+    return x;
+  };
+  const Magic magic;
+  const uint32_t block = block_bytes<D, NG>(T);
+  uint8_t* const ring = lds + wave * (S::RING * S::STAGE);
+  const uint32_t ring_at = __builtin_amdgcn_readfirstlane(
+      (uint32_t)reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) uint8_t*)ring));
+
+  const uint32_t first_unit = blockIdx.x * share, last_unit = min(first_unit + share, total);
+  uint32_t unit = first_unit;
+  while (unit < last_unit) {
+    // ---- the piece: steps [s0, s1) of a tile ----
+    int r = 0;  // the last request that begins at the unit or before
+    Request rq;
+    uint32_t r_begin;
+    if (few) {
+      r = 63 - __builtin_clzll(__ballot(lane < a.requests && begins[lane] <= unit));
+      rq = Request{few_first[r], few_n[r], few_kv[r]};
+    } else {
+      for (int hi = a.requests; hi - r > 1;) {
+        const int mid = (r + hi) >> 1;
+        if (__builtin_amdgcn_readfirstlane(begins[mid]) <= unit) r = mid;
+        else hi = mid;
+      }
+      rq = request_of(a, r);
+    }
+    r_begin = begins[r];
+    r = __builtin_amdgcn_readfirstlane(r);
+    rq.first = __builtin_amdgcn_readfirstlane(rq.first);
+    rq.n = __builtin_amdgcn_readfirstlane(rq.n);
+    rq.kv = __builtin_amdgcn_readfirstlane(rq.kv);
+    r_begin = __builtin_amdgcn_readfirstlane(r_begin);
+    const int rows = rq.n * G, row_blocks = blocks_of(rq), len = divided ? units_of(rq) : 1;
+    const int tile = (int)((unit - r_begin) / (uint32_t)len);
+    const uint32_t tile_unit = r_begin + (uint32_t)tile * len;
+    const int rb = row_blocks == 1 ? 0 : tile % row_blocks;
+    const int own_head = (row_blocks == 1 ? tile : tile / row_blocks) * HW + hw, head = min(own_head, a.kv_heads - 1);  // (a wave may have none)
+    const int row0 = rb * 16 * NB;
+    const int past = rq.kv - rq.n;  // token t sees tokens 0 .. past + t
+    const bool one = rq.n == 1;  // (spares the divisions of a row's index)
+    const int t_first = one ? 0 : row0 / G, t_last = one ? 0 : min((row0 + 16 * NB - 1) / G, rq.n - 1);
+    const int end = max(past + t_last + 1, 0);             // tokens that some row of the tile sees
+    const int all = min(max(past + t_first + 1, 0), end);  // ... that every row sees
+    const int steps = (end + kStep - 1) / kStep;
+    // this wave's steps: s0, s0 + KW, ...
+    const uint32_t next_unit = min(tile_unit + len, last_unit);
+    const int s0 = (divided ? (int)(unit - tile_unit) * KW : 0) + kw;
+    const int s1 = divided ? min(steps, (int)(next_unit - tile_unit) * KW) : steps;
+    const int count = own_head < a.kv_heads && s1 > s0 ? (s1 - s0 + KW - 1) >> a.log_kw : 0;
+    const bool whole = unit == tile_unit && next_unit == tile_unit + len;
+    const bool first_piece = unit == first_unit;
+    if (!first_piece) __syncthreads();  // the piece before is done with LDS
+
+    // ---- Q: lane (c, g) holds row c's dims [32 w + 8 g, + 8), slots in the order the
+    // unpacking gives ----
+    const int lane = per_piece(threadIdx.x) & 63, c = lane & 15, g = lane >> 4;
+    const int blk = c / S::PARTS, part = c % S::PARTS;
+    const uint32_t sel = S::PARTS == 1 ? 0u : part_selector<S::PARTS == 1 ? 2 : S::PARTS>(part);
+    half8_t qf[NB][S::KW];
+    float c1[NB];
+    int seen[NB];  // tokens the row sees
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+      const int row = row0 + 16 * b + c, t_row = one ? 0 : row / G, h_row = one ? min(row, G - 1) : row - t_row * G;
+      seen[b] = row < rows ? max(past + t_row + 1, 0) : 0;
+      c1[b] = a.c1;
+      float x[S::KW][8];
+      const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(rq.first + min(t_row, rq.n - 1)) * a.qt +
+                            (long long)(head * G + h_row) * a.qh + 8 * g;
+      float amax = 0.f;
+#pragma unroll
+      for (int w = 0; w < S::KW; w++) {
+        unpack8<TYPE>(*reinterpret_cast<const u32x4*>(src + 32 * w), x[w]);
+#pragma unroll
+        for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[w][i]));
+      }
+      if constexpr (TYPE == BF16) {
+        // bf16's range does not fit fp16: rows are brought to [2^7, 2^8) by a power of two
+        amax = column_max(amax);
+        const int e = amax > 0.f && amax < __builtin_inff() ? 8 - __builtin_amdgcn_frexp_expf(amax) : 0;
+#pragma unroll
+        for (int w = 0; w < S::KW; w++)
+#pragma unroll
+          for (int i = 0; i < 8; i++) x[w][i] = __builtin_amdgcn_ldexpf(x[w][i], e);
+        c1[b] = __builtin_amdgcn_ldexpf(c1[b], -e);
+      }
+      constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
 #pragma unroll
       for (int w = 0; w < S::KW; w++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) x[w][i] = __builtin_amdgcn_ldexpf(x[w][i], e);
-      c1 = __builtin_amdgcn_ldexpf(c1, -e);
+        for (int i = 0; i < 8; i++) qf[b][w][i] = (_Float16)x[w][order[i]];
     }
-    constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
-#pragma unroll
-    for (int w = 0; w < S::KW; w++)
-#pragma unroll
-      for (int i = 0; i < 8; i++) qf[w][i] = (_Float16)x[w][order[i]];
-  }
 
-  // ---- the loop ----
-  float4_t O[NG][S::OPS];
-  float M = kNone, L = 0.f;
+    // ---- the loop ----
+    float4_t O[NB][NG][S::OPS];
+    float M[NB], L[NB], x_top[NB];    // x_top: x above which M rises
+    float shift = 0.f, v_top = 0.f;  // v 2^shift <= 2^kVTop while v <= v_top
 #pragma unroll
-  for (int n = 0; n < NG; n++)
-#pragma unroll
-    for (int i = 0; i < S::OPS; i++) O[n][i] = (float4_t){0.f, 0.f, 0.f, 0.f};
-  float shift = 0.f, v_top = 0.f;  // v 2^shift <= 2^kVTop while v <= v_top
-  float x_top = kNone;              // x above which M rises
-  const int blk = c / S::PARTS, part = c % S::PARTS;
-  const uint32_t sel = S::PARTS == 1 ? 0u : part_selector<S::PARTS == 1 ? 2 : S::PARTS>(part);
-  const size_t block = block_bytes<D, NG>(T);
-  const int32_t* pages = a.table + (size_t)r * a.max_pages;
-
-  // page ids of the wave's next 32 steps: lane i holds the page of half i % 2 of step i / 2
-  auto fetch_ids = [&](int s) {
-    const int tok = (s + (lane >> 1) * kWaves) * kStep + 16 * (lane & 1);
-    const int id = tok < end ? pages[tok >> a.log_page] : -1;
-    return (uint32_t)id < (uint32_t)a.num_pages ? id : -1;
-  };
-  auto fetch = [&](int s, int id0, int id1, Codes<D, NG>& f) {
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      const int id = u ? id1 : id0;
-      const int o = (s * kStep + 16 * u) & (T - 1);
-      // a page that is not there is read as the first one and masked
-      const uint8_t* b = a.cache + ((size_t)max(id, 0) * a.kv_heads + head) * block;
-      const uint8_t* kp = b + (o + c) * (D / 2) + g * (D / 8);
-      if constexpr (D == 128) {
-        const u32x4 w = *reinterpret_cast<const u32x4*>(kp);
-        f.k[u][0] = w.x, f.k[u][1] = w.y, f.k[u][2] = w.z, f.k[u][3] = w.w;
-      } else {
-        const u32x2 w = *reinterpret_cast<const u32x2*>(kp);
-        f.k[u][0] = w.x, f.k[u][1] = w.y;
-      }
-#pragma unroll
-      for (int n = 0; n < NG; n++) {
-        f.v[u][n] = *reinterpret_cast<const u32x4*>(b + v_word<D>(T, o + 4 * g, n * S::BLOCKS + blk));
-        f.ks[u][n] = *reinterpret_cast<const half4_t*>(b + k_scale<D, NG>(T, o + 4 * g, n));
-        f.vs[u][n] = *reinterpret_cast<const half4_t*>(b + v_scale<D, NG>(T, o + 4 * g, n));
-      }
-    }
-  };
-  auto compute = [&](int s, int id0, int id1, const Codes<D, NG>& f) {
-    float x[2][4];
-#pragma unroll
-    for (int u = 0; u < 2; u++) {
-      float4_t sum[NG];
-#pragma unroll
-      for (int n = 0; n < NG; n++) {
-        sum[n] = (float4_t){0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int w = 0; w < S::STEPS; w++)
-          sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k_operand(f.k[u][n * S::STEPS + w]), qf[n * S::STEPS + w],
-                                                          sum[n], 0, 0, 0);
-      }
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        x[u][i] = sum[0][i] * (float)f.ks[u][0][i];
-#pragma unroll
-        for (int n = 1; n < NG; n++) x[u][i] = __builtin_fmaf(sum[n][i], (float)f.ks[u][n][i], x[u][i]);
-      }
-    }
-    half4_t vs[2][NG];
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int n = 0; n < NG; n++) vs[u][n] = f.vs[u][n];
-    // (wave-uniform) a step that some row does not see whole
-    const bool masked = (s + 1) * kStep > all || id0 < 0 || id1 < 0;
-    if (masked) {
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-          const int tok = s * kStep + 16 * u + 4 * g + i;
-          const bool in = tok < seen && (u ? id1 : id0) >= 0;
-          x[u][i] = in ? x[u][i] : -__builtin_inff();
-#pragma unroll
-          for (int n = 0; n < NG; n++) vs[u][n][i] = in ? vs[u][n][i] : (_Float16)0.f;
-        }
-    }
-    float xm = x[0][0], vm = 0.f;
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        xm = fmaxf(xm, x[u][i]);
-#pragma unroll
-        for (int n = 0; n < NG; n++) vm = fmaxf(vm, (float)vs[u][n][i]);
-      }
-    if (__any(xm > x_top || vm > v_top)) {
-      // new reference: the rows' maxima so far and the largest v of all lanes
-      xm = fmaxf(xm, __shfl_xor(xm, 16));
-      xm = fmaxf(xm, __shfl_xor(xm, 32));
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) vm = fmaxf(vm, __shfl_xor(vm, d));
-      float new_shift = shift;
-      if (vm > v_top) {
-        // vm <= 2^e; 2^24 bounds the shift where every v so far is tiny or zero
-        new_shift = fminf(kVTop - (float)__builtin_amdgcn_frexp_expf(vm), 24.f);
-        v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
-      }
-      // M = max - shift: rows keep the larger of the old maximum and this step's
-      const float old_max = M == kNone ? kNone : M + shift;
-      const float new_max = fmaxf(old_max, xm * c1);
-      const float new_M = new_max <= kNone ? kNone : new_max - new_shift;
-      const float f = M == kNone ? 0.f : __builtin_amdgcn_exp2f(M - new_M);
-      M = new_M;
-      shift = new_shift;
-      x_top = M == kNone ? kNone : (new_max + kSlack) / c1;
-      L *= f;
+    for (int b = 0; b < NB; b++) {
+      M[b] = x_top[b] = kNone;
+      L[b] = 0.f;
 #pragma unroll
       for (int n = 0; n < NG; n++)
 #pragma unroll
-        for (int i = 0; i < S::OPS; i++) O[n][i] *= f;
+        for (int i = 0; i < S::OPS; i++) O[b][n][i] = (float4_t){0.f, 0.f, 0.f, 0.f};
     }
-    half4_t ph[2][NG];
-#pragma unroll
-    for (int u = 0; u < 2; u++)
-#pragma unroll
-      for (int i = 0; i < 4; i++) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[u][i], c1, -M));
-        L += p;
-#pragma unroll
-        for (int n = 0; n < NG; n++) ph[u][n][i] = (_Float16)(p * (float)vs[u][n][i]);
-      }
-#pragma unroll
-    for (int n = 0; n < NG; n++) {
-      const half8_t P = {ph[0][n][0], ph[0][n][1], ph[0][n][2], ph[0][n][3],
-                         ph[1][n][0], ph[1][n][1], ph[1][n][2], ph[1][n][3]};
-      half8_t vo[S::OPS];
-      v_operands<S::PARTS>(f.v[0][n], f.v[1][n], sel, vo);
-#pragma unroll
-      for (int i = 0; i < S::OPS; i++) O[n][i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vo[i], P, O[n][i], 0, 0, 0);
-    }
-  };
+    const int32_t* pages = a.table + (size_t)r * a.max_pages;
+    const uint8_t* const cache = a.cache + (size_t)head * block;
 
-  for (int base = s0 + wave; base < s1; base += 32 * kWaves) {
-    const int ids = fetch_ids(base);
-    const int count = min((s1 - base + kWaves - 1) / kWaves, 32);
-    auto id = [&](int i) { return __builtin_amdgcn_readlane(ids, i); };
-    Codes<D, NG> f[2];
-    fetch(base, id(0), id(1), f[0]);
-    for (int k = 0; k < count; k += 2) {
-      if (k + 1 < count) fetch(base + (k + 1) * kWaves, id(2 * k + 2), id(2 * k + 3), f[1]);
-      compute(base + k * kWaves, id(2 * k), id(2 * k + 1), f[0]);
-      if (k + 1 < count) {
-        if (k + 2 < count) fetch(base + (k + 2) * kWaves, id(2 * k + 4), id(2 * k + 5), f[0]);
-        compute(base + (k + 1) * kWaves, id(2 * k + 2), id(2 * k + 3), f[1]);
+    // Places of 32 of the wave's steps from k on: lane i has half i % 2 of step k + i / 2,
+    // the byte offset of its K codes (bit 63: no such page).
+    auto places = [&](int k) {
+      const int tok = (s0 + (k + (lane >> 1)) * KW) * kStep + 16 * (lane & 1);
+      const int id = tok < end ? pages[tok >> a.log_page] : -1;
+      const bool there = (uint32_t)id < (uint32_t)a.num_pages;
+      // a page that is not there is read as the first one and masked
+      const uint64_t at = (uint64_t)(there ? (uint32_t)id : 0u) * ((uint64_t)block * a.kv_heads) + (tok & (T - 1)) * (D / 2);
+      return there ? at : at | 1ull << 63;
+    };
+    uint64_t now = places(0), then = places(32);  // of steps [32 b, 32 b + 32) and the 32 after
+    auto place = [&](uint64_t v, int i) {
+      return (uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), i) << 32 |
+             (uint32_t)__builtin_amdgcn_readlane((int)v, i);
+    };
+    // Sends step k into a stage of the ring.
+    auto send = [&](int k, uint64_t p0, uint64_t p1, uint32_t to) {
+      const uint8_t* k0 = cache + (p0 & ~(1ull << 63));
+      const uint8_t* k1 = cache + (p1 & ~(1ull << 63));
+      const uint32_t v_off = (uint32_t)T * (D / 2);
+      if constexpr (D == 128) {  // 16 tokens are 64 lanes' 16 bytes
+        sm24::dma16x1(to, 16 * lane, k0);
+        sm24::dma16x1(to + 1024, 16 * lane, k1);
+        sm24::dma16x1(to + S::V_AT, 16 * lane, k0 + v_off);
+        sm24::dma16x1(to + S::V_AT + 1024, 16 * lane, k1 + v_off);
+      } else {
+        const uint8_t* kl = (lane < 32 ? k0 : k1 - 512) + 16 * lane;
+        sm24::dma16(to, kl);
+        sm24::dma16(to + S::V_AT, kl + v_off);
       }
-    }
-  }
+      // scales: 8 NG lanes for K and for V of a half; they lie T D - o (D/2 - 2 NG) behind the K codes
+      constexpr int L8 = 8 * NG;
+      const uint32_t tok = (uint32_t)(s0 + k * KW) * kStep;
+      const uint32_t o0 = tok & (T - 1), o1 = (tok + 16) & (T - 1);
+      const uint8_t* sc0 = k0 + (uint32_t)T * D - o0 * (D / 2 - 2 * NG);
+      const uint8_t* sc1 = k1 + (uint32_t)T * D - o1 * (D / 2 - 2 * NG);
+      const uint32_t at = (lane % L8) * 4 + (lane / L8 % 2) * (2 * NG * (uint32_t)T);
+      if constexpr (NG == 4) {
+        dma4(to + S::S_AT, sc0 + at);
+        dma4(to + S::S_AT + 256, sc1 + at);
+      } else if (lane < 4 * L8) {
+        dma4(to + S::S_AT, (lane < 2 * L8 ? sc0 : sc1) + at);
+      }
+    };
+    auto receive = [&](const uint8_t* from, Codes<D, NG>& f) {
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        const uint8_t* kp = from + u * (8 * D) + c * (D / 2) + g * (D / 8);
+        if constexpr (D == 128) {
+          const u32x4 w = *reinterpret_cast<const u32x4*>(kp);
+          f.k[u][0] = w.x, f.k[u][1] = w.y, f.k[u][2] = w.z, f.k[u][3] = w.w;
+        } else {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(kp);
+          f.k[u][0] = w.x, f.k[u][1] = w.y;
+        }
+#pragma unroll
+        for (int n = 0; n < NG; n++) {
+          f.v[u][n] = *reinterpret_cast<const u32x4*>(from + S::V_AT + u * (8 * D) + g * (2 * D) + (n * S::BLOCKS + blk) * 16);
+          f.ks[u][n] = *reinterpret_cast<const half4_t*>(from + S::S_AT + u * (64 * NG) + (g * NG + n) * 8);
+          f.vs[u][n] = *reinterpret_cast<const half4_t*>(from + S::S_AT + u * (64 * NG) + 32 * NG + (g * NG + n) * 8);
+        }
+      }
+    };
+    auto compute = [&](int s, bool there0, bool there1, const Codes<D, NG>& f) {
+      float x[NB][2][4];
+#pragma unroll
+      for (int u = 0; u < 2; u++) {
+        float4_t sum[NB][NG];
+#pragma unroll
+        for (int n = 0; n < NG; n++) {
+#pragma unroll
+          for (int b = 0; b < NB; b++) sum[b][n] = (float4_t){0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int w = 0; w < S::STEPS; w++) {
+            const half8_t k = k_operand(magic, f.k[u][n * S::STEPS + w]);
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+              sum[b][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[b][n * S::STEPS + w], sum[b][n], 0, 0, 0);
+          }
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            x[b][u][i] = sum[b][0][i] * (float)f.ks[u][0][i];
+#pragma unroll
+            for (int n = 1; n < NG; n++) x[b][u][i] = __builtin_fmaf(sum[b][n][i], (float)f.ks[u][n][i], x[b][u][i]);
+          }
+      }
+      half4_t vs[2][NG];
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int n = 0; n < NG; n++) vs[u][n] = f.vs[u][n];
+      // (wave-uniform) a step that some row does not see whole
+      const bool masked = (s + 1) * kStep > all || !there0 || !there1;
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+          for (int i = 0; i < 4; i++) {
+            const int tok = s * kStep + 16 * u + 4 * g + i;
+            bool some = false;  // scales of tokens that no row here sees may be anything
+#pragma unroll
+            for (int b = 0; b < NB; b++) {
+              const bool in = tok < seen[b] && (u ? there1 : there0);
+              x[b][u][i] = in ? x[b][u][i] : -__builtin_inff();
+              some |= in;
+            }
+#pragma unroll
+            for (int n = 0; n < NG; n++) vs[u][n][i] = some ? vs[u][n][i] : (_Float16)0.f;
+          }
+      }
+      float xm[NB], vm = 0.f;
+      bool rise = false;
+#pragma unroll
+      for (int b = 0; b < NB; b++) {
+        xm[b] = x[b][0][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) xm[b] = fmaxf(xm[b], x[b][i / 4][i % 4]);
+        rise |= xm[b] > x_top[b];
+      }
+#pragma unroll
+      for (int i = 0; i < 8 * NG; i++) vm = fmaxf(vm, (float)vs[i / 4 / NG][i / 4 % NG][i % 4]);
+      if (__any(rise || vm > v_top)) {
+        // new reference: the rows' maxima so far and the largest v (the four lanes of a row agree)
+        vm = column_max(vm);
+        float new_shift = shift;
+        if (vm > v_top) {
+          // vm <= 2^e; 2^24 bounds the shift where every v so far is tiny
+          new_shift = fminf(kVTop - (float)__builtin_amdgcn_frexp_expf(vm), 24.f);
+          v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
+        }
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+          const float m = column_max(xm[b]);
+          // M = max - shift: rows keep the larger of the old maximum and this step's
+          const float old_max = M[b] == kNone ? kNone : M[b] + shift;
+          const float new_max = fmaxf(old_max, m * c1[b]);
+          const float new_M = new_max <= kNone ? kNone : new_max - new_shift;
+          const float f = M[b] == kNone ? 0.f : __builtin_amdgcn_exp2f(M[b] - new_M);
+          M[b] = new_M;
+          x_top[b] = new_M == kNone ? kNone : (new_max + kSlack) * __builtin_amdgcn_rcpf(c1[b]);
+          L[b] *= f;
+#pragma unroll
+          for (int n = 0; n < NG; n++)
+#pragma unroll
+            for (int i = 0; i < S::OPS; i++) O[b][n][i] *= f;
+        }
+        shift = new_shift;
+      }
+      half8_t P[NB][NG];
+#pragma unroll
+      for (int b = 0; b < NB; b++)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i / 4][i % 4], c1[b], -M[b]));
+          L[b] += p;
+#pragma unroll
+          for (int n = 0; n < NG; n++) P[b][n][i] = (_Float16)(p * (float)vs[i / 4][n][i % 4]);
+        }
+      if (NB > 1 && masked) {
+        // a scale that another row of the tile sees may be NaN: what this row does not see is zero
+#pragma unroll
+        for (int b = 0; b < NB; b++)
+#pragma unroll
+          for (int i = 0; i < 8; i++)
+#pragma unroll
+            for (int n = 0; n < NG; n++)
+              P[b][n][i] = x[b][i / 4][i % 4] == -__builtin_inff() ? (_Float16)0.f : P[b][n][i];
+      }
+#pragma unroll
+      for (int n = 0; n < NG; n++)
+#pragma unroll
+        for (int turn = 0; turn < kTurns<S::PARTS>; turn++) {
+          constexpr int OT = kTurnOps<S::PARTS>;
+          half8_t vo[OT];
+          v_operands<S::PARTS>(magic, f.v[0][n], f.v[1][n], sel, turn, vo);
+#pragma unroll
+          for (int i = 0; i < OT; i++)
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+              O[b][n][turn * OT + i] =
+                  __builtin_amdgcn_mfma_f32_16x16x32_f16(vo[i], P[b][n], O[b][n][turn * OT + i], 0, 0, 0);
+        }
+    };
 
-  // ---- the waves meet: lane (c, g) holds row c's dims of MFMA rows 4 g + i ----
-  L += __shfl_xor(L, 16);
-  L += __shfl_xor(L, 32);
 #pragma unroll
-  for (int n = 0; n < NG; n++)
-#pragma unroll
-    for (int i = 0; i < S::OPS; i++)
-#pragma unroll
-      for (int k = 0; k < 4; k++) {
-        const int m = 4 * g + k;
-        const int d = 8 * (n * S::BLOCKS + m / S::PARTS) + (8 / S::PARTS) * (m % S::PARTS) + i;
-        red[wave][c][d] = O[n][i][k];
+    for (int k = 0; k < S::RING; k++)
+      if (k < count) send(k, place(now, 2 * k), place(now, 2 * k + 1), ring_at + k * S::STAGE);
+    int stage = 0;
+#pragma unroll 1
+    for (int k = 0; k < count; k++) {
+      if (k > 0 && (k & 31) == 0) {
+        now = then;
+        then = places(k + 32);
       }
-  if (g == 0) {
-    red_m[wave][c] = M;
-    red_l[wave][c] = L;
-  }
-  __syncthreads();
-  // thread: row tid / 16, dims [D/16 * (tid % 16), + D/16)
-  constexpr int E = D / 16;
-  const int rr = tid >> 4, d0 = E * (tid & 15);
-  const bool exists = rb * 16 + rr < rows;
-  float m = red_m[0][rr];
-#pragma unroll
-  for (int w = 1; w < kWaves; w++) m = fmaxf(m, red_m[w][rr]);
-  float l = 0.f, o[E] = {};
-#pragma unroll
-  for (int w = 0; w < kWaves; w++) {
-    const float f = __builtin_amdgcn_exp2f(red_m[w][rr] - m);
-    l += f * red_l[w][rr];
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] += f * red[w][rr][d0 + e];
-  }
-  if (live > 1) {
-    constexpr int W = D + 2;
-    float* part = a.partial + ((size_t)tile * a.splits + split) * 16 * W + (size_t)rr * W;
-    if (exists) {
-#pragma unroll
-      for (int e = 0; e < E; e += 2) *reinterpret_cast<float2*>(part + d0 + e) = make_float2(o[e], o[e + 1]);
-      if ((tid & 15) == 0) *reinterpret_cast<float2*>(part + D) = make_float2(m, l);
+      const int i = 2 * (k & 31);
+      const bool there0 = __builtin_amdgcn_readlane((int)(now >> 32), i) >= 0;
+      const bool there1 = __builtin_amdgcn_readlane((int)(now >> 32), i + 1) >= 0;
+      if (k + S::RING <= count) sm24::wait_vm<(S::RING - 1) * S::LOADS>();
+      else sm24::wait_vm<0>();
+      Codes<D, NG> f;
+      receive(ring + stage * S::STAGE, f);
+      // the stage's reads are done before it is filled again
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_sched_barrier(0);
+      if (k + S::RING < count) {
+        const int j = 2 * ((k + S::RING) & 31);
+        if ((k & 31) + S::RING < 32) send(k + S::RING, place(now, j), place(now, j + 1), ring_at + stage * S::STAGE);
+        else send(k + S::RING, place(then, j), place(then, j + 1), ring_at + stage * S::STAGE);
+      }
+      stage = stage + 1 == S::RING ? 0 : stage + 1;
+      compute(s0 + k * KW, there0, there1, f);
     }
-    // every thread's stores are done before the barrier, the counter moves after it
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(0);
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __syncthreads();
-    if (tid == 0)
-      arrived = __hip_atomic_fetch_add(a.counters + tile, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
-    __syncthreads();
-    if (arrived != (uint32_t)live) return;
-    if (tid == 0) __hip_atomic_store(a.counters + tile, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (!exists) return;
-    const float* all_parts = a.partial + (size_t)tile * a.splits * 16 * W + (size_t)rr * W;
-    m = kNone;
-    l = 0.f;
+
+    // ---- a head's waves meet, 16 rows at a time: lane (c, g) holds row c's dims of MFMA
+    // rows 4 g + i; then the waves share out the items (row, four dims) ----
+    constexpr int RP = D + 4, Q4 = D / 4;  // floats of a row in LDS, items of a row
+    const int et = per_piece(threadIdx.x) & 63, ec = et & 15, eg = et >> 4;
+    const int item0 = et + 64 * kw, items = 64 << a.log_kw;
+    uint8_t* const group = lds + (hw << a.log_kw) * (S::RING * S::STAGE);  // the head's waves' rings
+    const bool exists = own_head < a.kv_heads;
+    const int live_rows = min(rows - row0, 16 * NB);
+    // a piece's place in the scratch, and a row of this head in it
+    auto slot_row = [&](uint32_t w, int second, int row) {
+      return (((size_t)w * 2 + second) * HW + hw) * (16 * NB) + row;
+    };
+    auto write = [&](int row, int d0, float m, float l, const float4_t& o) {
+      const int i = row0 + row, t = one ? 0 : i / G;
+      const size_t at = (size_t)(rq.first + t) * a.q_heads + head * G + i - t * G;
+      const float inv = l == 0.f ? 0.f : 1.f / l;  // no token seen: zeros (a NaN stays one)
+      uint16_t* dst = static_cast<uint16_t*>(a.out) + at * D + d0;
+      *reinterpret_cast<u32x2*>(dst) =
+          (u32x2){(uint32_t)from_float<TYPE>(o.x * inv) | (uint32_t)from_float<TYPE>(o.y * inv) << 16,
+                  (uint32_t)from_float<TYPE>(o.z * inv) | (uint32_t)from_float<TYPE>(o.w * inv) << 16};
+      if (a.lse != nullptr && d0 == 0)
+        a.lse[at] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+    };
 #pragma unroll
-    for (int e = 0; e < E; e++) o[e] = 0.f;
-    for (int s = 0; s < live; s++) {
-      const float* p = all_parts + (size_t)s * 16 * W;
-      const float2 ml = *reinterpret_cast<const float2*>(p + D);
-      const float nm = fmaxf(m, ml.x);
-      const float f0 = __builtin_amdgcn_exp2f(m - nm), f1 = __builtin_amdgcn_exp2f(ml.x - nm);
-      m = nm;
-      l = l * f0 + ml.y * f1;
+    for (int b = 0; b < NB; b++) {
+      __syncthreads();  // the rings, or the block of rows before, are done with
+      L[b] = column_sum(L[b]);
+      float* mine = reinterpret_cast<float*>(ring);
 #pragma unroll
-      for (int e = 0; e < E; e += 2) {
-        const float2 v = *reinterpret_cast<const float2*>(p + d0 + e);
-        o[e] = o[e] * f0 + v.x * f1;
-        o[e + 1] = o[e + 1] * f0 + v.y * f1;
+      for (int n = 0; n < NG; n++)
+#pragma unroll
+        for (int i = 0; i < S::OPS; i++)
+#pragma unroll
+          for (int k = 0; k < 4; k++) {
+            const int m = 4 * eg + k;
+            mine[ec * RP + 8 * (n * S::BLOCKS + m / S::PARTS) + (8 / S::PARTS) * (m % S::PARTS) + i] = O[b][n][i][k];
+          }
+      if (eg == 0) *reinterpret_cast<float2*>(mine + ec * RP + D) = make_float2(M[b], L[b]);
+      __syncthreads();
+#pragma unroll 1
+      for (int it = item0; it < 16 * Q4; it += items) {
+        const int row = it / Q4, d0 = it % Q4 * 4;
+        if (!exists || 16 * b + row >= live_rows) break;  // (rows ascend)
+        const float* from = reinterpret_cast<const float*>(group) + row * RP;
+        constexpr int NEXT = S::RING * S::STAGE / 4;  // floats from a wave's to the next
+        float m = kNone, l = 0.f;
+        float4_t o = {0.f, 0.f, 0.f, 0.f};
+        float2 ml[kWaves];
+        float4_t v[kWaves];
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {  // (all reads in flight; those past KW repeat the last and do not count)
+          const float* at = from + min(w, KW - 1) * NEXT;
+          ml[w] = *reinterpret_cast<const float2*>(at + D);
+          v[w] = *reinterpret_cast<const float4_t*>(at + d0);
+        }
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) m = fmaxf(m, ml[w].x);
+#pragma unroll
+        for (int w = 0; w < kWaves; w++) {
+          const float f = w < KW ? __builtin_amdgcn_exp2f(ml[w].x - m) : 0.f;
+          l += f * ml[w].y;
+          o += v[w] * f;
+        }
+        if (whole) {
+          write(16 * b + row, d0, m, l, o);
+        } else {
+          const size_t at = slot_row(blockIdx.x, first_piece ? 0 : 1, 16 * b + row);
+          *reinterpret_cast<float4_t*>(a.partial + at * D + d0) = o;
+          if (d0 == 0) *reinterpret_cast<float2*>(a.partial_ml + at * 2) = make_float2(m, l);
+        }
       }
     }
-  }
-  if (!exists) return;
-  const int t_out = (rb * 16 + rr) / G, h_out = head * G + (rb * 16 + rr) % G;
-  const size_t at = (size_t)(rq.first + t_out) * a.q_heads + h_out;
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // no token seen: zeros (a NaN stays one)
-  uint16_t* dst = static_cast<uint16_t*>(a.out) + at * D + d0;
+    if (!whole) {
+      // every thread's stores are done before the barrier, the counter (the first
+      // workgroup's: only its last piece is a tile's beginning) moves after it
+      const uint32_t w0 = tile_unit / share, pieces = (tile_unit + len - 1) / share - w0 + 1;
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      __builtin_amdgcn_s_waitcnt(0);
+      __atomic_signal_fence(__ATOMIC_SEQ_CST);
+      __syncthreads();
+      if (tid == 0)
+        arrived = __hip_atomic_fetch_add(a.counters + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+      __syncthreads();
+      if (arrived == pieces) {
+        if (tid == 0) __hip_atomic_store(a.counters + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        // only the first workgroup's piece may be its second
+        const int second0 = w0 * share < tile_unit ? 1 : 0;
+        float* weight = reinterpret_cast<float*>(group);  // [row][piece], then [row] {reference, sum}
+        float* row_ml = weight + 16 * kMaxSplits;
+#pragma unroll 1
+        for (int b = 0; b < NB; b++) {
+          const int left = exists ? min(live_rows - 16 * b, 16) : 0;
+          if (b > 0) __syncthreads();
+          // lane s reads a row's reference and sum of piece s; the wave weighs the pieces
+          float2 ml[16];
 #pragma unroll
-  for (int e = 0; e < E; e += 2)
-    *reinterpret_cast<uint32_t*>(dst + e) =
-        (uint32_t)from_float<TYPE>(o[e] * inv) | (uint32_t)from_float<TYPE>(o[e + 1] * inv) << 16;
-  if (a.lse != nullptr && (tid & 15) == 0)
-    a.lse[at] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+          for (int j = 0; j < 16; j++) {
+            const int row = kw + (j << a.log_kw);
+            ml[j] = make_float2(kNone, 0.f);
+            if (row < left && et < (int)pieces)
+              ml[j] = *reinterpret_cast<const float2*>(
+                  a.partial_ml + slot_row(w0 + et, et == 0 ? second0 : 0, 16 * b + row) * 2);
+          }
+#pragma unroll
+          for (int j = 0; j < 16; j++) {
+            const int row = kw + (j << a.log_kw);
+            if (row < left) {  // (wave-uniform)
+              float m = ml[j].x;
+#pragma unroll
+              for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+              const float f = et < (int)pieces ? __builtin_amdgcn_exp2f(ml[j].x - m) : 0.f;
+              float l = f * ml[j].y;
+#pragma unroll
+              for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+              weight[row * kMaxSplits + et] = f;
+              if (et == 0) row_ml[2 * row] = m, row_ml[2 * row + 1] = l;
+            }
+          }
+          __syncthreads();
+#pragma unroll 1
+          for (int it = item0; it < left * Q4; it += items) {
+            const int row = it / Q4, d0 = it % Q4 * 4;
+            float4_t o = {0.f, 0.f, 0.f, 0.f};
+            constexpr int FLIGHT = 8;  // pieces in flight
+#pragma unroll 1
+            for (uint32_t s = 0; s < pieces; s += FLIGHT) {
+              float4_t v[FLIGHT];
+#pragma unroll
+              for (int k = 0; k < FLIGHT; k++) {
+                const uint32_t p = min(s + k, pieces - 1);
+                v[k] = *reinterpret_cast<const float4_t*>(
+                    a.partial + slot_row(w0 + p, p == 0 ? second0 : 0, 16 * b + row) * D + d0);
+              }
+#pragma unroll
+              for (int k = 0; k < FLIGHT; k++) o += v[k] * weight[row * kMaxSplits + s + k];  // (zero past the last)
+            }
+            write(16 * b + row, d0, row_ml[2 * row], row_ml[2 * row + 1], o);
+          }
+        }
+      }
+    }
+    unit = next_unit;
+  }
 }
 
 }  // namespace kv4

@@ -61,15 +61,15 @@ def test_wrappers_refuse_cpu_tensors(built_lib):
 
 
 def test_plan(built_lib):
-    """Long caches of few heads are split until the compute units are covered; short ones and
-    large batches are not; a split has a step of 32 tokens for each of its four waves."""
-    assert marlin.plan_kv4_attention(1, 32, 32, 128, 1, 100)["splits"] == 1
-    assert marlin.plan_kv4_attention(1, 64, 8, 128, 1, 131072, sms=256)["splits"] >= 32
-    assert marlin.plan_kv4_attention(4096, 64, 8, 128, 1, 131072)["splits"] == 1
+    """Two workgroups a compute unit where there is that much work, fewer for short caches of few
+    heads, and no division (no scratch) where a tile has no step of 32 tokens for each wave."""
+    assert marlin.plan_kv4_attention(1, 32, 32, 128, 1, 100) == {"workgroups": 32, "split": False}
+    assert marlin.plan_kv4_attention(1, 64, 8, 128, 1, 131072, sms=256) == {"workgroups": 512, "split": True}
+    assert marlin.plan_kv4_attention(4096, 64, 8, 128, 1, 131072)["workgroups"] == 512
     assert marlin.plan_kv4_attention(0, 64, 8, 128, 1, 1024)["workgroups"] == 0
-    for kv in (1, 128, 129, 1000):
+    for kv in (1, 256, 257, 1000):
         p = marlin.plan_kv4_attention(1, 8, 8, 128, 1, kv)
-        assert 1 <= p["splits"] <= -(-kv // 128)
+        assert p["workgroups"] == 8 * -(-kv // 256) and p["split"] == (kv > 256)
     with pytest.raises(RuntimeError, match="multiple"):
         marlin.plan_kv4_attention(1, 9, 2, 128)
 
