@@ -2,7 +2,6 @@
 #include <hip/hip_runtime.h>
 #include <math.h>
 #include <stdint.h>
-#include <stdlib.h>
 
 #include "kv4_host.h"
 #include "kv4_split.h"
@@ -21,20 +20,20 @@ struct Plan {
 };
 
 // Two workgroups of eight waves fill a compute unit.  Waves of a workgroup that share a
-// head (KW) meet in LDS, pieces of a tile in memory: few tiles take all eight for a head,
-// many tiles fewer.
+// head (KW) meet in LDS, pieces of a tile in memory.  Few tiles take all eight waves for a
+// head (one request of 131072 tokens on 8 heads: 43 us with eight, 69 with two, 124 with
+// one); from an eighth of a tile a workgroup on, fewer, as a workgroup otherwise goes
+// through several tiles one after the other (24 requests on 32 heads: 86 us with eight, 60
+// with one; 64 requests on 8: 135, 133 with four, 147 with one).
 Plan plan(int requests, int q_heads, int kv_heads, int max_q, int max_kv, int cus) {
   Plan p;
   const long long rows = (long long)max_q * (q_heads / kv_heads);
   const long long row_blocks = (rows + 15) / 16;
   const long long steps = ((long long)max_kv + kStep - 1) / kStep;
-  const long long per_cu = getenv("KV4_PER_CU") ? atoi(getenv("KV4_PER_CU")) : 2;
-  const long long most = per_cu * cus;
+  const long long most = 2ll * cus;
   const long long heads = requests * row_blocks * kv_heads;
-  const long long div = getenv("KV4_DIV") ? atoi(getenv("KV4_DIV")) : 4;
-  p.log_kw = 3;
-  while (p.log_kw > 0 && heads * (1 << p.log_kw) / kWaves > most / div) p.log_kw--;
-  if (getenv("KV4_KW")) p.log_kw = atoi(getenv("KV4_KW"));
+  p.log_kw = kLogWaves;
+  while (p.log_kw > 0 && heads * (1 << p.log_kw) / kWaves > most / 4) p.log_kw--;
   const int hw = kWaves >> p.log_kw;
   const long long units = steps < 1 ? 1 : (steps + (1 << p.log_kw) - 1) >> p.log_kw;
   long long w = requests * row_blocks * ((kv_heads + hw - 1) / hw) * units;

@@ -44,11 +44,7 @@ namespace kv4 {
 
 constexpr int kLogWaves = 3, kWaves = 1 << kLogWaves;
 constexpr int kLogStep = 5, kStep = 1 << kLogStep;  // tokens per wave and step
-constexpr int kMaxSplits = 64;     // of one tile
-#ifndef KV4_MIN_SHARE
-#define KV4_MIN_SHARE 4
-#endif
-constexpr int kMinShare = KV4_MIN_SHARE;       // units of a piece
+constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last workgroup's read of it
 constexpr int kMaxRequests = 2 * 64 * kWaves;  // of a launch that divides by the requests' lengths
 constexpr float kSlack = 8.f;      // p <= 2^8 of the reference
 constexpr float kVTop = 7.f;       // v 2^shift <= 2^7, so p v <= 2^15 < 65504
@@ -299,9 +295,8 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
     }
     total = __builtin_amdgcn_readfirstlane((uint32_t)all);
     share = (total + gridDim.x - 1) / gridDim.x;
-    // a piece is worth its meeting in memory, and a tile lies in kMaxSplits shares at most
-    longest = __builtin_amdgcn_readfirstlane(longest);
-    if (divided) share = max(share, (uint32_t)max(min(longest, kMinShare), (longest + kMaxSplits - 2) / (kMaxSplits - 1)));
+    // a tile lies in kMaxSplits shares at most
+    if (divided) share = max(share, (uint32_t)((longest + kMaxSplits - 2) / (kMaxSplits - 1)));
     share = __builtin_amdgcn_readfirstlane(share);
     break;
   }
@@ -749,7 +744,7 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
               float l = f * ml[j].y;
 #pragma unroll
               for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-              weight[row * kMaxSplits + et] = f;
+              if (et < kMaxSplits) weight[row * kMaxSplits + et] = f;
               if (et == 0) row_ml[2 * row] = m, row_ml[2 * row + 1] = l;
             }
           }
