@@ -8,6 +8,13 @@
 
 namespace kv4 {
 
+hipError_t launch_prompt(const AttnArgs& a, int workgroups, int head_dim, int ng, int dtype, hipStream_t stream);
+
+// Requests of at most so many rows (new tokens times the query heads of a kv head) go to the
+// split kernel, the others to the prompt kernel, each of which passes over the other's.
+constexpr int kSplitRows = 48;
+constexpr int kPromptTile = 64;
+
 int compute_units(int dev) {
   int n = 0;
   if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
@@ -15,7 +22,7 @@ int compute_units(int dev) {
 }
 
 struct Plan {
-  int workgroups, log_kw;
+  int workgroups, log_kw, pieces;
   bool split;  // a tile may be divided: the call needs scratch
 };
 
@@ -43,6 +50,24 @@ Plan plan(int requests, int q_heads, int kv_heads, int max_q, int max_kv, int cu
   return p;
 }
 
+// The prompt kernel: a workgroup of eight waves fills a compute unit.  Fewer tiles (256 rows
+// of a head) than compute units are divided over their tokens on the device, which knows the
+// lengths; this is the grid, which bounds the tiles by the tokens.
+constexpr int kPromptRows = 256, kPromptWaves = 8;
+
+Plan prompt_plan(int tokens, int requests, int q_heads, int kv_heads, int max_q, int max_kv, int cus) {
+  const long long group = q_heads / kv_heads, rows = tokens * group;
+  long long kinds = rows / kPromptRows + (requests < rows / (kSplitRows + 1) ? requests : rows / (kSplitRows + 1));
+  const long long most = requests * ((max_q * group + kPromptRows - 1) / kPromptRows);
+  if (kinds > most) kinds = most;
+  Plan p{};
+  p.pieces = cus / kv_heads;
+  p.split = max_kv > kPromptTile && p.pieces > 1;
+  const long long w = (p.split && kinds < p.pieces ? p.pieces : kinds) * kv_heads;
+  p.workgroups = w > 0x7FFFFF ? -1 : (int)w;
+  return p;
+}
+
 int check(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int page_size, int num_pages,
           int max_pages, int groupsize, int max_q, int max_kv, float scale, int dtype) {
   const int err = check_geometry(kv_heads, head_dim, groupsize, page_size, num_pages, dtype);
@@ -50,6 +75,8 @@ int check(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int
   if (tokens < 0 || requests < 0 || max_pages < 0 || max_q < 0 || max_kv < 0)
     return refuse("kv4_attention takes no negative sizes");
   if (q_heads <= 0 || q_heads % kv_heads != 0) return refuse("kv4_attention needs q_heads to be a multiple of kv_heads");
+  if ((long long)tokens * (q_heads / kv_heads) > (1ll << 30) || (long long)max_q * (q_heads / kv_heads) > (1ll << 30))
+    return refuse("kv4_attention takes at most 2^30 rows (tokens times query heads of a kv head)");
   if ((long long)max_pages * page_size > (1ll << 30)) return refuse("a block table row covers more than 2^30 tokens");
   if (!(scale > 0.f) || !isfinite(scale)) return refuse("kv4_attention needs a positive, finite scale");
   return MARLIN_HIP_OK;
@@ -84,7 +111,6 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
   if (tokens == 0 || requests == 0 || max_q == 0) return MARLIN_HIP_OK;
   sm24::DeviceScope scope(dev);
   if (!scope.ok) return MARLIN_HIP_ERR_LAUNCH;
-  Plan p = plan(requests, q_heads, kv_heads, max_q, max_kv, compute_units(dev));
   AttnArgs a{};
   a.q = q;
   a.cache = static_cast<const uint8_t*>(cache);
@@ -96,30 +122,62 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
   a.qt = q_token_stride;
   a.qh = q_head_stride;
   a.tokens = tokens;
-  a.requests = requests;
   a.q_heads = q_heads;
   a.kv_heads = kv_heads;
+  const int group = q_heads / kv_heads, ng = groups(head_dim, groupsize);
+  const long long page_bytes = (long long)page_size * (head_dim + 4 * ng) * kv_heads;
+  if (page_bytes > 0xFFFFFFFFll) return refuse("kv4_attention: a page of 2^32 bytes or more");
+  a.page_stride = (uint32_t)page_bytes;
   a.num_pages = num_pages;
   a.max_pages = max_pages;
   a.log_page = 31 - __builtin_clz((unsigned)page_size);
-  a.max_rows = 0x7FFFFFFF;
-  a.log_kw = p.log_kw;
-  a.group = q_heads / kv_heads;
+  a.max_rows = kSplitRows;
+  a.group = group;
   a.c1 = scale * 1.4426950408889634f;
-  if (p.split) {
-    const size_t rows = (size_t)p.workgroups * 2 * 16 * (kWaves >> p.log_kw);
-    err = sm24::get_scratch(dev, stream, rows * (head_dim + 2) * sizeof(float), &a.counters, &a.partial);
-    if (err != MARLIN_HIP_OK) return err;
-    // (null while the stream is captured and has no scratch yet: tiles stay whole)
-    if (a.partial) a.partial_ml = a.partial + rows * head_dim;
+  const int cus = compute_units(dev);
+  const bool prompts = (long long)max_q * group > kSplitRows, few = !prompts || cu_q != nullptr;
+  const int split_q = prompts ? kSplitRows / group : max_q;
+  for (a.first = 0; a.first < requests; a.first += kMaxRequests) {
+    a.requests = requests - a.first < kMaxRequests ? requests - a.first : kMaxRequests;
+    if (prompts) {
+      const Plan p = prompt_plan(tokens, a.requests, q_heads, kv_heads, max_q, max_kv, cus);
+      if (p.workgroups < 0) return refuse("kv4_attention: too many rows for one launch");
+      a.pieces = p.pieces;
+      if (p.split) {
+        const size_t rows = (size_t)p.pieces * kv_heads * kPromptRows;
+        err = sm24::get_scratch(dev, stream, (rows * head_dim + 2 * rows * 2) * sizeof(float), &a.counters, &a.partial);
+        if (err != MARLIN_HIP_OK) return err;
+        if (a.partial) a.partial_ml = a.partial + rows * head_dim;  // (a null: see below)
+      }
+      err = sm24::launch_error(launch_prompt(a, p.workgroups, head_dim, ng, dtype, stream));
+      if (err != MARLIN_HIP_OK) return err;
+      a.partial = nullptr;
+    }
+    if (few && split_q > 0) {
+      const Plan p = plan(a.requests, q_heads, kv_heads, split_q, max_kv, cus);
+      a.log_kw = p.log_kw;
+      if (p.split) {
+        const size_t rows = (size_t)p.workgroups * 2 * 16 * (kWaves >> p.log_kw);
+        err = sm24::get_scratch(dev, stream, rows * (head_dim + 2) * sizeof(float), &a.counters, &a.partial);
+        if (err != MARLIN_HIP_OK) return err;
+        // (null while the stream is captured and has no scratch yet: tiles stay whole)
+        if (a.partial) a.partial_ml = a.partial + rows * head_dim;
+      }
+      dispatch(head_dim, ng, [&](auto d, auto g) {
+        constexpr int D = decltype(d)::value, NG = decltype(g)::value;
+        const dim3 grid((unsigned)p.workgroups), block(64 * kWaves);
+        if (dtype == F16) hipLaunchKernelGGL((kv4_split_kernel<D, NG, F16, 1>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((kv4_split_kernel<D, NG, BF16, 1>), grid, block, 0, stream, a);
+      });
+      err = sm24::launch_error(hipGetLastError());
+      if (err != MARLIN_HIP_OK) return err;
+      a.partial = nullptr;
+    }
+    a.kv_lens += a.requests;
+    a.table += (size_t)a.requests * max_pages;
+    if (a.cu_q) a.cu_q += a.requests;
   }
-  dispatch(head_dim, groups(head_dim, groupsize), [&](auto d, auto g) {
-    constexpr int D = decltype(d)::value, NG = decltype(g)::value;
-    const dim3 grid((unsigned)p.workgroups), block(64 * kWaves);
-    if (dtype == F16) hipLaunchKernelGGL((kv4_split_kernel<D, NG, F16, 1>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((kv4_split_kernel<D, NG, BF16, 1>), grid, block, 0, stream, a);
-  });
-  return sm24::launch_error(hipGetLastError());
+  return MARLIN_HIP_OK;
 }
 
 }  // extern "C"

@@ -1,0 +1,545 @@
+// Attention of many query rows (prompts, chunks of prompts) over the 4-bit paged cache.
+//
+// The sums of kv4_split.h, on 32x32x16 MFMAs: a wave keeps 32 rows, a workgroup of eight
+// goes through the tokens that its rows see, 64 at a time.  Its waves turn the tile's codes
+// into fp16 (less 8, exact) once for all eight, straight into the MFMAs' operand order in
+// LDS, one tile ahead of the products; the codes come from memory two tiles ahead.
+//   S^T = K Q^T    A = K from LDS, B = Q in registers; lane (c, h) gets row c's sums of tokens
+//                  8 b + 4 h + i of a half tile (32 tokens)
+//   O^T = V^T P^T  A = V from LDS, B = p v, whose reduction index counts those tokens: p
+//                  stays in its lane
+// Sixteen tokens lie in one page, and are what a wave loads at once: the page is the wave's,
+// so that a tile costs it a few scalar operations and one load; the scales go to LDS as
+// they are (LDS-DMA), and are fp16 operands of mixed-precision FMAs.
+//
+// Measured on this part: a wave issues an operation of any kind every 4.1 to 4.8 cycles, two
+// waves of a SIMD in parallel; an MFMA takes its 32 cycles and hides nearly no other
+// operation of either wave (32 + 2.1 n cycles for one beside n of the vector ALU, with two
+// waves).  So what counts is operations per score, of any kind, and neither LDS (254 of
+// 256 bytes a clock with eight waves) nor the order of products and softmax.
+#pragma once
+#include "kv4_split.h"
+
+namespace kv4 {
+
+constexpr int kTile = 64;       // tokens
+constexpr int kPromptWaves = 8;
+constexpr int kPromptRows = 32 * kPromptWaves;
+constexpr int kMaxKinds = 256;     // row blocks of a launch whose tokens are divided
+constexpr int kMaxParts = 32;      // of a row block's tokens
+constexpr float kMinShare = 4.f;   // tiles: a part costs its write and its read
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+// Place of dim 8 blk + i of V among the MFMA rows: the rows of a scale group fill
+// whole MFMAs, and consecutive words go to consecutive rows.
+template <int D, int NG>
+__device__ __forceinline__ constexpr int v_row(int blk, int i) {
+  constexpr int BL = D / 8 / NG;
+  return blk / BL * (8 * BL) + i * BL + blk % BL;
+}
+
+__device__ __forceinline__ uint32_t pack2(float lo, float hi) {
+  return __builtin_bit_cast(uint32_t, (half2_t){(_Float16)lo, (_Float16)hi});
+}
+
+template <int D, int NG, int TYPE>
+__global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnArgs a) {
+  constexpr int W = kPromptWaves;
+  constexpr int KU = D / 16;          // k-steps of the first product
+  constexpr int GU = KU / NG;         // ... per scale group
+  constexpr int DT = D / 32;          // MFMAs of 32 dims of the second
+  constexpr int BL = D / 8 / NG;      // words of a scale group
+  constexpr int K_BYTES = kTile * D * 2, V_BYTES = K_BYTES, S_BYTES = 2 * NG * kTile * 2;
+  constexpr int BUF = K_BYTES + V_BYTES;  // operands of a tile, two tiles; then the scales of four
+  constexpr int PIECES = kTile * D / 2 / 16;  // 16-byte pieces of K codes, and of V codes
+  constexpr int GROUPS = kTile / 16;          // of tokens in one page
+  __shared__ __align__(16) uint8_t lds[2 * BUF + 4 * S_BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int c = lane & 31, h = lane >> 5;
+  const int G = a.group, T = 1 << a.log_page;
+
+  // ---- the piece: which request's, which block of rows, which part of its tokens ----
+  // Heads fastest, so that a head stays on one XCD; a request's last block, the longest, first.
+  __shared__ int kinds[kMaxKinds], kind_tiles[kMaxKinds];
+  const int head = blockIdx.x % a.kv_heads, index = blockIdx.x / a.kv_heads;
+  auto blocks_of = [&](const Request& q) { return q.n * G > a.max_rows ? (q.n * G + kPromptRows - 1) / kPromptRows : 0; };
+  // tokens that some row of a block sees
+  auto end_of = [&](const Request& q, int block) {
+    return max(q.kv - q.n + min((block * kPromptRows + kPromptRows - 1) / G, q.n - 1) + 1, 0);
+  };
+  const int per = (a.requests + 63) / 64, r_lane = lane * per;  // a lane's requests
+  int own = 0;
+  for (int r = r_lane; r < min(r_lane + per, a.requests); r++) own += blocks_of(request_of(a, r));
+  auto scan = [&](int x) {  // what the lanes before have
+    int sum = x;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int y = __shfl_up(sum, d);
+      if (lane >= d) sum += y;
+    }
+    return sum - x;
+  };
+  const int before = scan(own), all = __builtin_amdgcn_readlane(before + own, 63);
+  if (all == 0) return;
+  int r, block, part = 0, parts = 1;
+  if (a.partial == nullptr || all > min(a.pieces, kMaxKinds)) {
+    // workgroups for all compute units: whole
+    if (index >= all) return;
+    const int at = __builtin_ctzll(__ballot(before + own > index));
+    int i = index - __builtin_amdgcn_readlane(before, at);
+    r = at * per;
+    int n = blocks_of(request_of(a, r));
+    while (i >= n) {
+      i -= n;
+      n = blocks_of(request_of(a, ++r));
+    }
+    block = n - 1 - i;
+  } else {
+    // Divided: parts of (nearly) one length, the shortest of 64 that give no more parts than
+    // there are workgroups for this head.
+    if (wave == 0) {
+      int i = before;
+      for (int r = r_lane; r < min(r_lane + per, a.requests); r++) {
+        const Request q = request_of(a, r);
+        for (int b = blocks_of(q) - 1; b >= 0; b--, i++) {
+          kinds[i] = r * kMaxKinds + b;
+          kind_tiles[i] = max((end_of(q, b) + kTile - 1) / kTile, 1);
+        }
+      }
+    }
+    __syncthreads();
+    float sum = 0.f, longest = 0.f;
+    for (int i = 0; i < all; i++) {
+      sum += (float)kind_tiles[i];
+      longest = fmaxf(longest, (float)kind_tiles[i]);
+    }
+    const float lo = fmaxf(fmaxf(sum / (float)a.pieces, kMinShare), longest / (float)kMaxParts), hi = fmaxf(lo, longest);
+    const float per_tile = 1.f / (lo + (hi - lo) * ((float)(lane + 1) / 64.f));
+    auto parts_of = [&](int tiles, float f) { return max((int)ceilf((float)tiles * f - 0.001f), 1); };
+    int n = 0;
+    for (int i = 0; i < all; i++) n += parts_of(kind_tiles[i], per_tile);
+    const float f = __builtin_bit_cast(
+        float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, per_tile), __builtin_ctzll(__ballot(n <= a.pieces || lane == 63))));
+    int i = 0;
+    part = index;
+    for (; i < all; i++) {
+      parts = __builtin_amdgcn_readfirstlane(parts_of(kind_tiles[i], f));
+      if (part < parts) break;
+      part -= parts;
+    }
+    if (i == all) return;
+    const int kind = __builtin_amdgcn_readfirstlane(kinds[i]);
+    r = kind / kMaxKinds, block = kind % kMaxKinds;
+  }
+  const Request rq = request_of(a, r);
+  const int rows = rq.n * G, row0 = block * kPromptRows;
+  const int past = rq.kv - rq.n;
+  const int w_row0 = row0 + 32 * wave;
+  // tokens that some row of the workgroup, some row of the wave and every row of it sees
+  const int end = end_of(rq, block);
+  const int w_end = w_row0 < rows ? max(past + min((w_row0 + 31) / G, rq.n - 1) + 1, 0) : 0;
+  const int w_all = min(max(past + w_row0 / G + 1, 0), w_end);
+
+  typedef __attribute__((address_space(3))) uint8_t lds_u8;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_u8*)lds;
+
+  // ---- Q ----
+  const int seen = w_row0 + c < rows ? max(past + min((w_row0 + c) / G, rq.n - 1) + 1, 0) : 0;
+  half8_t qf[KU];
+  float c1 = a.c1;
+  {
+    const int row = w_row0 + c, t_row = min(row / G, rq.n - 1), h_row = head * G + row % G;
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(rq.first + t_row) * a.qt +
+                          (long long)h_row * a.qh + 8 * h;
+    u32x4 raw[KU];
+#pragma unroll
+    for (int u = 0; u < KU; u++) raw[u] = *reinterpret_cast<const u32x4*>(src + 16 * u);
+    if constexpr (TYPE == BF16) {
+      float amax = 0.f;
+#pragma unroll
+      for (int u = 0; u < KU; u++) {
+        float x[8];
+        unpack8<TYPE>(raw[u], x);
+#pragma unroll
+        for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[i]));
+      }
+      const Pair p = across32(amax);
+      amax = fmaxf(p.a, p.b);
+      const int e = amax > 0.f && amax < __builtin_inff() ? 8 - __builtin_amdgcn_frexp_expf(amax) : 0;
+#pragma unroll
+      for (int u = 0; u < KU; u++) {
+        float x[8];
+        unpack8<TYPE>(raw[u], x);
+        constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+        for (int i = 0; i < 8; i++) qf[u][i] = (_Float16)__builtin_amdgcn_ldexpf(x[order[i]], e);
+      }
+      c1 = __builtin_amdgcn_ldexpf(c1, -e);
+    } else {
+#pragma unroll
+      for (int u = 0; u < KU; u++) {
+        const half8_t q = __builtin_bit_cast(half8_t, raw[u]);
+        qf[u] = (half8_t){q[0], q[4], q[1], q[5], q[2], q[6], q[3], q[7]};
+      }
+    }
+  }
+
+  // ---- the codes of a tile: a wave's pieces are all of K or all of V ----
+  const Magic magic;
+  const int32_t* pages = a.table + (size_t)r * a.max_pages;
+  const uint8_t* const cache = a.cache + (size_t)head * block_bytes<D, NG>(T);
+  // a wave's pieces: of K (the first waves) or of V, of one group (D = 128) or of two
+  constexpr int KWAVES = PIECES / 64;
+  static_assert(2 * KWAVES <= W && (KWAVES == GROUPS || 2 * KWAVES == GROUPS), "");
+  const bool is_k = wave < KWAVES, is_v = !is_k && wave < 2 * KWAVES;
+
+  // Where 64 groups (16 tiles) from 64 b on begin, one a lane: the table's entries as they
+  // come (a look at once would wait for them and for every load before them), then the byte
+  // offset of the K codes (bit 63: no such page, which is read as the first one and masked).
+  auto entries = [&](int b) { return pages[min((64 * b + lane) * 16, end - 1) >> a.log_page]; };
+  auto places = [&](int b, int entry) {
+    const int tok = (64 * b + lane) * 16;
+    const bool there = (uint32_t)entry < (uint32_t)a.num_pages;
+    const uint64_t at = (uint64_t)(there ? (uint32_t)entry : 0u) * a.page_stride + (uint32_t)(tok & (T - 1)) * (D / 2);
+    return there || tok >= end ? at : at | 1ull << 63;
+  };
+  int entry = 0;              // of the block of 16 tiles after the one in `then`
+  uint64_t now = 0, then = 0;  // of the block of the tile in use, and of the one after
+  auto place = [&](int tile, int g, int block_now) {
+    const int i = (tile & 15) * GROUPS + g;
+    const uint64_t v = tile >> 4 == block_now ? now : then;
+    return cache + ((uint64_t)(uint32_t)(__builtin_amdgcn_readlane((int)(v >> 32), i) & 0x7FFFFFFF) << 32 |
+                    (uint32_t)__builtin_amdgcn_readlane((int)v, i));
+  };
+  u32x4 raw;
+  auto fetch = [&](int tile, int block_now) {
+    if (!is_k && !is_v) return;
+    const uint32_t v_off = is_k ? 0u : (uint32_t)T * (D / 2);
+    if constexpr (KWAVES == GROUPS) {
+      raw = *reinterpret_cast<const u32x4*>(place(tile, wave % GROUPS, block_now) + v_off + (uint32_t)(16 * lane));
+    } else {
+      const int g = wave % KWAVES * 2;
+      const uint8_t *p0 = place(tile, g, block_now) + v_off, *p1 = place(tile, g + 1, block_now) + v_off;
+      raw = *reinterpret_cast<const u32x4*>((lane < 32 ? p0 : p1) + (uint32_t)(16 * (lane & 31)));
+    }
+  };
+  // Scales of a group: 8 NG lanes of K, as many of V.  (The waves without V's longer unpacking.)
+  const int s_group = KWAVES == GROUPS ? wave : wave - 2 * KWAVES;
+  const bool s_mine = s_group >= 0 && s_group < GROUPS;
+  const uint32_t s_lane = (lane % (8 * NG)) * 4 + (lane / (8 * NG)) * (2 * NG * (uint32_t)T) + (uint32_t)T * D;
+  auto fetch_scales = [&](int tile, int block_now) {
+    if (s_mine) {
+      const uint32_t o = (uint32_t)(tile * kTile + 16 * s_group) & (T - 1);
+      const uint8_t* b = place(tile, s_group, block_now) - o * (D / 2 - 2 * NG);
+      if (lane < 16 * NG)
+        dma4(__builtin_amdgcn_readfirstlane(lds_at + 2 * BUF + (tile & 3) * S_BYTES + s_group * (64 * NG)), b + s_lane);
+    }
+  };
+  // Slot of token t among a tile's of a K operand: turned by the reader's lane group, so that
+  // the writing lanes (four words of a row side by side) hit different banks.
+  auto k_slot = [](int t, int g) { return (t + 4 * g) & (kTile - 1); };
+  // Where a thread writes V's operands in a tile: quad q gives reduction steps of 16 tokens,
+  // lanes' halves, first or second four.  (One register: the compiler would keep its terms.)
+  const int v_piece = tid - PIECES, v_quad = v_piece / (D / 8), v_blk = v_piece % (D / 8);
+  uint32_t v_to = K_BYTES + ((v_quad >> 2) * 2 + (v_quad & 1)) * (D * 16) + (v_quad >> 1 & 1) * 8 + v_row<D, NG>(v_blk, 0) * 16;
+  asm volatile("" : "+v"(v_to));
+  auto unpack = [&](int tile) {
+    uint8_t* const to = lds + (tile & 1) * BUF;
+    if (is_k) {
+      constexpr int PT = D / 32;  // pieces of a token
+      const int t = tid / PT;
+#pragma unroll
+      for (int j = 0; j < 4; j++) {
+        const int word = tid % PT * 4 + j, g = word / (D / 32), b = 4 * (word % (D / 32)) + g;
+        *reinterpret_cast<half8_t*>(to + (b * kTile + k_slot(t, g)) * 16) = k_operand(magic, raw[j]);
+      }
+    } else if (is_v) {
+      uint8_t* const v = to + v_to;
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        const uint32_t s = half ? 0x07060302u : 0x05040100u;
+        const uint32_t x = __builtin_amdgcn_perm(raw.y, raw.x, s), y = __builtin_amdgcn_perm(raw.w, raw.z, s);
+#pragma unroll
+        for (int k = 0; k < 2; k++) {
+          const half4_t lo = magic.codes(k ? x >> 8 : x), hi = magic.codes(k ? y >> 8 : y);
+          const int i = 4 * half + 2 * k;
+          *reinterpret_cast<half4_t*>(v + i * BL * 16) = (half4_t){lo.x, lo.y, hi.x, hi.y};
+          *reinterpret_cast<half4_t*>(v + (i + 1) * BL * 16) = (half4_t){lo.z, lo.w, hi.z, hi.w};
+        }
+      }
+    }
+  };
+
+  float16_t O[DT];
+  float M = kNone, L = 0.f, x_top = kNone, shift = 0.f, v_top = 0.f;
+#pragma unroll
+  for (int t = 0; t < DT; t++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) O[t][i] = 0.f;
+
+  // LDS addresses of this lane's operands in the tile in use: everything else of an address
+  // is an instruction's constant.
+  auto read16 = [](uint32_t at, int more) {
+    return *(const __attribute__((address_space(3))) half8_t*)(uintptr_t)(at + more);
+  };
+  // Scales [group of 16][K, V][quad][NG][4] of tokens 8 b + 4 h + (0 .. 3) of half j.
+  auto scale_of = [&](uint32_t scales, int kv, int n, int j, int b) {
+    const int more = (2 * j + b / 2) * (64 * NG) + kv * (32 * NG) + (2 * (b & 1) * NG + n) * 8;
+    return *(const __attribute__((address_space(3))) half4_t*)(uintptr_t)(scales + 8 * NG * h + more);
+  };
+  // The scale of V of token `lane` of the tile, the largest of its groups.
+  auto v_of_lane = [&](uint32_t scales) {
+    _Float16 v = (_Float16)0.f;
+#pragma unroll
+    for (int n = 0; n < NG; n++) {
+      const uint32_t at = scales + (lane >> 4) * (64 * NG) + 32 * NG + (lane >> 2 & 3) * (8 * NG) + (lane & 3) * 2;
+      v = __builtin_fmaxf16(v, *(const __attribute__((address_space(3))) _Float16*)(uintptr_t)(at + n * 8));
+    }
+    return (float)v;
+  };
+  auto compute = [&](int tile, uint32_t hole) {
+    const uint32_t buf = lds_at + (tile & 1) * BUF, scales = lds_at + 2 * BUF + (tile & 3) * S_BYTES;
+    const uint32_t even[2] = {buf + (h * kTile + k_slot(c, h)) * 16, buf + (h * kTile + k_slot(32 + c, h)) * 16};
+    const uint32_t odd[2] = {buf + (h * kTile + k_slot(c, 2 + h)) * 16, buf + (h * kTile + k_slot(32 + c, 2 + h)) * 16};
+    float x[2][16];
+#pragma unroll
+    for (int j = 0; j < 2; j++)
+#pragma unroll
+      for (int n = 0; n < NG; n++) {
+        float16_t S;
+#pragma unroll
+        for (int i = 0; i < 16; i++) S[i] = 0.f;
+#pragma unroll
+        for (int u = n * GU; u < (n + 1) * GU; u++)
+          S = __builtin_amdgcn_mfma_f32_32x32x16_f16(read16((u & 1 ? odd : even)[j], u * (2 * kTile * 16)), qf[u], S, 0, 0, 0);
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          const half4_t s = scale_of(scales, 0, n, j, b);
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            x[j][4 * b + i] = __builtin_fmaf(S[4 * b + i], (float)s[i], n == 0 ? 0.f : x[j][4 * b + i]);
+        }
+      }
+    float vm = v_of_lane(scales);
+    const bool masked = (tile + 1) * kTile > w_all || hole != 0;
+    if (masked) {
+      vm = tile * kTile + lane < w_end && !(hole >> (lane >> 4) & 1) ? vm : 0.f;
+#pragma unroll
+      for (int j = 0; j < 2; j++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+          const int t = 32 * j + 8 * (i / 4) + 4 * h + i % 4;
+          const bool in = tile * kTile + t < seen && !(hole >> (2 * j + i / 8) & 1);
+          x[j][i] = in ? x[j][i] : -__builtin_inff();
+        }
+    }
+    float xm = x[0][0];
+#pragma unroll
+    for (int i = 1; i < 32; i++) xm = fmaxf(xm, x[i / 16][i % 16]);
+    if (__any(xm > x_top || vm > v_top)) {
+      const Pair px = across32(xm);
+      xm = fmaxf(px.a, px.b);
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) vm = fmaxf(vm, __shfl_xor(vm, d));
+      float new_shift = shift;
+      if (vm > v_top) {
+        // vm <= 2^e; 2^24 bounds the shift where every v so far is tiny
+        new_shift = fminf(kVTop - (float)__builtin_amdgcn_frexp_expf(vm), 24.f);
+        v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
+      }
+      const float old_max = M == kNone ? kNone : M + shift;
+      const float new_max = fmaxf(old_max, xm * c1);
+      const float new_M = new_max <= kNone ? kNone : new_max - new_shift;
+      const float f = M == kNone ? 0.f : __builtin_amdgcn_exp2f(M - new_M);
+      M = new_M;
+      shift = new_shift;
+      x_top = M == kNone ? kNone : (new_max + kSlack) * __builtin_amdgcn_rcpf(c1);
+      L *= f;
+#pragma unroll
+      for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) O[t][i] *= f;
+    }
+    const uint32_t v_at = buf + K_BYTES + (h * D + c) * 16;
+#pragma unroll
+    for (int j = 0; j < 2; j++) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        x[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j][i], c1, -M));
+        L += x[j][i];
+      }
+#pragma unroll
+      for (int n = 0; n < NG; n++) {
+        u32x4 P[2];  // fp16 pairs
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          const half4_t s = scale_of(scales, 1, n, j, b);
+#pragma unroll
+          for (int i = 0; i < 4; i += 2)
+            P[b >> 1][2 * (b & 1) + i / 2] = pack2(__builtin_fmaf(x[j][4 * b + i], (float)s[i], 0.f),
+                                                   __builtin_fmaf(x[j][4 * b + i + 1], (float)s[i + 1], 0.f));
+        }
+        if (masked) {  // what a row does not see is zero, whatever its scale
+#pragma unroll
+          for (int i = 0; i < 16; i += 2)
+            P[i / 8][i % 8 / 2] &= (x[j][i] == 0.f ? 0u : 0xFFFFu) | (x[j][i + 1] == 0.f ? 0u : 0xFFFF0000u);
+        }
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+          for (int t = n * (DT / NG); t < (n + 1) * (DT / NG); t++)
+            O[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read16(v_at, ((2 * j + s) * 2 * D + 32 * t) * 16),
+                                                          __builtin_bit_cast(half8_t, P[s]), O[t], 0, 0, 0);
+      }
+    }
+  };
+
+  const int tiles = (end + kTile - 1) / kTile;
+  const int t0 = tiles * part / parts, t1 = tiles * (part + 1) / parts;
+  if (t0 < t1) {
+    const int b0 = t0 >> 4;
+    now = places(b0, entries(b0));
+    then = places(b0 + 1, entries(b0 + 1));
+    entry = entries(b0 + 2);
+    uint64_t missing = __ballot((int64_t)now < 0);  // groups of the block whose page is not there
+    fetch(t0, b0);
+    fetch_scales(t0, b0);
+    unpack(t0);
+    sm24::wait_vm<0>();  // the first tile's scales
+    fetch_scales(t0 + 1, b0);
+    fetch(t0 + 1, b0);
+    __syncthreads();
+#pragma unroll 1
+    for (int tile = t0; tile < t1; tile++) {
+      const int b = tile >> 4;
+      if (tile > t0 && (tile & 15) == 0) {
+        now = then;
+        then = places(b + 1, entry);
+        entry = entries(b + 2);
+        missing = __ballot((int64_t)now < 0);
+      }
+      if (tile * kTile < w_end)
+        compute(tile, (uint32_t)(missing >> ((tile & 15) * GROUPS)) & ((1u << GROUPS) - 1));
+      if (tile + 1 < t1) {
+        unpack(tile + 1);
+        // the next tile's scales are there: sent before its codes, which the unpacking waited
+        // for, or the only loads of a wave without codes
+        if (!is_k && !is_v) sm24::wait_vm<0>();
+        fetch_scales(tile + 2, b);
+        fetch(tile + 2, b);
+      }
+      __syncthreads();
+    }
+  }
+
+  // (the thread's index anew: what is made from it is not kept in registers through the loop)
+  int thread = threadIdx.x;
+  asm volatile("" : "+v"(thread));
+  const int out_lane = thread & 63, out_c = out_lane & 31, out_h = out_lane >> 5;
+  const int row = w_row0 + out_c, t_row = row / G, h_row = head * G + row - t_row * G;
+  // ---- out: lane (c, h) holds row c's dims of MFMA rows 8 (k / 4) + 4 h + k % 4 ----
+  const Pair pl = across32(L);
+  float l = pl.a + pl.b;
+  if (parts > 1) {
+    // The waves of the same rows meet in memory; the last to arrive (its own stores and
+    // those it reads are ordered by its wait and by the counter) adds the parts in order.
+    if (w_row0 >= rows) return;
+    constexpr int kPart = DT * 16 * 64;  // floats of a wave's part
+    const uint32_t stride = (uint32_t)a.kv_heads * W;  // from a part's waves to the next one's
+    const uint32_t first = (blockIdx.x - (uint32_t)(part * a.kv_heads)) * W + wave, mine = first + part * stride;
+    float* const o_mine = a.partial + (size_t)mine * kPart + 4 * out_lane;
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+      for (int i = 0; i < 4; i++)
+        *reinterpret_cast<float4_t*>(o_mine + (4 * t + i) * 256) =
+            (float4_t){O[t][4 * i], O[t][4 * i + 1], O[t][4 * i + 2], O[t][4 * i + 3]};
+    float* const ml = a.partial_ml + 2 * out_lane;
+    *reinterpret_cast<float2*>(ml + (size_t)mine * 128) = make_float2(M, l);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    uint32_t arrived = 0;
+    if (out_lane == 0) arrived = __hip_atomic_fetch_add(a.counters + first, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+    if ((int)__builtin_amdgcn_readfirstlane(arrived) != parts) return;
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    if (out_lane == 0) __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    float top = M;
+    for (int p = 0; p < parts; p += 8) {
+      float m[8];  // (those past the last repeat it)
+#pragma unroll
+      for (int i = 0; i < 8; i++) m[i] = ml[(size_t)(first + min(p + i, parts - 1) * stride) * 128];
+#pragma unroll
+      for (int i = 0; i < 8; i++) top = fmaxf(top, m[i]);
+    }
+    float16_t sum[DT];
+#pragma unroll
+    for (int t = 0; t < DT; t++)
+#pragma unroll
+      for (int i = 0; i < 16; i++) sum[t][i] = 0.f;
+    l = 0.f;
+#pragma unroll 1
+    for (int p = 0; p < parts; p++) {
+      const uint32_t at = first + p * stride;
+      const float2 x = *reinterpret_cast<const float2*>(ml + (size_t)at * 128);
+      const float* o = a.partial + (size_t)at * kPart + 4 * out_lane;
+      float4_t v[DT * 4];
+#pragma unroll
+      for (int i = 0; i < DT * 4; i++) v[i] = *reinterpret_cast<const float4_t*>(o + i * 256);
+      const float f = __builtin_amdgcn_exp2f(x.x - top);
+      l += f * x.y;
+#pragma unroll
+      for (int i = 0; i < DT * 16; i++) sum[i / 16][i % 16] = __builtin_fmaf(v[i / 4][i % 4], f, sum[i / 16][i % 16]);
+    }
+    M = top;
+#pragma unroll
+    for (int t = 0; t < DT; t++) O[t] = sum[t];
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;  // no token seen: zeros (a NaN stays one)
+  const size_t at = (size_t)(rq.first + t_row) * a.q_heads + h_row;
+  uint16_t* const dst = static_cast<uint16_t*>(a.out) + at * D;
+#pragma unroll
+  for (int t = 0; t < DT; t++)
+#pragma unroll
+    for (int i = 0; i < 16; i++) O[t][i] *= inv;
+  if constexpr (BL >= 8) {
+    // all eight dims of a word: row v_row(blk, i) of the group
+#pragma unroll
+    for (int n = 0; n < NG; n++)
+#pragma unroll
+      for (int k = 0; k < BL / 2; k++) {  // words 4 out_h + k % 4 + 8 (k / 4) of the group
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const int m = i * BL + 8 * (k / 4);  // MFMA row less 4 out_h + k % 4
+          x[i] = O[n * (BL / 4) + m / 32][m % 32 / 8 * 4 + k % 4];
+        }
+        if (row < rows) *reinterpret_cast<u32x4*>(dst + 8 * (n * BL + 8 * (k / 4) + 4 * out_h + k % 4)) = pack8<TYPE>(x);
+      }
+  } else {
+    // a lane has every other dim (2 e + out_h) of each of the group's four words: the lanes of a
+    // row exchange, and write two words each
+#pragma unroll
+    for (int n = 0; n < NG; n++)
+#pragma unroll
+      for (int k = 0; k < 2; k++) {
+        float x[8];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const float keep = out_h ? O[n][4 * e + k + 2] : O[n][4 * e + k];
+          const float give = out_h ? O[n][4 * e + k] : O[n][4 * e + k + 2];
+          const float got = __shfl_xor(give, 32);
+          x[2 * e] = out_h ? got : keep;
+          x[2 * e + 1] = out_h ? keep : got;
+        }
+        if (row < rows) *reinterpret_cast<u32x4*>(dst + 8 * (n * 4 + k + 2 * out_h)) = pack8<TYPE>(x);
+      }
+  }
+  if (a.lse != nullptr && out_h == 0 && row < rows)
+    a.lse[at] = l == 0.f ? -__builtin_inff() : (M + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
+}
+
+}  // namespace kv4

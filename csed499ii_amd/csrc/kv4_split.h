@@ -63,8 +63,11 @@ struct AttnArgs {
   uint32_t* counters;   // [workgroup], zero between launches
   long long qt, qh;     // strides of q in elements
   int tokens, requests, q_heads, kv_heads;
+  uint32_t page_stride; // bytes of a page, all heads
   int num_pages, max_pages, log_page;
-  int max_rows;         // rows of a request above this are another kernel's
+  int first;            // token of request 0 where cu_q is null
+  int pieces;           // of the prompt kernel: workgroups a head that fill the machine
+  int max_rows;         // requests of at most so many rows a head are the split kernel's, others the prompt kernel's
   int log_kw;           // KW waves of a workgroup share a head (KW HW = kWaves)
   int group;            // query heads of a kv head
   float c1;             // softmax scale * log2 e
@@ -77,7 +80,7 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
   Request q;
   q.kv = min(max(a.kv_lens[r], 0), a.max_pages << a.log_page);  // (at most 2^30)
   if (a.cu_q == nullptr) {
-    q.first = r;
+    q.first = a.first + r;
     q.n = 1;
   } else {
     q.first = min(max(a.cu_q[r], 0), a.tokens);
@@ -421,7 +424,7 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
       const int id = tok < end ? pages[tok >> a.log_page] : -1;
       const bool there = (uint32_t)id < (uint32_t)a.num_pages;
       // a page that is not there is read as the first one and masked
-      const uint64_t at = (uint64_t)(there ? (uint32_t)id : 0u) * ((uint64_t)block * a.kv_heads) + (tok & (T - 1)) * (D / 2);
+      const uint64_t at = (uint64_t)(there ? (uint32_t)id : 0u) * a.page_stride + (uint32_t)(tok & (T - 1)) * (D / 2);
       return there ? at : at | 1ull << 63;
     };
     uint64_t now = places(0), then = places(32);  // of steps [32 b, 32 b + 32) and the 32 after
@@ -537,7 +540,7 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
         rise |= xm[b] > x_top[b];
       }
 #pragma unroll
-      for (int i = 0; i < 8 * NG; i++) vm = fmaxf(vm, (float)vs[i / 4 / NG][i / 4 % NG][i % 4]);
+      for (int i = 0; i < 8 * NG; i++) vm = fmaxf(vm, fabsf((float)vs[i / 4 / NG][i / 4 % NG][i % 4]));
       if (__any(rise || vm > v_top)) {
         // new reference: the rows' maxima so far and the largest v (the four lanes of a row agree)
         vm = column_max(vm);
