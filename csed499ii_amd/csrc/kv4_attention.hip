@@ -22,30 +22,29 @@ int compute_units(int dev) {
 }
 
 struct Plan {
-  int workgroups, log_kw, pieces;
+  int workgroups, log_kw, lead, pieces;
   bool split;  // a tile may be divided: the call needs scratch
 };
 
-// Two workgroups of eight waves fill a compute unit.  Waves of a workgroup that share a
-// head (KW) meet in LDS, pieces of a tile in memory.  Few tiles take all eight waves for a
-// head (one request of 131072 tokens on 8 heads: 43 us with eight, 69 with two, 124 with
-// one); from an eighth of a tile a workgroup on, fewer, as a workgroup otherwise goes
-// through several tiles one after the other (24 requests on 32 heads: 86 us with eight, 60
-// with one; 64 requests on 8: 135, 133 with four, 147 with one).
-Plan plan(int requests, int q_heads, int kv_heads, int max_q, int max_kv, int cus) {
-  Plan p;
-  const long long rows = (long long)max_q * (q_heads / kv_heads);
-  const long long row_blocks = (rows + 15) / 16;
+// Two workgroups of eight waves fill a compute unit, one where their registers and rings are
+// larger (Shape::TWO).  All eight waves take one block of 16 rows, and meet in LDS; a piece of
+// it costs its write and read in memory, fewer where the waves are together (one request of
+// 131072 tokens on 8 heads: 37.8 us with eight, 59 with four, 107 with two; 64 requests of
+// 4096: 57, 64, 70).  From two blocks a workgroup on, a workgroup goes through many short
+// ones instead, and two waves take a block (64 requests of 4096 tokens on 32 heads: 232 us
+// with eight, 229 with four, 219 with two; 200 of 1000: 220, 196, 189).
+Plan plan(int requests, int q_heads, int kv_heads, int head_dim, int ng, int max_q, int max_kv, int cus) {
+  Plan p{};
+  const long long row_blocks = ((long long)max_q * (q_heads / kv_heads) + 15) / 16;
   const long long steps = ((long long)max_kv + kStep - 1) / kStep;
-  const long long most = 2ll * cus;
-  const long long heads = requests * row_blocks * kv_heads;
-  p.log_kw = kLogWaves;
-  while (p.log_kw > 0 && heads * (1 << p.log_kw) / kWaves > most / 4) p.log_kw--;
+  const long long most = ng == 1 || head_dim == 64 ? 2ll * cus : cus;
+  const long long blocks = requests * row_blocks * kv_heads;
+  p.log_kw = blocks <= 2 * most ? kLogWaves : 1;
   const int hw = kWaves >> p.log_kw;
   const long long units = steps < 1 ? 1 : (steps + (1 << p.log_kw) - 1) >> p.log_kw;
-  long long w = requests * row_blocks * ((kv_heads + hw - 1) / hw) * units;
-  if (w > most) w = most;
-  p.workgroups = (int)w;
+  const long long w = requests * ((row_blocks * kv_heads + hw - 1) / hw) * units;
+  p.lead = w > most ? kLead : 0;
+  p.workgroups = (int)(w < most ? w : most);
   p.split = units > 1;
   return p;
 }
@@ -90,7 +89,7 @@ int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, i
                         int sms, int* out) {
   const int err = kv4::check(0, requests, q_heads, kv_heads, head_dim, 16, 1, 0, groupsize, max_q, max_kv, 1.f, 0);
   if (err != MARLIN_HIP_OK) return err;
-  const kv4::Plan p = kv4::plan(requests, q_heads, kv_heads, max_q, max_kv, sms > 0 ? sms : 256);
+  const kv4::Plan p = kv4::plan(requests, q_heads, kv_heads, head_dim, kv4::groups(head_dim, groupsize), max_q, max_kv, sms > 0 ? sms : 256);
   out[0] = 0;
   out[1] = p.workgroups;
   out[2] = p.split;
@@ -154,8 +153,9 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
       a.partial = nullptr;
     }
     if (few && split_q > 0) {
-      const Plan p = plan(a.requests, q_heads, kv_heads, split_q, max_kv, cus);
+      const Plan p = plan(a.requests, q_heads, kv_heads, head_dim, ng, split_q, max_kv, cus);
       a.log_kw = p.log_kw;
+      a.lead = p.lead;
       if (p.split) {
         const size_t rows = (size_t)p.workgroups * 2 * 16 * (kWaves >> p.log_kw);
         err = sm24::get_scratch(dev, stream, rows * (head_dim + 2) * sizeof(float), &a.counters, &a.partial);
@@ -166,8 +166,8 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
       dispatch(head_dim, ng, [&](auto d, auto g) {
         constexpr int D = decltype(d)::value, NG = decltype(g)::value;
         const dim3 grid((unsigned)p.workgroups), block(64 * kWaves);
-        if (dtype == F16) hipLaunchKernelGGL((kv4_split_kernel<D, NG, F16, 1>), grid, block, 0, stream, a);
-        else hipLaunchKernelGGL((kv4_split_kernel<D, NG, BF16, 1>), grid, block, 0, stream, a);
+        if (dtype == F16) hipLaunchKernelGGL((kv4_split_kernel<D, NG, F16>), grid, block, 0, stream, a);
+        else hipLaunchKernelGGL((kv4_split_kernel<D, NG, BF16>), grid, block, 0, stream, a);
       });
       err = sm24::launch_error(hipGetLastError());
       if (err != MARLIN_HIP_OK) return err;

@@ -9,9 +9,12 @@
 // so that the scales leave both products and the matrix cores multiply small integers,
 // which fp16 holds exactly.
 //
-// A tile is 16 NB rows (NB MFMAs' columns) of HW heads over all their tokens.  A workgroup
-// gives each head KW of its eight waves, which take turns at the 32-token steps: a unit is a
-// step for each.  The tiles' units, end to end, are divided evenly over the workgroups,
+// A tile is HW blocks of 16 rows (an MFMA's columns) over all the tokens that they see: all
+// of a head's rows, then the next head's, so that blocks that read the same codes mostly
+// share a compute unit's path to memory.  (Several blocks to a wave, which unpacks for all:
+// 66.9 us where this takes 65.9, 12 requests of 5 tokens and 8 query heads to a kv head.)
+// A workgroup gives each block KW of its eight waves, which take turns at the 32-token
+// steps: a unit is a step for each.  The tiles' units, end to end, are divided evenly over the workgroups,
 // whatever the requests' lengths: a workgroup takes the end of one tile, whole tiles, the
 // beginning of another.  Per step and wave:
 //   S^T = K Q^T  16x16x32 MFMAs, A = codes (rows = 16 tokens), B = Q, held in registers;
@@ -44,6 +47,11 @@ namespace kv4 {
 
 constexpr int kLogWaves = 3, kWaves = 1 << kLogWaves;
 constexpr int kLogStep = 5, kStep = 1 << kLogStep;  // tokens per wave and step
+// Units that a tile counts more than it has, for what a workgroup's turn to another tile costs,
+// where there are more units than workgroups
+// (24 requests of 17 to 4096 tokens on 32 heads: 87.0 us with none, 58.0 with 2, 59.5 with 4;
+// 64 of 1024 to 16384 on 8: 134.6, 130.7, 129.7; one of 131072: 40.2, 37.8, 37.3).
+constexpr int kLead = 2;
 constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last workgroup's read of it
 constexpr int kMaxRequests = 2 * 64 * kWaves;  // of a launch that divides by the requests' lengths
 constexpr float kSlack = 8.f;      // p <= 2^8 of the reference
@@ -69,6 +77,7 @@ struct AttnArgs {
   int pieces;           // of the prompt kernel: workgroups a head that fill the machine
   int max_rows;         // requests of at most so many rows a head are the split kernel's, others the prompt kernel's
   int log_kw;           // KW waves of a workgroup share a head (KW HW = kWaves)
+  int lead;             // units that a tile counts more than it has
   int group;            // query heads of a kv head
   float c1;             // softmax scale * log2 e
 };
@@ -206,8 +215,8 @@ __device__ __forceinline__ void v_operands(const Magic& m, const u32x4& a, const
   }
 }
 
-template <int D, int NG, int TYPE, int NB>
-__global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)) void kv4_split_kernel(AttnArgs a) {
+template <int D, int NG, int TYPE>
+__global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_split_kernel(AttnArgs a) {
   using S = Shape<D, NG>;
   // the waves' rings; later 16 rows of D + 4 floats in each
   static_assert(S::RING * S::STAGE >= 16 * (D + 4) * 4 && S::RING * S::STAGE >= 16 * (kMaxSplits + 2) * 4, "");
@@ -224,13 +233,12 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
   const int T = 1 << a.log_page;
   const int KW = 1 << a.log_kw, HW = kWaves >> a.log_kw;
   const int kw = wave & (KW - 1), hw = wave >> a.log_kw;
-  const int head_groups = (a.kv_heads + HW - 1) >> (kLogWaves - a.log_kw);
 
   // ---- the division: every request's tiles are as long as its last one; rows that see
   // nothing take a unit, to write their zeros.  Without scratch, and where the units do
   // not fit 31 bits, tiles count as one and stay whole ----
-  auto blocks_of = [&](const Request& q) { return q.n * G > a.max_rows ? 0 : (q.n * G + 16 * NB - 1) / (16 * NB); };
-  auto units_of = [&](const Request& q) { return max((q.kv + kStep * KW - 1) >> (kLogStep + a.log_kw), 1); };
+  auto blocks_of = [&](const Request& q) { return q.n * G > a.max_rows ? 0 : (q.n * G + 16 - 1) / 16; };
+  auto units_of = [&](const Request& q) { return max((q.kv + kStep * KW - 1) >> (kLogStep + a.log_kw), 1) + a.lead; };
   bool divided = a.partial != nullptr;
   uint32_t total, share;
   // Up to 64 requests are one to a lane, in every wave alike, and found by a ballot; more
@@ -242,7 +250,7 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
     long long mine[2] = {0, 0};
     int longest = 1;
     auto cost = [&](const Request& q) {
-      long long n = (long long)blocks_of(q) * head_groups;
+      long long n = ((long long)blocks_of(q) * a.kv_heads + HW - 1) >> (kLogWaves - a.log_kw);
       if (divided) {
         if (n > 0) longest = max(longest, units_of(q));
         n *= units_of(q);
@@ -343,21 +351,23 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
     const int rows = rq.n * G, row_blocks = blocks_of(rq), len = divided ? units_of(rq) : 1;
     const int tile = (int)((unit - r_begin) / (uint32_t)len);
     const uint32_t tile_unit = r_begin + (uint32_t)tile * len;
-    const int rb = row_blocks == 1 ? 0 : tile % row_blocks;
-    const int own_head = (row_blocks == 1 ? tile : tile / row_blocks) * HW + hw, head = min(own_head, a.kv_heads - 1);  // (a wave may have none)
-    const int row0 = rb * 16 * NB;
+    // the wave's blocks of rows of all heads (it may have none)
+    const int own_block = tile * HW + hw, own = min(own_block, row_blocks * a.kv_heads - 1);
+    const bool exists = own == own_block;
+    const int head = row_blocks == 1 ? own : own / row_blocks, row0 = (own - head * row_blocks) * 16;
     const int past = rq.kv - rq.n;  // token t sees tokens 0 .. past + t
     const bool one = rq.n == 1;  // (spares the divisions of a row's index)
-    const int t_first = one ? 0 : row0 / G, t_last = one ? 0 : min((row0 + 16 * NB - 1) / G, rq.n - 1);
+    const int t_first = one ? 0 : row0 / G, t_last = one ? 0 : min((row0 + 15) / G, rq.n - 1);
     const int end = max(past + t_last + 1, 0);             // tokens that some row of the tile sees
     const int all = min(max(past + t_first + 1, 0), end);  // ... that every row sees
     const int steps = (end + kStep - 1) / kStep;
-    // this wave's steps: s0, s0 + KW, ...
-    const uint32_t next_unit = min(tile_unit + len, last_unit);
-    const int s0 = (divided ? (int)(unit - tile_unit) * KW : 0) + kw;
-    const int s1 = divided ? min(steps, (int)(next_unit - tile_unit) * KW) : steps;
-    const int count = own_head < a.kv_heads && s1 > s0 ? (s1 - s0 + KW - 1) >> a.log_kw : 0;
-    const bool whole = unit == tile_unit && next_unit == tile_unit + len;
+    // this wave's steps: s0, s0 + KW, ... (the tile's first units are its lead)
+    const uint32_t next_unit = min(tile_unit + len, last_unit), work_unit = tile_unit + (divided ? a.lead : 0);
+    if (next_unit <= work_unit) break;
+    const int s0 = (divided ? (int)(max(unit, work_unit) - work_unit) * KW : 0) + kw;
+    const int s1 = divided ? min(steps, (int)(next_unit - work_unit) * KW) : steps;
+    const int count = exists && s1 > s0 ? (s1 - s0 + KW - 1) >> a.log_kw : 0;
+    const bool whole = unit <= work_unit && next_unit == tile_unit + len;
     const bool first_piece = unit == first_unit;
     if (!first_piece) __syncthreads();  // the piece before is done with LDS
 
@@ -366,54 +376,44 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
     const int lane = per_piece(threadIdx.x) & 63, c = lane & 15, g = lane >> 4;
     const int blk = c / S::PARTS, part = c % S::PARTS;
     const uint32_t sel = S::PARTS == 1 ? 0u : part_selector<S::PARTS == 1 ? 2 : S::PARTS>(part);
-    half8_t qf[NB][S::KW];
-    float c1[NB];
-    int seen[NB];  // tokens the row sees
+    half8_t qf[S::KW];
+    float c1 = a.c1;
+    const int row = row0 + c, t_row = one ? 0 : row / G, h_row = one ? min(row, G - 1) : row - t_row * G;
+    const int seen = row < rows ? max(past + t_row + 1, 0) : 0;  // tokens the row sees
+    float x[S::KW][8];
+    const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(rq.first + min(t_row, rq.n - 1)) * a.qt +
+                          (long long)(head * G + h_row) * a.qh + 8 * g;
+    float amax = 0.f;
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
-      const int row = row0 + 16 * b + c, t_row = one ? 0 : row / G, h_row = one ? min(row, G - 1) : row - t_row * G;
-      seen[b] = row < rows ? max(past + t_row + 1, 0) : 0;
-      c1[b] = a.c1;
-      float x[S::KW][8];
-      const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(rq.first + min(t_row, rq.n - 1)) * a.qt +
-                            (long long)(head * G + h_row) * a.qh + 8 * g;
-      float amax = 0.f;
+    for (int w = 0; w < S::KW; w++) {
+      unpack8<TYPE>(*reinterpret_cast<const u32x4*>(src + 32 * w), x[w]);
 #pragma unroll
-      for (int w = 0; w < S::KW; w++) {
-        unpack8<TYPE>(*reinterpret_cast<const u32x4*>(src + 32 * w), x[w]);
-#pragma unroll
-        for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[w][i]));
-      }
-      if constexpr (TYPE == BF16) {
-        // bf16's range does not fit fp16: rows are brought to [2^7, 2^8) by a power of two
-        amax = column_max(amax);
-        const int e = amax > 0.f && amax < __builtin_inff() ? 8 - __builtin_amdgcn_frexp_expf(amax) : 0;
-#pragma unroll
-        for (int w = 0; w < S::KW; w++)
-#pragma unroll
-          for (int i = 0; i < 8; i++) x[w][i] = __builtin_amdgcn_ldexpf(x[w][i], e);
-        c1[b] = __builtin_amdgcn_ldexpf(c1[b], -e);
-      }
-      constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+      for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[w][i]));
+    }
+    if constexpr (TYPE == BF16) {
+      // bf16's range does not fit fp16: rows are brought to [2^7, 2^8) by a power of two
+      amax = column_max(amax);
+      const int e = amax > 0.f && amax < __builtin_inff() ? 8 - __builtin_amdgcn_frexp_expf(amax) : 0;
 #pragma unroll
       for (int w = 0; w < S::KW; w++)
 #pragma unroll
-        for (int i = 0; i < 8; i++) qf[b][w][i] = (_Float16)x[w][order[i]];
+        for (int i = 0; i < 8; i++) x[w][i] = __builtin_amdgcn_ldexpf(x[w][i], e);
+      c1 = __builtin_amdgcn_ldexpf(c1, -e);
     }
+    constexpr int order[8] = {0, 4, 1, 5, 2, 6, 3, 7};
+#pragma unroll
+    for (int w = 0; w < S::KW; w++)
+#pragma unroll
+      for (int i = 0; i < 8; i++) qf[w][i] = (_Float16)x[w][order[i]];
 
     // ---- the loop ----
-    float4_t O[NB][NG][S::OPS];
-    float M[NB], L[NB], x_top[NB];    // x_top: x above which M rises
+    float4_t O[NG][S::OPS];
+    float M = kNone, L = 0.f, x_top = kNone;  // x_top: x above which M rises
     float shift = 0.f, v_top = 0.f;  // v 2^shift <= 2^kVTop while v <= v_top
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
-      M[b] = x_top[b] = kNone;
-      L[b] = 0.f;
+    for (int n = 0; n < NG; n++)
 #pragma unroll
-      for (int n = 0; n < NG; n++)
-#pragma unroll
-        for (int i = 0; i < S::OPS; i++) O[b][n][i] = (float4_t){0.f, 0.f, 0.f, 0.f};
-    }
+      for (int i = 0; i < S::OPS; i++) O[n][i] = (float4_t){0.f, 0.f, 0.f, 0.f};
     const int32_t* pages = a.table + (size_t)r * a.max_pages;
     const uint8_t* const cache = a.cache + (size_t)head * block;
 
@@ -481,30 +481,25 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
       }
     };
     auto compute = [&](int s, bool there0, bool there1, const Codes<D, NG>& f) {
-      float x[NB][2][4];
+      float x[2][4];
 #pragma unroll
       for (int u = 0; u < 2; u++) {
-        float4_t sum[NB][NG];
+        float4_t sum[NG];
 #pragma unroll
         for (int n = 0; n < NG; n++) {
-#pragma unroll
-          for (int b = 0; b < NB; b++) sum[b][n] = (float4_t){0.f, 0.f, 0.f, 0.f};
+          sum[n] = (float4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
           for (int w = 0; w < S::STEPS; w++) {
             const half8_t k = k_operand(magic, f.k[u][n * S::STEPS + w]);
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-              sum[b][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[b][n * S::STEPS + w], sum[b][n], 0, 0, 0);
+            sum[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[n * S::STEPS + w], sum[n], 0, 0, 0);
           }
         }
 #pragma unroll
-        for (int b = 0; b < NB; b++)
+        for (int i = 0; i < 4; i++) {
+          x[u][i] = sum[0][i] * (float)f.ks[u][0][i];
 #pragma unroll
-          for (int i = 0; i < 4; i++) {
-            x[b][u][i] = sum[b][0][i] * (float)f.ks[u][0][i];
-#pragma unroll
-            for (int n = 1; n < NG; n++) x[b][u][i] = __builtin_fmaf(sum[b][n][i], (float)f.ks[u][n][i], x[b][u][i]);
-          }
+          for (int n = 1; n < NG; n++) x[u][i] = __builtin_fmaf(sum[n][i], (float)f.ks[u][n][i], x[u][i]);
+        }
       }
       half4_t vs[2][NG];
 #pragma unroll
@@ -519,29 +514,19 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
             const int tok = s * kStep + 16 * u + 4 * g + i;
-            bool some = false;  // scales of tokens that no row here sees may be anything
+            const bool in = tok < seen && (u ? there1 : there0);
+            x[u][i] = in ? x[u][i] : -__builtin_inff();
+            // (the scale of a token that the row does not see may be anything)
 #pragma unroll
-            for (int b = 0; b < NB; b++) {
-              const bool in = tok < seen[b] && (u ? there1 : there0);
-              x[b][u][i] = in ? x[b][u][i] : -__builtin_inff();
-              some |= in;
-            }
-#pragma unroll
-            for (int n = 0; n < NG; n++) vs[u][n][i] = some ? vs[u][n][i] : (_Float16)0.f;
+            for (int n = 0; n < NG; n++) vs[u][n][i] = in ? vs[u][n][i] : (_Float16)0.f;
           }
       }
-      float xm[NB], vm = 0.f;
-      bool rise = false;
+      float xm = x[0][0], vm = 0.f;
 #pragma unroll
-      for (int b = 0; b < NB; b++) {
-        xm[b] = x[b][0][0];
-#pragma unroll
-        for (int i = 1; i < 8; i++) xm[b] = fmaxf(xm[b], x[b][i / 4][i % 4]);
-        rise |= xm[b] > x_top[b];
-      }
+      for (int i = 1; i < 8; i++) xm = fmaxf(xm, x[i / 4][i % 4]);
 #pragma unroll
       for (int i = 0; i < 8 * NG; i++) vm = fmaxf(vm, fabsf((float)vs[i / 4 / NG][i / 4 % NG][i % 4]));
-      if (__any(rise || vm > v_top)) {
+      if (__any(xm > x_top || vm > v_top)) {
         // new reference: the rows' maxima so far and the largest v (the four lanes of a row agree)
         vm = column_max(vm);
         float new_shift = shift;
@@ -550,43 +535,28 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
           new_shift = fminf(kVTop - (float)__builtin_amdgcn_frexp_expf(vm), 24.f);
           v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
         }
+        const float m = column_max(xm);
+        // M = max - shift: rows keep the larger of the old maximum and this step's
+        const float old_max = M == kNone ? kNone : M + shift;
+        const float new_max = fmaxf(old_max, m * c1);
+        const float new_M = new_max <= kNone ? kNone : new_max - new_shift;
+        const float f = M == kNone ? 0.f : __builtin_amdgcn_exp2f(M - new_M);
+        M = new_M;
+        x_top = new_M == kNone ? kNone : (new_max + kSlack) * __builtin_amdgcn_rcpf(c1);
+        L *= f;
 #pragma unroll
-        for (int b = 0; b < NB; b++) {
-          const float m = column_max(xm[b]);
-          // M = max - shift: rows keep the larger of the old maximum and this step's
-          const float old_max = M[b] == kNone ? kNone : M[b] + shift;
-          const float new_max = fmaxf(old_max, m * c1[b]);
-          const float new_M = new_max <= kNone ? kNone : new_max - new_shift;
-          const float f = M[b] == kNone ? 0.f : __builtin_amdgcn_exp2f(M[b] - new_M);
-          M[b] = new_M;
-          x_top[b] = new_M == kNone ? kNone : (new_max + kSlack) * __builtin_amdgcn_rcpf(c1[b]);
-          L[b] *= f;
+        for (int n = 0; n < NG; n++)
 #pragma unroll
-          for (int n = 0; n < NG; n++)
-#pragma unroll
-            for (int i = 0; i < S::OPS; i++) O[b][n][i] *= f;
-        }
+          for (int i = 0; i < S::OPS; i++) O[n][i] *= f;
         shift = new_shift;
       }
-      half8_t P[NB][NG];
+      half8_t P[NG];
 #pragma unroll
-      for (int b = 0; b < NB; b++)
+      for (int i = 0; i < 8; i++) {
+        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4], c1, -M));
+        L += p;
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[b][i / 4][i % 4], c1[b], -M[b]));
-          L[b] += p;
-#pragma unroll
-          for (int n = 0; n < NG; n++) P[b][n][i] = (_Float16)(p * (float)vs[i / 4][n][i % 4]);
-        }
-      if (NB > 1 && masked) {
-        // a scale that another row of the tile sees may be NaN: what this row does not see is zero
-#pragma unroll
-        for (int b = 0; b < NB; b++)
-#pragma unroll
-          for (int i = 0; i < 8; i++)
-#pragma unroll
-            for (int n = 0; n < NG; n++)
-              P[b][n][i] = x[b][i / 4][i % 4] == -__builtin_inff() ? (_Float16)0.f : P[b][n][i];
+        for (int n = 0; n < NG; n++) P[n][i] = (_Float16)(p * (float)vs[i / 4][n][i % 4]);
       }
 #pragma unroll
       for (int n = 0; n < NG; n++)
@@ -597,10 +567,8 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
           v_operands<S::PARTS>(magic, f.v[0][n], f.v[1][n], sel, turn, vo);
 #pragma unroll
           for (int i = 0; i < OT; i++)
-#pragma unroll
-            for (int b = 0; b < NB; b++)
-              O[b][n][turn * OT + i] =
-                  __builtin_amdgcn_mfma_f32_16x16x32_f16(vo[i], P[b][n], O[b][n][turn * OT + i], 0, 0, 0);
+            O[n][turn * OT + i] =
+                __builtin_amdgcn_mfma_f32_16x16x32_f16(vo[i], P[n], O[n][turn * OT + i], 0, 0, 0);
         }
     };
 
@@ -633,17 +601,16 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
       compute(s0 + k * KW, there0, there1, f);
     }
 
-    // ---- a head's waves meet, 16 rows at a time: lane (c, g) holds row c's dims of MFMA
+    // ---- the waves of a block of rows meet: lane (c, g) holds row c's dims of MFMA
     // rows 4 g + i; then the waves share out the items (row, four dims) ----
     constexpr int RP = D + 4, Q4 = D / 4;  // floats of a row in LDS, items of a row
     const int et = per_piece(threadIdx.x) & 63, ec = et & 15, eg = et >> 4;
     const int item0 = et + 64 * kw, items = 64 << a.log_kw;
-    uint8_t* const group = lds + (hw << a.log_kw) * (S::RING * S::STAGE);  // the head's waves' rings
-    const bool exists = own_head < a.kv_heads;
-    const int live_rows = min(rows - row0, 16 * NB);
+    uint8_t* const group = lds + (hw << a.log_kw) * (S::RING * S::STAGE);  // those waves' rings
+    const int live_rows = min(rows - row0, 16);
     // a piece's place in the scratch, and a row of this head in it
     auto slot_row = [&](uint32_t w, int second, int row) {
-      return (((size_t)w * 2 + second) * HW + hw) * (16 * NB) + row;
+      return (((size_t)w * 2 + second) * HW + hw) * 16 + row;
     };
     auto write = [&](int row, int d0, float m, float l, const float4_t& o) {
       const int i = row0 + row, t = one ? 0 : i / G;
@@ -656,59 +623,56 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
       if (a.lse != nullptr && d0 == 0)
         a.lse[at] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
     };
+    __syncthreads();  // the rings are done with
+    L = column_sum(L);
+    float* mine = reinterpret_cast<float*>(ring);
 #pragma unroll
-    for (int b = 0; b < NB; b++) {
-      __syncthreads();  // the rings, or the block of rows before, are done with
-      L[b] = column_sum(L[b]);
-      float* mine = reinterpret_cast<float*>(ring);
+    for (int n = 0; n < NG; n++)
 #pragma unroll
-      for (int n = 0; n < NG; n++)
+      for (int i = 0; i < S::OPS; i++)
 #pragma unroll
-        for (int i = 0; i < S::OPS; i++)
-#pragma unroll
-          for (int k = 0; k < 4; k++) {
-            const int m = 4 * eg + k;
-            mine[ec * RP + 8 * (n * S::BLOCKS + m / S::PARTS) + (8 / S::PARTS) * (m % S::PARTS) + i] = O[b][n][i][k];
-          }
-      if (eg == 0) *reinterpret_cast<float2*>(mine + ec * RP + D) = make_float2(M[b], L[b]);
-      __syncthreads();
+        for (int k = 0; k < 4; k++) {
+          const int m = 4 * eg + k;
+          mine[ec * RP + 8 * (n * S::BLOCKS + m / S::PARTS) + (8 / S::PARTS) * (m % S::PARTS) + i] = O[n][i][k];
+        }
+    if (eg == 0) *reinterpret_cast<float2*>(mine + ec * RP + D) = make_float2(M, L);
+    __syncthreads();
 #pragma unroll 1
-      for (int it = item0; it < 16 * Q4; it += items) {
-        const int row = it / Q4, d0 = it % Q4 * 4;
-        if (!exists || 16 * b + row >= live_rows) break;  // (rows ascend)
-        const float* from = reinterpret_cast<const float*>(group) + row * RP;
-        constexpr int NEXT = S::RING * S::STAGE / 4;  // floats from a wave's to the next
-        float m = kNone, l = 0.f;
-        float4_t o = {0.f, 0.f, 0.f, 0.f};
-        float2 ml[kWaves];
-        float4_t v[kWaves];
+    for (int it = item0; it < 16 * Q4; it += items) {
+      const int row = it / Q4, d0 = it % Q4 * 4;
+      if (!exists || row >= live_rows) break;  // (rows ascend)
+      const float* from = reinterpret_cast<const float*>(group) + row * RP;
+      constexpr int NEXT = S::RING * S::STAGE / 4;  // floats from a wave's to the next
+      float m = kNone, l = 0.f;
+      float4_t o = {0.f, 0.f, 0.f, 0.f};
+      float2 ml[kWaves];
+      float4_t v[kWaves];
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {  // (all reads in flight; those past KW repeat the last and do not count)
-          const float* at = from + min(w, KW - 1) * NEXT;
-          ml[w] = *reinterpret_cast<const float2*>(at + D);
-          v[w] = *reinterpret_cast<const float4_t*>(at + d0);
-        }
+      for (int w = 0; w < kWaves; w++) {  // (all reads in flight; those past KW repeat the last and do not count)
+        const float* at = from + min(w, KW - 1) * NEXT;
+        ml[w] = *reinterpret_cast<const float2*>(at + D);
+        v[w] = *reinterpret_cast<const float4_t*>(at + d0);
+      }
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) m = fmaxf(m, ml[w].x);
+      for (int w = 0; w < kWaves; w++) m = fmaxf(m, ml[w].x);
 #pragma unroll
-        for (int w = 0; w < kWaves; w++) {
-          const float f = w < KW ? __builtin_amdgcn_exp2f(ml[w].x - m) : 0.f;
-          l += f * ml[w].y;
-          o += v[w] * f;
-        }
-        if (whole) {
-          write(16 * b + row, d0, m, l, o);
-        } else {
-          const size_t at = slot_row(blockIdx.x, first_piece ? 0 : 1, 16 * b + row);
-          *reinterpret_cast<float4_t*>(a.partial + at * D + d0) = o;
-          if (d0 == 0) *reinterpret_cast<float2*>(a.partial_ml + at * 2) = make_float2(m, l);
-        }
+      for (int w = 0; w < kWaves; w++) {
+        const float f = w < KW ? __builtin_amdgcn_exp2f(ml[w].x - m) : 0.f;
+        l += f * ml[w].y;
+        o += v[w] * f;
+      }
+      if (whole) {
+        write(row, d0, m, l, o);
+      } else {
+        const size_t at = slot_row(blockIdx.x, first_piece ? 0 : 1, row);
+        *reinterpret_cast<float4_t*>(a.partial + at * D + d0) = o;
+        if (d0 == 0) *reinterpret_cast<float2*>(a.partial_ml + at * 2) = make_float2(m, l);
       }
     }
     if (!whole) {
       // every thread's stores are done before the barrier, the counter (the first
       // workgroup's: only its last piece is a tile's beginning) moves after it
-      const uint32_t w0 = tile_unit / share, pieces = (tile_unit + len - 1) / share - w0 + 1;
+      const uint32_t w0 = work_unit / share, pieces = (tile_unit + len - 1) / share - w0 + 1;
       __atomic_signal_fence(__ATOMIC_SEQ_CST);
       __builtin_amdgcn_s_waitcnt(0);
       __atomic_signal_fence(__ATOMIC_SEQ_CST);
@@ -722,55 +686,51 @@ __global__ __launch_bounds__(64 * kWaves, (NB == 1 && Shape<D, NG>::TWO ? 4 : 2)
         const int second0 = w0 * share < tile_unit ? 1 : 0;
         float* weight = reinterpret_cast<float*>(group);  // [row][piece], then [row] {reference, sum}
         float* row_ml = weight + 16 * kMaxSplits;
-#pragma unroll 1
-        for (int b = 0; b < NB; b++) {
-          const int left = exists ? min(live_rows - 16 * b, 16) : 0;
-          if (b > 0) __syncthreads();
-          // lane s reads a row's reference and sum of piece s; the wave weighs the pieces
-          float2 ml[16];
+        const int left = exists ? live_rows : 0;
+        // lane s reads a row's reference and sum of piece s; the wave weighs the pieces
+        float2 ml[16];
 #pragma unroll
-          for (int j = 0; j < 16; j++) {
-            const int row = kw + (j << a.log_kw);
-            ml[j] = make_float2(kNone, 0.f);
-            if (row < left && et < (int)pieces)
-              ml[j] = *reinterpret_cast<const float2*>(
-                  a.partial_ml + slot_row(w0 + et, et == 0 ? second0 : 0, 16 * b + row) * 2);
+        for (int j = 0; j < 16; j++) {
+          const int row = kw + (j << a.log_kw);
+          ml[j] = make_float2(kNone, 0.f);
+          if (row < left && et < (int)pieces)
+            ml[j] = *reinterpret_cast<const float2*>(
+                a.partial_ml + slot_row(w0 + et, et == 0 ? second0 : 0, row) * 2);
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+          const int row = kw + (j << a.log_kw);
+          if (row < left) {  // (wave-uniform)
+            float m = ml[j].x;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
+            const float f = et < (int)pieces ? __builtin_amdgcn_exp2f(ml[j].x - m) : 0.f;
+            float l = f * ml[j].y;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
+            if (et < kMaxSplits) weight[row * kMaxSplits + et] = f;
+            if (et == 0) row_ml[2 * row] = m, row_ml[2 * row + 1] = l;
           }
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (int it = item0; it < left * Q4; it += items) {
+          const int row = it / Q4, d0 = it % Q4 * 4;
+          float4_t o = {0.f, 0.f, 0.f, 0.f};
+          constexpr int FLIGHT = 8;  // pieces in flight
+#pragma unroll 1
+          for (uint32_t s = 0; s < pieces; s += FLIGHT) {
+            float4_t v[FLIGHT];
 #pragma unroll
-          for (int j = 0; j < 16; j++) {
-            const int row = kw + (j << a.log_kw);
-            if (row < left) {  // (wave-uniform)
-              float m = ml[j].x;
-#pragma unroll
-              for (int d = 1; d < 64; d <<= 1) m = fmaxf(m, __shfl_xor(m, d));
-              const float f = et < (int)pieces ? __builtin_amdgcn_exp2f(ml[j].x - m) : 0.f;
-              float l = f * ml[j].y;
-#pragma unroll
-              for (int d = 1; d < 64; d <<= 1) l += __shfl_xor(l, d);
-              if (et < kMaxSplits) weight[row * kMaxSplits + et] = f;
-              if (et == 0) row_ml[2 * row] = m, row_ml[2 * row + 1] = l;
+            for (int k = 0; k < FLIGHT; k++) {
+              const uint32_t p = min(s + k, pieces - 1);
+              v[k] = *reinterpret_cast<const float4_t*>(
+                  a.partial + slot_row(w0 + p, p == 0 ? second0 : 0, row) * D + d0);
             }
-          }
-          __syncthreads();
-#pragma unroll 1
-          for (int it = item0; it < left * Q4; it += items) {
-            const int row = it / Q4, d0 = it % Q4 * 4;
-            float4_t o = {0.f, 0.f, 0.f, 0.f};
-            constexpr int FLIGHT = 8;  // pieces in flight
-#pragma unroll 1
-            for (uint32_t s = 0; s < pieces; s += FLIGHT) {
-              float4_t v[FLIGHT];
 #pragma unroll
-              for (int k = 0; k < FLIGHT; k++) {
-                const uint32_t p = min(s + k, pieces - 1);
-                v[k] = *reinterpret_cast<const float4_t*>(
-                    a.partial + slot_row(w0 + p, p == 0 ? second0 : 0, 16 * b + row) * D + d0);
-              }
-#pragma unroll
-              for (int k = 0; k < FLIGHT; k++) o += v[k] * weight[row * kMaxSplits + s + k];  // (zero past the last)
-            }
-            write(16 * b + row, d0, row_ml[2 * row], row_ml[2 * row + 1], o);
+            for (int k = 0; k < FLIGHT; k++) o += v[k] * weight[row * kMaxSplits + s + k];  // (zero past the last)
           }
+          write(row, d0, row_ml[2 * row], row_ml[2 * row + 1], o);
         }
       }
     }

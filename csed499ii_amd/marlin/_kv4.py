@@ -143,7 +143,7 @@ def kv4_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: t
                            f"{block_table.size(0)}")
     if num_tokens < 0:
         raise RuntimeError("num_tokens must not be negative")
-    out = torch.empty(num_tokens + 2 * R + 2, dtype=torch.int32, device=context_lens.device)
+    out = context_lens.new_empty(num_tokens + 2 * R + 2)
     slots, cu, kv, used = out.split_with_sizes((num_tokens, R + 1, R, 1))
     at = out.data_ptr()
     err = _lib.load().marlin_hip_kv4_tables(ctx, new, free, table, at, at + 4 * num_tokens,
@@ -193,7 +193,7 @@ def kv4_gather(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, groupsiz
     sp = _ints("slots", slots, dev)
     N, H = slots.size(0), cache.size(1)
     k = torch.empty((N, H, head_dim), dtype=dtype, device=cache.device)
-    v = torch.empty((N, H, head_dim), dtype=dtype, device=cache.device)
+    v = torch.empty_like(k)
     err = _lib.load().marlin_hip_kv4_gather(cache.data_ptr(), sp, k.data_ptr(), v.data_ptr(), N, H, head_dim, page,
                                             cache.size(0), groupsize, _DTYPES[dtype], dev, _raw_stream(dev))
     if err:
@@ -250,7 +250,7 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     if max_kv is None:
         max_kv = block_table.size(1) * page
     if out is None:
-        out = torch.empty((N, Hq, D), dtype=q.dtype, device=q.device)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((N, Hq, D))  # (torch.empty costs the host more)
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise RuntimeError(f"out must be a contiguous, 16-byte aligned {q.dtype} {tuple(q.shape)} tensor on cuda:{dev}")
