@@ -11,8 +11,16 @@ namespace kv4 {
 hipError_t launch_prompt(const AttnArgs& a, int workgroups, int head_dim, int ng, int dtype, hipStream_t stream);
 
 // Requests of at most so many rows (new tokens times the query heads of a kv head) go to the
-// split kernel, the others to the prompt kernel, each of which passes over the other's.
-constexpr int kSplitRows = 48;
+// split kernel, the others to the prompt kernel, each of which passes over the other's.  The
+// split kernel's time grows with the rows, the prompt kernel's is the same up to 256: 12
+// requests of 4096 tokens on 8 heads of 128 dims, 64, 80, 96 and 128 rows, 57, 64, 74 and 87
+// us beside 67 to 69; with groups of 32, which cost the prompt kernel most, 65, 78, 91 and 108
+// beside 148, and 160 beside 165 at 192.  Few tiles leave the prompt kernel's large parts
+// waiting: one request of 8192 tokens, 24 us beside 34 at 64 rows, 41 beside 59 at 256.
+int split_rows(int requests, int kv_heads, int head_dim, int ng, int cus) {
+  if ((long long)requests * kv_heads <= cus / 16) return 256;
+  return head_dim == 128 && ng == 4 ? 160 : 80;
+}
 constexpr int kPromptTile = 64;
 
 int compute_units(int dev) {
@@ -37,7 +45,7 @@ Plan plan(int requests, int q_heads, int kv_heads, int head_dim, int ng, int max
   Plan p{};
   const long long row_blocks = ((long long)max_q * (q_heads / kv_heads) + 15) / 16;
   const long long steps = ((long long)max_kv + kStep - 1) / kStep;
-  const long long most = ng == 1 || head_dim == 64 ? 2ll * cus : cus;
+  const long long most = 2ll * cus;
   const long long blocks = requests * row_blocks * kv_heads;
   p.log_kw = blocks <= 2 * most ? kLogWaves : 1;
   const int hw = kWaves >> p.log_kw;
@@ -54,9 +62,9 @@ Plan plan(int requests, int q_heads, int kv_heads, int head_dim, int ng, int max
 // lengths; this is the grid, which bounds the tiles by the tokens.
 constexpr int kPromptRows = 256, kPromptWaves = 8;
 
-Plan prompt_plan(int tokens, int requests, int q_heads, int kv_heads, int max_q, int max_kv, int cus) {
+Plan prompt_plan(int tokens, int requests, int q_heads, int kv_heads, int max_q, int max_kv, int max_rows, int cus) {
   const long long group = q_heads / kv_heads, rows = tokens * group;
-  long long kinds = rows / kPromptRows + (requests < rows / (kSplitRows + 1) ? requests : rows / (kSplitRows + 1));
+  long long kinds = rows / kPromptRows + (requests < rows / (max_rows + 1) ? requests : rows / (max_rows + 1));
   const long long most = requests * ((max_q * group + kPromptRows - 1) / kPromptRows);
   if (kinds > most) kinds = most;
   Plan p{};
@@ -130,16 +138,19 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
   a.num_pages = num_pages;
   a.max_pages = max_pages;
   a.log_page = 31 - __builtin_clz((unsigned)page_size);
-  a.max_rows = kSplitRows;
   a.group = group;
   a.c1 = scale * 1.4426950408889634f;
   const int cus = compute_units(dev);
-  const bool prompts = (long long)max_q * group > kSplitRows, few = !prompts || cu_q != nullptr;
-  const int split_q = prompts ? kSplitRows / group : max_q;
+  const int few_rows = split_rows(requests, kv_heads, head_dim, ng, cus);
+  const bool prompts = (long long)max_q * group > few_rows;
+  const int split_q = prompts ? few_rows / group : max_q;
+  // (where the tokens say that no request can be short, the prompt kernel takes all)
+  const bool split = !prompts || (cu_q != nullptr && split_q > 0 && tokens <= split_q + (long long)(requests - 1) * max_q);
+  a.max_rows = split ? few_rows : 0;
   for (a.first = 0; a.first < requests; a.first += kMaxRequests) {
     a.requests = requests - a.first < kMaxRequests ? requests - a.first : kMaxRequests;
     if (prompts) {
-      const Plan p = prompt_plan(tokens, a.requests, q_heads, kv_heads, max_q, max_kv, cus);
+      const Plan p = prompt_plan(tokens, a.requests, q_heads, kv_heads, max_q, max_kv, a.max_rows, cus);
       if (p.workgroups < 0) return refuse("kv4_attention: too many rows for one launch");
       a.pieces = p.pieces;
       if (p.split) {
@@ -152,7 +163,7 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
       if (err != MARLIN_HIP_OK) return err;
       a.partial = nullptr;
     }
-    if (few && split_q > 0) {
+    if (split) {
       const Plan p = plan(a.requests, q_heads, kv_heads, head_dim, ng, split_q, max_kv, cus);
       a.log_kw = p.log_kw;
       a.lead = p.lead;

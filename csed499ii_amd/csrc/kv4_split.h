@@ -110,10 +110,10 @@ struct Shape {
   // A step in LDS: K codes of 32 tokens, V codes, scales [half][K, V][quad][NG][4].
   static constexpr int V_AT = kStep * D / 2, S_AT = kStep * D, STAGE = S_AT + 128 * NG;
   static constexpr int LOADS = D / 32 + (NG == 4 ? 2 : 1);  // DMA instructions of a step
-  // 128 registers let two workgroups share a compute unit; with several groups of 128 dims
-  // one has it to itself, and its waves twice the steps in flight.
-  static constexpr bool TWO = NG == 1 || D == 64;
-  static constexpr int RING = TWO ? 2 : 4;  // steps of a wave in flight or in use
+  // 128 registers let two workgroups share a compute unit.  With several groups of 128 dims
+  // V's codes and scales do not fit them, and are read from LDS as they are needed.
+  static constexpr bool LATE = NG > 1 && D == 128;
+  static constexpr int RING = 2;  // steps of a wave in flight or in use
 };
 
 // x and its value in the lane 16 (32) places over, in one order or the other.  (In assembly:
@@ -216,7 +216,7 @@ __device__ __forceinline__ void v_operands(const Magic& m, const u32x4& a, const
 }
 
 template <int D, int NG, int TYPE>
-__global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_split_kernel(AttnArgs a) {
+__global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
   using S = Shape<D, NG>;
   // the waves' rings; later 16 rows of D + 4 floats in each
   static_assert(S::RING * S::STAGE >= 16 * (D + 4) * 4 && S::RING * S::STAGE >= 16 * (kMaxSplits + 2) * 4, "");
@@ -312,11 +312,12 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_
     break;
   }
 
-  // The thread's index as a value of this piece only: what is computed from it is not kept
-  // in registers through the loop.
-  auto per_piece = [](int x) {
-    asm volatile("" : "+v"(x));
-    return x;
+  // The lane's index anew, as a value of this piece only: neither it nor what is computed from
+  // it is kept in registers through the loop.
+  auto lane_again = [] {
+    uint32_t ones = ~0u;
+    asm volatile("" : "+s"(ones));
+    return (int)__builtin_amdgcn_mbcnt_hi(ones, __builtin_amdgcn_mbcnt_lo(ones, 0));
   };
   const Magic magic;
   const uint32_t block = block_bytes<D, NG>(T);
@@ -332,7 +333,8 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_
     Request rq;
     uint32_t r_begin;
     if (few) {
-      r = 63 - __builtin_clzll(__ballot(lane < a.requests && begins[lane] <= unit));
+      const int i = lane_again();
+      r = 63 - __builtin_clzll(__ballot(i < a.requests && begins[i] <= unit));
       rq = Request{few_first[r], few_n[r], few_kv[r]};
     } else {
       for (int hi = a.requests; hi - r > 1;) {
@@ -373,7 +375,7 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_
 
     // ---- Q: lane (c, g) holds row c's dims [32 w + 8 g, + 8), slots in the order the
     // unpacking gives ----
-    const int lane = per_piece(threadIdx.x) & 63, c = lane & 15, g = lane >> 4;
+    const int lane = lane_again(), c = lane & 15, g = lane >> 4;
     const int blk = c / S::PARTS, part = c % S::PARTS;
     const uint32_t sel = S::PARTS == 1 ? 0u : part_selector<S::PARTS == 1 ? 2 : S::PARTS>(part);
     half8_t qf[S::KW];
@@ -461,29 +463,38 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_
         dma4(to + S::S_AT, (lane < 2 * L8 ? sc0 : sc1) + at);
       }
     };
-    auto receive = [&](const uint8_t* from, Codes<D, NG>& f) {
+    auto read_v = [&](const uint8_t* from, int u, int n) {
+      return *reinterpret_cast<const u32x4*>(from + S::V_AT + u * (8 * D) + g * (2 * D) + (n * S::BLOCKS + blk) * 16);
+    };
+    auto read_ks = [&](const uint8_t* from, int u, int n) {
+      return *reinterpret_cast<const half4_t*>(from + S::S_AT + u * (64 * NG) + (g * NG + n) * 8);
+    };
+    auto read_vs = [&](const uint8_t* from, int u, int n) {
+      return *reinterpret_cast<const half4_t*>(from + S::S_AT + u * (64 * NG) + 32 * NG + (g * NG + n) * 8);
+    };
+    auto receive = [&](const uint8_t* from, int u, Codes<D, NG>& f) {
+      const uint8_t* kp = from + u * (8 * D) + c * (D / 2) + g * (D / 8);
+      if constexpr (D == 128) {
+        const u32x4 w = *reinterpret_cast<const u32x4*>(kp);
+        f.k[u][0] = w.x, f.k[u][1] = w.y, f.k[u][2] = w.z, f.k[u][3] = w.w;
+      } else {
+        const u32x2 w = *reinterpret_cast<const u32x2*>(kp);
+        f.k[u][0] = w.x, f.k[u][1] = w.y;
+      }
 #pragma unroll
-      for (int u = 0; u < 2; u++) {
-        const uint8_t* kp = from + u * (8 * D) + c * (D / 2) + g * (D / 8);
-        if constexpr (D == 128) {
-          const u32x4 w = *reinterpret_cast<const u32x4*>(kp);
-          f.k[u][0] = w.x, f.k[u][1] = w.y, f.k[u][2] = w.z, f.k[u][3] = w.w;
-        } else {
-          const u32x2 w = *reinterpret_cast<const u32x2*>(kp);
-          f.k[u][0] = w.x, f.k[u][1] = w.y;
+      for (int n = 0; n < NG; n++) {
+        if (!S::LATE) {
+          f.v[u][n] = read_v(from, u, n);
+          f.vs[u][n] = read_vs(from, u, n);
         }
-#pragma unroll
-        for (int n = 0; n < NG; n++) {
-          f.v[u][n] = *reinterpret_cast<const u32x4*>(from + S::V_AT + u * (8 * D) + g * (2 * D) + (n * S::BLOCKS + blk) * 16);
-          f.ks[u][n] = *reinterpret_cast<const half4_t*>(from + S::S_AT + u * (64 * NG) + (g * NG + n) * 8);
-          f.vs[u][n] = *reinterpret_cast<const half4_t*>(from + S::S_AT + u * (64 * NG) + 32 * NG + (g * NG + n) * 8);
-        }
+        f.ks[u][n] = read_ks(from, u, n);
       }
     };
-    auto compute = [&](int s, bool there0, bool there1, const Codes<D, NG>& f) {
+    auto compute = [&](int s, bool there0, bool there1, Codes<D, NG>& f, const uint8_t* from) {
       float x[2][4];
 #pragma unroll
       for (int u = 0; u < 2; u++) {
+        if constexpr (S::LATE) receive(from, u, f);
         float4_t sum[NG];
 #pragma unroll
         for (int n = 0; n < NG; n++) {
@@ -505,7 +516,7 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_
 #pragma unroll
       for (int u = 0; u < 2; u++)
 #pragma unroll
-        for (int n = 0; n < NG; n++) vs[u][n] = f.vs[u][n];
+        for (int n = 0; n < NG; n++) vs[u][n] = S::LATE ? read_vs(from, u, n) : f.vs[u][n];
       // (wave-uniform) a step that some row does not see whole
       const bool masked = (s + 1) * kStep > all || !there0 || !there1;
       if (masked) {
@@ -555,21 +566,40 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_
       for (int i = 0; i < 8; i++) {
         const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4], c1, -M));
         L += p;
+        if constexpr (S::LATE) {
+          x[i / 4][i % 4] = p;
+        } else {
 #pragma unroll
-        for (int n = 0; n < NG; n++) P[n][i] = (_Float16)(p * (float)vs[i / 4][n][i % 4]);
+          for (int n = 0; n < NG; n++) P[n][i] = (_Float16)(p * (float)vs[i / 4][n][i % 4]);
+        }
       }
 #pragma unroll
-      for (int n = 0; n < NG; n++)
+      for (int n = 0; n < NG; n++) {
+        u32x4 v0, v1;
+        if constexpr (S::LATE) {
+          v0 = read_v(from, 0, n), v1 = read_v(from, 1, n);
+          const half4_t s[2] = {read_vs(from, 0, n), read_vs(from, 1, n)};
+#pragma unroll
+          for (int i = 0; i < 8; i++) P[n][i] = (_Float16)(x[i / 4][i % 4] * (float)s[i / 4][i % 4]);
+          if (masked) {  // zero, whatever the scale
+#pragma unroll
+            for (int i = 0; i < 8; i++) P[n][i] = x[i / 4][i % 4] == 0.f ? (_Float16)0.f : P[n][i];
+          }
+        } else {
+          v0 = f.v[0][n], v1 = f.v[1][n];
+        }
 #pragma unroll
         for (int turn = 0; turn < kTurns<S::PARTS>; turn++) {
           constexpr int OT = kTurnOps<S::PARTS>;
           half8_t vo[OT];
-          v_operands<S::PARTS>(magic, f.v[0][n], f.v[1][n], sel, turn, vo);
+          v_operands<S::PARTS>(magic, v0, v1, sel, turn, vo);
 #pragma unroll
           for (int i = 0; i < OT; i++)
             O[n][turn * OT + i] =
                 __builtin_amdgcn_mfma_f32_16x16x32_f16(vo[i], P[n], O[n][turn * OT + i], 0, 0, 0);
         }
+        if constexpr (S::LATE) __builtin_amdgcn_sched_barrier(0);  // (registers: a group at a time)
+      }
     };
 
 #pragma unroll
@@ -588,7 +618,11 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_
       if (k + S::RING <= count) sm24::wait_vm<(S::RING - 1) * S::LOADS>();
       else sm24::wait_vm<0>();
       Codes<D, NG> f;
-      receive(ring + stage * S::STAGE, f);
+      if constexpr (!S::LATE) {
+        receive(ring + stage * S::STAGE, 0, f);
+        receive(ring + stage * S::STAGE, 1, f);
+      }
+      if (S::LATE) compute(s0 + k * KW, there0, there1, f, ring + stage * S::STAGE);
       // the stage's reads are done before it is filled again
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_sched_barrier(0);
@@ -598,13 +632,13 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_
         else send(k + S::RING, place(then, j), place(then, j + 1), ring_at + stage * S::STAGE);
       }
       stage = stage + 1 == S::RING ? 0 : stage + 1;
-      compute(s0 + k * KW, there0, there1, f);
+      if (!S::LATE) compute(s0 + k * KW, there0, there1, f, nullptr);
     }
 
     // ---- the waves of a block of rows meet: lane (c, g) holds row c's dims of MFMA
     // rows 4 g + i; then the waves share out the items (row, four dims) ----
     constexpr int RP = D + 4, Q4 = D / 4;  // floats of a row in LDS, items of a row
-    const int et = per_piece(threadIdx.x) & 63, ec = et & 15, eg = et >> 4;
+    const int et = lane_again(), ec = et & 15, eg = et >> 4;
     const int item0 = et + 64 * kw, items = 64 << a.log_kw;
     uint8_t* const group = lds + (hw << a.log_kw) * (S::RING * S::STAGE);  // those waves' rings
     const int live_rows = min(rows - row0, 16);
@@ -677,11 +711,11 @@ __global__ __launch_bounds__(64 * kWaves, (Shape<D, NG>::TWO ? 4 : 2)) void kv4_
       __builtin_amdgcn_s_waitcnt(0);
       __atomic_signal_fence(__ATOMIC_SEQ_CST);
       __syncthreads();
-      if (tid == 0)
+      if (wave == 0 && et == 0)
         arrived = __hip_atomic_fetch_add(a.counters + w0, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
       __syncthreads();
       if (arrived == pieces) {
-        if (tid == 0) __hip_atomic_store(a.counters + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (wave == 0 && et == 0) __hip_atomic_store(a.counters + w0, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         // only the first workgroup's piece may be its second
         const int second0 = w0 * share < tile_unit ? 1 : 0;
         float* weight = reinterpret_cast<float*>(group);  // [row][piece], then [row] {reference, sum}
