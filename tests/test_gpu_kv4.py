@@ -442,3 +442,100 @@ def test_refusals():
     no("requests", marlin.kv4_tables, kv, kv[:2], slots, table, 3, T)
     no("page_size", marlin.kv4_tables, kv, kv, slots, table, 3, 20)
     no("negative", marlin.kv4_tables, kv, kv, slots, table, -1, T)
+
+
+# ---- many rows: the prompt kernel (more rows a head than the split kernel's, more than a few heads) ----
+
+
+PROMPTS = [
+    ([170, 1, 3], [200, 513, 3], 6, 6),          # beside requests that are the split kernel's
+    ([300, 170, 290], [300, 330, 290], 6, 6),    # no short request: one launch
+    ([200, 2], [190, 700], 18, 9),               # rows that see nothing
+    ([41], [1200], 68, 17),                      # one block of rows, divided over its tokens
+    ([90, 0, 1, 90], [400, 0, 70, 90], 10, 5),
+]
+
+
+@pytest.mark.parametrize("D,g,T", GEOMETRIES)
+@pytest.mark.parametrize("q_lens,kv_lens,Hq,Hkv", PROMPTS)
+def test_prompts(D, g, T, q_lens, kv_lens, Hq, Hkv):
+    dtype = torch.bfloat16 if len(kv_lens) == 3 else torch.float16
+    p = _problem(q_lens, kv_lens, Hq, Hkv, D, g, T, dtype, seed=sum(kv_lens) + D)
+    want = ref.attention(p[0].double().numpy(), *p[1:5], D, p[5], T)
+    out, lse = _run(p, g, dtype)
+    _check(out, lse, want, dtype, f"D={D} g={g} T={T} q={q_lens} kv={kv_lens}")
+
+
+@pytest.mark.parametrize("k_gain,v_gain", [(30.0, 1.0), (1.0, 1e-4), (1.0, 3000.0), (6.0, 1e-3), (0.0, 1.0), (1.0, 0.0)])
+def test_prompts_peaked_flat_tiny_and_large(k_gain, v_gain):
+    D, g, T = 128, 64, 16
+    p = _problem([90, 170], [500, 300], 10, 10, D, g, T, torch.float16, seed=6, k_gain=k_gain, v_gain=v_gain)
+    want = ref.attention(p[0].double().numpy(), *p[1:5], D, p[5], T)
+    out, lse = _run(p, g, torch.float16)
+    _check(out, lse, want, torch.float16, f"gains {k_gain} {v_gain}", x_max=1000.0 * max(1.0, k_gain) / 30)
+
+
+def test_prompts_with_missing_pages_and_nan():
+    D, T = 128, 16
+    p = list(_problem([170, 3, 180], [260, 90, 200], 6, 6, D, -1, T, torch.float16, seed=4))
+    p[2][0, 3], p[2][0, 7], p[2][1, 0] = -1, 10 ** 6, -7
+    p[2][2, :] = -1
+    want = ref.attention(p[0].double().numpy(), *p[1:5], D, 1, T)
+    assert np.isneginf(want[1][-180:]).all()
+    out, lse = _run(p, -1, torch.float16)
+    _check(out, lse, want, torch.float16, "missing pages")
+    # a NaN scale of V at position 200 reaches the rows that see it and no others
+    p = _problem([170], [260], 17, 17, D, -1, T, torch.float16, seed=52)
+    p[1][p[2][0, 200 // T]].view(np.float16)[:, ref.places(T, D, 1)[3][200 % T]] = np.nan
+    out, _ = _run(p, -1, torch.float16)
+    nan = torch.isnan(out).flatten(1)
+    first = 200 - (260 - 170)
+    assert nan[first:].all() and not nan[:first].any()
+
+
+def test_divided_prompt_same_bits_and_in_a_graph():
+    """A divided block of rows gives the same bits from run to run and on replays between eager
+    work; captured on a stream without scratch it stays whole, the same product."""
+    D, T = 128, 16
+    q, cache, table, kv, cu, _ = _problem([41], [1200], 68, 17, D, -1, T, torch.float16, seed=42)
+    q, cache, table, kv, cu = q.to(DEV), torch.from_numpy(cache).to(DEV), ints(table), ints(kv), ints(cu)
+    call = lambda: marlin.kv4_attention(q, cache, table, kv, cu, max_q=41, max_kv=1200, return_lse=True)  # noqa: E731
+    want, want_lse = call()
+    for _ in range(4):
+        out, lse = call()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out, lse = call()
+    for _ in range(4):
+        out.fill_(float("nan"))
+        call()
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    fresh, graph2 = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph2, stream=fresh):
+        out2, _ = call()
+    graph2.replay()
+    torch.cuda.synchronize()
+    assert (out2.float() - want.float()).abs().max() <= 2.0 ** -9 * want.float().abs().max()
+
+
+@pytest.mark.parametrize("long", [0, 3, 170])
+def test_more_requests_than_one_launch_takes(long):
+    """1100 requests of 0 to 40 tokens; the last but fifty with ``long`` new tokens (0: no cu_q)."""
+    D, T, R = 64, 16, 1100
+    q_lens = [1] * R
+    kv_lens = [(7 * i) % 41 for i in range(R)]
+    if long:
+        q_lens[R - 50], kv_lens[R - 50], kv_lens[R - 51] = long, long + 5, 20
+    p = _problem(q_lens, kv_lens, 2, 1, D, -1, T, torch.float16, seed=81)
+    want = ref.attention(p[0].double().numpy(), *p[1:5], D, 1, T)
+    out, lse = _run(p, -1, torch.float16, one=not long)
+    _check(out, lse, want, torch.float16, f"{R} requests, {long}")
