@@ -3,6 +3,8 @@
 #include <math.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "kv4_host.h"
 #include "kv4_split.h"
 
@@ -23,9 +25,14 @@ int split_rows(int requests, int kv_heads, int head_dim, int ng, int cus) {
 }
 constexpr int kPromptTile = 64;
 
+// (the query takes the host 0.2 us of each call, so its answer is kept)
 int compute_units(int dev) {
+  static std::atomic<int> known[64];
+  if (dev >= 0 && dev < 64 && known[dev].load(std::memory_order_relaxed) > 0)
+    return known[dev].load(std::memory_order_relaxed);
   int n = 0;
-  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+  if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
+  if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
 

@@ -22,6 +22,7 @@ stream of the tensors' device and nothing waits for the GPU.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 
 import torch
@@ -37,6 +38,16 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 def _raise(err: int):
     raise RuntimeError(_lib.last_error() or f"marlin_hip error {err}")
+
+
+@functools.lru_cache(maxsize=None)
+def _page_of(width: int, head_dim: int, groupsize: int) -> int:
+    """Page size of a cache whose blocks are ``width`` bytes."""
+    page, rest = divmod(width, _row_bytes(head_dim, groupsize))
+    if rest or page not in (16, 32, 64, 128, 256):
+        raise RuntimeError(f"cache blocks of {width} bytes hold no whole page of head_dim={head_dim}, "
+                           f"groupsize={groupsize}")
+    return page
 
 
 def _row_bytes(head_dim: int, groupsize: int) -> int:
@@ -72,7 +83,7 @@ def _ints(name: str, t: torch.Tensor, dev: int, dim: int = 1) -> int:
 
 
 def _page_size(cache: torch.Tensor, dev: int, kv_heads: int | None, head_dim: int, groupsize: int) -> int:
-    row = _row_bytes(head_dim, groupsize)
+    _row_bytes(head_dim, groupsize)
     if not isinstance(cache, torch.Tensor):
         raise TypeError("cache must be a torch.Tensor")
     if cache.dtype != torch.uint8 or cache.dim() != 3 or cache.get_device() != dev or not cache.is_contiguous():
@@ -81,11 +92,7 @@ def _page_size(cache: torch.Tensor, dev: int, kv_heads: int | None, head_dim: in
         raise RuntimeError("cache must be 16-byte aligned")
     if kv_heads is not None and cache.size(1) != kv_heads:
         raise RuntimeError(f"cache has {cache.size(1)} heads, k and v have {kv_heads}")
-    page, rest = divmod(cache.size(2), row)
-    if rest or page not in (16, 32, 64, 128, 256):
-        raise RuntimeError(f"cache blocks of {cache.size(2)} bytes hold no whole page of head_dim={head_dim}, "
-                           f"groupsize={groupsize}")
-    return page
+    return _page_of(cache.size(2), head_dim, groupsize)
 
 
 def _rows(name: str, t: torch.Tensor, dev: int):
@@ -133,23 +140,36 @@ def kv4_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: t
     captured step may pass its padded size); tokens past it get no slot and no page.
     Lengths below zero count as zero.  The sum of ``new_lens`` must stay below 2^31.
     """
-    dev = _device_of("context_lens", context_lens)
-    _check_page(page_size)
-    ctx, new = _ints("context_lens", context_lens, dev), _ints("new_lens", new_lens, dev)
-    free, table = _ints("free_pages", free_pages, dev), _ints("block_table", block_table, dev, 2)
-    R = context_lens.size(0)
-    if new_lens.size(0) != R or block_table.size(0) != R:
-        raise RuntimeError(f"context_lens has {R} requests, new_lens {new_lens.size(0)}, block_table "
-                           f"{block_table.size(0)}")
+    try:  # (as in kv4_append)
+        R, = shape = context_lens.shape
+        F, = free_pages.shape
+        rows, P = block_table.shape
+        dev, ctx, new = context_lens.get_device(), context_lens.data_ptr(), new_lens.data_ptr()
+        free, table, kind = free_pages.data_ptr(), block_table.data_ptr(), torch.int32
+        fits = (dev >= 0 and rows == R and page_size in (16, 32, 64, 128, 256) and new_lens.shape == shape
+                and context_lens.dtype is new_lens.dtype is free_pages.dtype is block_table.dtype is kind
+                and new_lens.get_device() == free_pages.get_device() == block_table.get_device() == dev
+                and context_lens.is_contiguous() and new_lens.is_contiguous() and free_pages.is_contiguous()
+                and block_table.is_contiguous())
+    except (AttributeError, TypeError, ValueError):
+        fits = False
+    if not fits:
+        dev = _device_of("context_lens", context_lens)
+        _check_page(page_size)
+        ctx, new = _ints("context_lens", context_lens, dev), _ints("new_lens", new_lens, dev)
+        free, table = _ints("free_pages", free_pages, dev), _ints("block_table", block_table, dev, 2)
+        R, F, P = context_lens.size(0), free_pages.size(0), block_table.size(1)
+        if new_lens.size(0) != R or block_table.size(0) != R:
+            raise RuntimeError(f"context_lens has {R} requests, new_lens {new_lens.size(0)}, block_table "
+                               f"{block_table.size(0)}")
     if num_tokens < 0:
         raise RuntimeError("num_tokens must not be negative")
     out = context_lens.new_empty(num_tokens + 2 * R + 2)
     slots, cu, kv, used = out.split_with_sizes((num_tokens, R + 1, R, 1))
     at = out.data_ptr()
     err = _lib.load().marlin_hip_kv4_tables(ctx, new, free, table, at, at + 4 * num_tokens,
-                                            at + 4 * (num_tokens + R + 1), at + 4 * (num_tokens + 2 * R + 1), R,
-                                            free_pages.size(0), block_table.size(1), page_size, num_tokens, dev,
-                                            _raw_stream(dev))
+                                            at + 4 * (num_tokens + R + 1), at + 4 * (num_tokens + 2 * R + 1), R, F,
+                                            P, page_size, num_tokens, dev, _raw_stream(dev))
     if err:
         _raise(err)
     return slots, cu, kv, used
@@ -164,19 +184,37 @@ def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: tor
     slices of a fused qkv projection.  A slot that is negative or past the last page is
     skipped; two tokens must not share one.  Scales saturate at 65504; a NaN makes its
     group NaN."""
-    dev = _device_of("k", k)
-    _device_of("v", v)
-    kt, kh = _rows("k", k, dev)
-    vt, vh = _rows("v", v, dev)
-    N, H, D = k.shape
-    if v.shape != k.shape or v.dtype != k.dtype:
-        raise RuntimeError(f"k is {k.dtype} {tuple(k.shape)}, v is {v.dtype} {tuple(v.shape)}")
-    page = _page_size(cache, dev, H, D, groupsize)
-    sp = _ints("slots", slots, dev)
-    if slots.size(0) != N:
-        raise RuntimeError(f"slots has {slots.size(0)} entries, k has {N} tokens")
-    err = _lib.load().marlin_hip_kv4_append(k.data_ptr(), v.data_ptr(), cache.data_ptr(), sp, N, H, D, kt, kh, vt, vh,
-                                            page, cache.size(0), groupsize, _DTYPES[k.dtype], dev, _raw_stream(dev))
+    # What fits as it is passes in one look (the calls of a decoding step wait for the host);
+    # anything else is checked step by step, for the message or for strides that do not count.
+    try:
+        N, H, D = shape = k.shape
+        (kt, kh, kd), (vt, vh, vd) = k.stride(), v.stride()
+        pages, heads, width = cache.shape
+        dev, dtype = k.get_device(), _DTYPES.get(k.dtype)
+        kp, vp, cp, sp = k.data_ptr(), v.data_ptr(), cache.data_ptr(), slots.data_ptr()
+        fits = (dtype is not None and dev >= 0 and v.dtype is k.dtype and v.shape == shape and v.get_device() == dev
+                and kd == vd == 1 and not (kt | kh | vt | vh) & 7 and not (kp | vp | cp) & 15 and heads == H
+                and cache.dtype is torch.uint8 and cache.get_device() == dev and cache.is_contiguous()
+                and slots.dtype is torch.int32 and slots.get_device() == dev and slots.is_contiguous()
+                and slots.shape == (N,))
+    except (AttributeError, TypeError, ValueError):
+        fits = False
+    if not fits:
+        dev = _device_of("k", k)
+        _device_of("v", v)
+        kt, kh = _rows("k", k, dev)
+        vt, vh = _rows("v", v, dev)
+        N, H, D = k.shape
+        if v.shape != k.shape or v.dtype != k.dtype:
+            raise RuntimeError(f"k is {k.dtype} {tuple(k.shape)}, v is {v.dtype} {tuple(v.shape)}")
+        _page_size(cache, dev, H, D, groupsize)
+        sp = _ints("slots", slots, dev)
+        if slots.size(0) != N:
+            raise RuntimeError(f"slots has {slots.size(0)} entries, k has {N} tokens")
+        pages, _, width = cache.shape
+        kp, vp, cp, dtype = k.data_ptr(), v.data_ptr(), cache.data_ptr(), _DTYPES[k.dtype]
+    err = _lib.load().marlin_hip_kv4_append(kp, vp, cp, sp, N, H, D, kt, kh, vt, vh, _page_of(width, D, groupsize), pages,
+                                            groupsize, dtype, dev, _raw_stream(dev))
     if err:
         _raise(err)
 
@@ -186,16 +224,26 @@ def kv4_gather(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, groupsiz
     """The values ``(k, v)``, each ``[tokens, kv_heads, head_dim]``, that the cache holds in
     ``slots``: what :func:`kv4_attention` computes with.  Zeros for slots that are negative or
     past the last page."""
-    dev = _device_of("cache", cache)
-    if dtype not in _DTYPES:
-        raise RuntimeError(f"dtype must be fp16 or bf16, got {dtype}")
-    page = _page_size(cache, dev, None, head_dim, groupsize)
-    sp = _ints("slots", slots, dev)
-    N, H = slots.size(0), cache.size(1)
+    try:  # (as in kv4_append)
+        pages, H, width = cache.shape
+        N, = slots.shape
+        dev, kind, cp, sp = cache.get_device(), _DTYPES.get(dtype), cache.data_ptr(), slots.data_ptr()
+        fits = (kind is not None and dev >= 0 and cache.dtype is torch.uint8 and cache.is_contiguous() and not cp & 15
+                and slots.dtype is torch.int32 and slots.get_device() == dev and slots.is_contiguous())
+    except (AttributeError, TypeError, ValueError):
+        fits = False
+    if not fits:
+        dev = _device_of("cache", cache)
+        if dtype not in _DTYPES:
+            raise RuntimeError(f"dtype must be fp16 or bf16, got {dtype}")
+        _page_size(cache, dev, None, head_dim, groupsize)
+        sp = _ints("slots", slots, dev)
+        (pages, H, width), N, kind, cp = cache.shape, slots.size(0), _DTYPES[dtype], cache.data_ptr()
+    page = _page_of(width, head_dim, groupsize)
     k = torch.empty((N, H, head_dim), dtype=dtype, device=cache.device)
     v = torch.empty_like(k)
-    err = _lib.load().marlin_hip_kv4_gather(cache.data_ptr(), sp, k.data_ptr(), v.data_ptr(), N, H, head_dim, page,
-                                            cache.size(0), groupsize, _DTYPES[dtype], dev, _raw_stream(dev))
+    err = _lib.load().marlin_hip_kv4_gather(cp, sp, k.data_ptr(), v.data_ptr(), N, H, head_dim, page, pages, groupsize,
+                                            kind, dev, _raw_stream(dev))
     if err:
         _raise(err)
     return k, v
@@ -225,15 +273,33 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     of the cache (e.g. -1) are left out; slots past ``kv_lens`` may hold anything.
     A call that splits uses the stream's split-K scratch, as :func:`mul_2_4` does: under
     stream capture make an eager call of the shape first, else it runs unsplit."""
-    dev = _device_of("q", q)
-    qt, qh = _rows("q", q, dev)
-    N, Hq, D = q.shape
-    page = _page_size(cache, dev, None, D, groupsize)
-    H, R = cache.size(1), kv_lens.size(0)
-    table, lens = _ints("block_table", block_table, dev, 2), _ints("kv_lens", kv_lens, dev)
-    if block_table.size(0) != R:
-        raise RuntimeError(f"kv_lens has {R} requests, block_table {block_table.size(0)}")
-    if Hq % H:
+    try:  # (as in kv4_append)
+        N, Hq, D = q.shape
+        qt, qh, qd = q.stride()
+        pages, H, width = cache.shape
+        R, P = block_table.shape
+        dev, dtype = q.get_device(), _DTYPES.get(q.dtype)
+        qp, cp, table, lens = q.data_ptr(), cache.data_ptr(), block_table.data_ptr(), kv_lens.data_ptr()
+        fits = (dtype is not None and dev >= 0 and qd == 1 and not (qt | qh) & 7 and not (qp | cp) & 15
+                and cache.dtype is torch.uint8 and cache.get_device() == dev and cache.is_contiguous()
+                and block_table.dtype is torch.int32 and block_table.get_device() == dev and block_table.is_contiguous()
+                and kv_lens.dtype is torch.int32 and kv_lens.get_device() == dev and kv_lens.is_contiguous()
+                and kv_lens.shape == (R,))
+    except (AttributeError, TypeError, ValueError):
+        fits = False
+    if not fits:
+        dev = _device_of("q", q)
+        qt, qh = _rows("q", q, dev)
+        N, Hq, D = q.shape
+        _page_size(cache, dev, None, D, groupsize)
+        table, lens = _ints("block_table", block_table, dev, 2), _ints("kv_lens", kv_lens, dev)
+        R, P = block_table.shape
+        if kv_lens.size(0) != R:
+            raise RuntimeError(f"kv_lens has {kv_lens.size(0)} requests, block_table {R}")
+        pages, H, width = cache.shape
+        qp, cp, dtype = q.data_ptr(), cache.data_ptr(), _DTYPES[q.dtype]
+    page = _page_of(width, D, groupsize)
+    if H == 0 or Hq % H:
         raise RuntimeError(f"{Hq} query heads are no multiple of the cache's {H}")
     if cu_q is None:
         cu = 0
@@ -248,7 +314,7 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
         if max_q is None:
             max_q = N
     if max_kv is None:
-        max_kv = block_table.size(1) * page
+        max_kv = P * page
     if out is None:
         out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((N, Hq, D))  # (torch.empty costs the host more)
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous() \
@@ -256,9 +322,9 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
         raise RuntimeError(f"out must be a contiguous, 16-byte aligned {q.dtype} {tuple(q.shape)} tensor on cuda:{dev}")
     lse = torch.empty((N, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     err = _lib.load().marlin_hip_kv4_attention(
-        q.data_ptr(), cache.data_ptr(), table, lens, cu, out.data_ptr(), 0 if lse is None else lse.data_ptr(), N, R,
-        Hq, H, D, qt, qh, page, cache.size(0), block_table.size(1), groupsize, min(max_q, N), max_kv,
-        1.0 / math.sqrt(D) if scale is None else scale, _DTYPES[q.dtype], dev, _raw_stream(dev))
+        qp, cp, table, lens, cu, out.data_ptr(), 0 if lse is None else lse.data_ptr(), N, R, Hq, H, D, qt, qh, page,
+        pages, P, groupsize, min(max_q, N), max_kv, 1.0 / math.sqrt(D) if scale is None else scale, dtype, dev,
+        _raw_stream(dev))
     if err:
         _raise(err)
     return (out, lse) if return_lse else out
