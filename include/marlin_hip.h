@@ -224,9 +224,9 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
                              int page_size, int num_pages, int max_pages, int groupsize, int max_q, int max_kv,
                              float scale, int dtype, int dev, hipStream_t stream);
 
-/* The launch plan of a marlin_hip_kv4_attention call, computed on the host without a GPU
- * (sms <= 0: 256 compute units): out[0] 0 (the split kernel), out[1] workgroups, out[2]
- * splits of the cache's length (> 1: the call uses its stream's split-K scratch). */
+/* The launch plan of a marlin_hip_kv4_attention call of few rows, computed on the host without
+ * a GPU (sms <= 0: 256 compute units): out[0] 0, out[1] workgroups, out[2] whether a request's
+ * cache may be divided among workgroups (the call then uses its stream's split-K scratch). */
 int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, int groupsize, int max_q, int max_kv,
                         int sms, int* out);
 

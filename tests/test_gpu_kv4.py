@@ -539,3 +539,21 @@ def test_more_requests_than_one_launch_takes(long):
     want = ref.attention(p[0].double().numpy(), *p[1:5], D, 1, T)
     out, lse = _run(p, -1, torch.float16, one=not long)
     _check(out, lse, want, torch.float16, f"{R} requests, {long}")
+
+
+# ---- the example: projections, tables, append, attention and read-back in one path ----
+
+
+@pytest.mark.parametrize("args", [[], ["--head-dim", "64", "--groupsize", "32", "--page", "64", "--prompt", "70"],
+                                  ["--requests", "3", "--heads", "8", "--kv-heads", "8", "--prompt", "33", "--steps", "40"]])
+def test_example(args, capsys):
+    """Off by fp16's rounding of p v and of the output (2^-11 each, of sums no larger than
+    twice the largest output) at most."""
+    import importlib.util
+    import pathlib
+    path = pathlib.Path(__file__).resolve().parents[1] / "examples" / "kv4_decode.py"
+    spec = importlib.util.spec_from_file_location("kv4_decode", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    assert module.main(["--check", *args]) <= 4 * 2.0 ** -11
+    assert "tokens/s" in capsys.readouterr().out
