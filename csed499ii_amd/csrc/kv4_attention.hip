@@ -146,6 +146,7 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
   a.max_pages = max_pages;
   a.log_page = 31 - __builtin_clz((unsigned)page_size);
   a.group = group;
+  a.max_q = max_q;
   a.c1 = scale * 1.4426950408889634f;
   const int cus = compute_units(dev);
   const int few_rows = split_rows(requests, kv_heads, head_dim, ng, cus);

@@ -65,7 +65,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   // Heads fastest, so that a head stays on one XCD; a request's last block, the longest, first.
   __shared__ int kinds[kMaxKinds], kind_tiles[kMaxKinds];
   const int head = blockIdx.x % a.kv_heads, index = blockIdx.x / a.kv_heads;
-  auto blocks_of = [&](const Request& q) { return q.n * G > a.max_rows ? (q.n * G + kPromptRows - 1) / kPromptRows : 0; };
+  auto blocks_of = [&](const Request& q) { return rows_of(a, q) > a.max_rows ? (rows_of(a, q) + kPromptRows - 1) / kPromptRows : 0; };
   // tokens that some row of a block sees
   auto end_of = [&](const Request& q, int block) {
     return max(q.kv - q.n + min((block * kPromptRows + kPromptRows - 1) / G, q.n - 1) + 1, 0);
@@ -135,7 +135,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     r = kind / kMaxKinds, block = kind % kMaxKinds;
   }
   const Request rq = request_of(a, r);
-  const int rows = rq.n * G, row0 = block * kPromptRows;
+  const int rows = rows_of(a, rq), row0 = block * kPromptRows;
   const int past = rq.kv - rq.n;
   const int w_row0 = row0 + 32 * wave;
   // tokens that some row of the workgroup, some row of the wave and every row of it sees

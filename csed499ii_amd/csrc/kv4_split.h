@@ -75,6 +75,7 @@ struct AttnArgs {
   int num_pages, max_pages, log_page;
   int first;            // token of request 0 where cu_q is null
   int pieces;           // of the prompt kernel: workgroups a head that fill the machine
+  int max_q;            // a request's later tokens are not computed
   int max_rows;         // requests of at most so many rows a head are the split kernel's, others the prompt kernel's
   int log_kw;           // KW waves of a workgroup share a head (KW HW = kWaves)
   int lead;             // units that a tile counts more than it has
@@ -97,6 +98,9 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
   }
   return q;
 }
+
+// Rows of a head that are computed.
+__device__ __forceinline__ int rows_of(const AttnArgs& a, const Request& q) { return min(q.n, a.max_q) * a.group; }
 
 // Codes of one 32-token step as loaded.  BLOCKS: 8-dim words of a scale group, whose 16
 // MFMA rows are word row / PARTS, part row % PARTS.
@@ -237,7 +241,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
   // ---- the division: every request's tiles are as long as its last one; rows that see
   // nothing take a unit, to write their zeros.  Without scratch, and where the units do
   // not fit 31 bits, tiles count as one and stay whole ----
-  auto blocks_of = [&](const Request& q) { return q.n * G > a.max_rows ? 0 : (q.n * G + 16 - 1) / 16; };
+  auto blocks_of = [&](const Request& q) { return rows_of(a, q) > a.max_rows ? 0 : (rows_of(a, q) + 15) / 16; };
   auto units_of = [&](const Request& q) { return max((q.kv + kStep * KW - 1) >> (kLogStep + a.log_kw), 1) + a.lead; };
   bool divided = a.partial != nullptr;
   uint32_t total, share;
@@ -350,7 +354,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     rq.n = __builtin_amdgcn_readfirstlane(rq.n);
     rq.kv = __builtin_amdgcn_readfirstlane(rq.kv);
     r_begin = __builtin_amdgcn_readfirstlane(r_begin);
-    const int rows = rq.n * G, row_blocks = blocks_of(rq), len = divided ? units_of(rq) : 1;
+    const int rows = rows_of(a, rq), row_blocks = blocks_of(rq), len = divided ? units_of(rq) : 1;
     const int tile = (int)((unit - r_begin) / (uint32_t)len);
     const uint32_t tile_unit = r_begin + (uint32_t)tile * len;
     // the wave's blocks of rows of all heads (it may have none)

@@ -557,3 +557,17 @@ def test_example(args, capsys):
     spec.loader.exec_module(module)
     assert module.main(["--check", *args]) <= 4 * 2.0 ** -11
     assert "tokens/s" in capsys.readouterr().out
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,H,most", [([5, 2, 9], [40, 70, 9], 2, 3), ([700, 3, 400], [700, 90, 600], 6, 300),
+                                                   ([700, 300, 400], [700, 300, 600], 6, 300), ([40, 700], [40, 700], 9, 4)])
+def test_more_new_tokens_than_max_q(q_lens, kv_lens, H, most):
+    """The first max_q tokens of every request are computed, and no other row is touched."""
+    D, T = 64, 16
+    p = _problem(q_lens, kv_lens, H, H, D, -1, T, torch.float16, seed=91)
+    want = ref.attention(p[0].double().numpy(), *p[1:5], D, 1, T)
+    buf = torch.full(p[0].shape, 7.0, dtype=torch.float16, device=DEV)
+    out, lse = _run(p, -1, torch.float16, max_q=most, out=buf)
+    keep = np.concatenate([np.arange(n) < most for n in q_lens])
+    _check(out[torch.from_numpy(keep).to(DEV)], lse[torch.from_numpy(keep).to(DEV)], [w[keep] for w in want], torch.float16, "first")
+    assert (out[torch.from_numpy(~keep).to(DEV)] == 7).all()
