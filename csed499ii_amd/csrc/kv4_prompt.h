@@ -50,11 +50,11 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   constexpr int GU = KU / NG;         // ... per scale group
   constexpr int DT = D / 32;          // MFMAs of 32 dims of the second
   constexpr int BL = D / 8 / NG;      // words of a scale group
-  constexpr int K_BYTES = kTile * D * 2, V_BYTES = K_BYTES, S_BYTES = 2 * NG * kTile * 2;
-  constexpr int BUF = K_BYTES + V_BYTES;  // operands of a tile, two tiles; then the scales of four
+  constexpr int K_BYTES = kTile * D * 2, V_BYTES = K_BYTES, S_BYTES = 2 * NG * kTile * 4;
+  constexpr int BUF = K_BYTES + V_BYTES + S_BYTES;  // operands and scales of a tile
   constexpr int PIECES = kTile * D / 2 / 16;  // 16-byte pieces of K codes, and of V codes
   constexpr int GROUPS = kTile / 16;          // of tokens in one page
-  __shared__ __align__(16) uint8_t lds[2 * BUF + 4 * S_BYTES];
+  __shared__ __align__(16) uint8_t lds[2 * BUF];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -146,10 +146,24 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   typedef __attribute__((address_space(3))) uint8_t lds_u8;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_u8*)lds;
 
+  // Where 64 groups of 16 tokens (16 tiles) from 64 b on begin, one a lane: the table's entries
+  // as they come (a look at once would wait for them and for every load before them), then the
+  // byte offset of the K codes (bit 63: no such page, which is read as the first one and masked).
+  const int tiles = (end + kTile - 1) / kTile;
+  const int t0 = tiles * part / parts, t1 = tiles * (part + 1) / parts;
+  const int32_t* pages = a.table + (size_t)r * a.max_pages;
+  auto entries = [&](int b) { return pages[min((64 * b + lane) * 16, end - 1) >> a.log_page]; };
+  int entry0 = 0, entry1 = 0, entry = 0;  // (here, so that they and Q come together)
+  if (t0 < t1) {
+    entry0 = entries(t0 >> 4);
+    entry1 = entries((t0 >> 4) + 1);
+    entry = entries((t0 >> 4) + 2);
+  }
+
   // ---- Q ----
   const int seen = w_row0 + c < rows ? max(past + min((w_row0 + c) / G, rq.n - 1) + 1, 0) : 0;
   half8_t qf[KU];
-  float c1 = a.c1;
+  float down = 1.f;  // scores per product of the row's operands
   {
     const int row = w_row0 + c, t_row = min(row / G, rq.n - 1), h_row = head * G + row % G;
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(rq.first + t_row) * a.qt +
@@ -177,7 +191,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 #pragma unroll
         for (int i = 0; i < 8; i++) qf[u][i] = (_Float16)__builtin_amdgcn_ldexpf(x[order[i]], e);
       }
-      c1 = __builtin_amdgcn_ldexpf(c1, -e);
+      down = __builtin_amdgcn_ldexpf(1.f, -e);
     } else {
 #pragma unroll
       for (int u = 0; u < KU; u++) {
@@ -189,24 +203,18 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 
   // ---- the codes of a tile: a wave's pieces are all of K or all of V ----
   const Magic magic;
-  const int32_t* pages = a.table + (size_t)r * a.max_pages;
   const uint8_t* const cache = a.cache + (size_t)head * block_bytes<D, NG>(T);
   // a wave's pieces: of K (the first waves) or of V, of one group (D = 128) or of two
   constexpr int KWAVES = PIECES / 64;
   static_assert(2 * KWAVES <= W && (KWAVES == GROUPS || 2 * KWAVES == GROUPS), "");
   const bool is_k = wave < KWAVES, is_v = !is_k && wave < 2 * KWAVES;
 
-  // Where 64 groups (16 tiles) from 64 b on begin, one a lane: the table's entries as they
-  // come (a look at once would wait for them and for every load before them), then the byte
-  // offset of the K codes (bit 63: no such page, which is read as the first one and masked).
-  auto entries = [&](int b) { return pages[min((64 * b + lane) * 16, end - 1) >> a.log_page]; };
   auto places = [&](int b, int entry) {
     const int tok = (64 * b + lane) * 16;
     const bool there = (uint32_t)entry < (uint32_t)a.num_pages;
     const uint64_t at = (uint64_t)(there ? (uint32_t)entry : 0u) * a.page_stride + (uint32_t)(tok & (T - 1)) * (D / 2);
     return there || tok >= end ? at : at | 1ull << 63;
   };
-  int entry = 0;              // of the block of 16 tiles after the one in `then`
   uint64_t now = 0, then = 0;  // of the block of the tile in use, and of the one after
   auto place = [&](int tile, int g, int block_now) {
     const int i = (tile & 15) * GROUPS + g;
@@ -215,6 +223,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
                     (uint32_t)__builtin_amdgcn_readlane((int)v, i));
   };
   u32x4 raw;
+  uint32_t raw_scales;
   auto fetch = [&](int tile, int block_now) {
     if (!is_k && !is_v) return;
     const uint32_t v_off = is_k ? 0u : (uint32_t)T * (D / 2);
@@ -231,11 +240,11 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   const bool s_mine = s_group >= 0 && s_group < GROUPS;
   const uint32_t s_lane = (lane % (8 * NG)) * 4 + (lane / (8 * NG)) * (2 * NG * (uint32_t)T) + (uint32_t)T * D;
   auto fetch_scales = [&](int tile, int block_now) {
+    raw_scales = 0;
     if (s_mine) {
       const uint32_t o = (uint32_t)(tile * kTile + 16 * s_group) & (T - 1);
       const uint8_t* b = place(tile, s_group, block_now) - o * (D / 2 - 2 * NG);
-      if (lane < 16 * NG)
-        dma4(__builtin_amdgcn_readfirstlane(lds_at + 2 * BUF + (tile & 3) * S_BYTES + s_group * (64 * NG)), b + s_lane);
+      if (lane < 16 * NG) raw_scales = *reinterpret_cast<const uint32_t*>(b + s_lane);
     }
   };
   // Slot of token t among a tile's of a K operand: turned by the reader's lane group, so that
@@ -248,6 +257,15 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   asm volatile("" : "+v"(v_to));
   auto unpack = [&](int tile) {
     uint8_t* const to = lds + (tile & 1) * BUF;
+    if (s_mine && lane < 16 * NG) {
+      // fp32, K's with the softmax's factor: a score is one FMA.  (Kept as fp16 for mixed FMAs,
+      // which issue at half the rate, and the factor apart: 168 us where this takes 164, 4096
+      // tokens on 32 heads; with groups of 32 465 and 448, 2048 on 64 and 8 heads of 4096.)
+      const half2_t v = __builtin_bit_cast(half2_t, raw_scales);
+      const float f = lane < 8 * NG ? a.c1 : 1.f;
+      *reinterpret_cast<float2*>(to + K_BYTES + V_BYTES + s_group * (128 * NG) + lane * 8) =
+          make_float2((float)v.x * f, (float)v.y * f);
+    }
     if (is_k) {
       constexpr int PT = D / 32;  // pieces of a token
       const int t = tid / PT;
@@ -274,7 +292,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   };
 
   float16_t O[DT];
-  float M = kNone, L = 0.f, x_top = kNone, shift = 0.f, v_top = 0.f;
+  // M as in kv4_split.h; the scores are taken less `base`, which is M, or 0 before there is one
+  float M = kNone, base = 0.f, top = kNone, L = 0.f, shift = 0.f, v_top = 0.f;
 #pragma unroll
   for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -287,21 +306,21 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   };
   // Scales [group of 16][K, V][quad][NG][4] of tokens 8 b + 4 h + (0 .. 3) of half j.
   auto scale_of = [&](uint32_t scales, int kv, int n, int j, int b) {
-    const int more = (2 * j + b / 2) * (64 * NG) + kv * (32 * NG) + (2 * (b & 1) * NG + n) * 8;
-    return *(const __attribute__((address_space(3))) half4_t*)(uintptr_t)(scales + 8 * NG * h + more);
+    const int more = (2 * j + b / 2) * (128 * NG) + kv * (64 * NG) + (2 * (b & 1) * NG + n) * 16;
+    return *(const __attribute__((address_space(3))) float4_t*)(uintptr_t)(scales + 16 * NG * h + more);
   };
   // The scale of V of token `lane` of the tile, the largest of its groups.
   auto v_of_lane = [&](uint32_t scales) {
-    _Float16 v = (_Float16)0.f;
+    float v = 0.f;
 #pragma unroll
     for (int n = 0; n < NG; n++) {
-      const uint32_t at = scales + (lane >> 4) * (64 * NG) + 32 * NG + (lane >> 2 & 3) * (8 * NG) + (lane & 3) * 2;
-      v = __builtin_fmaxf16(v, *(const __attribute__((address_space(3))) _Float16*)(uintptr_t)(at + n * 8));
+      const uint32_t at = scales + (lane >> 4) * (128 * NG) + 64 * NG + (lane >> 2 & 3) * (16 * NG) + (lane & 3) * 4;
+      v = fmaxf(v, *(const __attribute__((address_space(3))) float*)(uintptr_t)(at + n * 16));
     }
-    return (float)v;
+    return v;
   };
   auto compute = [&](int tile, uint32_t hole) {
-    const uint32_t buf = lds_at + (tile & 1) * BUF, scales = lds_at + 2 * BUF + (tile & 3) * S_BYTES;
+    const uint32_t buf = lds_at + (tile & 1) * BUF, scales = buf + K_BYTES + V_BYTES;
     const uint32_t even[2] = {buf + (h * kTile + k_slot(c, h)) * 16, buf + (h * kTile + k_slot(32 + c, h)) * 16};
     const uint32_t odd[2] = {buf + (h * kTile + k_slot(c, 2 + h)) * 16, buf + (h * kTile + k_slot(32 + c, 2 + h)) * 16};
     float x[2][16];
@@ -317,10 +336,11 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
           S = __builtin_amdgcn_mfma_f32_32x32x16_f16(read16((u & 1 ? odd : even)[j], u * (2 * kTile * 16)), qf[u], S, 0, 0, 0);
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-          const half4_t s = scale_of(scales, 0, n, j, b);
+          const float4_t s = scale_of(scales, 0, n, j, b);
 #pragma unroll
           for (int i = 0; i < 4; i++)
-            x[j][4 * b + i] = __builtin_fmaf(S[4 * b + i], (float)s[i], n == 0 ? 0.f : x[j][4 * b + i]);
+            x[j][4 * b + i] = __builtin_fmaf(TYPE == BF16 ? S[4 * b + i] * down : S[4 * b + i], s[i],
+                                             n == 0 ? -base : x[j][4 * b + i]);
         }
       }
     float vm = v_of_lane(scales);
@@ -339,7 +359,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     float xm = x[0][0];
 #pragma unroll
     for (int i = 1; i < 32; i++) xm = fmaxf(xm, x[i / 16][i % 16]);
-    if (__any(xm > x_top || vm > v_top)) {
+    if (__any(xm > top || vm > v_top)) {
       const Pair px = across32(xm);
       xm = fmaxf(px.a, px.b);
 #pragma unroll
@@ -351,13 +371,16 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
       }
       const float old_max = M == kNone ? kNone : M + shift;
-      const float new_max = fmaxf(old_max, xm * c1);
-      const float new_M = new_max <= kNone ? kNone : new_max - new_shift;
-      const float f = M == kNone ? 0.f : __builtin_amdgcn_exp2f(M - new_M);
+      const float new_max = fmaxf(old_max, xm + base);
+      const float new_M = new_max <= kNone ? kNone : new_max - new_shift, new_base = new_max <= kNone ? 0.f : new_M;
+      const float f = M == kNone ? 0.f : __builtin_amdgcn_exp2f(M - new_M), less = new_base - base;
       M = new_M;
+      base = new_base;
       shift = new_shift;
-      x_top = M == kNone ? kNone : (new_max + kSlack) * __builtin_amdgcn_rcpf(c1);
+      top = M == kNone ? kNone : shift + kSlack;
       L *= f;
+#pragma unroll
+      for (int i = 0; i < 32; i++) x[i / 16][i % 16] -= less;
 #pragma unroll
       for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -368,7 +391,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     for (int j = 0; j < 2; j++) {
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        x[j][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(x[j][i], c1, -M));
+        x[j][i] = __builtin_amdgcn_exp2f(x[j][i]);
         L += x[j][i];
       }
 #pragma unroll
@@ -376,11 +399,10 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         u32x4 P[2];  // fp16 pairs
 #pragma unroll
         for (int b = 0; b < 4; b++) {
-          const half4_t s = scale_of(scales, 1, n, j, b);
+          const float4_t s = scale_of(scales, 1, n, j, b);
 #pragma unroll
           for (int i = 0; i < 4; i += 2)
-            P[b >> 1][2 * (b & 1) + i / 2] = pack2(__builtin_fmaf(x[j][4 * b + i], (float)s[i], 0.f),
-                                                   __builtin_fmaf(x[j][4 * b + i + 1], (float)s[i + 1], 0.f));
+            P[b >> 1][2 * (b & 1) + i / 2] = pack2(x[j][4 * b + i] * s[i], x[j][4 * b + i + 1] * s[i + 1]);
         }
         if (masked) {  // what a row does not see is zero, whatever its scale
 #pragma unroll
@@ -397,18 +419,14 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     }
   };
 
-  const int tiles = (end + kTile - 1) / kTile;
-  const int t0 = tiles * part / parts, t1 = tiles * (part + 1) / parts;
   if (t0 < t1) {
     const int b0 = t0 >> 4;
-    now = places(b0, entries(b0));
-    then = places(b0 + 1, entries(b0 + 1));
-    entry = entries(b0 + 2);
+    now = places(b0, entry0);
+    then = places(b0 + 1, entry1);
     uint64_t missing = __ballot((int64_t)now < 0);  // groups of the block whose page is not there
     fetch(t0, b0);
     fetch_scales(t0, b0);
     unpack(t0);
-    sm24::wait_vm<0>();  // the first tile's scales
     fetch_scales(t0 + 1, b0);
     fetch(t0 + 1, b0);
     __syncthreads();
@@ -425,9 +443,6 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         compute(tile, (uint32_t)(missing >> ((tile & 15) * GROUPS)) & ((1u << GROUPS) - 1));
       if (tile + 1 < t1) {
         unpack(tile + 1);
-        // the next tile's scales are there: sent before its codes, which the unpacking waited
-        // for, or the only loads of a wave without codes
-        if (!is_k && !is_v) sm24::wait_vm<0>();
         fetch_scales(tile + 2, b);
         fetch(tile + 2, b);
       }
@@ -467,13 +482,13 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     if ((int)__builtin_amdgcn_readfirstlane(arrived) != parts) return;
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
     if (out_lane == 0) __hip_atomic_store(a.counters + first, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    float top = M;
+    float most = M;
     for (int p = 0; p < parts; p += 8) {
       float m[8];  // (those past the last repeat it)
 #pragma unroll
       for (int i = 0; i < 8; i++) m[i] = ml[(size_t)(first + min(p + i, parts - 1) * stride) * 128];
 #pragma unroll
-      for (int i = 0; i < 8; i++) top = fmaxf(top, m[i]);
+      for (int i = 0; i < 8; i++) most = fmaxf(most, m[i]);
     }
     float16_t sum[DT];
 #pragma unroll
@@ -489,12 +504,12 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       float4_t v[DT * 4];
 #pragma unroll
       for (int i = 0; i < DT * 4; i++) v[i] = *reinterpret_cast<const float4_t*>(o + i * 256);
-      const float f = __builtin_amdgcn_exp2f(x.x - top);
+      const float f = __builtin_amdgcn_exp2f(x.x - most);
       l += f * x.y;
 #pragma unroll
       for (int i = 0; i < DT * 16; i++) sum[i / 16][i % 16] = __builtin_fmaf(v[i / 4][i % 4], f, sum[i / 16][i % 16]);
     }
-    M = top;
+    M = most;
 #pragma unroll
     for (int t = 0; t < DT; t++) O[t] = sum[t];
   }
