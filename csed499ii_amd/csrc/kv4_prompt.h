@@ -63,7 +63,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 
   // ---- the piece: which request's, which block of rows, which part of its tokens ----
   // Heads fastest, so that a head stays on one XCD; a request's last block, the longest, first.
-  __shared__ int kinds[kMaxKinds], kind_tiles[kMaxKinds];
+  __shared__ __align__(16) int kinds[kMaxKinds], kind_tiles[kMaxKinds];
   const int head = blockIdx.x % a.kv_heads, index = blockIdx.x / a.kv_heads;
   auto blocks_of = [&](const Request& q) { return rows_of(a, q) > a.max_rows ? (rows_of(a, q) + kPromptRows - 1) / kPromptRows : 0; };
   // tokens that some row of a block sees
@@ -101,36 +101,59 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     // Divided: parts of (nearly) one length, the shortest of 64 that give no more parts than
     // there are workgroups for this head.
     if (wave == 0) {
-      int i = before;
-      for (int r = r_lane; r < min(r_lane + per, a.requests); r++) {
-        const Request q = request_of(a, r);
-        for (int b = blocks_of(q) - 1; b >= 0; b--, i++) {
-          kinds[i] = r * kMaxKinds + b;
-          kind_tiles[i] = max((end_of(q, b) + kTile - 1) / kTile, 1);
+      // a request after the other, its blocks over the lanes
+      for (uint64_t with = __ballot(own > 0); with != 0; with &= with - 1) {
+        const int at = __builtin_ctzll(with);
+        int i = __builtin_amdgcn_readlane(before, at);
+        for (int r = at * per; r < min(at * per + per, a.requests); r++) {
+          const Request q = request_of(a, r);
+          const int n = blocks_of(q);
+          for (int b = lane; b < n; b += 64) {
+            kinds[i + b] = r * kMaxKinds + n - 1 - b;
+            kind_tiles[i + b] = max((end_of(q, n - 1 - b) + kTile - 1) / kTile, 1);
+          }
+          i += n;
         }
       }
     }
     __syncthreads();
+    int tiles_of[4];  // of the kinds 4 lane + (0 .. 3)
     float sum = 0.f, longest = 0.f;
-    for (int i = 0; i < all; i++) {
-      sum += (float)kind_tiles[i];
-      longest = fmaxf(longest, (float)kind_tiles[i]);
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      tiles_of[k] = 4 * lane + k < all ? kind_tiles[4 * lane + k] : 0;
+      sum += (float)tiles_of[k];
+      longest = fmaxf(longest, (float)tiles_of[k]);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      sum += __shfl_xor(sum, d);
+      longest = fmaxf(longest, __shfl_xor(longest, d));
     }
     const float lo = fmaxf(fmaxf(sum / (float)a.pieces, kMinShare), longest / (float)kMaxParts), hi = fmaxf(lo, longest);
     const float per_tile = 1.f / (lo + (hi - lo) * ((float)(lane + 1) / 64.f));
     auto parts_of = [&](int tiles, float f) { return max((int)ceilf((float)tiles * f - 0.001f), 1); };
     int n = 0;
-    for (int i = 0; i < all; i++) n += parts_of(kind_tiles[i], per_tile);
+    for (int i = 0; i < all; i += 4) {
+      const int4 t = *reinterpret_cast<const int4*>(kind_tiles + i);
+      n += parts_of(t.x, per_tile) + (i + 1 < all ? parts_of(t.y, per_tile) : 0) +
+           (i + 2 < all ? parts_of(t.z, per_tile) : 0) + (i + 3 < all ? parts_of(t.w, per_tile) : 0);
+    }
     const float f = __builtin_bit_cast(
         float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, per_tile), __builtin_ctzll(__ballot(n <= a.pieces || lane == 63))));
+    int parts_to[5] = {0};  // of this lane's kinds, up to each
+#pragma unroll
+    for (int k = 0; k < 4; k++) parts_to[k + 1] = parts_to[k] + (tiles_of[k] > 0 ? parts_of(tiles_of[k], f) : 0);
+    const int ahead = scan(parts_to[4]);
+    const uint64_t past_it = __ballot(ahead + parts_to[4] > index);
+    if (past_it == 0) return;
+    const int at = __builtin_ctzll(past_it), left = index - __builtin_amdgcn_readlane(ahead, at);
     int i = 0;
-    part = index;
-    for (; i < all; i++) {
-      parts = __builtin_amdgcn_readfirstlane(parts_of(kind_tiles[i], f));
-      if (part < parts) break;
-      part -= parts;
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+      const int from = __builtin_amdgcn_readlane(parts_to[k], at), to = __builtin_amdgcn_readlane(parts_to[k + 1], at);
+      if (left >= from && left < to) i = 4 * at + k, part = left - from, parts = to - from;
     }
-    if (i == all) return;
     const int kind = __builtin_amdgcn_readfirstlane(kinds[i]);
     r = kind / kMaxKinds, block = kind % kMaxKinds;
   }
