@@ -186,7 +186,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   // ---- Q ----
   const int seen = w_row0 + c < rows ? max(past + min((w_row0 + c) / G, rq.n - 1) + 1, 0) : 0;
   half8_t qf[KU];
-  float down = 1.f;  // scores per product of the row's operands
+  float down = 1.f, up = 1.f;  // scores per product of the row's operands (a power of two), and back
   {
     const int row = w_row0 + c, t_row = min(row / G, rq.n - 1), h_row = head * G + row % G;
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(rq.first + t_row) * a.qt +
@@ -215,6 +215,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         for (int i = 0; i < 8; i++) qf[u][i] = (_Float16)__builtin_amdgcn_ldexpf(x[order[i]], e);
       }
       down = __builtin_amdgcn_ldexpf(1.f, -e);
+      up = __builtin_amdgcn_ldexpf(1.f, e);
     } else {
 #pragma unroll
       for (int u = 0; u < KU; u++) {
@@ -315,7 +316,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   };
 
   float16_t O[DT];
-  // M as in kv4_split.h; the scores are taken less `base`, which is M, or 0 before there is one
+  // M as in kv4_split.h; the scores, in units of `down`, are taken less `base`, which is M, or
+  // 0 before there is one, and M rises where one passes `top`
   float M = kNone, base = 0.f, top = kNone, L = 0.f, shift = 0.f, v_top = 0.f;
 #pragma unroll
   for (int t = 0; t < DT; t++)
@@ -362,8 +364,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
           const float4_t s = scale_of(scales, 0, n, j, b);
 #pragma unroll
           for (int i = 0; i < 4; i++)
-            x[j][4 * b + i] = __builtin_fmaf(TYPE == BF16 ? S[4 * b + i] * down : S[4 * b + i], s[i],
-                                             n == 0 ? -base : x[j][4 * b + i]);
+            x[j][4 * b + i] = __builtin_fmaf(S[4 * b + i], s[i], n == 0 ? -base : x[j][4 * b + i]);
         }
       }
     float vm = v_of_lane(scales);
@@ -394,13 +395,13 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
       }
       const float old_max = M == kNone ? kNone : M + shift;
-      const float new_max = fmaxf(old_max, xm + base);
-      const float new_M = new_max <= kNone ? kNone : new_max - new_shift, new_base = new_max <= kNone ? 0.f : new_M;
+      const float new_max = fmaxf(old_max, (xm + base) * down);
+      const float new_M = new_max <= kNone ? kNone : new_max - new_shift, new_base = new_max <= kNone ? 0.f : new_M * up;
       const float f = M == kNone ? 0.f : __builtin_amdgcn_exp2f(M - new_M), less = new_base - base;
       M = new_M;
       base = new_base;
       shift = new_shift;
-      top = M == kNone ? kNone : shift + kSlack;
+      top = M == kNone ? kNone : (shift + kSlack) * up;
       L *= f;
 #pragma unroll
       for (int i = 0; i < 32; i++) x[i / 16][i % 16] -= less;
@@ -414,7 +415,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     for (int j = 0; j < 2; j++) {
 #pragma unroll
       for (int i = 0; i < 16; i++) {
-        x[j][i] = __builtin_amdgcn_exp2f(x[j][i]);
+        x[j][i] = __builtin_amdgcn_exp2f(x[j][i] * down);
         L += x[j][i];
       }
 #pragma unroll
