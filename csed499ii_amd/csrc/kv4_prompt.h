@@ -9,14 +9,23 @@
 //   O^T = V^T P^T  A = V from LDS, B = p v, whose reduction index counts those tokens: p
 //                  stays in its lane
 // Sixteen tokens lie in one page, and are what a wave loads at once: the page is the wave's,
-// so that a tile costs it a few scalar operations and one load; the scales go to LDS as
-// they are (LDS-DMA), and are fp16 operands of mixed-precision FMAs.
+// so that a tile costs it a few scalar operations and one load.
 //
-// Measured on this part: a wave issues an operation of any kind every 4.1 to 4.8 cycles, two
-// waves of a SIMD in parallel; an MFMA takes its 32 cycles and hides nearly no other
-// operation of either wave (32 + 2.1 n cycles for one beside n of the vector ALU, with two
-// waves).  So what counts is operations per score, of any kind, and neither LDS (254 of
-// 256 bytes a clock with eight waves) nor the order of products and softmax.
+// Bound by issue: a wave issues an operation of any kind every 4.1 to 4.8 cycles, two waves of
+// a SIMD in parallel, and an MFMA takes its 32 cycles and hides nearly no other operation of
+// either wave (32 + 2.1 n cycles for one beside n of the vector ALU, with two waves).  So what
+// counts is operations per score, of any kind, and neither LDS (254 of 256 bytes a clock with
+// eight waves) nor the order of products and softmax.  A tile of 128 dims takes 4400 cycles:
+// 2048 of MFMAs, some 1600 of vector operations at their rates, the rest waits.  4096 tokens
+// on 32 heads of 128 dims: 164 us, 840 TFLOP/s, where a large library product reaches 1161.
+// Tried: four waves and 128 rows (198), 32-token tiles and three workgroups a compute unit
+// (232), scales as fp16 in mixed FMAs (168), products and softmax of two tiles interleaved
+// (186 to 191); 64 dims in 128 registers, for two workgroups a compute unit, spill.
+//
+// Fewer blocks of rows than compute units are divided over their tokens, one part a
+// workgroup; the waves of the same rows meet in the uncached scratch, and the last to arrive
+// adds the parts in order.  A 512-token chunk on 64 and 8 heads with 4096 in all: 151 us
+// whole, 100 in two parts, whose write and read take 6.
 #pragma once
 #include "kv4_split.h"
 

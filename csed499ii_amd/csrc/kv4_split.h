@@ -37,6 +37,13 @@
 // entry is not a page, slots never written (their scales may be NaN).  Their p v is set to
 // zero after the product, not multiplied by zero.
 //
+// Bound by HBM where the cache is long and one block of rows reads it: 64 requests of 1024 to
+// 16384 tokens on 8 heads of 128 dims, eight query heads each, take 128 us, 4.6 TB/s of the
+// 5.1 that a large copy reaches.  From two blocks on, by the unpacking, which every block
+// repeats (12 requests of five tokens, 40 rows, 4096 in all: 47 us, 36 at 24 rows).  Short ones
+// by latencies one after the other (lengths, table, codes, the meeting): one request of 1000
+// tokens on 32 heads, 10.3 us.
+//
 // The waves meet in LDS; the partial sums of a divided tile go through the uncached
 // scratch, and the last of its workgroups to arrive on its counter adds them in order: one
 // launch, and the same bits from run to run.
@@ -115,7 +122,9 @@ struct Shape {
   static constexpr int V_AT = kStep * D / 2, S_AT = kStep * D, STAGE = S_AT + 128 * NG;
   static constexpr int LOADS = D / 32 + (NG == 4 ? 2 : 1);  // DMA instructions of a step
   // 128 registers let two workgroups share a compute unit.  With several groups of 128 dims
-  // V's codes and scales do not fit them, and are read from LDS as they are needed.
+  // V's codes and scales do not fit them, and are read from LDS as they are needed (12 requests
+  // of five tokens with groups of 32: 53.5 us; all at once, one workgroup a unit and four
+  // steps in flight, 56.6).
   static constexpr bool LATE = NG > 1 && D == 128;
   static constexpr int RING = 2;  // steps of a wave in flight or in use
 };
