@@ -214,7 +214,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       }
       const Pair p = across32(amax);
       amax = fmaxf(p.a, p.b);
-      const int e = amax > 0.f && amax < __builtin_inff() ? 8 - __builtin_amdgcn_frexp_expf(amax) : 0;
+      // (2^100 where all is so small that its scores are zero anyway)
+      const int e = amax > 0.f && amax < __builtin_inff() ? min(8 - __builtin_amdgcn_frexp_expf(amax), 100) : 0;
 #pragma unroll
       for (int u = 0; u < KU; u++) {
         float x[8];
@@ -403,13 +404,17 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         new_shift = fminf(kVTop - (float)__builtin_amdgcn_frexp_expf(vm), 24.f);
         v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
       }
-      const float old_max = M == kNone ? kNone : M + shift;
-      const float new_max = fmaxf(old_max, (xm + base) * down);
-      const float new_M = new_max <= kNone ? kNone : new_max - new_shift, new_base = new_max <= kNone ? 0.f : new_M * up;
-      const float f = M == kNone ? 0.f : __builtin_amdgcn_exp2f(M - new_M), less = new_base - base;
-      M = new_M;
+      // the largest so far lies at `shift`, a larger one of this tile comes to new_shift.  Where
+      // scores are so large that base's rounding would move it by more than the slack, it is
+      // the tile's that stay together.
+      const bool none = M == kNone, risen = none ? xm > -__builtin_inff() : xm > shift * up;
+      const float new_base = base + (risen ? xm - new_shift * up : none ? 0.f : (shift - new_shift) * up);
+      float less = new_base - base;
+      if (risen) less = __builtin_amdgcn_fmed3f(less, xm - (new_shift + kSlack) * up, xm - (new_shift - kSlack) * up);
+      const float f = none ? 0.f : __builtin_amdgcn_exp2f(-less * down);
       base = new_base;
       shift = new_shift;
+      M = none && !risen ? kNone : base * down;
       top = M == kNone ? kNone : (shift + kSlack) * up;
       L *= f;
 #pragma unroll

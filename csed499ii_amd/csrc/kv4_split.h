@@ -63,6 +63,7 @@ constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last wo
 constexpr int kMaxRequests = 2 * 64 * kWaves;  // of a launch that divides by the requests' lengths
 constexpr float kSlack = 8.f;      // p <= 2^8 of the reference
 constexpr float kVTop = 7.f;       // v 2^shift <= 2^7, so p v <= 2^15 < 65504
+constexpr float kBig = 1 << 20;    // of a row's largest score, in log2 units
 constexpr float kNone = -1.0e30f;  // reference of a row that has seen nothing
 
 struct AttnArgs {
@@ -423,6 +424,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
 
     // ---- the loop ----
     float4_t O[NG][S::OPS];
+    bool big = false, some_big = false;       // the row, some row
     float M = kNone, L = 0.f, x_top = kNone;  // x_top: x above which M rises
     float shift = 0.f, v_top = 0.f;  // v 2^shift <= 2^kVTop while v <= v_top
 #pragma unroll
@@ -560,13 +562,19 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
           v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
         }
         const float m = column_max(xm);
-        // M = max - shift: rows keep the larger of the old maximum and this step's
+        // M = max - shift: rows keep the larger of the old maximum and this step's.  Past kBig,
+        // where M's rounding would show, scores are taken less the largest one, x_top.
         const float old_max = M == kNone ? kNone : M + shift;
-        const float new_max = fmaxf(old_max, m * c1);
+        const bool risen = big ? m > x_top : m * c1 > old_max;
+        const float new_max = risen ? m * c1 : old_max;
         const float new_M = new_max <= kNone ? kNone : new_max - new_shift;
-        const float f = M == kNone ? 0.f : __builtin_amdgcn_exp2f(M - new_M);
+        const float f = M == kNone ? 0.f
+                        : __builtin_amdgcn_exp2f(big ? __builtin_fmaf(risen ? x_top - m : 0.f, c1, new_shift - shift) : M - new_M);
+        if (risen) big = fabsf(new_max) > kBig;
+        if (!big) x_top = new_M == kNone ? kNone : (new_max + kSlack) * __builtin_amdgcn_rcpf(c1);
+        else if (risen) x_top = m;
         M = new_M;
-        x_top = new_M == kNone ? kNone : (new_max + kSlack) * __builtin_amdgcn_rcpf(c1);
+        some_big = __any(big);
         L *= f;
 #pragma unroll
         for (int n = 0; n < NG; n++)
@@ -575,9 +583,19 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
         shift = new_shift;
       }
       half8_t P[NG];
+      if (some_big) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float v = x[i / 4][i % 4];
+          x[i / 4][i % 4] = big ? __builtin_fmaf(v - x_top, c1, shift) : __builtin_fmaf(v, c1, -M);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i / 4][i % 4] = __builtin_fmaf(x[i / 4][i % 4], c1, -M);
+      }
 #pragma unroll
       for (int i = 0; i < 8; i++) {
-        const float p = __builtin_amdgcn_exp2f(__builtin_fmaf(x[i / 4][i % 4], c1, -M));
+        const float p = __builtin_amdgcn_exp2f(x[i / 4][i % 4]);
         L += p;
         if constexpr (S::LATE) {
           x[i / 4][i % 4] = p;

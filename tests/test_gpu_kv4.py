@@ -571,3 +571,26 @@ def test_more_new_tokens_than_max_q(q_lens, kv_lens, H, most):
     keep = np.concatenate([np.arange(n) < most for n in q_lens])
     _check(out[torch.from_numpy(keep).to(DEV)], lse[torch.from_numpy(keep).to(DEV)], [w[keep] for w in want], torch.float16, "first")
     assert (out[torch.from_numpy(~keep).to(DEV)] == 7).all()
+
+
+@pytest.mark.parametrize("gain", [1e-39, 1e-36, 1e-20, 1e20, 1e30])
+@pytest.mark.parametrize("q_lens,kv_lens,H", [([1, 1], [300, 40], 2), ([170, 90], [260, 90], 9)])
+def test_tiny_and_huge_bf16_queries(q_lens, kv_lens, H, gain):
+    """Queries near the type's limits: scores that are all zero, or one token that takes all."""
+    D, g, T = 128, 64, 16
+    p = list(_problem(q_lens, kv_lens, H, H, D, g, T, torch.bfloat16, seed=101))
+    p[0] = (p[0].double() * gain).to(torch.bfloat16)
+    want = ref.attention(p[0].double().numpy(), *p[1:5], D, p[5], T)
+    out, _ = _run(p, g, torch.bfloat16)
+    _check(out, None, want, torch.bfloat16, f"q times {gain}")
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,H", [([1, 1], [700, 40], 2), ([5], [300], 4), ([170, 90], [260, 90], 9)])
+def test_scores_at_fp16_limits(q_lens, kv_lens, H):
+    """Queries and keys of tens of thousands, values of hundreds: scores of 10^11, one token takes all."""
+    D, T = 128, 16
+    p = _problem(q_lens, kv_lens, H, H, D, -1, T, torch.float16, seed=102, k_gain=1e4, v_gain=300.0)
+    p = (p[0] * 1e4, *p[1:])
+    want = ref.attention(p[0].double().numpy(), *p[1:5], D, 1, T)
+    out, lse = _run(p, -1, torch.float16)
+    _check(out, lse, want, torch.float16, "limits", x_max=1e12)
