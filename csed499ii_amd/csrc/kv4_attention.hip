@@ -104,6 +104,10 @@ int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, i
                         int sms, int* out) {
   const int err = kv4::check(0, requests, q_heads, kv_heads, head_dim, 16, 1, 0, groupsize, max_q, max_kv, 1.f, 0);
   if (err != MARLIN_HIP_OK) return err;
+  // (a launch takes so many requests, and of each so many rows)
+  if (requests > kv4::kMaxRequests) requests = kv4::kMaxRequests;
+  const int most_q = 256 / (q_heads / kv_heads) > 1 ? 256 / (q_heads / kv_heads) : 1;
+  if (max_q > most_q) max_q = most_q;
   const kv4::Plan p = kv4::plan(requests, q_heads, kv_heads, head_dim, kv4::groups(head_dim, groupsize), max_q, max_kv, sms > 0 ? sms : 256);
   out[0] = 0;
   out[1] = p.workgroups;

@@ -350,7 +350,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 #pragma unroll
     for (int n = 0; n < NG; n++) {
       const uint32_t at = scales + (lane >> 4) * (128 * NG) + 64 * NG + (lane >> 2 & 3) * (16 * NG) + (lane & 3) * 4;
-      v = fmaxf(v, *(const __attribute__((address_space(3))) float*)(uintptr_t)(at + n * 16));
+      v = fmaxf(v, fabsf(*(const __attribute__((address_space(3))) float*)(uintptr_t)(at + n * 16)));
     }
     return v;
   };
