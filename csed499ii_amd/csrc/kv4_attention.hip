@@ -179,6 +179,7 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
       const Plan p = plan(a.requests, q_heads, kv_heads, head_dim, ng, split_q, max_kv, cus);
       a.log_kw = p.log_kw;
       a.lead = p.lead;
+      a.slots = 2 * cus;
       if (p.split) {
         const size_t rows = (size_t)p.workgroups * 2 * 16 * (kWaves >> p.log_kw);
         err = sm24::get_scratch(dev, stream, rows * (head_dim + 2) * sizeof(float), &a.counters, &a.partial);

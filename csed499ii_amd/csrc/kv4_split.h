@@ -59,6 +59,12 @@ constexpr int kLogStep = 5, kStep = 1 << kLogStep;  // tokens per wave and step
 // (24 requests of 17 to 4096 tokens on 32 heads: 87.0 us with none, 58.0 with 2, 59.5 with 4;
 // 64 of 1024 to 16384 on 8: 134.6, 130.7, 129.7; one of 131072: 40.2, 37.8, 37.3).
 constexpr int kLead = 2;
+// Units that a whole tile may take beyond an even share before tiles are divided: what the
+// meeting of the pieces costs.  16 requests of 1000 tokens on 8 heads (four units) 17.1 us
+// divided, 14.7 whole; four of 1000, 40 rows on 20 heads, 24.8 and 16.4; one of 1000 on 32
+// heads, which stays divided, 10.7 and 12.3.
+constexpr int kWhole = 3;
+constexpr int kTilesAt = 43;       // bit of a sum of units
 constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last workgroup's read of it
 constexpr int kMaxRequests = 2 * 64 * kWaves;  // of a launch that divides by the requests' lengths
 constexpr float kSlack = 8.f;      // p <= 2^8 of the reference
@@ -86,6 +92,7 @@ struct AttnArgs {
   int max_q;            // a request's later tokens are not computed
   int max_rows;         // requests of at most so many rows a head are the split kernel's, others the prompt kernel's
   int log_kw;           // KW waves of a workgroup share a head (KW HW = kWaves)
+  int slots;            // workgroups that fill the machine
   int lead;             // units that a tile counts more than it has
   int group;            // query heads of a kv head
   float c1;             // softmax scale * log2 e
@@ -96,7 +103,9 @@ struct Request {
 };
 __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
   Request q;
-  q.kv = min(max(a.kv_lens[r], 0), a.max_pages << a.log_page);  // (at most 2^30)
+  int cap = a.max_pages << a.log_page;  // (at most 2^30)
+  asm volatile("" : "+s"(cap));         // (else kept in a vector register all the while)
+  q.kv = min(max(a.kv_lens[r], 0), cap);
   if (a.cu_q == nullptr) {
     q.first = a.first + r;
     q.n = 1;
@@ -265,14 +274,15 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     int longest = 1;
     auto cost = [&](const Request& q) {
       long long n = ((long long)blocks_of(q) * a.kv_heads + HW - 1) >> (kLogWaves - a.log_kw);
-      if (divided) {
+      if (divided) {  // units, and above them tiles: as many as the sums have room for
         if (n > 0) longest = max(longest, units_of(q));
-        n *= units_of(q);
+        n = min(n * units_of(q), 1ll << 32) + (min(n, 1023ll) << kTilesAt);
       }
       return n;
     };
     if (few) {
       mine[0] = cost(own);
+      if (__ballot(mine[0] > 0) == 0) return;  // beside prompts, no request of few rows
     } else {
 #pragma unroll
       for (int u = 0; u < 2; u++)
@@ -314,12 +324,22 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
       begins[2 * tid + 1] = (uint32_t)(before + mine[0]);
       __syncthreads();
     }
-    if (divided && __builtin_amdgcn_readfirstlane((int)(all > 0x7FFFFFFFll))) {
-      divided = false;
-      continue;
+    if (divided) {
+      const long long tiles = all >> kTilesAt, units = all & ((1ll << kTilesAt) - 1);
+      // tiles stay whole, one a workgroup, where none takes much more than an even share
+      const bool whole = tiles <= gridDim.x &&
+                         (longest - a.lead - kWhole) * (long long)a.slots <= units - tiles * a.lead;
+      if (__builtin_amdgcn_readfirstlane((int)(whole || units > 0x7FFFFFFFll))) {
+        divided = false;
+        continue;
+      }
+      all = units;
     }
     total = __builtin_amdgcn_readfirstlane((uint32_t)all);
     share = (total + gridDim.x - 1) / gridDim.x;
+    // pieces of one unit: no more than one a compute unit (one request of 4000 tokens on 32
+    // heads 16.3 us with two, 13.3 so)
+    if (divided && share == 1 && total > (uint32_t)a.slots / 2) share = 2;
     // a tile lies in kMaxSplits shares at most
     if (divided) share = max(share, (uint32_t)((longest + kMaxSplits - 2) / (kMaxSplits - 1)));
     share = __builtin_amdgcn_readfirstlane(share);
