@@ -15,13 +15,13 @@ hipError_t launch_prompt(const AttnArgs& a, int workgroups, int head_dim, int ng
 // Requests of at most so many rows (new tokens times the query heads of a kv head) go to the
 // split kernel, the others to the prompt kernel, each of which passes over the other's.  The
 // split kernel's time grows with the rows, the prompt kernel's is the same up to 256: 12
-// requests of 4096 tokens on 8 heads of 128 dims, 64, 80, 96 and 128 rows, 57, 64, 74 and 87
-// us beside 67 to 69; with groups of 32, which cost the prompt kernel most, 65, 78, 91 and 108
-// beside 148, and 160 beside 165 at 192.  Few tiles leave the prompt kernel's large parts
-// waiting: one request of 8192 tokens, 24 us beside 34 at 64 rows, 41 beside 59 at 256.
+// requests of 4096 tokens on 8 heads of 128 dims, 64, 80, 96 and 128 rows, 54, 58, 74 and 87
+// us beside 67 to 69; with groups of 32, 128, 144 and 160 rows, 118, 134 and 142 beside 133.
+// Few tiles leave the prompt kernel's large parts waiting: one request of 8192 tokens, 24 us
+// beside 34 at 64 rows, 41 beside 59 at 256.
 int split_rows(int requests, int kv_heads, int head_dim, int ng, int cus) {
   if ((long long)requests * kv_heads <= cus / 16) return 256;
-  return head_dim == 128 && ng == 4 ? 160 : 80;
+  return head_dim == 128 && ng == 4 ? 144 : 80;
 }
 constexpr int kPromptTile = 64;
 

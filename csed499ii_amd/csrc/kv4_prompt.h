@@ -63,6 +63,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   constexpr int BUF = K_BYTES + V_BYTES + S_BYTES;  // operands and scales of a tile
   constexpr int PIECES = kTile * D / 2 / 16;  // 16-byte pieces of K codes, and of V codes
   constexpr int GROUPS = kTile / 16;          // of tokens in one page
+  constexpr int HALVES = NG == 4 ? 1 : 2;     // of a tile whose scores are held at once (four
+                                              // groups: 439 us with both, 367; two: 268, 285)
   __shared__ __align__(16) uint8_t lds[2 * BUF];
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -358,101 +360,107 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     const uint32_t buf = lds_at + (tile & 1) * BUF, scales = buf + K_BYTES + V_BYTES;
     const uint32_t even[2] = {buf + (h * kTile + k_slot(c, h)) * 16, buf + (h * kTile + k_slot(32 + c, h)) * 16};
     const uint32_t odd[2] = {buf + (h * kTile + k_slot(c, 2 + h)) * 16, buf + (h * kTile + k_slot(32 + c, 2 + h)) * 16};
-    float x[2][16];
-#pragma unroll
-    for (int j = 0; j < 2; j++)
-#pragma unroll
-      for (int n = 0; n < NG; n++) {
-        float16_t S;
-#pragma unroll
-        for (int i = 0; i < 16; i++) S[i] = 0.f;
-#pragma unroll
-        for (int u = n * GU; u < (n + 1) * GU; u++)
-          S = __builtin_amdgcn_mfma_f32_32x32x16_f16(read16((u & 1 ? odd : even)[j], u * (2 * kTile * 16)), qf[u], S, 0, 0, 0);
-#pragma unroll
-        for (int b = 0; b < 4; b++) {
-          const float4_t s = scale_of(scales, 0, n, j, b);
-#pragma unroll
-          for (int i = 0; i < 4; i++)
-            x[j][4 * b + i] = __builtin_fmaf(S[4 * b + i], s[i], n == 0 ? -base : x[j][4 * b + i]);
-        }
-      }
-    float vm = v_of_lane(scales);
     const bool masked = (tile + 1) * kTile > w_all || hole != 0;
-    if (masked) {
-      vm = tile * kTile + lane < w_end && !(hole >> (lane >> 4) & 1) ? vm : 0.f;
+    float vm = 0.f;
 #pragma unroll
-      for (int j = 0; j < 2; j++)
+    for (int j0 = 0; j0 < 2; j0 += HALVES) {
+      float x[HALVES][16];
+#pragma unroll
+      for (int jj = 0; jj < HALVES; jj++)
+#pragma unroll
+        for (int n = 0; n < NG; n++) {
+          const int j = j0 + jj;
+          float16_t S;
+#pragma unroll
+          for (int i = 0; i < 16; i++) S[i] = 0.f;
+#pragma unroll
+          for (int u = n * GU; u < (n + 1) * GU; u++)
+            S = __builtin_amdgcn_mfma_f32_32x32x16_f16(read16((u & 1 ? odd : even)[j], u * (2 * kTile * 16)), qf[u], S, 0, 0, 0);
+#pragma unroll
+          for (int b = 0; b < 4; b++) {
+            const float4_t s = scale_of(scales, 0, n, j, b);
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              x[jj][4 * b + i] = __builtin_fmaf(S[4 * b + i], s[i], n == 0 ? -base : x[jj][4 * b + i]);
+          }
+        }
+      if (j0 == 0) vm = v_of_lane(scales);
+      if (masked) {
+        vm = tile * kTile + lane < w_end && !(hole >> (lane >> 4) & 1) ? vm : 0.f;
+#pragma unroll
+        for (int jj = 0; jj < HALVES; jj++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) {
+            const int j = j0 + jj, t = 32 * j + 8 * (i / 4) + 4 * h + i % 4;
+            const bool in = tile * kTile + t < seen && !(hole >> (2 * j + i / 8) & 1);
+            x[jj][i] = in ? x[jj][i] : -__builtin_inff();
+          }
+      }
+      float xm = x[0][0];
+#pragma unroll
+      for (int i = 1; i < 16 * HALVES; i++) xm = fmaxf(xm, x[i / 16][i % 16]);
+      if (__any(xm > top || vm > v_top)) {
+        const Pair px = across32(xm);
+        xm = fmaxf(px.a, px.b);
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) vm = fmaxf(vm, __shfl_xor(vm, d));
+        float new_shift = shift;
+        if (vm > v_top) {
+          // vm <= 2^e; 2^24 bounds the shift where every v so far is tiny
+          new_shift = fminf(kVTop - (float)__builtin_amdgcn_frexp_expf(vm), 24.f);
+          v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
+        }
+        // the largest so far lies at `shift`, a larger one of this tile comes to new_shift.  Where
+        // scores are so large that base's rounding would move it by more than the slack, it is
+        // the tile's that stay together.
+        const bool none = M == kNone, risen = none ? xm > -__builtin_inff() : xm > shift * up;
+        const float new_base = base + (risen ? xm - new_shift * up : none ? 0.f : (shift - new_shift) * up);
+        float less = new_base - base;
+        if (risen) less = __builtin_amdgcn_fmed3f(less, xm - (new_shift + kSlack) * up, xm - (new_shift - kSlack) * up);
+        const float f = none ? 0.f : __builtin_amdgcn_exp2f(-less * down);
+        base = new_base;
+        shift = new_shift;
+        M = none && !risen ? kNone : base * down;
+        top = M == kNone ? kNone : (shift + kSlack) * up;
+        L *= f;
+#pragma unroll
+        for (int i = 0; i < 16 * HALVES; i++) x[i / 16][i % 16] -= less;
+#pragma unroll
+        for (int t = 0; t < DT; t++)
+#pragma unroll
+          for (int i = 0; i < 16; i++) O[t][i] *= f;
+      }
+      const uint32_t v_at = buf + K_BYTES + (h * D + c) * 16;
+#pragma unroll
+      for (int jj = 0; jj < HALVES; jj++) {
+        const int j = j0 + jj;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-          const int t = 32 * j + 8 * (i / 4) + 4 * h + i % 4;
-          const bool in = tile * kTile + t < seen && !(hole >> (2 * j + i / 8) & 1);
-          x[j][i] = in ? x[j][i] : -__builtin_inff();
-        }
-    }
-    float xm = x[0][0];
-#pragma unroll
-    for (int i = 1; i < 32; i++) xm = fmaxf(xm, x[i / 16][i % 16]);
-    if (__any(xm > top || vm > v_top)) {
-      const Pair px = across32(xm);
-      xm = fmaxf(px.a, px.b);
-#pragma unroll
-      for (int d = 1; d < 64; d <<= 1) vm = fmaxf(vm, __shfl_xor(vm, d));
-      float new_shift = shift;
-      if (vm > v_top) {
-        // vm <= 2^e; 2^24 bounds the shift where every v so far is tiny
-        new_shift = fminf(kVTop - (float)__builtin_amdgcn_frexp_expf(vm), 24.f);
-        v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
-      }
-      // the largest so far lies at `shift`, a larger one of this tile comes to new_shift.  Where
-      // scores are so large that base's rounding would move it by more than the slack, it is
-      // the tile's that stay together.
-      const bool none = M == kNone, risen = none ? xm > -__builtin_inff() : xm > shift * up;
-      const float new_base = base + (risen ? xm - new_shift * up : none ? 0.f : (shift - new_shift) * up);
-      float less = new_base - base;
-      if (risen) less = __builtin_amdgcn_fmed3f(less, xm - (new_shift + kSlack) * up, xm - (new_shift - kSlack) * up);
-      const float f = none ? 0.f : __builtin_amdgcn_exp2f(-less * down);
-      base = new_base;
-      shift = new_shift;
-      M = none && !risen ? kNone : base * down;
-      top = M == kNone ? kNone : (shift + kSlack) * up;
-      L *= f;
-#pragma unroll
-      for (int i = 0; i < 32; i++) x[i / 16][i % 16] -= less;
-#pragma unroll
-      for (int t = 0; t < DT; t++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) O[t][i] *= f;
-    }
-    const uint32_t v_at = buf + K_BYTES + (h * D + c) * 16;
-#pragma unroll
-    for (int j = 0; j < 2; j++) {
-#pragma unroll
-      for (int i = 0; i < 16; i++) {
-        x[j][i] = __builtin_amdgcn_exp2f(x[j][i] * down);
-        L += x[j][i];
-      }
-#pragma unroll
-      for (int n = 0; n < NG; n++) {
-        u32x4 P[2];  // fp16 pairs
-#pragma unroll
-        for (int b = 0; b < 4; b++) {
-          const float4_t s = scale_of(scales, 1, n, j, b);
-#pragma unroll
-          for (int i = 0; i < 4; i += 2)
-            P[b >> 1][2 * (b & 1) + i / 2] = pack2(x[j][4 * b + i] * s[i], x[j][4 * b + i + 1] * s[i + 1]);
-        }
-        if (masked) {  // what a row does not see is zero, whatever its scale
-#pragma unroll
-          for (int i = 0; i < 16; i += 2)
-            P[i / 8][i % 8 / 2] &= (x[j][i] == 0.f ? 0u : 0xFFFFu) | (x[j][i + 1] == 0.f ? 0u : 0xFFFF0000u);
+          x[jj][i] = __builtin_amdgcn_exp2f(x[jj][i] * down);
+          L += x[jj][i];
         }
 #pragma unroll
-        for (int s = 0; s < 2; s++)
+        for (int n = 0; n < NG; n++) {
+          u32x4 P[2];  // fp16 pairs
 #pragma unroll
-          for (int t = n * (DT / NG); t < (n + 1) * (DT / NG); t++)
-            O[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read16(v_at, ((2 * j + s) * 2 * D + 32 * t) * 16),
-                                                          __builtin_bit_cast(half8_t, P[s]), O[t], 0, 0, 0);
+          for (int b = 0; b < 4; b++) {
+            const float4_t s = scale_of(scales, 1, n, j, b);
+#pragma unroll
+            for (int i = 0; i < 4; i += 2)
+              P[b >> 1][2 * (b & 1) + i / 2] = pack2(x[jj][4 * b + i] * s[i], x[jj][4 * b + i + 1] * s[i + 1]);
+          }
+          if (masked) {  // what a row does not see is zero, whatever its scale
+#pragma unroll
+            for (int i = 0; i < 16; i += 2)
+              P[i / 8][i % 8 / 2] &= (x[jj][i] == 0.f ? 0u : 0xFFFFu) | (x[jj][i + 1] == 0.f ? 0u : 0xFFFF0000u);
+          }
+#pragma unroll
+          for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int t = n * (DT / NG); t < (n + 1) * (DT / NG); t++)
+              O[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read16(v_at, ((2 * j + s) * 2 * D + 32 * t) * 16),
+                                                            __builtin_bit_cast(half8_t, P[s]), O[t], 0, 0, 0);
+        }
       }
     }
   };
