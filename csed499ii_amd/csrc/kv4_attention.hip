@@ -39,6 +39,7 @@ int compute_units(int dev) {
 struct Plan {
   int workgroups, log_kw, lead, pieces;
   bool split;  // a tile may be divided: the call needs scratch
+  bool rest;
 };
 
 // Two workgroups of eight waves fill a compute unit, one where their registers and rings are
@@ -77,7 +78,10 @@ Plan prompt_plan(int tokens, int requests, int q_heads, int kv_heads, int max_q,
   Plan p{};
   p.pieces = cus / kv_heads;
   p.split = max_kv > kPromptTile && p.pieces > 1;
-  const long long w = (p.split && kinds < p.pieces ? p.pieces : kinds) * kv_heads;
+  // (of one fresh prompt the last blocks see few tokens: 65 us whole, 69 with workgroups for
+  // them, 1500 tokens on 64 and 8 heads)
+  p.rest = p.split && kinds > p.pieces && (requests > 1 || max_kv >= 2ll * max_q);
+  const long long w = (p.rest ? kinds + p.pieces : p.split && kinds < p.pieces ? p.pieces : kinds) * kv_heads;
   p.workgroups = w > 0x7FFFFF ? -1 : (int)w;
   return p;
 }
@@ -165,6 +169,7 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
       const Plan p = prompt_plan(tokens, a.requests, q_heads, kv_heads, max_q, max_kv, a.max_rows, cus);
       if (p.workgroups < 0) return refuse("kv4_attention: too many rows for one launch");
       a.pieces = p.pieces;
+      a.rest = p.rest;
       if (p.split) {
         const size_t rows = (size_t)p.pieces * kv_heads * kPromptRows;
         err = sm24::get_scratch(dev, stream, (rows * head_dim + 2 * rows * 2) * sizeof(float), &a.counters, &a.partial);

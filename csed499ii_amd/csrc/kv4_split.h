@@ -89,6 +89,7 @@ struct AttnArgs {
   int num_pages, max_pages, log_page;
   int first;            // token of request 0 where cu_q is null
   int pieces;           // of the prompt kernel: workgroups a head that fill the machine
+  bool rest;            // whether its grid has as many more, to divide the last blocks
   int max_q;            // a request's later tokens are not computed
   int max_rows;         // requests of at most so many rows a head are the split kernel's, others the prompt kernel's
   int log_kw;           // KW waves of a workgroup share a head (KW HW = kWaves)

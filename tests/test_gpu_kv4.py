@@ -594,3 +594,20 @@ def test_scores_at_fp16_limits(q_lens, kv_lens, H):
     want = ref.attention(p[0].double().numpy(), *p[1:5], D, 1, T)
     out, lse = _run(p, -1, torch.float16)
     _check(out, lse, want, torch.float16, "limits", x_max=1e12)
+
+
+@pytest.mark.parametrize("D,g,T", [(128, -1, 16), (128, 32, 32), (64, 64, 16)])
+def test_more_blocks_of_rows_than_compute_units(D, g, T):
+    """Whole blocks for every unit and a few more, which are divided over their tokens: the
+    rows of the first and the last request against 64 bits, all of them run to run."""
+    H, R, n, kv = 64, 5, 90, 700  # 320 blocks of 90 rows
+    p = _problem([n] * R, [kv] * R, H, H, D, g, T, torch.float16, seed=111)
+    first, lse = _run(p, g, torch.float16)
+    q, cache, table, kvs, cu, G = p
+    for i, h in ((0, 0), (0, 63), (4, 0), (4, 31), (4, 63)):
+        sl = slice(n * i, n * (i + 1))
+        want = ref.attention(q[sl, h:h + 1].double().numpy(), cache[:, h:h + 1], table[i:i + 1], kvs[i:i + 1], [0, n], D, G, T)
+        _check(first[sl, h:h + 1], lse[sl, h:h + 1], want, torch.float16, f"request {i} head {h}")
+    for _ in range(3):
+        again, lse2 = _run(p, g, torch.float16)
+        assert torch.equal(first, again) and torch.equal(lse, lse2)
