@@ -17,9 +17,9 @@
 // counts is operations per score, of any kind, and neither LDS (254 of 256 bytes a clock with
 // eight waves) nor the order of products and softmax.  A tile of 128 dims takes 4400 cycles:
 // 2048 of MFMAs, some 1600 of vector operations at their rates, the rest waits.  4096 tokens
-// on 32 heads of 128 dims: 164 us, 840 TFLOP/s, where a large library product reaches 1161.
+// on 32 heads of 128 dims: 160 us, 860 TFLOP/s, where a large library product reaches 1161.
 // Tried: four waves and 128 rows (198), 32-token tiles and three workgroups a compute unit
-// (232), scales as fp16 in mixed FMAs (168), products and softmax of two tiles interleaved
+// (232), scales as fp16 in mixed FMAs (168 where this took 164), products and softmax of two tiles interleaved
 // (186 to 191); 64 dims in 128 registers, for two workgroups a compute unit, spill.
 //
 // Fewer blocks of rows than compute units are divided over their tokens, one part a
