@@ -23,7 +23,6 @@ int split_rows(int requests, int kv_heads, int head_dim, int ng, int cus) {
   if ((long long)requests * kv_heads <= cus / 16) return 256;
   return head_dim == 128 && ng == 4 ? 144 : 80;
 }
-constexpr int kPromptTile = 64;
 
 // (the query takes the host 0.2 us of each call, so its answer is kept)
 int compute_units(int dev) {
@@ -39,17 +38,16 @@ int compute_units(int dev) {
 struct Plan {
   int workgroups, log_kw, lead, pieces;
   bool split;  // a tile may be divided: the call needs scratch
-  bool rest;
+  bool rest;   // the prompt kernel's last blocks, too, where they are few
 };
 
-// Two workgroups of eight waves fill a compute unit, one where their registers and rings are
-// larger (Shape::TWO).  All eight waves take one block of 16 rows, and meet in LDS; a piece of
-// it costs its write and read in memory, fewer where the waves are together (one request of
-// 131072 tokens on 8 heads: 37.8 us with eight, 59 with four, 107 with two; 64 requests of
+// Two workgroups of eight waves fill a compute unit.  All eight waves take one block of 16
+// rows and meet in LDS: a piece of a block costs its write and read in memory, and so there
+// are few (one request of 131072 tokens on 8 heads: 37.8 us with eight, 59 with four, 107 with two; 64 requests of
 // 4096: 57, 64, 70).  From two blocks a workgroup on, a workgroup goes through many short
 // ones instead, and two waves take a block (64 requests of 4096 tokens on 32 heads: 232 us
 // with eight, 229 with four, 219 with two; 200 of 1000: 220, 196, 189).
-Plan plan(int requests, int q_heads, int kv_heads, int head_dim, int ng, int max_q, int max_kv, int cus) {
+Plan plan(int requests, int q_heads, int kv_heads, int max_q, int max_kv, int cus) {
   Plan p{};
   const long long row_blocks = ((long long)max_q * (q_heads / kv_heads) + 15) / 16;
   const long long steps = ((long long)max_kv + kStep - 1) / kStep;
@@ -68,8 +66,6 @@ Plan plan(int requests, int q_heads, int kv_heads, int head_dim, int ng, int max
 // The prompt kernel: a workgroup of eight waves fills a compute unit.  Fewer tiles (256 rows
 // of a head) than compute units are divided over their tokens on the device, which knows the
 // lengths; this is the grid, which bounds the tiles by the tokens.
-constexpr int kPromptRows = 256, kPromptWaves = 8;
-
 Plan prompt_plan(int tokens, int requests, int q_heads, int kv_heads, int max_q, int max_kv, int max_rows, int cus) {
   const long long group = q_heads / kv_heads, rows = tokens * group;
   long long kinds = rows / kPromptRows + (requests < rows / (max_rows + 1) ? requests : rows / (max_rows + 1));
@@ -77,7 +73,7 @@ Plan prompt_plan(int tokens, int requests, int q_heads, int kv_heads, int max_q,
   if (kinds > most) kinds = most;
   Plan p{};
   p.pieces = cus / kv_heads;
-  p.split = max_kv > kPromptTile && p.pieces > 1;
+  p.split = max_kv > kTile && p.pieces > 1;
   // (of one fresh prompt the last blocks see few tokens: 65 us whole, 69 with workgroups for
   // them, 1500 tokens on 64 and 8 heads)
   p.rest = p.split && kinds > p.pieces && (requests > 1 || max_kv >= 2ll * max_q);
@@ -112,7 +108,7 @@ int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, i
   if (requests > kv4::kMaxRequests) requests = kv4::kMaxRequests;
   const int most_q = 256 / (q_heads / kv_heads) > 1 ? 256 / (q_heads / kv_heads) : 1;
   if (max_q > most_q) max_q = most_q;
-  const kv4::Plan p = kv4::plan(requests, q_heads, kv_heads, head_dim, kv4::groups(head_dim, groupsize), max_q, max_kv, sms > 0 ? sms : 256);
+  const kv4::Plan p = kv4::plan(requests, q_heads, kv_heads, max_q, max_kv, sms > 0 ? sms : 256);
   out[0] = 0;
   out[1] = p.workgroups;
   out[2] = p.split;
@@ -174,14 +170,14 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
         const size_t rows = (size_t)p.pieces * kv_heads * kPromptRows;
         err = sm24::get_scratch(dev, stream, (rows * head_dim + 2 * rows * 2) * sizeof(float), &a.counters, &a.partial);
         if (err != MARLIN_HIP_OK) return err;
-        if (a.partial) a.partial_ml = a.partial + rows * head_dim;  // (a null: see below)
+        if (a.partial) a.partial_ml = a.partial + rows * head_dim;  // (null: blocks stay whole)
       }
       err = sm24::launch_error(launch_prompt(a, p.workgroups, head_dim, ng, dtype, stream));
       if (err != MARLIN_HIP_OK) return err;
       a.partial = nullptr;
     }
     if (split) {
-      const Plan p = plan(a.requests, q_heads, kv_heads, head_dim, ng, split_q, max_kv, cus);
+      const Plan p = plan(a.requests, q_heads, kv_heads, split_q, max_kv, cus);
       a.log_kw = p.log_kw;
       a.lead = p.lead;
       a.slots = 2 * cus;

@@ -31,9 +31,6 @@
 
 namespace kv4 {
 
-constexpr int kTile = 64;       // tokens
-constexpr int kPromptWaves = 8;
-constexpr int kPromptRows = 32 * kPromptWaves;
 constexpr int kMaxKinds = 256;     // row blocks of a launch whose tokens are divided
 constexpr int kMaxParts = 32;      // of a row block's tokens
 constexpr float kMinShare = 4.f;   // tiles: a part costs its write and its read

@@ -66,6 +66,8 @@ constexpr int kLead = 2;
 constexpr int kWhole = 3;
 constexpr int kTilesAt = 43;       // bit of a sum of units
 constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last workgroup's read of it
+constexpr int kTile = 64;          // tokens of a tile of the prompt kernel
+constexpr int kPromptWaves = 8, kPromptRows = 32 * kPromptWaves;
 constexpr int kMaxRequests = 2 * 64 * kWaves;  // of a launch that divides by the requests' lengths
 constexpr float kSlack = 8.f;      // p <= 2^8 of the reference
 constexpr float kVTop = 7.f;       // v 2^shift <= 2^7, so p v <= 2^15 < 65504
@@ -80,9 +82,9 @@ struct AttnArgs {
   const int32_t* cu_q;  // null: request i is token i
   void* out;
   float* lse;           // null: not wanted
-  float* partial;       // [workgroup][first, last][row][D]; null: no tile is divided
-  float* partial_ml;    // [workgroup][first, last][row][2]: reference and sum
-  uint32_t* counters;   // [workgroup], zero between launches
+  float* partial;       // [workgroup][first, last][row][D] (prompt kernel: [part][wave][..]); null: no tile is divided
+  float* partial_ml;    // as many pairs of a reference and a sum
+  uint32_t* counters;   // [workgroup] (prompt kernel: [block of rows][wave]), zero between launches
   long long qt, qh;     // strides of q in elements
   int tokens, requests, q_heads, kv_heads;
   uint32_t page_stride; // bytes of a page, all heads
