@@ -127,6 +127,8 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
   if ((q_token_stride | q_head_stride) & 7) return refuse("kv4_attention needs strides that are multiples of 8 elements");
   if (num_pages < 1) return refuse("kv4_attention needs a cache of at least one page");
   if (tokens == 0 || requests == 0 || max_q == 0) return MARLIN_HIP_OK;
+  // (request i is token i: its row of q, and of the output, must be there)
+  if (cu_q == nullptr && tokens < requests) return refuse("kv4_attention without cu_q needs a token for every request");
   sm24::DeviceScope scope(dev);
   if (!scope.ok) return MARLIN_HIP_ERR_LAUNCH;
   AttnArgs a{};

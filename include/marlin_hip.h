@@ -210,7 +210,8 @@ int marlin_hip_kv4_gather(const void* cache, const void* slots, void* k, void* v
                           hipStream_t stream);
 
 /* Causal attention.  q [tokens][q_heads][head_dim] (strides in elements, multiples of 8)
- * holds request i's new tokens at [cu_q[i], cu_q[i + 1]) (cu_q null: one a request); they
+ * holds request i's new tokens at [cu_q[i], cu_q[i + 1]) (cu_q null: token i, and fewer
+ * tokens than requests are refused); they
  * are the last of its kv_lens[i] tokens, in the pages block_table[i][max_pages] (entries
  * outside [0, num_pages): left out; max_pages * page_size at most 2^30).  out is contiguous
  * [tokens][q_heads][head_dim]; lse fp32 [tokens][q_heads] or null.  A row that sees no token:
