@@ -121,6 +121,9 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
                              int page_size, int num_pages, int max_pages, int groupsize, int max_q, int max_kv,
                              float scale, int dtype, int dev, hipStream_t stream) {
   using namespace kv4;
+  // (a bound that may be far above what there is, e.g. a fixed one of all steps: the choice of
+  // kernels and their grids go by rows that exist)
+  if (tokens >= 0 && max_q > tokens) max_q = tokens;
   int err = check(tokens, requests, q_heads, kv_heads, head_dim, page_size, num_pages, max_pages, groupsize, max_q,
                   max_kv, scale, dtype);
   if (err != MARLIN_HIP_OK) return err;
