@@ -76,7 +76,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   auto blocks_of = [&](const Request& q) { return rows_of(a, q) > a.max_rows ? (rows_of(a, q) + kPromptRows - 1) / kPromptRows : 0; };
   // tokens that some row of a block sees
   auto end_of = [&](const Request& q, int block) {
-    return max(q.kv - q.n + min((block * kPromptRows + kPromptRows - 1) / G, q.n - 1) + 1, 0);
+    return seen_by(q, min((block * kPromptRows + kPromptRows - 1) / G, q.n - 1));
   };
   const int per = (a.requests + 63) / 64, r_lane = lane * per;  // a lane's requests
   int own = 0;
@@ -180,7 +180,6 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   }
   const Request rq = request_of(a, r);
   const int rows = rows_of(a, rq), row0 = block * kPromptRows;
-  const int past = rq.kv - rq.n;
   const int w_row0 = row0 + 32 * wave;
   // tokens that some row of the workgroup, some row of the wave and every row of it sees
   const int end = end_of(rq, block);
@@ -188,8 +187,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     parts = max(min(most, (end + kTile - 1) / (kTile * (int)kMinShare)), 1);
     if (part >= parts) return;
   }
-  const int w_end = w_row0 < rows ? max(past + min((w_row0 + 31) / G, rq.n - 1) + 1, 0) : 0;
-  const int w_all = min(max(past + w_row0 / G + 1, 0), w_end);
+  const int w_end = w_row0 < rows ? seen_by(rq, min((w_row0 + 31) / G, rq.n - 1)) : 0;
+  const int w_all = min(seen_by(rq, w_row0 / G), w_end);
 
   typedef __attribute__((address_space(3))) uint8_t lds_u8;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_u8*)lds;
@@ -209,7 +208,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   }
 
   // ---- Q ----
-  const int seen = w_row0 + c < rows ? max(past + min((w_row0 + c) / G, rq.n - 1) + 1, 0) : 0;
+  const int seen = w_row0 + c < rows ? seen_by(rq, min((w_row0 + c) / G, rq.n - 1)) : 0;
   half8_t qf[KU];
   float down = 1.f, up = 1.f;  // scores per product of the row's operands (a power of two), and back
   {

@@ -102,22 +102,32 @@ struct AttnArgs {
 };
 
 struct Request {
-  int first, n, kv;  // first token, new tokens, tokens in all
+  int first, n, kv;  // first token, new tokens in q, tokens in all that the table covers
+  int past;          // position of the first new token
 };
 __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
   Request q;
   int cap = a.max_pages << a.log_page;  // (at most 2^30)
   asm volatile("" : "+s"(cap));         // (else kept in a vector register all the while)
-  q.kv = min(max(a.kv_lens[r], 0), cap);
+  const int kv = max(a.kv_lens[r], 0);
+  q.kv = min(kv, cap);
+  int n = 1;
   if (a.cu_q == nullptr) {
     q.first = a.first + r;
     q.n = 1;
   } else {
-    q.first = min(max(a.cu_q[r], 0), a.tokens);
-    q.n = max(min(a.cu_q[r + 1], a.tokens) - q.first, 0);
+    const int begin = max(a.cu_q[r], 0), end = max(a.cu_q[r + 1], 0);
+    n = max(end - begin, 0);
+    q.first = min(begin, a.tokens);
+    q.n = max(min(end, a.tokens) - q.first, 0);
   }
+  // positions go by the lengths as they are: what the table or q cuts off moves no token
+  q.past = min(kv - n, 1 << 30);
   return q;
 }
+
+// Tokens that new token t sees.
+__device__ __forceinline__ int seen_by(const Request& q, int t) { return max(min(q.past + t + 1, q.kv), 0); }
 
 // Rows of a head that are computed.
 __device__ __forceinline__ int rows_of(const AttnArgs& a, const Request& q) { return min(q.n, a.max_q) * a.group; }
@@ -248,7 +258,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
   static_assert(S::RING * S::STAGE >= 16 * (D + 4) * 4 && S::RING * S::STAGE >= 16 * (kMaxSplits + 2) * 4, "");
   __shared__ __align__(16) uint8_t lds[kWaves * S::RING * S::STAGE];
   __shared__ uint32_t begins[kMaxRequests];
-  __shared__ int few_first[64], few_n[64], few_kv[64];
+  __shared__ int few_first[64], few_n[64], few_kv[64], few_past[64];
   __shared__ long long wave_sum[kWaves];
   __shared__ int wave_max[kWaves];
   __shared__ uint32_t arrived;
@@ -270,7 +280,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
   // Up to 64 requests are one to a lane, in every wave alike, and found by a ballot; more
   // are two to a thread and searched for.
   const bool few = a.requests <= 64;
-  Request own{0, 0, 0};
+  Request own{0, 0, 0, 0};
   if (few && lane < a.requests) own = request_of(a, lane);
   while (true) {
     long long mine[2] = {0, 0};
@@ -307,7 +317,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
             (uint32_t)__builtin_amdgcn_readlane((int)sum, at);
       if (wave == 0) {
         begins[lane] = (uint32_t)before;
-        few_first[lane] = own.first, few_n[lane] = own.n, few_kv[lane] = own.kv;
+        few_first[lane] = own.first, few_n[lane] = own.n, few_kv[lane] = own.kv, few_past[lane] = own.past;
       }
       __syncthreads();
     } else {
@@ -372,7 +382,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     if (few) {
       const int i = lane_again();
       r = 63 - __builtin_clzll(__ballot(i < a.requests && begins[i] <= unit));
-      rq = Request{few_first[r], few_n[r], few_kv[r]};
+      rq = Request{few_first[r], few_n[r], few_kv[r], few_past[r]};
     } else {
       for (int hi = a.requests; hi - r > 1;) {
         const int mid = (r + hi) >> 1;
@@ -386,6 +396,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     rq.first = __builtin_amdgcn_readfirstlane(rq.first);
     rq.n = __builtin_amdgcn_readfirstlane(rq.n);
     rq.kv = __builtin_amdgcn_readfirstlane(rq.kv);
+    rq.past = __builtin_amdgcn_readfirstlane(rq.past);
     r_begin = __builtin_amdgcn_readfirstlane(r_begin);
     const int rows = rows_of(a, rq), row_blocks = blocks_of(rq), len = divided ? units_of(rq) : 1;
     const int tile = (int)((unit - r_begin) / (uint32_t)len);
@@ -394,11 +405,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     const int own_block = tile * HW + hw, own = min(own_block, row_blocks * a.kv_heads - 1);
     const bool exists = own == own_block;
     const int head = row_blocks == 1 ? own : own / row_blocks, row0 = (own - head * row_blocks) * 16;
-    const int past = rq.kv - rq.n;  // token t sees tokens 0 .. past + t
     const bool one = rq.n == 1;  // (spares the divisions of a row's index)
     const int t_first = one ? 0 : row0 / G, t_last = one ? 0 : min((row0 + 15) / G, rq.n - 1);
-    const int end = max(past + t_last + 1, 0);             // tokens that some row of the tile sees
-    const int all = min(max(past + t_first + 1, 0), end);  // ... that every row sees
+    const int end = seen_by(rq, t_last);   // tokens that some row of the tile sees
+    const int all = seen_by(rq, t_first);  // ... that every row sees
     const int steps = (end + kStep - 1) / kStep;
     // this wave's steps: s0, s0 + KW, ... (the tile's first units are its lead)
     const uint32_t next_unit = min(tile_unit + len, last_unit), work_unit = tile_unit + (divided ? a.lead : 0);
@@ -418,7 +428,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     half8_t qf[S::KW];
     float c1 = a.c1;
     const int row = row0 + c, t_row = one ? 0 : row / G, h_row = one ? min(row, G - 1) : row - t_row * G;
-    const int seen = row < rows ? max(past + t_row + 1, 0) : 0;  // tokens the row sees
+    const int seen = row < rows ? seen_by(rq, t_row) : 0;  // tokens the row sees
     float x[S::KW][8];
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(rq.first + min(t_row, rq.n - 1)) * a.qt +
                           (long long)(head * G + h_row) * a.qh + 8 * g;
