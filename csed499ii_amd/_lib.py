@@ -43,6 +43,7 @@ SIGNATURES = {
     "marlin_hip_kv4_append": (_i, [_vp] * 4 + [_i] * 3 + [_ll] * 4 + [_i] * 5 + [_vp]),
     "marlin_hip_kv4_gather": (_i, [_vp] * 4 + [_i] * 8 + [_vp]),
     "marlin_hip_kv4_attention": (_i, [_vp] * 7 + [_i] * 5 + [_ll] * 2 + [_i] * 6 + [_f, _i, _i, _vp]),
+    "marlin_hip_kv4_attention_ctx": (_i, [_vp] * 8 + [_i] * 5 + [_ll] * 2 + [_i] * 6 + [_f, _i, _i, _vp]),
     "marlin_hip_kv4_plan": (_i, [_i] * 8 + [ctypes.POINTER(_i)]),
     "marlin_hip_last_error": (ctypes.c_char_p, []),
 }

@@ -115,11 +115,11 @@ int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, i
   return MARLIN_HIP_OK;
 }
 
-int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block_table, const void* kv_lens,
-                             const void* cu_q, void* out, void* lse, int tokens, int requests, int q_heads,
-                             int kv_heads, int head_dim, long long q_token_stride, long long q_head_stride,
-                             int page_size, int num_pages, int max_pages, int groupsize, int max_q, int max_kv,
-                             float scale, int dtype, int dev, hipStream_t stream) {
+int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* block_table, const void* kv_lens,
+                                 const void* cu_q, const void* context_lens, void* out, void* lse, int tokens,
+                                 int requests, int q_heads, int kv_heads, int head_dim, long long q_token_stride,
+                                 long long q_head_stride, int page_size, int num_pages, int max_pages, int groupsize,
+                                 int max_q, int max_kv, float scale, int dtype, int dev, hipStream_t stream) {
   using namespace kv4;
   // (a bound that may be far above what there is, e.g. a fixed one of all steps: the choice of
   // kernels and their grids go by rows that exist)
@@ -140,6 +140,7 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
   a.table = static_cast<const int32_t*>(block_table);
   a.kv_lens = static_cast<const int32_t*>(kv_lens);
   a.cu_q = static_cast<const int32_t*>(cu_q);
+  a.ctx = static_cast<const int32_t*>(context_lens);
   a.out = out;
   a.lse = static_cast<float*>(lse);
   a.qt = q_token_stride;
@@ -206,8 +207,19 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
     a.kv_lens += a.requests;
     a.table += (size_t)a.requests * max_pages;
     if (a.cu_q) a.cu_q += a.requests;
+    if (a.ctx) a.ctx += a.requests;
   }
   return MARLIN_HIP_OK;
+}
+
+int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block_table, const void* kv_lens,
+                             const void* cu_q, void* out, void* lse, int tokens, int requests, int q_heads,
+                             int kv_heads, int head_dim, long long q_token_stride, long long q_head_stride,
+                             int page_size, int num_pages, int max_pages, int groupsize, int max_q, int max_kv,
+                             float scale, int dtype, int dev, hipStream_t stream) {
+  return marlin_hip_kv4_attention_ctx(q, cache, block_table, kv_lens, cu_q, nullptr, out, lse, tokens, requests,
+                                      q_heads, kv_heads, head_dim, q_token_stride, q_head_stride, page_size, num_pages,
+                                      max_pages, groupsize, max_q, max_kv, scale, dtype, dev, stream);
 }
 
 }  // extern "C"

@@ -80,6 +80,7 @@ struct AttnArgs {
   const int32_t* table;
   const int32_t* kv_lens;
   const int32_t* cu_q;  // null: request i is token i
+  const int32_t* ctx;   // positions of the first new tokens; null: the new ones are the last of kv_lens
   void* out;
   float* lse;           // null: not wanted
   float* partial;       // [workgroup][first, last][row][D] (prompt kernel: [part][wave][..]); null: no tile is divided
@@ -122,7 +123,7 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
     q.n = max(min(end, a.tokens) - q.first, 0);
   }
   // positions go by the lengths as they are: what the table or q cuts off moves no token
-  q.past = min(kv - n, 1 << 30);
+  q.past = min(a.ctx != nullptr ? max(a.ctx[r], 0) : kv - n, 1 << 30);
   return q;
 }
 

@@ -14,7 +14,7 @@ One decoding step of a layer, for requests in a batch::
 
     slots, cu, kv_lens, used = kv4_tables(context_lens, new_lens, free_pages, block_table, tokens, T)
     kv4_append(k, v, cache, slots)
-    out = kv4_attention(q, cache, block_table, kv_lens, cu, max_q=..., max_kv=...)
+    out = kv4_attention(q, cache, block_table, kv_lens, cu, max_q=..., max_kv=..., context_lens=context_lens)
 
 The tables are made once a step and serve all layers.  Everything runs on the current
 stream of the tensors' device and nothing waits for the GPU.
@@ -132,12 +132,14 @@ def kv4_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: t
     * ``slots [num_tokens]``: the slot of each new token, for :func:`kv4_append`; -1 past the
       last one, where ``free_pages`` has run out and where the table is full;
     * ``cu_new [R + 1]``: the first new token of each request, and their number;
-    * ``kv_lens [R]``: ``context + new``, cut at the table's ``P * page_size``;
+    * ``kv_lens [R]``: ``context + new``, cut at the table's ``P * page_size`` (where that may
+      happen :func:`kv4_attention` needs ``context_lens``, too, for the positions);
     * ``pages_used [1]``: pages wanted from ``free_pages``.  More than ``F`` means that some
       requests have entries of -1 in the table, whose tokens :func:`kv4_attention` leaves out.
 
     ``num_tokens`` is the length of the slot map, an upper bound known on the host (a
-    captured step may pass its padded size); tokens past it get no slot and no page.
+    captured step may pass its padded size); tokens past it get no slot and no page, but count
+    in ``cu_new``, ``kv_lens`` and ``pages_used``.
     Lengths below zero count as zero.  The sum of ``new_lens`` must stay below 2^31.
     """
     try:  # (as in kv4_append)
@@ -252,14 +254,17 @@ def kv4_gather(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, groupsiz
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
                   cu_q: torch.Tensor | None = None, max_q: int | None = None, max_kv: int | None = None,
                   groupsize: int = -1, scale: float | None = None, return_lse: bool = False,
-                  out: torch.Tensor | None = None):
+                  out: torch.Tensor | None = None, context_lens: torch.Tensor | None = None):
     """Causal attention of new tokens over the requests' cached rows, theirs included.
 
     ``q [tokens, q_heads, D]`` (fp16 or bf16; a view as in :func:`kv4_append`) holds the new
     tokens request by request: those of request ``i`` are ``q[cu_q[i]:cu_q[i + 1]]`` (int32
-    ``[R + 1]``; None: one token a request).  They are the last of its ``kv_lens[i]`` (int32
-    ``[R]``) tokens, whose rows lie in the pages ``block_table[i]`` (int32 ``[R, P]``); the
-    token at position ``p`` sees the positions up to ``p``.  ``q_heads`` is a multiple of the
+    ``[R + 1]``; None: one token a request).  Their positions start at ``context_lens[i]``
+    (int32 ``[R]``; None: they are the last of the ``kv_lens[i]`` tokens).  The request has
+    ``kv_lens[i]`` (int32 ``[R]``) tokens in all, whose rows lie in the pages ``block_table[i]``
+    (int32 ``[R, P]``); the token at position ``p`` sees the positions up to ``p``.  After
+    :func:`kv4_tables` pass its ``context_lens`` here, too: the ``kv_lens`` that it returns are
+    cut where the table is full, and no longer tell the new tokens' positions.  ``q_heads`` is a multiple of the
     cache's heads, and query head ``h`` reads kv head ``h // (q_heads / kv_heads)``.
 
     ``max_q`` is the most new tokens of a request (a longer one's later tokens are not
@@ -313,6 +318,12 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
             raise RuntimeError(f"cu_q has {cu_q.size(0)} entries, expected {R + 1}")
         if max_q is None:
             max_q = N
+    if context_lens is None:
+        ctx = 0
+    else:
+        ctx = _ints("context_lens", context_lens, dev)
+        if context_lens.size(0) != R:
+            raise RuntimeError(f"context_lens has {context_lens.size(0)} requests, block_table {R}")
     if max_kv is None:
         max_kv = P * page
     if out is None:
@@ -321,8 +332,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
             or out.data_ptr() % 16:
         raise RuntimeError(f"out must be a contiguous, 16-byte aligned {q.dtype} {tuple(q.shape)} tensor on cuda:{dev}")
     lse = torch.empty((N, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-    err = _lib.load().marlin_hip_kv4_attention(
-        qp, cp, table, lens, cu, out.data_ptr(), 0 if lse is None else lse.data_ptr(), N, R, Hq, H, D, qt, qh, page,
+    err = _lib.load().marlin_hip_kv4_attention_ctx(
+        qp, cp, table, lens, cu, ctx, out.data_ptr(), 0 if lse is None else lse.data_ptr(), N, R, Hq, H, D, qt, qh, page,
         pages, P, groupsize, min(max_q, N), max_kv, 1.0 / math.sqrt(D) if scale is None else scale, dtype, dev,
         _raw_stream(dev))
     if err:

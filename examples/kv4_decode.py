@@ -50,11 +50,12 @@ class Attention(nn.Module):
         self.cache = marlin.kv4_cache(pages, kv_heads, head_dim, page, groupsize, device=device)
         self.last = None  # q and out of the last step, for the check
 
-    def forward(self, x, slots, table, kv_lens, cu, max_q, max_kv):
+    def forward(self, x, slots, table, kv_lens, cu, max_q, max_kv, context_lens):
         y = self.qkv(rms(x)).view(x.size(0), self.heads + 2 * self.kv_heads, self.head_dim)
         q, k, v = y.split_with_sizes((self.heads, self.kv_heads, self.kv_heads), 1)  # views: no copy
         marlin.kv4_append(k, v, self.cache, slots, self.groupsize)
-        out = marlin.kv4_attention(q, self.cache, table, kv_lens, cu, max_q, max_kv, self.groupsize)
+        out = marlin.kv4_attention(q, self.cache, table, kv_lens, cu, max_q, max_kv, self.groupsize,
+                                   context_lens=context_lens)
         self.last = q, out
         return x + self.o(out.view(x.size(0), -1))
 
@@ -82,10 +83,10 @@ class Decoder:
         taken = sum(pages(c + n) - pages(c) for c, n in zip(self.lens, new))
         self.free = self.free[taken:]
         self.lens = [c + n for c, n in zip(self.lens, new)]
-        self.kv_lens = kv_lens
+        context_lens, self.kv_lens = self.kv_lens, kv_lens
         one = None if all(n == 1 for n in new) else cu
         for layer in self.layers:
-            x = layer(x, slots, self.table, kv_lens, one, max(new), max(self.lens))
+            x = layer(x, slots, self.table, kv_lens, one, max(new), max(self.lens), context_lens)
         return x, cu
 
     def check(self, new):

@@ -212,7 +212,7 @@ int marlin_hip_kv4_gather(const void* cache, const void* slots, void* k, void* v
 /* Causal attention.  q [tokens][q_heads][head_dim] (strides in elements, multiples of 8)
  * holds request i's new tokens at [cu_q[i], cu_q[i + 1]) (cu_q null: token i, and fewer
  * tokens than requests are refused); they
- * are the last of its kv_lens[i] tokens, in the pages block_table[i][max_pages] (entries
+ * are the last of its kv_lens[i] tokens (which may pass the table's width), in the pages block_table[i][max_pages] (entries
  * outside [0, num_pages): left out; max_pages * page_size at most 2^30).  out is contiguous
  * [tokens][q_heads][head_dim]; lse fp32 [tokens][q_heads] or null.  A row that sees no token:
  * zeros and -inf.  max_q bounds a request's new tokens (later ones are not computed);
@@ -224,6 +224,15 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
                              int kv_heads, int head_dim, long long q_token_stride, long long q_head_stride,
                              int page_size, int num_pages, int max_pages, int groupsize, int max_q, int max_kv,
                              float scale, int dtype, int dev, hipStream_t stream);
+
+/* The same, the position of each request's first new token given as context_lens[requests]
+ * (null: kv_lens[i] less the new tokens that cu_q counts): the call that goes with
+ * marlin_hip_kv4_tables, which cuts kv_lens at the table's width. */
+int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* block_table, const void* kv_lens,
+                                 const void* cu_q, const void* context_lens, void* out, void* lse, int tokens,
+                                 int requests, int q_heads, int kv_heads, int head_dim, long long q_token_stride,
+                                 long long q_head_stride, int page_size, int num_pages, int max_pages, int groupsize,
+                                 int max_q, int max_kv, float scale, int dtype, int dev, hipStream_t stream);
 
 /* The launch plan of a marlin_hip_kv4_attention call of few rows, computed on the host without
  * a GPU (sms <= 0: 256 compute units): out[0] 0, out[1] workgroups, out[2] whether a request's

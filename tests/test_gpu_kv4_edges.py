@@ -42,3 +42,61 @@ def test_fewer_rows_of_q_than_new_tokens(Hq, Hkv):
     out, lse = marlin.kv4_attention(q[:65].to(DEV), torch.from_numpy(cache).to(DEV), ints(table), ints(kv), ints(cu),
                                     max_q=70, max_kv=90, return_lse=True)
     _check(out, lse, want, torch.float16, "cut by q")
+
+
+def _step(Hq, Hkv, ctx, new, P, rows, seed):
+    """Tables, append and attention of a step over a cache that holds the contexts and, in every
+    other slot, NaN scales: the outputs, and those in 64 bits at the true positions."""
+    T, D, R = 16, 128, len(ctx)
+    gen = torch.Generator().manual_seed(seed)
+    have = [min(-(-c // T), P) for c in ctx]
+    size = R * P + 8
+    order = torch.randperm(size, generator=gen).tolist()
+    table, at = np.full((R, P), size + 5, np.int32), 0  # (stale entries: no page)
+    cache = np.full((size, Hkv, T * (D + 4)), 0xFF, np.uint8)
+    filled = ref.random_cache(size, Hkv, T, D, 1, gen)
+    scales = ref.places(T, D, 1)[2:]
+    for i, n in enumerate(have):
+        table[i, :n] = order[at:at + n]
+        at += n
+        for j in range(n):
+            cache[table[i, j]] = filled[table[i, j]]
+            for o in range(ctx[i] - j * T, T):
+                for s in scales:
+                    cache[table[i, j]].view(np.float16)[:, s[o]] = np.nan
+    free = ints(order[at:])
+    q, k, v = (torch.randn((sum(new), h, D), generator=gen).half() for h in (Hq, Hkv, Hkv))
+    dev_table, dev_cache = ints(table), torch.from_numpy(cache).to(DEV)
+    slots, cu, kv, _ = marlin.kv4_tables(ints(ctx), ints(new), free, dev_table, rows, T)
+    marlin.kv4_append(k[:rows].to(DEV), v[:rows].to(DEV), dev_cache, slots)
+    out, lse = marlin.kv4_attention(q[:rows].to(DEV), dev_cache, dev_table, kv, cu, max_q=max(new), max_kv=P * T,
+                                    return_lse=True, context_lens=ints(ctx))
+    total = [c + n for c, n in zip(ctx, new)]
+    want = ref.attention(q.double().numpy(), dev_cache.cpu().numpy(), _wider(dev_table.cpu().numpy(), P + max(total) // T + 1),
+                         total, cu.cpu().numpy(), D, 1, T)
+    return out, lse, [w[:rows] for w in want], slots
+
+
+@pytest.mark.parametrize("Hq,Hkv", KERNELS)
+def test_step_that_fills_its_tables(Hq, Hkv):
+    """Requests that pass their tables' 64 tokens in this step, had passed them before, and fit."""
+    out, lse, want, slots = _step(Hq, Hkv, [30, 70, 5, 0], [50, 40, 3, 64], 4, 157, 203)
+    assert (slots[:34] >= 0).all() and (slots[34:90] == -1).all() and (slots[90:] >= 0).all()
+    _check(out, lse, want, torch.float16, "full tables")
+
+
+@pytest.mark.parametrize("Hq,Hkv", KERNELS)
+def test_step_with_fewer_slots_than_new_tokens(Hq, Hkv):
+    """A slot map that ends inside the second request: its tokens see those before them only."""
+    out, lse, want, slots = _step(Hq, Hkv, [0, 9], [40, 40], 8, 65, 204)
+    assert (slots >= 0).all()
+    _check(out, lse, want, torch.float16, "short map")
+
+
+def test_context_lens_are_checked():
+    D, T = 128, 16
+    cache = marlin.kv4_cache(4, 2, D, T, device=DEV)
+    q, table, kv = torch.zeros((2, 2, D), dtype=torch.float16, device=DEV), ints([[0], [1]]), ints([3, 3])
+    for bad in (ints([1]), ints([1, 2]).long(), ints([1, 2]).cpu()):
+        with pytest.raises(RuntimeError, match="context_lens"):
+            marlin.kv4_attention(q, cache, table, kv, context_lens=bad)
