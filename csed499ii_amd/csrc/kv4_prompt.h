@@ -342,8 +342,9 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 
   float16_t O[DT];
   // M as in kv4_split.h; the scores, in units of `down`, are taken less `base`, which is M, or
-  // 0 before there is one, and M rises where one passes `top`
-  float M = kNone, base = 0.f, top = kNone, L = 0.f, shift = 0.f, v_top = 0.f;
+  // 0 before there is one
+  float M = kNone, base = 0.f, L = 0.f;
+  bool some_none = true;  // some row of the wave that has tokens here has no M
 #pragma unroll
   for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -355,125 +356,168 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     return *(const __attribute__((address_space(3))) half8_t*)(uintptr_t)(at + more);
   };
   // Scales [group of 16][K, V][quad][NG][4] of tokens 8 b + 4 h + (0 .. 3) of half j.
-  auto scale_of = [&](uint32_t scales, int kv, int n, int j, int b) {
+  auto scale_of = [&](uint32_t scales_lane, int kv, int n, int j, int b) {
     const int more = (2 * j + b / 2) * (128 * NG) + kv * (64 * NG) + (2 * (b & 1) * NG + n) * 16;
-    return *(const __attribute__((address_space(3))) float4_t*)(uintptr_t)(scales + 16 * NG * h + more);
-  };
-  // The scale of V of token `lane` of the tile, the largest of its groups.
-  auto v_of_lane = [&](uint32_t scales) {
-    float v = 0.f;
-#pragma unroll
-    for (int n = 0; n < NG; n++) {
-      const uint32_t at = scales + (lane >> 4) * (128 * NG) + 64 * NG + (lane >> 2 & 3) * (16 * NG) + (lane & 3) * 4;
-      v = fmaxf(v, fabsf(*(const __attribute__((address_space(3))) float*)(uintptr_t)(at + n * 16)));
-    }
-    return v;
+    return *(const __attribute__((address_space(3))) float4_t*)(uintptr_t)(scales_lane + more);
   };
   auto compute = [&](int tile, uint32_t hole) {
-    const uint32_t buf = lds_at + (tile & 1) * BUF, scales = buf + K_BYTES + V_BYTES;
-    const uint32_t even[2] = {buf + (h * kTile + k_slot(c, h)) * 16, buf + (h * kTile + k_slot(32 + c, h)) * 16};
-    const uint32_t odd[2] = {buf + (h * kTile + k_slot(c, 2 + h)) * 16, buf + (h * kTile + k_slot(32 + c, 2 + h)) * 16};
+    const uint32_t buf = lds_at + (tile & 1) * BUF;
+    uint32_t scales_lane = buf + K_BYTES + V_BYTES + 16 * NG * h;
+    uint32_t even[2] = {buf + (h * kTile + k_slot(c, h)) * 16, buf + (h * kTile + k_slot(32 + c, h)) * 16};
+    uint32_t odd[2] = {buf + (h * kTile + k_slot(c, 2 + h)) * 16, buf + (h * kTile + k_slot(32 + c, 2 + h)) * 16};
     const bool masked = (tile + 1) * kTile > w_all || hole != 0;
-    float vm = 0.f;
+    // Scores of half j, less base.
+    auto scores_of = [&](int j, float (&x)[16]) {
+#pragma unroll
+      for (int n = 0; n < NG; n++) {
+        float16_t S;
+#pragma unroll
+        for (int i = 0; i < 16; i++) S[i] = 0.f;
+#pragma unroll
+        for (int u = n * GU; u < (n + 1) * GU; u++)
+          S = __builtin_amdgcn_mfma_f32_32x32x16_f16(read16((u & 1 ? odd : even)[j], u * (2 * kTile * 16)), qf[u], S, 0, 0, 0);
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          const float4_t s = scale_of(scales_lane, 0, n, j, b);
+#pragma unroll
+          for (int i = 0; i < 4; i++)
+            x[4 * b + i] = __builtin_fmaf(S[4 * b + i], s[i], n == 0 ? -base : x[4 * b + i]);
+        }
+      }
+    };
+    // -infinity for what a row does not see.
+    auto mask = [&](int j, float (&x)[16]) {
+      int left = seen - tile * kTile - 4 * h;
+      asm volatile("" : "+v"(left));  // (else done for every tile)
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const int t = 32 * j + 8 * (i / 4) + i % 4;
+        const bool in = t < left && !(hole >> (2 * j + i / 8) & 1);
+        x[i] = in ? x[i] : -__builtin_inff();
+      }
+    };
+    // p and p v (fp16 pairs) of half j; sum of p, the largest p v.
+    auto weigh = [&](int j, float (&x)[16], u32x4 (&P)[NG][2], float& sum, float& most) {
+      sum = 0.f, most = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        x[i] = __builtin_amdgcn_exp2f(x[i] * down);
+        sum += x[i];
+      }
+#pragma unroll
+      for (int n = 0; n < NG; n++) {
+#pragma unroll
+        for (int b = 0; b < 4; b++) {
+          const float4_t s = scale_of(scales_lane, 1, n, j, b);
+#pragma unroll
+          for (int i = 0; i < 4; i += 2) {
+            const float lo = x[4 * b + i] * s[i], hi = x[4 * b + i + 1] * s[i + 1];
+            most = fmaxf(fmaxf(most, fabsf(lo)), fabsf(hi));
+            P[n][b >> 1][2 * (b & 1) + i / 2] = pack2(lo, hi);
+          }
+        }
+        asm volatile("" : "+v"(sum), "+v"(most));  // (now, not when all of p v is in registers)
+      }
+      if (masked) {  // what a row does not see is zero, whatever its scale
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+          const uint32_t keep = (x[i] == 0.f ? 0u : 0xFFFFu) | (x[i + 1] == 0.f ? 0u : 0xFFFF0000u);
+#pragma unroll
+          for (int n = 0; n < NG; n++) P[n][i / 8][i % 8 / 2] &= keep;
+        }
+      }
+    };
+    // A new reference from the scores x of half j, which come to lie less it; what it is higher by.
+    // In log2 units: the largest score xm and the largest p v, which lies e over it, are brought
+    // to 2^-rel and to 2^kVTop at most.
+    auto refer = [&](int j, float (&x)[16]) {
+      float xm = -__builtin_inff(), e = xm;
+#pragma unroll
+      for (int i = 0; i < 16; i++) xm = fmaxf(xm, x[i]);
+      const Pair px = across32(xm);
+      xm = fmaxf(px.a, px.b);
+#pragma unroll
+      for (int b = 0; b < 4; b++) {
+        float4_t v = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int n = 0; n < NG; n++) {
+          const float4_t s = scale_of(scales_lane, 1, n, j, b);
+#pragma unroll
+          for (int i = 0; i < 4; i++) v[i] = fmaxf(v[i], fabsf(s[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)  // (what is not seen makes -inf or NaN, which count for nothing)
+          e = fmaxf(e, __builtin_fmaf(x[4 * b + i] - xm, down, __builtin_amdgcn_logf(v[i])));
+      }
+      const Pair pe = across32(e);
+      e = fmaxf(pe.a, pe.b);
+      const bool none = M == kNone, any = xm > -__builtin_inff();
+      // (2^24: below the least v; where all v so far are zero the next may be any)
+      const float rel = fmaxf(e - kVTop, none ? -(kVTop + 24.f) : -kMostShift);
+      const bool rises = any && (none || __builtin_fmaf(xm, down, rel) > 0.f);
+      const float new_base = rises ? base + __builtin_fmaf(rel, up, xm) : base;
+      float less = new_base - base;
+      // (scores so large that base's rounding moves it by more than the slack: p = 1 for the largest)
+      const bool coarse = rises && !(fabsf(__builtin_fmaf(xm - less, down, rel)) <= kSlack);
+      if (coarse) less = xm;
+      base = coarse ? base + xm : new_base;
+      const float f = none ? 0.f : __builtin_amdgcn_exp2f(-less * down);
+      M = none && !any ? kNone : base * down;
+      some_none = __any(M == kNone && seen > t0 * kTile);
+      L *= f;
+#pragma unroll
+      for (int i = 0; i < 16; i++) x[i] -= less;
+#pragma unroll
+      for (int t = 0; t < DT; t++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) O[t][i] *= f;
+      return less;
+    };
+    const uint32_t v_at = buf + K_BYTES + (h * D + c) * 16;
 #pragma unroll
     for (int j0 = 0; j0 < 2; j0 += HALVES) {
       float x[HALVES][16];
 #pragma unroll
-      for (int jj = 0; jj < HALVES; jj++)
-#pragma unroll
-        for (int n = 0; n < NG; n++) {
-          const int j = j0 + jj;
-          float16_t S;
-#pragma unroll
-          for (int i = 0; i < 16; i++) S[i] = 0.f;
-#pragma unroll
-          for (int u = n * GU; u < (n + 1) * GU; u++)
-            S = __builtin_amdgcn_mfma_f32_32x32x16_f16(read16((u & 1 ? odd : even)[j], u * (2 * kTile * 16)), qf[u], S, 0, 0, 0);
-#pragma unroll
-          for (int b = 0; b < 4; b++) {
-            const float4_t s = scale_of(scales, 0, n, j, b);
-#pragma unroll
-            for (int i = 0; i < 4; i++)
-              x[jj][4 * b + i] = __builtin_fmaf(S[4 * b + i], s[i], n == 0 ? -base : x[jj][4 * b + i]);
-          }
-        }
-      if (j0 == 0) vm = v_of_lane(scales);
+      for (int jj = 0; jj < HALVES; jj++) scores_of(j0 + jj, x[jj]);
       if (masked) {
-        vm = tile * kTile + lane < w_end && !(hole >> (lane >> 4) & 1) ? vm : 0.f;
 #pragma unroll
-        for (int jj = 0; jj < HALVES; jj++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) {
-            const int j = j0 + jj, t = 32 * j + 8 * (i / 4) + 4 * h + i % 4;
-            const bool in = tile * kTile + t < seen && !(hole >> (2 * j + i / 8) & 1);
-            x[jj][i] = in ? x[jj][i] : -__builtin_inff();
-          }
+        for (int jj = 0; jj < HALVES; jj++) mask(j0 + jj, x[jj]);
       }
-      float xm = x[0][0];
-#pragma unroll
-      for (int i = 1; i < 16 * HALVES; i++) xm = fmaxf(xm, x[i / 16][i % 16]);
-      if (__any(xm > top || vm > v_top)) {
-        const Pair px = across32(xm);
-        xm = fmaxf(px.a, px.b);
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) vm = fmaxf(vm, __shfl_xor(vm, d));
-        float new_shift = shift;
-        if (vm > v_top) {
-          // vm <= 2^e; 2^24 bounds the shift where every v so far is tiny
-          new_shift = fminf(kVTop - (float)__builtin_amdgcn_frexp_expf(vm), 24.f);
-          v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
-        }
-        // the largest so far lies at `shift`, a larger one of this tile comes to new_shift.  Where
-        // scores are so large that base's rounding would move it by more than the slack, it is
-        // the tile's that stay together.
-        const bool none = M == kNone, risen = none ? xm > -__builtin_inff() : xm > shift * up;
-        const float new_base = base + (risen ? xm - new_shift * up : none ? 0.f : (shift - new_shift) * up);
-        float less = new_base - base;
-        if (risen) less = __builtin_amdgcn_fmed3f(less, xm - (new_shift + kSlack) * up, xm - (new_shift - kSlack) * up);
-        const float f = none ? 0.f : __builtin_amdgcn_exp2f(-less * down);
-        base = new_base;
-        shift = new_shift;
-        M = none && !risen ? kNone : base * down;
-        top = M == kNone ? kNone : (shift + kSlack) * up;
-        L *= f;
-#pragma unroll
-        for (int i = 0; i < 16 * HALVES; i++) x[i / 16][i % 16] -= less;
-#pragma unroll
-        for (int t = 0; t < DT; t++)
-#pragma unroll
-          for (int i = 0; i < 16; i++) O[t][i] *= f;
-      }
-      const uint32_t v_at = buf + K_BYTES + (h * D + c) * 16;
 #pragma unroll
       for (int jj = 0; jj < HALVES; jj++) {
         const int j = j0 + jj;
+        u32x4 P[NG][2];
+        float sum = 0.f, most = 0.f;
+        auto refer_to = [&] {
+          const float less = refer(j, x[jj]);
+          if (jj + 1 < HALVES) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) {
-          x[jj][i] = __builtin_amdgcn_exp2f(x[jj][i] * down);
-          L += x[jj][i];
+            for (int i = 0; i < 16; i++) x[HALVES - 1][i] -= less;
+          }
+          asm volatile("" ::: "memory");  // (else V's scales are kept in registers)
+        };
+        const bool first = some_none;
+        if (!first) weigh(j, x[jj], P, sum, most);
+        if (first || __any(!(L + sum < kMostL) || most > kMostPV)) {
+          // Rare; from the scores on once more, which are not kept, for their registers.  (Else
+          // what is read both times is, and addresses by the dozen.)
+          if (!first) {
+            asm volatile("" : "+v"(even[j]), "+v"(odd[j]), "+v"(scales_lane)::"memory");
+            scores_of(j, x[jj]);
+            if (masked) mask(j, x[jj]);
+          }
+          refer_to();
+          weigh(j, x[jj], P, sum, most);
         }
+        L += sum;
 #pragma unroll
-        for (int n = 0; n < NG; n++) {
-          u32x4 P[2];  // fp16 pairs
-#pragma unroll
-          for (int b = 0; b < 4; b++) {
-            const float4_t s = scale_of(scales, 1, n, j, b);
-#pragma unroll
-            for (int i = 0; i < 4; i += 2)
-              P[b >> 1][2 * (b & 1) + i / 2] = pack2(x[jj][4 * b + i] * s[i], x[jj][4 * b + i + 1] * s[i + 1]);
-          }
-          if (masked) {  // what a row does not see is zero, whatever its scale
-#pragma unroll
-            for (int i = 0; i < 16; i += 2)
-              P[i / 8][i % 8 / 2] &= (x[jj][i] == 0.f ? 0u : 0xFFFFu) | (x[jj][i + 1] == 0.f ? 0u : 0xFFFF0000u);
-          }
+        for (int n = 0; n < NG; n++)
 #pragma unroll
           for (int s = 0; s < 2; s++)
 #pragma unroll
             for (int t = n * (DT / NG); t < (n + 1) * (DT / NG); t++)
               O[t] = __builtin_amdgcn_mfma_f32_32x32x16_f16(read16(v_at, ((2 * j + s) * 2 * D + 32 * t) * 16),
-                                                            __builtin_bit_cast(half8_t, P[s]), O[t], 0, 0, 0);
-        }
+                                                            __builtin_bit_cast(half8_t, P[n][s]), O[t], 0, 0, 0);
       }
     }
   };

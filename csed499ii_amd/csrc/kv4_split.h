@@ -26,12 +26,14 @@
 // and subtracted from the sums it costs less, but the sums then grow to 8 sum p v and lose
 // in fp32 what a small output has: 10^-6 of the largest v was seen.)
 //
-// M is not the running maximum but a reference it may exceed by 2^kSlack before
-// accumulators are rescaled, which a wave-uniform branch does then: rare after the first
-// steps, and the exact maximum is not needed for an exact softmax.  M also carries the
-// power of two that keeps p v in fp16's normal range (p v is rounded to fp16 for the
-// matrix cores, relative error 2^-12, averaged over the tokens; sums are fp32): M rises
-// when a larger v is met, too.
+// M is not the running maximum but a reference that is only changed, by a wave-uniform branch,
+// when a row's p v, which is rounded to fp16 for the matrix cores, would pass 2^15 (or its sum
+// of p 2^100): rare after the first step.  The branch brings the row's largest p v so far to 2^7,
+// however large the v of tokens of little weight.  So p v has fp16's 11 bits where it is not
+// below 2^-14, and is off by 2^-25 at most there: an output by 2^-11 sum_j w_j |v_j| (w: the
+// softmax) and 2^-32 a token of the largest w_j s_j of the row, all its scale groups alike, which
+// share M.  With the largest v in M's place, however small its weight, values 2^21 below it lost
+// bits, and all of them 2^31 below.  Sums are fp32.
 //
 // What does not exist must not count: tokens past the row's last one, pages whose table
 // entry is not a page, slots never written (their scales may be NaN).  Their p v is set to
@@ -69,8 +71,11 @@ constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last wo
 constexpr int kTile = 64;          // tokens of a tile of the prompt kernel
 constexpr int kPromptWaves = 8, kPromptRows = 32 * kPromptWaves;
 constexpr int kMaxRequests = 2 * 64 * kWaves;  // of a launch that divides by the requests' lengths
-constexpr float kSlack = 8.f;      // p <= 2^8 of the reference
-constexpr float kVTop = 7.f;       // v 2^shift <= 2^7, so p v <= 2^15 < 65504
+constexpr float kVTop = 7.f;       // a new reference brings the row's largest p v to 2^7
+constexpr float kMostPV = 1 << 15; // ... which later ones may pass by 2^8 (65504 is the largest fp16)
+constexpr float kSlack = 8.f;      // of a reference that is rounded, in log2 units
+constexpr float kMostL = 0x1p100f; // of a row's sum of p, before it gets a new reference
+constexpr float kMostShift = 90.f; // p <= 2^90 at a new reference, however small its v
 constexpr float kBig = 1 << 20;    // of a row's largest score, in log2 units
 constexpr float kNone = -1.0e30f;  // reference of a row that has seen nothing
 
@@ -80,7 +85,6 @@ struct AttnArgs {
   const int32_t* table;
   const int32_t* kv_lens;
   const int32_t* cu_q;  // null: request i is token i
-  const int32_t* ctx;   // positions of the first new tokens; null: the new ones are the last of kv_lens
   void* out;
   float* lse;           // null: not wanted
   float* partial;       // [workgroup][first, last][row][D] (prompt kernel: [part][wave][..]); null: no tile is divided
@@ -100,6 +104,8 @@ struct AttnArgs {
   int lead;             // units that a tile counts more than it has
   int group;            // query heads of a kv head
   float c1;             // softmax scale * log2 e
+  const int32_t* ctx;   // positions of the first new tokens; where there are none kv_lens
+  bool has_ctx;
 };
 
 struct Request {
@@ -110,7 +116,7 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
   Request q;
   int cap = a.max_pages << a.log_page;  // (at most 2^30)
   asm volatile("" : "+s"(cap));         // (else kept in a vector register all the while)
-  const int kv = max(a.kv_lens[r], 0);
+  const int kv = max(a.kv_lens[r], 0), ctx = a.ctx[r];
   q.kv = min(kv, cap);
   int n = 1;
   if (a.cu_q == nullptr) {
@@ -123,7 +129,7 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
     q.n = max(min(end, a.tokens) - q.first, 0);
   }
   // positions go by the lengths as they are: what the table or q cuts off moves no token
-  q.past = min(a.ctx != nullptr ? max(a.ctx[r], 0) : kv - n, 1 << 30);
+  q.past = min(a.has_ctx ? max(ctx, 0) : kv - n, 1 << 30);
   return q;
 }
 
@@ -217,6 +223,15 @@ struct Magic {
 __device__ __forceinline__ half8_t k_operand(const Magic& m, uint32_t w) {
   const half4_t a = m.codes(w), b = m.codes(w >> 8);
   return (half8_t){a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+}
+
+// Of four fp16 numbers, without their signs; of two such, the larger (a NaN is larger still).
+__device__ __forceinline__ half4_t magnitude(half4_t v) {
+  return __builtin_bit_cast(half4_t, __builtin_bit_cast(u32x2, v) & 0x7FFF7FFFu);
+}
+__device__ __forceinline__ half4_t larger(half4_t a, half4_t b) {
+  typedef uint16_t quad __attribute__((ext_vector_type(4)));
+  return __builtin_bit_cast(half4_t, __builtin_elementwise_max(__builtin_bit_cast(quad, a), __builtin_bit_cast(quad, b)));
 }
 
 // Selectors of v_perm_b32 that pair the parts of two tokens' words (first token low).
@@ -458,9 +473,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
 
     // ---- the loop ----
     float4_t O[NG][S::OPS];
-    bool big = false, some_big = false;       // the row, some row
-    float M = kNone, L = 0.f, x_top = kNone;  // x_top: x above which M rises
-    float shift = 0.f, v_top = 0.f;  // v 2^shift <= 2^kVTop while v <= v_top
+    bool big = false, some_big = false;  // the row, some row
+    bool fresh = true;                   // (wave-uniform) no step yet
+    float M = kNone, L = 0.f, shift = 0.f, x_top = 0.f;  // M = x_top c1 - shift, x_top a score
 #pragma unroll
     for (int n = 0; n < NG; n++)
 #pragma unroll
@@ -581,63 +596,91 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
             for (int n = 0; n < NG; n++) vs[u][n][i] = in ? vs[u][n][i] : (_Float16)0.f;
           }
       }
-      float xm = x[0][0], vm = 0.f;
+      half4_t vt[2];  // of V, a token's largest scale (of the sizes: bits order as they do)
 #pragma unroll
-      for (int i = 1; i < 8; i++) xm = fmaxf(xm, x[i / 4][i % 4]);
+      for (int u = 0; u < 2; u++) {
+        vt[u] = magnitude(vs[u][0]);
 #pragma unroll
-      for (int i = 0; i < 8 * NG; i++) vm = fmaxf(vm, fabsf((float)vs[i / 4 / NG][i / 4 % NG][i % 4]));
-      if (__any(xm > x_top || vm > v_top)) {
-        // new reference: the rows' maxima so far and the largest v (the four lanes of a row agree)
-        vm = column_max(vm);
-        float new_shift = shift;
-        if (vm > v_top) {
-          // vm <= 2^e; 2^24 bounds the shift where every v so far is tiny
-          new_shift = fminf(kVTop - (float)__builtin_amdgcn_frexp_expf(vm), 24.f);
-          v_top = __builtin_amdgcn_exp2f(kVTop - new_shift);
-        }
-        const float m = column_max(xm);
-        // M = max - shift: rows keep the larger of the old maximum and this step's.  Past kBig,
-        // where M's rounding would show, scores are taken less the largest one, x_top.
-        const float old_max = M == kNone ? kNone : M + shift;
+        for (int n = 1; n < NG; n++) vt[u] = larger(vt[u], magnitude(vs[u][n]));
+      }
+      half8_t P[NG];
+      float p[8], sum = 0.f, most = 0.f;  // of this step's tokens: their sum, the largest p v
+      auto refer = [&] {
+        // A new reference (the four lanes of a row agree): the row's largest score m, and the
+        // largest p v of this step, e, and of those before, e_old, in log2 of 2^m's units.
+        float m = x[0][0];
+#pragma unroll
+        for (int i = 1; i < 8; i++) m = fmaxf(m, x[i / 4][i % 4]);
+        m = column_max(m);
+        const bool none = M == kNone;
+        const float old_max = none ? kNone : M + shift;
+        // Past kBig, where M's rounding would show, scores are taken less the largest one, x_top.
         const bool risen = big ? m > x_top : m * c1 > old_max;
         const float new_max = risen ? m * c1 : old_max;
+        const float drop = big ? (risen ? x_top - m : 0.f) * c1 : old_max - new_max;  // (<= 0)
+        if (risen) {
+          big = fabsf(new_max) > kBig;
+          x_top = m;
+        }
+        float e = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          const float v = x[i / 4][i % 4];
+          e = fmaxf(e, (big ? (v - x_top) * c1 : __builtin_fmaf(v, c1, -new_max)) +
+                           __builtin_amdgcn_logf((float)vt[i / 4][i % 4]));
+        }
+        e = column_max(e);
+        const float e_old = none ? e : kVTop - shift + drop;
+        // (2^24: below the least v; where all v so far are zero the next may be any)
+        const float new_shift = fminf(kVTop - fmaxf(e, e_old), none ? kVTop + 24.f : kMostShift);
         const float new_M = new_max <= kNone ? kNone : new_max - new_shift;
-        const float f = M == kNone ? 0.f
-                        : __builtin_amdgcn_exp2f(big ? __builtin_fmaf(risen ? x_top - m : 0.f, c1, new_shift - shift) : M - new_M);
-        if (risen) big = fabsf(new_max) > kBig;
-        if (!big) x_top = new_M == kNone ? kNone : (new_max + kSlack) * __builtin_amdgcn_rcpf(c1);
-        else if (risen) x_top = m;
+        const float f = none ? 0.f : __builtin_amdgcn_exp2f(big ? drop + (new_shift - shift) : M - new_M);
         M = new_M;
+        shift = new_shift;
         some_big = __any(big);
         L *= f;
 #pragma unroll
         for (int n = 0; n < NG; n++)
 #pragma unroll
           for (int i = 0; i < S::OPS; i++) O[n][i] *= f;
-        shift = new_shift;
-      }
-      half8_t P[NG];
-      if (some_big) {
+      };
+      auto weigh = [&] {
+        if (some_big) {
 #pragma unroll
-        for (int i = 0; i < 8; i++) {
-          const float v = x[i / 4][i % 4];
-          x[i / 4][i % 4] = big ? __builtin_fmaf(v - x_top, c1, shift) : __builtin_fmaf(v, c1, -M);
-        }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; i++) x[i / 4][i % 4] = __builtin_fmaf(x[i / 4][i % 4], c1, -M);
-      }
-#pragma unroll
-      for (int i = 0; i < 8; i++) {
-        const float p = __builtin_amdgcn_exp2f(x[i / 4][i % 4]);
-        L += p;
-        if constexpr (S::LATE) {
-          x[i / 4][i % 4] = p;
+          for (int i = 0; i < 8; i++) {
+            const float v = x[i / 4][i % 4];
+            p[i] = big ? __builtin_fmaf(v - x_top, c1, shift) : __builtin_fmaf(v, c1, -M);
+          }
         } else {
 #pragma unroll
-          for (int n = 0; n < NG; n++) P[n][i] = (_Float16)(p * (float)vs[i / 4][n][i % 4]);
+          for (int i = 0; i < 8; i++) p[i] = __builtin_fmaf(x[i / 4][i % 4], c1, -M);
         }
+        sum = 0.f, most = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+          p[i] = __builtin_amdgcn_exp2f(p[i]);
+          sum += p[i];
+          if constexpr (NG > 1) {
+            most = fmaxf(most, p[i] * (float)vt[i / 4][i % 4]);
+          }
+          if constexpr (!S::LATE) {
+#pragma unroll
+            for (int n = 0; n < NG; n++) {
+              const float pv = p[i] * (float)vs[i / 4][n][i % 4];
+              if constexpr (NG == 1) most = fmaxf(most, fabsf(pv));
+              P[n][i] = (_Float16)pv;
+            }
+          }
+        }
+      };
+      if (!fresh) weigh();
+      // (a row without a reference has p = 2^(10^30) of what it sees)
+      if (fresh || __any(!(L + sum < kMostL) || most > kMostPV)) {
+        refer();
+        fresh = false;
+        weigh();
       }
+      L += sum;
 #pragma unroll
       for (int n = 0; n < NG; n++) {
         u32x4 v0, v1;
@@ -645,10 +688,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
           v0 = read_v(from, 0, n), v1 = read_v(from, 1, n);
           const half4_t s[2] = {read_vs(from, 0, n), read_vs(from, 1, n)};
 #pragma unroll
-          for (int i = 0; i < 8; i++) P[n][i] = (_Float16)(x[i / 4][i % 4] * (float)s[i / 4][i % 4]);
+          for (int i = 0; i < 8; i++) P[n][i] = (_Float16)(p[i] * (float)s[i / 4][i % 4]);
           if (masked) {  // zero, whatever the scale
 #pragma unroll
-            for (int i = 0; i < 8; i++) P[n][i] = x[i / 4][i % 4] == 0.f ? (_Float16)0.f : P[n][i];
+            for (int i = 0; i < 8; i++) P[n][i] = p[i] == 0.f ? (_Float16)0.f : P[n][i];
           }
         } else {
           v0 = f.v[0][n], v1 = f.v[1][n];

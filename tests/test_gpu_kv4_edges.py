@@ -100,3 +100,66 @@ def test_context_lens_are_checked():
     for bad in (ints([1]), ints([1, 2]).long(), ints([1, 2]).cpu()):
         with pytest.raises(RuntimeError, match="context_lens"):
             marlin.kv4_attention(q, cache, table, kv, context_lens=bad)
+
+
+# ---- values over many orders of magnitude ----
+
+
+def _set_token(cache, table, T, D, G, pos, code, ks, vs):
+    """Position ``pos`` of request 0: every code of K ``code``, scales of K and V."""
+    page, o = table[0, pos // T], pos % T
+    k, _, k_at, v_at = ref.places(T, D, G)
+    for n in k[o]:
+        b = cache[page][:, n // 2]
+        cache[page][:, n // 2] = (b & 0xF0) | code if n % 2 == 0 else (b & 0x0F) | code << 4
+    halves = cache[page].view(np.float16)
+    halves[:, k_at[o]], halves[:, v_at[o]] = ks, vs
+
+
+WIDE = ["outlier first", "outlier inside", "outlier last", "sink of tiny v", "zeros first", "weightless zeros last",
+        "rising"]
+
+
+@pytest.mark.parametrize("n,Hq,Hkv", [(3, 4, 2), (50, 34, 17)])
+@pytest.mark.parametrize("D,g", [(128, -1), (128, 64), (128, 32), (64, 32)])
+@pytest.mark.parametrize("case", WIDE)
+def test_values_over_many_orders_of_magnitude(case, D, g, n, Hq, Hkv):
+    """Scales of V from fp16's least to its largest in one row.  p v is rounded to fp16 around a
+    power of two that follows the row's largest p v, not its largest v: 2^-11 of sum_j w_j |v_jd|
+    holds whatever v a token of little weight has, but for what lies 2^-32 a token below the
+    row's largest w_j s_j (a code is 8 at most).  bf16, so that no output is below the type's range."""
+    T, kv = 32, 400
+    q, cache, table, kvs, cu, G = _problem([n], [kv], Hq, Hkv, D, g, T, torch.bfloat16, seed=211)
+    q = q.abs()  # a token whose codes are all alike has the same sign of score for every row
+    pl = ref.places(T, D, G)
+    at = {p: (table[0, p // T], p % T) for p in range(kv)}
+
+    def scale(tokens, f):
+        for p in tokens:
+            cache[at[p][0]].view(np.float16)[:, pl[3][at[p][1]]] *= np.float16(f)
+
+    unit = float(q.double().sum(-1).mean()) / np.sqrt(D)  # of a token of codes 1 and scale 1
+    if case.startswith("outlier"):  # no weight (2^-60 or less), the largest scale; the others near the least
+        scale(range(kv), 2.0 ** -17)
+        _set_token(cache, table, T, D, G, {"first": 0, "inside": 170, "last": kv - n}[case.split()[1]], 0,
+                   80 / (8 * unit), 60000.0)
+    elif case == "sink of tiny v":
+        _set_token(cache, table, T, D, G, 0, 15, 12 / (7 * unit), 2.0 ** -24)
+    elif case == "zeros first":
+        scale(range(150), 0.0)
+        scale(range(150, 300), 2.0 ** -20)
+        scale(range(300, kv), 3000.0)
+    elif case == "weightless zeros last":  # a token that takes nearly all weight and has no v
+        _set_token(cache, table, T, D, G, kv - n, 15, 40 / (7 * unit), 0.0)
+    else:
+        for p in range(kv):
+            scale([p], 2.0 ** (-17 + p / 12.5))  # 2^-17 to 2^14.9
+    want = ref.attention(q.double().numpy(), cache, table, kvs, cu, D, G, T)
+    out, lse = marlin.kv4_attention(q.to(DEV), torch.from_numpy(cache).to(DEV), ints(table), ints(kvs), ints(cu),
+                                    max_q=n, max_kv=kv, groupsize=g, return_lse=True)
+    o, (w, ref_lse, weight) = out.double().cpu().numpy(), want
+    top = weight.max(-1, keepdims=True)  # >= the largest w_j s_j: some code is not 8
+    tol = (2.0 ** -11 + 2.0 ** -13) * weight + 2.0 ** -8 * np.abs(w) + kv * 8 * 2.0 ** -32 * top
+    bad = ~(np.abs(o - w) <= tol)
+    assert not bad.any(), f"{bad.sum()} of {bad.size} off, worst {np.nanmax(np.abs(o - w) / tol):.2f} of the bound"
+    assert np.abs(lse.double().cpu().numpy() - ref_lse).max() <= 2.0 ** -16 * 100
