@@ -385,16 +385,17 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         }
       }
     };
-    // -infinity for what a row does not see.
+    // -infinity for what a row does not see: score i of half j where not sees(j, i, left()).
+    auto left = [&] {
+      int n = seen - tile * kTile - 4 * h;
+      asm volatile("" : "+v"(n));  // (else done for every tile)
+      return n;
+    };
+    auto sees = [&](int j, int i, int n) { return 32 * j + 8 * (i / 4) + i % 4 < n && !(hole >> (2 * j + i / 8) & 1); };
     auto mask = [&](int j, float (&x)[16]) {
-      int left = seen - tile * kTile - 4 * h;
-      asm volatile("" : "+v"(left));  // (else done for every tile)
+      const int n = left();
 #pragma unroll
-      for (int i = 0; i < 16; i++) {
-        const int t = 32 * j + 8 * (i / 4) + i % 4;
-        const bool in = t < left && !(hole >> (2 * j + i / 8) & 1);
-        x[i] = in ? x[i] : -__builtin_inff();
-      }
+      for (int i = 0; i < 16; i++) x[i] = sees(j, i, n) ? x[i] : -__builtin_inff();
     };
     // p and p v (fp16 pairs) of half j; sum of p, the largest p v.
     auto weigh = [&](int j, float (&x)[16], u32x4 (&P)[NG][2], float& sum, float& most) {
@@ -418,10 +419,11 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         }
         asm volatile("" : "+v"(sum), "+v"(most));  // (now, not when all of p v is in registers)
       }
-      if (masked) {  // what a row does not see is zero, whatever its scale
+      if (masked) {  // what a row does not see is zero, whatever its scale (a seen NaN shows)
+        const int to = left();
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const uint32_t keep = (x[i] == 0.f ? 0u : 0xFFFFu) | (x[i + 1] == 0.f ? 0u : 0xFFFF0000u);
+          const uint32_t keep = (sees(j, i, to) ? 0xFFFFu : 0u) | (sees(j, i + 1, to) ? 0xFFFF0000u : 0u);
 #pragma unroll
           for (int n = 0; n < NG; n++) P[n][i / 8][i % 8 / 2] &= keep;
         }

@@ -681,6 +681,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
         weigh();
       }
       L += sum;
+      if (S::LATE && masked) {  // (a sign marks what is not seen)
+#pragma unroll
+        for (int i = 0; i < 8; i++) p[i] = x[i / 4][i % 4] == -__builtin_inff() ? -0.f : p[i];
+      }
 #pragma unroll
       for (int n = 0; n < NG; n++) {
         u32x4 v0, v1;
@@ -689,9 +693,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
           const half4_t s[2] = {read_vs(from, 0, n), read_vs(from, 1, n)};
 #pragma unroll
           for (int i = 0; i < 8; i++) P[n][i] = (_Float16)(p[i] * (float)s[i / 4][i % 4]);
-          if (masked) {  // zero, whatever the scale
+          if (masked) {  // what is not seen is zero, whatever its scale (a seen NaN shows)
 #pragma unroll
-            for (int i = 0; i < 8; i++) P[n][i] = p[i] == 0.f ? (_Float16)0.f : P[n][i];
+            for (int i = 0; i < 8; i++) P[n][i] = __builtin_signbit(p[i]) ? (_Float16)0.f : P[n][i];
           }
         } else {
           v0 = f.v[0][n], v1 = f.v[1][n];

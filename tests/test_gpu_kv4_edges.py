@@ -163,3 +163,20 @@ def test_values_over_many_orders_of_magnitude(case, D, g, n, Hq, Hkv):
     bad = ~(np.abs(o - w) <= tol)
     assert not bad.any(), f"{bad.sum()} of {bad.size} off, worst {np.nanmax(np.abs(o - w) / tol):.2f} of the bound"
     assert np.abs(lse.double().cpu().numpy() - ref_lse).max() <= 2.0 ** -16 * 100
+
+
+@pytest.mark.parametrize("n,Hq,Hkv", [(3, 4, 2), (50, 34, 17)])
+@pytest.mark.parametrize("D,g", [(128, -1), (128, 64), (128, 32), (64, 32)])
+@pytest.mark.parametrize("pos", [100, 396])
+def test_nan_of_a_seen_row_without_weight_shows(pos, D, g, n, Hq, Hkv):
+    """A NaN scale of V whose token's weight is zero in fp32, among tokens that all rows see and
+    among those that some do not: the rows that see it are NaN, no others."""
+    T, kv = 32, 399
+    q, cache, table, kvs, cu, G = _problem([n], [kv], Hq, Hkv, D, g, T, torch.float16, seed=221)
+    q = q.abs()
+    unit = float(q.double().sum(-1).mean()) / np.sqrt(D)
+    _set_token(cache, table, T, D, G, pos, 0, 300 / (8 * unit), np.nan)
+    out = marlin.kv4_attention(q.to(DEV), torch.from_numpy(cache).to(DEV), ints(table), ints(kvs), ints(cu), max_q=n,
+                               max_kv=kv, groupsize=g)
+    nan, first = torch.isnan(out).flatten(1), max(pos - (kv - n), 0)
+    assert nan[first:].all() and not nan[:first].any()
