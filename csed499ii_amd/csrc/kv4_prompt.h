@@ -385,17 +385,17 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         }
       }
     };
-    // -infinity for what a row does not see: score i of half j where not sees(j, i, left()).
-    auto left = [&] {
-      int n = seen - tile * kTile - 4 * h;
-      asm volatile("" : "+v"(n));  // (else done for every tile)
-      return n;
-    };
-    auto sees = [&](int j, int i, int n) { return 32 * j + 8 * (i / 4) + i % 4 < n && !(hole >> (2 * j + i / 8) & 1); };
-    auto mask = [&](int j, float (&x)[16]) {
-      const int n = left();
+    // -infinity for what a row does not see, `least` at least for what it does (NaN stays): once
+    // there is a reference so much that p is not zero, which what is not seen is told by.
+    auto mask = [&](int j, float (&x)[16], float least) {
+      int left = seen - tile * kTile - 4 * h;
+      asm volatile("" : "+v"(left));  // (else done for every tile)
 #pragma unroll
-      for (int i = 0; i < 16; i++) x[i] = sees(j, i, n) ? x[i] : -__builtin_inff();
+      for (int i = 0; i < 16; i++) {
+        const int t = 32 * j + 8 * (i / 4) + i % 4;
+        const bool in = t < left && !(hole >> (2 * j + i / 8) & 1);
+        x[i] = in ? x[i] < least ? least : x[i] : -__builtin_inff();
+      }
     };
     // p and p v (fp16 pairs) of half j; sum of p, the largest p v.
     auto weigh = [&](int j, float (&x)[16], u32x4 (&P)[NG][2], float& sum, float& most) {
@@ -419,11 +419,10 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         }
         asm volatile("" : "+v"(sum), "+v"(most));  // (now, not when all of p v is in registers)
       }
-      if (masked) {  // what a row does not see is zero, whatever its scale (a seen NaN shows)
-        const int to = left();
+      if (masked) {  // what a row does not see is zero, whatever its scale
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const uint32_t keep = (sees(j, i, to) ? 0xFFFFu : 0u) | (sees(j, i + 1, to) ? 0xFFFF0000u : 0u);
+          const uint32_t keep = (x[i] == 0.f ? 0u : 0xFFFFu) | (x[i + 1] == 0.f ? 0u : 0xFFFF0000u);
 #pragma unroll
           for (int n = 0; n < NG; n++) P[n][i / 8][i % 8 / 2] &= keep;
         }
@@ -475,6 +474,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         for (int i = 0; i < 16; i++) O[t][i] *= f;
       return less;
     };
+    const float least = -126.f * up;
     const uint32_t v_at = buf + K_BYTES + (h * D + c) * 16;
 #pragma unroll
     for (int j0 = 0; j0 < 2; j0 += HALVES) {
@@ -483,7 +483,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       for (int jj = 0; jj < HALVES; jj++) scores_of(j0 + jj, x[jj]);
       if (masked) {
 #pragma unroll
-        for (int jj = 0; jj < HALVES; jj++) mask(j0 + jj, x[jj]);
+        for (int jj = 0; jj < HALVES; jj++) mask(j0 + jj, x[jj], some_none ? -__builtin_inff() : least);
       }
 #pragma unroll
       for (int jj = 0; jj < HALVES; jj++) {
@@ -496,6 +496,10 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 #pragma unroll
             for (int i = 0; i < 16; i++) x[HALVES - 1][i] -= less;
           }
+          if (masked) {
+#pragma unroll
+            for (int k = jj; k < HALVES; k++) mask(j0 + k, x[k], least);
+          }
           asm volatile("" ::: "memory");  // (else V's scales are kept in registers)
         };
         const bool first = some_none;
@@ -506,7 +510,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
           if (!first) {
             asm volatile("" : "+v"(even[j]), "+v"(odd[j]), "+v"(scales_lane)::"memory");
             scores_of(j, x[jj]);
-            if (masked) mask(j, x[jj]);
+            if (masked) mask(j, x[jj], -__builtin_inff());
           }
           refer_to();
           weigh(j, x[jj], P, sum, most);
