@@ -274,7 +274,9 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     scores.  Returns ``out [tokens, q_heads, D]`` in ``q``'s type, and with ``return_lse`` the
     rows' log-sum-exp, fp32 ``[tokens, q_heads]``.
 
-    A row that sees no token gets zeros and ``-inf``; positions whose table entry is no page
+    A row that sees no token gets zeros and ``-inf``.  Rows that belong to no request (before
+    ``cu_q[0]``, from ``cu_q[R]`` on: a captured step's padding) and those past a request's
+    ``max_q`` are not written: they keep what ``out`` held, or hold anything.  No gradient flows through the call, as through the other kernels.  Positions whose table entry is no page
     of the cache (e.g. -1) are left out; slots past ``kv_lens`` may hold anything.
     A call that splits uses the stream's split-K scratch, as :func:`mul_2_4` does: under
     stream capture make an eager call of the shape first, else it runs unsplit."""

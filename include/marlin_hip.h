@@ -211,14 +211,15 @@ int marlin_hip_kv4_gather(const void* cache, const void* slots, void* k, void* v
 
 /* Causal attention.  q [tokens][q_heads][head_dim] (strides in elements, multiples of 8)
  * holds request i's new tokens at [cu_q[i], cu_q[i + 1]) (cu_q null: token i, and fewer
- * tokens than requests are refused); they
- * are the last of its kv_lens[i] tokens (which may pass the table's width), in the pages block_table[i][max_pages] (entries
- * outside [0, num_pages): left out; max_pages * page_size at most 2^30).  out is contiguous
- * [tokens][q_heads][head_dim]; lse fp32 [tokens][q_heads] or null.  A row that sees no token:
- * zeros and -inf.  max_q bounds a request's new tokens (later ones are not computed);
- * max_kv plans the split of the cache's length and does not change what is computed.  A
- * split call uses the stream's split-K scratch, and runs unsplit where a captured stream has
- * none yet.  scale is positive and finite. */
+ * tokens than requests are refused); they are the last of its kv_lens[i] tokens (which may
+ * pass the table's width), in the pages block_table[i][max_pages] (entries outside
+ * [0, num_pages): left out; max_pages * page_size at most 2^30).  out is contiguous
+ * [tokens][q_heads][head_dim]; lse fp32 [tokens][q_heads] or null.  A
+ * row that sees no token: zeros and -inf.  Rows of no request (before cu_q[0], from
+ * cu_q[requests] on) are not written.  max_q bounds a request's new tokens (later ones are not
+ * computed nor written); max_kv plans the split of the cache's length and does not change what
+ * is computed.  A split call uses the stream's split-K scratch, and runs unsplit where a
+ * captured stream has none yet.  scale is positive and finite. */
 int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block_table, const void* kv_lens,
                              const void* cu_q, void* out, void* lse, int tokens, int requests, int q_heads,
                              int kv_heads, int head_dim, long long q_token_stride, long long q_head_stride,

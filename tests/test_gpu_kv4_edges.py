@@ -180,3 +180,22 @@ def test_nan_of_a_seen_row_without_weight_shows(pos, D, g, n, Hq, Hkv):
                                max_kv=kv, groupsize=g)
     nan, first = torch.isnan(out).flatten(1), max(pos - (kv - n), 0)
     assert nan[first:].all() and not nan[:first].any()
+
+
+@pytest.mark.parametrize("q_lens,kv_lens,Hq,Hkv", [([1, 3], [300, 40], 4, 2), ([60, 90], [100, 90], 34, 17),
+                                                   ([1, 200], [50, 200], 6, 6), ([1] * 1100, [3] * 1100, 2, 1), ([0, 0], [9, 9], 4, 2)])
+@pytest.mark.parametrize("D,before,after", [(128, 0, 37), (64, 5, 1)])
+def test_rows_of_no_request_are_left_alone(q_lens, kv_lens, Hq, Hkv, D, before, after):
+    """Rows of q before the first request and after the last one, as in a step padded to a fixed
+    size, hold NaN and change nothing; ``out`` keeps what it had there.  In the kernel of few
+    rows, of prompts, both, and over several launches."""
+    T = 16
+    q, cache, table, kv, cu, G = _problem(q_lens, kv_lens, Hq, Hkv, D, -1, T, torch.float16, seed=231)
+    want = ref.attention(q.double().numpy(), cache, table, kv, cu, D, G, T)
+    q = torch.from_numpy(np.pad(q.numpy(), ((before, after), (0, 0), (0, 0)), constant_values=np.nan)).to(DEV)
+    out = torch.full(q.shape, 7.0, dtype=torch.float16, device=DEV)
+    _, lse = marlin.kv4_attention(q, torch.from_numpy(cache).to(DEV), ints(table), ints(kv), ints(cu + before),
+                                  max_q=max(max(q_lens), 1), max_kv=max(kv_lens), return_lse=True, out=out)
+    mine = slice(before, before + sum(q_lens))
+    _check(out[mine], lse[mine], want, torch.float16, "between the padding")
+    assert (out[:before] == 7).all() and (out[before + sum(q_lens):] == 7).all()
