@@ -276,7 +276,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
 
     A row that sees no token gets zeros and ``-inf``.  Rows that belong to no request (before
     ``cu_q[0]``, from ``cu_q[R]`` on: a captured step's padding) and those past a request's
-    ``max_q`` are not written: they keep what ``out`` held, or hold anything.  No gradient flows through the call, as through the other kernels.  Positions whose table entry is no page
+    ``max_q`` are not written: they keep what ``out`` held, or hold anything.  ``out`` must not
+    overlap ``q``.  No gradient flows through the call, as through the other kernels.  Positions whose table entry is no page
     of the cache (e.g. -1) are left out; slots past ``kv_lens`` may hold anything.
     A call that splits uses the stream's split-K scratch, as :func:`mul_2_4` does: under
     stream capture make an eager call of the shape first, else it runs unsplit."""
@@ -333,6 +334,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != dev or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise RuntimeError(f"out must be a contiguous, 16-byte aligned {q.dtype} {tuple(q.shape)} tensor on cuda:{dev}")
+    elif N and out.data_ptr() < qp + 2 * ((N - 1) * qt + (Hq - 1) * qh + D) and qp < out.data_ptr() + 2 * N * Hq * D:
+        raise RuntimeError("out must not overlap q, whose rows are read while out's are written")
     lse = torch.empty((N, Hq), dtype=torch.float32, device=q.device) if return_lse else None
     err = _lib.load().marlin_hip_kv4_attention_ctx(
         qp, cp, table, lens, cu, ctx, out.data_ptr(), 0 if lse is None else lse.data_ptr(), N, R, Hq, H, D, qt, qh, page,

@@ -214,7 +214,7 @@ int marlin_hip_kv4_gather(const void* cache, const void* slots, void* k, void* v
  * tokens than requests are refused); they are the last of its kv_lens[i] tokens (which may
  * pass the table's width), in the pages block_table[i][max_pages] (entries outside
  * [0, num_pages): left out; max_pages * page_size at most 2^30).  out is contiguous
- * [tokens][q_heads][head_dim]; lse fp32 [tokens][q_heads] or null.  A
+ * [tokens][q_heads][head_dim] and must not overlap q; lse fp32 [tokens][q_heads] or null.  A
  * row that sees no token: zeros and -inf.  Rows of no request (before cu_q[0], from
  * cu_q[requests] on) are not written.  max_q bounds a request's new tokens (later ones are not
  * computed nor written); max_kv plans the split of the cache's length and does not change what

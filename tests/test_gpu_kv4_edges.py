@@ -199,3 +199,18 @@ def test_rows_of_no_request_are_left_alone(q_lens, kv_lens, Hq, Hkv, D, before, 
     mine = slice(before, before + sum(q_lens))
     _check(out[mine], lse[mine], want, torch.float16, "between the padding")
     assert (out[:before] == 7).all() and (out[before + sum(q_lens):] == 7).all()
+
+
+def test_an_output_over_q_is_refused():
+    """Rows are written while others of q are still read."""
+    D, T = 128, 16
+    cache = marlin.kv4_cache(4, 2, D, T, device=DEV)
+    buf = torch.zeros((3, 8, D), dtype=torch.float16, device=DEV)
+    table, kv = ints([[0], [1], [2]]), ints([3, 3, 3])
+    flat = buf.view(-1)
+    for q, out in ((buf, buf), (buf[:, :4], buf.view(6, 4, D)[:3]), (buf[:, 2:6], flat[-3 * 4 * D:].view(3, 4, D)),
+                   (buf.view(6, 4, D)[:3], buf.view(6, 4, D)[2:5])):
+        with pytest.raises(RuntimeError, match="overlap"):
+            marlin.kv4_attention(q, cache, table, kv, out=out)
+    halves = buf.view(6, 4, D)
+    marlin.kv4_attention(halves[:3], cache, table, kv, out=halves[3:])  # side by side
