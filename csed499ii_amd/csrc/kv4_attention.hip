@@ -82,6 +82,22 @@ Plan prompt_plan(int tokens, int requests, int q_heads, int kv_heads, int max_q,
   return p;
 }
 
+// Which kernels a call launches, and what each is given.
+struct Choice {
+  bool prompts, split;
+  int few_rows, split_q;  // rows of a request that go to the split kernel, new tokens of one
+};
+Choice choose(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int ng, int max_q, bool cu, int cus) {
+  Choice c;
+  const int group = q_heads / kv_heads;
+  c.few_rows = split_rows(requests, kv_heads, head_dim, ng, cus);
+  c.prompts = (long long)max_q * group > c.few_rows;
+  c.split_q = c.prompts ? c.few_rows / group : max_q;
+  // (where the tokens say that no request can be short, the prompt kernel takes all)
+  c.split = !c.prompts || (cu && c.split_q > 0 && tokens <= c.split_q + (long long)(requests - 1) * max_q);
+  return c;
+}
+
 int check(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int page_size, int num_pages,
           int max_pages, int groupsize, int max_q, int max_kv, float scale, int dtype) {
   const int err = check_geometry(kv_heads, head_dim, groupsize, page_size, num_pages, dtype);
@@ -104,14 +120,25 @@ int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, i
                         int sms, int* out) {
   const int err = kv4::check(0, requests, q_heads, kv_heads, head_dim, 16, 1, 0, groupsize, max_q, max_kv, 1.f, 0);
   if (err != MARLIN_HIP_OK) return err;
-  // (a launch takes so many requests, and of each so many rows)
-  if (requests > kv4::kMaxRequests) requests = kv4::kMaxRequests;
-  const int most_q = 256 / (q_heads / kv_heads) > 1 ? 256 / (q_heads / kv_heads) : 1;
-  if (max_q > most_q) max_q = most_q;
-  const kv4::Plan p = kv4::plan(requests, q_heads, kv_heads, max_q, max_kv, sms > 0 ? sms : 256);
-  out[0] = 0;
-  out[1] = p.workgroups;
-  out[2] = p.split;
+  out[0] = out[1] = out[2] = 0;
+  if (requests == 0 || max_q == 0) return MARLIN_HIP_OK;
+  using namespace kv4;
+  const int cus = sms > 0 ? sms : 256, ng = groups(head_dim, groupsize), most = (1 << 30) / (q_heads / kv_heads);
+  const int tokens = (long long)requests * max_q < most ? requests * max_q : most;
+  const Choice c = choose(tokens, requests, q_heads, kv_heads, head_dim, ng, max_q, max_q > 1, cus);
+  if (requests > kMaxRequests) requests = kMaxRequests;  // (of the first launch)
+  if (c.split_q > 0) {
+    const Plan p = plan(requests, q_heads, kv_heads, c.split_q, max_kv, cus);
+    out[1] = p.workgroups;
+    out[2] = p.split;
+  }
+  if (c.prompts) {
+    const Plan p = prompt_plan(tokens, requests, q_heads, kv_heads, max_q, max_kv, c.split ? c.few_rows : 0, cus);
+    if (p.workgroups < 0) return refuse("kv4_attention: too many rows for one launch");
+    out[0] = 1;
+    out[1] = p.workgroups;
+    out[2] |= p.split;  // (shorter requests may go to the other kernel)
+  }
   return MARLIN_HIP_OK;
 }
 
@@ -160,15 +187,11 @@ int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* b
   a.max_q = max_q;
   a.c1 = scale * 1.4426950408889634f;
   const int cus = compute_units(dev);
-  const int few_rows = split_rows(requests, kv_heads, head_dim, ng, cus);
-  const bool prompts = (long long)max_q * group > few_rows;
-  const int split_q = prompts ? few_rows / group : max_q;
-  // (where the tokens say that no request can be short, the prompt kernel takes all)
-  const bool split = !prompts || (cu_q != nullptr && split_q > 0 && tokens <= split_q + (long long)(requests - 1) * max_q);
-  a.max_rows = split ? few_rows : 0;
+  const Choice c = choose(tokens, requests, q_heads, kv_heads, head_dim, ng, max_q, cu_q != nullptr, cus);
+  a.max_rows = c.split ? c.few_rows : 0;
   for (a.first = 0; a.first < requests; a.first += kMaxRequests) {
     a.requests = requests - a.first < kMaxRequests ? requests - a.first : kMaxRequests;
-    if (prompts) {
+    if (c.prompts) {
       const Plan p = prompt_plan(tokens, a.requests, q_heads, kv_heads, max_q, max_kv, a.max_rows, cus);
       if (p.workgroups < 0) return refuse("kv4_attention: too many rows for one launch");
       a.pieces = p.pieces;
@@ -183,8 +206,8 @@ int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* b
       if (err != MARLIN_HIP_OK) return err;
       a.partial = nullptr;
     }
-    if (split) {
-      const Plan p = plan(a.requests, q_heads, kv_heads, split_q, max_kv, cus);
+    if (c.split) {
+      const Plan p = plan(a.requests, q_heads, kv_heads, c.split_q, max_kv, cus);
       a.log_kw = p.log_kw;
       a.lead = p.lead;
       a.slots = 2 * cus;

@@ -348,10 +348,12 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
 
 def plan_kv4_attention(requests: int, q_heads: int, kv_heads: int, head_dim: int, max_q: int = 1, max_kv: int = 1,
                        groupsize: int = -1, sms: int = -1) -> dict:
-    """The launch plan of a :func:`kv4_attention` call of few rows (new tokens times the query
-    heads of a kv head), computed on the host without a GPU (``sms``: compute units, -1: 256):
-    ``workgroups``, and ``split``: whether a request's cache may be divided among them, through
-    the stream's split-K scratch.  How it is divided follows from the real lengths, on the GPU."""
+    """The launch plan of a :func:`kv4_attention` call for ``requests`` requests of ``max_q`` new
+    tokens each, computed on the host without a GPU (``sms``: compute units, -1: 256):
+    ``workgroups`` of the kernel that runs (of few rows or of prompts, which the rows, new tokens
+    times the query heads of a kv head, decide), and ``split``: whether a request's cache may be
+    divided among workgroups, through the stream's split-K scratch, in such a call or one with
+    shorter requests among them.  How it is divided follows from the real lengths, on the GPU."""
     out = (ctypes.c_int * 3)()
     err = _lib.load().marlin_hip_kv4_plan(requests, q_heads, kv_heads, head_dim, groupsize, max_q, max_kv, sms, out)
     if err:

@@ -235,9 +235,12 @@ int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* b
                                  long long q_head_stride, int page_size, int num_pages, int max_pages, int groupsize,
                                  int max_q, int max_kv, float scale, int dtype, int dev, hipStream_t stream);
 
-/* The launch plan of a marlin_hip_kv4_attention call of few rows, computed on the host without
- * a GPU (sms <= 0: 256 compute units): out[0] 0, out[1] workgroups, out[2] whether a request's
- * cache may be divided among workgroups (the call then uses its stream's split-K scratch). */
+/* The launch plan of a marlin_hip_kv4_attention call, computed on the host without a GPU (sms
+ * <= 0: 256 compute units), for `requests` requests of max_q new tokens each (cu_q null where
+ * max_q is 1): out[0] 0 (kernel of few rows) or 1 (of prompts), out[1] its workgroups (of the
+ * first launch where requests take several), out[2] whether such a call, or one with shorter
+ * requests among them, may divide a request's cache among workgroups (it then uses its
+ * stream's split-K scratch). */
 int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, int groupsize, int max_q, int max_kv,
                         int sms, int* out);
 

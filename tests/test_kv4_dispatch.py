@@ -18,12 +18,12 @@ from tests.launches import _base, build_fake  # noqa: E402
 NULL = ctypes.c_void_p(0)
 
 
-def attention(lib, at, tokens, requests, q_heads, kv_heads, head_dim, max_q, max_kv, cu_q, groupsize=-1):
+def attention(lib, at, tokens, requests, q_heads, kv_heads, head_dim, max_q, max_kv, cu_q, groupsize=-1, stream=64):
     """One call with operands at address ``at``, which is never read on the host."""
     p = ctypes.c_void_p(at)
     return lib.marlin_hip_kv4_attention(p, p, p, p, p if cu_q else NULL, p, NULL, tokens, requests, q_heads, kv_heads,
                                         head_dim, q_heads * head_dim, head_dim, 16, 1 << 16, 1 << 14, groupsize, max_q,
-                                        max_kv, 1.0, 0, 0, ctypes.c_void_p(64))
+                                        max_kv, 1.0, 0, 0, ctypes.c_void_p(stream))
 
 
 def test_one_token_a_request_needs_as_many_tokens(built_lib):
@@ -38,8 +38,8 @@ def fake(built_lib, tmp_path_factory):
 
 
 def launches(fake, calls):
-    """Per call (the arguments of ``attention`` after ``at``) its launches, kernel and grid, seen
-    in a process of its own."""
+    """Per call (the arguments of ``attention`` after ``at``) its launches: kernel, grid, and whether
+    the call asked for scratch (each on a stream of its own), seen in another process."""
     out = subprocess.run([sys.executable, str(pathlib.Path(__file__)), json.dumps({"fake": str(fake), "calls": calls})],
                          capture_output=True, text=True, cwd=ROOT, timeout=120)
     assert out.returncode == 0, out.stdout + out.stderr
@@ -56,18 +56,45 @@ def test_every_launch_has_workgroups(fake, tokens, requests, heads, kv_heads, D,
     assert ls and all(x["grid"] > 0 for x in ls), ls
 
 
+@pytest.mark.parametrize("D,g", [(128, -1), (128, 32), (64, -1)])
+@pytest.mark.parametrize("heads,kv_heads", [(32, 32), (64, 8), (64, 64), (16, 4), (24, 2), (160, 160), (128, 1)])
+def test_plan_names_what_runs(fake, D, g, heads, kv_heads):
+    """The plan query against the launches: kernel, workgroups and whether scratch is asked for;
+    with a shorter request among them scratch is asked for only where the plan says so."""
+    shapes = [(r, n, kv) for r in (1, 2, 17, 64, 1030) for n in (1, 2, 5, 9, 40, 81, 200, 600) for kv in (60, 65, 257, 5000)]
+    calls = [[r * n, r, heads, kv_heads, D, n, kv, n > 1, g] for r, n, kv in shapes]
+    shorter = [[r * n - n + 1, r, heads, kv_heads, D, n, kv, True, g] for r, n, kv in shapes]
+    out = (ctypes.c_int * 3)()
+    for (r, n, kv), full, mixed in zip(shapes, launches(fake, calls), launches(fake, shorter)):
+        assert _lib.load().marlin_hip_kv4_plan(r, heads, kv_heads, D, g, n, kv, 256, out) == 0
+        kernel, workgroups, split = out
+        assert full[0]["kernel"] == ("kv4_split_kernel", "kv4_prompt_kernel")[kernel], (r, n, kv)
+        assert full[0]["grid"] == workgroups, (r, n, kv, full, list(out))
+        assert len(full) == -(-r // 1024)
+        asked = any(x["scratch"] for x in full)
+        assert asked == bool(split) if kernel == 0 else asked <= split, (r, n, kv, full, list(out))
+        assert any(x["scratch"] for x in mixed) <= split, (r, n, kv, mixed, list(out))
+
+
 def _main(req):
     fake = ctypes.CDLL(req["fake"], mode=ctypes.RTLD_GLOBAL)
     fake.fake_hip_launch.restype = ctypes.c_char_p
     lib = _lib.load()
     u, out, seen = [ctypes.c_uint(), ctypes.c_uint(), ctypes.c_int(), ctypes.c_int()], [], 0
-    for call in req["calls"]:
-        err = attention(lib, 4096, *call)
+    at = ctypes.c_void_p()
+
+    def allocated():  # (the stand-in's allocator only counts up)
+        fake.hipMalloc(ctypes.byref(at), ctypes.c_size_t(4096))
+        return at.value
+
+    for n, call in enumerate(req["calls"]):
+        before = allocated()
+        err = attention(lib, 4096, *call, *[-1] * (len(call) == 8), 64 * (n + 1))
         assert err == 0, (call, err, _lib.last_error())
-        mine = []
+        scratch, mine = allocated() - before > 4096, []
         for i in range(seen, fake.fake_hip_launches()):
             name = fake.fake_hip_launch(i, *map(ctypes.byref, u)).decode()
-            mine.append({"kernel": _base(name), "grid": u[0].value})
+            mine.append({"kernel": _base(name), "grid": u[0].value, "scratch": scratch})
         seen += len(mine)
         out.append(mine)
     print(json.dumps(out))
