@@ -278,6 +278,8 @@ int marlin_hip_kv4_tables(const void* context_lens, const void* new_lens, const 
   if (requests < 0 || num_free < 0 || max_pages < 0 || tokens < 0)
     return kv4::refuse("kv4_tables takes no negative sizes");
   if (!kv4::page_ok(page_size)) return kv4::refuse("the KV cache's page_size must be 16, 32, 64, 128 or 256");
+  // (lengths are cut there, and are int32)
+  if ((long long)max_pages * page_size > (1ll << 30)) return kv4::refuse("a block table row covers more than 2^30 tokens");
   sm24::DeviceScope scope(dev);
   if (!scope.ok) return MARLIN_HIP_ERR_LAUNCH;
   kv4::TableArgs a{};

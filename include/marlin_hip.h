@@ -189,8 +189,8 @@ int marlin_hip_mul_2_4_native(const void* A, const void* Bn, const void* metan, 
  * goes to block_table[requests][max_pages].  Writes slots[tokens] (-1: past the last new
  * token, no free page left, or past the table's width), cu_new[requests + 1], kv_lens
  * [requests] (cut at the table's width) and pages_used[1] (pages wanted, which may exceed
- * num_free; entries without a page are -1).  Tokens past `tokens` get no slot and no page.
- * One launch. */
+ * num_free; entries without a page are -1).  Tokens past `tokens` get no slot and no page, but
+ * count in cu_new, kv_lens and pages_used.  max_pages * page_size is at most 2^30.  One launch. */
 int marlin_hip_kv4_tables(const void* context_lens, const void* new_lens, const void* free_pages, void* block_table,
                           void* slots, void* cu_new, void* kv_lens, void* pages_used, int requests, int num_free,
                           int max_pages, int page_size, int tokens, int dev, hipStream_t stream);

@@ -32,6 +32,13 @@ def test_one_token_a_request_needs_as_many_tokens(built_lib):
     assert "cu_q" in _lib.last_error()
 
 
+@pytest.mark.parametrize("width,page,code", [(1 << 26, 16, "OK"), (1 << 22, 256, "OK"), ((1 << 26) + 1, 16, "ERR_PROB_SHAPE"),
+                                             (1 << 30, 16, "ERR_PROB_SHAPE")])
+def test_table_width(fake, width, page, code):
+    """A table row covers 2^30 tokens at most, as attention asks for: kv_lens, cut there, is an int32."""
+    assert tables_in_child(fake, width, page) == getattr(_lib, code)
+
+
 @pytest.fixture(scope="module")
 def fake(built_lib, tmp_path_factory):
     return build_fake(tmp_path_factory.mktemp("fake_hip"))
@@ -41,6 +48,13 @@ def launches(fake, calls):
     """Per call (the arguments of ``attention`` after ``at``) its launches: kernel, grid, and whether
     the call asked for scratch (each on a stream of its own), seen in another process."""
     out = subprocess.run([sys.executable, str(pathlib.Path(__file__)), json.dumps({"fake": str(fake), "calls": calls})],
+                         capture_output=True, text=True, cwd=ROOT, timeout=120)
+    assert out.returncode == 0, out.stdout + out.stderr
+    return json.loads(out.stdout.splitlines()[-1])
+
+
+def tables_in_child(fake, width, page):
+    out = subprocess.run([sys.executable, str(pathlib.Path(__file__)), json.dumps({"fake": str(fake), "tables": [width, page]})],
                          capture_output=True, text=True, cwd=ROOT, timeout=120)
     assert out.returncode == 0, out.stdout + out.stderr
     return json.loads(out.stdout.splitlines()[-1])
@@ -80,6 +94,10 @@ def _main(req):
     fake = ctypes.CDLL(req["fake"], mode=ctypes.RTLD_GLOBAL)
     fake.fake_hip_launch.restype = ctypes.c_char_p
     lib = _lib.load()
+    if "tables" in req:
+        p, (width, page) = ctypes.c_void_p(4096), req["tables"]
+        print(lib.marlin_hip_kv4_tables(p, p, p, p, p, p, p, p, 1, 1, width, page, 1, 0, ctypes.c_void_p(64)))
+        return
     u, out, seen = [ctypes.c_uint(), ctypes.c_uint(), ctypes.c_int(), ctypes.c_int()], [], 0
     at = ctypes.c_void_p()
 
