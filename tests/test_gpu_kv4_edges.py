@@ -214,3 +214,41 @@ def test_an_output_over_q_is_refused():
             marlin.kv4_attention(q, cache, table, kv, out=out)
     halves = buf.view(6, 4, D)
     marlin.kv4_attention(halves[:3], cache, table, kv, out=halves[3:])  # side by side
+
+
+@pytest.mark.parametrize("streams", [1, 2])
+def test_divided_calls_of_two_host_threads(streams):
+    """Calls that divide their caches (few rows, prompts, both kernels in one call), issued by two
+    host threads at once, on one stream and on one each: the bits of a call by itself."""
+    import threading
+
+    D, T = 128, 16
+    calls = []
+    for seed, (q_lens, kv_lens, Hq, Hkv) in enumerate([([1] * 3, [4000, 700, 2900], 8, 1), ([41], [1200], 68, 17),
+                                                       ([120, 1, 2], [900, 3000, 40], 20, 20)]):
+        q, cache, table, kv, cu, _ = _problem(q_lens, kv_lens, Hq, Hkv, D, -1, T, torch.float16, seed=241 + seed)
+        args = (q.to(DEV), torch.from_numpy(cache).to(DEV), ints(table), ints(kv), ints(cu), max(q_lens), max(kv_lens))
+        calls.append((args, marlin.kv4_attention(*args)))
+    assert marlin.plan_kv4_attention(3, 8, 1, D, 1, 4000)["split"] and marlin.plan_kv4_attention(1, 68, 17, D, 41, 1200)["split"]
+    torch.cuda.synchronize()
+    own = [torch.cuda.Stream() for _ in range(streams)]
+    got, errors = [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(own[i % streams]):
+                for k in range(24):
+                    args, want = calls[(k + i) % 3]
+                    got[i].append((marlin.kv4_attention(*args), want))
+        except Exception as e:  # noqa: BLE001 (shown by the test's own thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors
+    for out, want in got[0] + got[1]:
+        assert torch.equal(out, want)
