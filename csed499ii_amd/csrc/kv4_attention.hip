@@ -167,8 +167,7 @@ int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* b
   a.table = static_cast<const int32_t*>(block_table);
   a.kv_lens = static_cast<const int32_t*>(kv_lens);
   a.cu_q = static_cast<const int32_t*>(cu_q);
-  a.has_ctx = context_lens != nullptr;
-  a.ctx = a.has_ctx ? static_cast<const int32_t*>(context_lens) : a.kv_lens;
+  a.ctx = static_cast<const int32_t*>(context_lens);
   a.out = out;
   a.lse = static_cast<float*>(lse);
   a.qt = q_token_stride;
@@ -231,7 +230,7 @@ int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* b
     a.kv_lens += a.requests;
     a.table += (size_t)a.requests * max_pages;
     if (a.cu_q) a.cu_q += a.requests;
-    a.ctx += a.requests;
+    if (a.ctx) a.ctx += a.requests;
   }
   return MARLIN_HIP_OK;
 }

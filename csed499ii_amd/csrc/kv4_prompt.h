@@ -127,7 +127,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         const int at = __builtin_ctzll(with);
         int i = __builtin_amdgcn_readlane(before, at);
         for (int r = at * per; r < min(at * per + per, a.requests); r++) {
-          const Request q = request_of(a, r);
+          Request q = request_of(a, r);
+          set_past(a, r, q);
           const int n = blocks_of(q);
           for (int b = lane; b < n; b += 64) {
             kinds[i + b] = r * kMaxKinds + n - 1 - b;
@@ -178,7 +179,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     const int kind = __builtin_amdgcn_readfirstlane(kinds[i]);
     r = kind / kMaxKinds, block = kind % kMaxKinds;
   }
-  const Request rq = request_of(a, r);
+  Request rq = request_of(a, r);
+  set_past(a, r, rq);
   const int rows = rows_of(a, rq), row0 = block * kPromptRows;
   const int w_row0 = row0 + 32 * wave;
   // tokens that some row of the workgroup, some row of the wave and every row of it sees
