@@ -1,5 +1,7 @@
 """The 4-bit KV cache's attention where lengths, tables and q do not fit each other, and where
 values span many orders of magnitude, against tests/kv4_ref.py.  Bounds as in test_gpu_kv4.py."""
+import ctypes
+
 import numpy as np
 import pytest
 import torch
@@ -216,6 +218,15 @@ def test_an_output_over_q_is_refused():
     marlin.kv4_attention(halves[:3], cache, table, kv, out=halves[3:])  # side by side
 
 
+def _new_stream():
+    """A stream of its own, kept for good: torch hands out a pool's in turn, and other tests count
+    on getting one that no call has used."""
+    hip, handle = ctypes.CDLL("libamdhip64.so"), ctypes.c_void_p()
+    with torch.cuda.device(DEV):
+        assert hip.hipStreamCreateWithFlags(ctypes.byref(handle), 1) == 0  # (does not wait for the null stream)
+    return torch.cuda.ExternalStream(handle.value, device=DEV)
+
+
 @pytest.mark.parametrize("streams", [1, 2])
 def test_divided_calls_of_two_host_threads(streams):
     """Calls that divide their caches (few rows, prompts, both kernels in one call), issued by two
@@ -231,7 +242,7 @@ def test_divided_calls_of_two_host_threads(streams):
         calls.append((args, marlin.kv4_attention(*args)))
     assert marlin.plan_kv4_attention(3, 8, 1, D, 1, 4000)["split"] and marlin.plan_kv4_attention(1, 68, 17, D, 41, 1200)["split"]
     torch.cuda.synchronize()
-    own = [torch.cuda.Stream() for _ in range(streams)]
+    own = [_new_stream() for _ in range(streams)]
     got, errors = [[], []], []
 
     def work(i):
