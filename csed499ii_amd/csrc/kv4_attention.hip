@@ -15,10 +15,11 @@ hipError_t launch_prompt(const AttnArgs& a, int workgroups, int head_dim, int ng
 // Requests of at most so many rows (new tokens times the query heads of a kv head) go to the
 // split kernel, the others to the prompt kernel, each of which passes over the other's.  The
 // split kernel's time grows with the rows, the prompt kernel's is the same up to 256: 12
-// requests of 4096 tokens on 8 heads of 128 dims, 64, 80, 96 and 128 rows, 54, 58, 74 and 87
-// us beside 67 to 69; with groups of 32, 128, 144 and 160 rows, 118, 134 and 142 beside 133.
+// requests of 4096 tokens on 8 heads of 128 dims, 64, 80, 96 and 128 rows, 53, 55, 70 and 82
+// us beside 72 to 73; with groups of 32, 128, 144 and 160 rows, 104, 123 and 133 beside 108,
+// 125 and 125.
 // Few tiles leave the prompt kernel's large parts waiting: one request of 8192 tokens, 24 us
-// beside 34 at 64 rows, 41 beside 59 at 256.
+// beside 34 at 64 rows, 41 beside 57 at 256.
 int split_rows(int requests, int kv_heads, int head_dim, int ng, int cus) {
   if ((long long)requests * kv_heads <= cus / 16) return 256;
   return head_dim == 128 && ng == 4 ? 144 : 80;
@@ -43,10 +44,10 @@ struct Plan {
 
 // Two workgroups of eight waves fill a compute unit.  All eight waves take one block of 16
 // rows and meet in LDS: a piece of a block costs its write and read in memory, and so there
-// are few (one request of 131072 tokens on 8 heads: 37.8 us with eight, 59 with four, 107 with two; 64 requests of
-// 4096: 57, 64, 70).  From two blocks a workgroup on, a workgroup goes through many short
-// ones instead, and two waves take a block (64 requests of 4096 tokens on 32 heads: 232 us
-// with eight, 229 with four, 219 with two; 200 of 1000: 220, 196, 189).
+// are few (one request of 131072 tokens on 8 heads: 38.4 us with eight, 63 with four, 113 with two; 64 requests of
+// 4096: 61, 65, 66).  From two blocks a workgroup on, a workgroup goes through many short
+// ones instead, and two waves take a block (64 requests of 4096 tokens on 32 heads: 220 us
+// with eight, 215 with four, 210 with two; 200 of 1000: 208, 187, 177).
 Plan plan(int requests, int q_heads, int kv_heads, int max_q, int max_kv, int cus) {
   Plan p{};
   const long long row_blocks = ((long long)max_q * (q_heads / kv_heads) + 15) / 16;
@@ -74,7 +75,7 @@ Plan prompt_plan(int tokens, int requests, int q_heads, int kv_heads, int max_q,
   Plan p{};
   p.pieces = cus / kv_heads;
   p.split = max_kv > kTile && p.pieces > 1;
-  // (of one fresh prompt the last blocks see few tokens: 65 us whole, 69 with workgroups for
+  // (of one fresh prompt the last blocks see few tokens: 60 us whole, 67 with workgroups for
   // them, 1500 tokens on 64 and 8 heads)
   p.rest = p.split && kinds > p.pieces && (requests > 1 || max_kv >= 2ll * max_q);
   const long long w = (p.rest ? kinds + p.pieces : p.split && kinds < p.pieces ? p.pieces : kinds) * kv_heads;

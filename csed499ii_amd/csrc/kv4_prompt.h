@@ -17,15 +17,16 @@
 // counts is operations per score, of any kind, and neither LDS (254 of 256 bytes a clock with
 // eight waves) nor the order of products and softmax.  A tile of 128 dims takes 4400 cycles:
 // 2048 of MFMAs, some 1600 of vector operations at their rates, the rest waits.  4096 tokens
-// on 32 heads of 128 dims: 160 us, 860 TFLOP/s, where a large library product reaches 1161.
+// on 32 heads of 128 dims: 161 us, 854 TFLOP/s, where a large library product reaches 1161;
+// MFMAs are 36 % of all its cycles, beginnings, ends and the division included.
 // Tried: four waves and 128 rows (198), 32-token tiles and three workgroups a compute unit
 // (232), scales as fp16 in mixed FMAs (168 where this took 164), products and softmax of two tiles interleaved
 // (186 to 191); 64 dims in 128 registers, for two workgroups a compute unit, spill.
 //
 // Fewer blocks of rows than compute units are divided over their tokens, one part a
 // workgroup; the waves of the same rows meet in the uncached scratch, and the last to arrive
-// adds the parts in order.  A 512-token chunk on 64 and 8 heads with 4096 in all: 151 us
-// whole, 100 in two parts, whose write and read take 6.
+// adds the parts in order.  A 512-token chunk on 64 and 8 heads with 4096 in all: 134 us
+// whole, 87 in two parts, whose write and read take 6.
 #pragma once
 #include "kv4_split.h"
 
@@ -60,8 +61,11 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   constexpr int BUF = K_BYTES + V_BYTES + S_BYTES;  // operands and scales of a tile
   constexpr int PIECES = kTile * D / 2 / 16;  // 16-byte pieces of K codes, and of V codes
   constexpr int GROUPS = kTile / 16;          // of tokens in one page
-  constexpr int HALVES = NG == 4 ? 1 : 2;     // of a tile whose scores are held at once (four
-                                              // groups: 439 us with both, 367; two: 268, 285)
+  // Halves of a tile whose scores are held at once: both, for products and softmax side by
+  // side, where the products are long enough for it (2048 tokens of 4096 on 64 and 8 heads of 128
+  // dims, groups of 32: 339 us with both, 353 one by one, of 64 272 and 274; 4000 on 16 and 4
+  // heads of 64 dims 109 and 100).
+  constexpr int HALVES = D == 128 ? 2 : 1;
   __shared__ __align__(16) uint8_t lds[2 * BUF];
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -97,7 +101,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   if (a.partial == nullptr || all > min(a.pieces, kMaxKinds)) {
     // Workgroups for all compute units: whole, but for the last ones, where they would keep
     // less than half of the units busy (nine requests of 256 new tokens, 2048 in all, on 32
-    // heads, 288 blocks: 153 us whole, 123 with the last 32 divided).
+    // heads, 288 blocks: 155 us whole, 116 with the last 32 divided).
     const int rest = a.partial != nullptr && a.rest ? all % a.pieces : 0;
     const int ways = 2 * rest <= a.pieces && rest > 0 ? min(a.pieces / rest, kMaxParts) : 1;
     const int whole = ways > 1 ? all - rest : all;

@@ -44,7 +44,7 @@
 // 5.1 that a large copy reaches.  From two blocks on, by the unpacking, which every block
 // repeats (12 requests of five tokens, 40 rows, 4096 in all: 47 us, 36 at 24 rows).  Short ones
 // by latencies one after the other (lengths, table, codes, the meeting): one request of 1000
-// tokens on 32 heads, 10.3 us.
+// tokens on 32 heads, 11.0 us.
 //
 // The waves meet in LDS; the partial sums of a divided tile go through the uncached
 // scratch, and the last of its workgroups to arrive on its counter adds them in order: one
@@ -58,13 +58,13 @@ constexpr int kLogWaves = 3, kWaves = 1 << kLogWaves;
 constexpr int kLogStep = 5, kStep = 1 << kLogStep;  // tokens per wave and step
 // Units that a tile counts more than it has, for what a workgroup's turn to another tile costs,
 // where there are more units than workgroups
-// (24 requests of 17 to 4096 tokens on 32 heads: 87.0 us with none, 58.0 with 2, 59.5 with 4;
-// 64 of 1024 to 16384 on 8: 134.6, 130.7, 129.7; one of 131072: 40.2, 37.8, 37.3).
+// (24 requests of 17 to 4096 tokens on 32 heads: 94.3 us with none, 57.8 with 2, 59.6 with 4;
+// 64 of 1024 to 16384 on 8: 133.0, 128.2, 129.3; one of 131072: 41.4, 38.4, 37.8).
 constexpr int kLead = 2;
 // Units that a whole tile may take beyond an even share before tiles are divided: what the
-// meeting of the pieces costs.  16 requests of 1000 tokens on 8 heads (four units) 17.1 us
-// divided, 14.7 whole; four of 1000, 40 rows on 20 heads, 24.8 and 16.4; one of 1000 on 32
-// heads, which stays divided, 10.7 and 12.3.
+// meeting of the pieces costs.  four requests of 1000 tokens (four units), 40 rows on 20 heads,
+// 23.3 us divided, 16.6 whole; 16 of 1000 on 8 heads 14.3 and 14.2; one of 1000 on 32 heads,
+// which stays divided, 11.0 and 12.7.
 constexpr int kWhole = 3;
 constexpr int kTilesAt = 43;       // bit of a sum of units
 constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last workgroup's read of it
@@ -157,8 +157,8 @@ struct Shape {
   static constexpr int LOADS = D / 32 + (NG == 4 ? 2 : 1);  // DMA instructions of a step
   // 128 registers let two workgroups share a compute unit.  With several groups of 128 dims
   // V's codes and scales do not fit them, and are read from LDS as they are needed (12 requests
-  // of five tokens with groups of 32: 53.5 us; all at once, one workgroup a unit and four
-  // steps in flight, 56.6).
+  // of five tokens with groups of 32, as first built: 53.5 us; all at once, one workgroup a unit
+  // and four steps in flight, 56.6).
   static constexpr bool LATE = NG > 1 && D == 128;
   static constexpr int RING = 2;  // steps of a wave in flight or in use
 };
