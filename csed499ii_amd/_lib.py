@@ -40,11 +40,15 @@ SIGNATURES = {
     "marlin_hip_native_unpack": (_i, [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp]),
     "marlin_hip_mul_2_4_native": (_i, [_vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _i, _vp, _i]),
     "marlin_hip_kv4_tables": (_i, [_vp] * 8 + [_i] * 6 + [_vp]),
+    "marlin_hip_kv4_tables_pos": (_i, [_vp] * 9 + [_i] * 6 + [_vp]),
     "marlin_hip_kv4_append": (_i, [_vp] * 4 + [_i] * 3 + [_ll] * 4 + [_i] * 5 + [_vp]),
     "marlin_hip_kv4_gather": (_i, [_vp] * 4 + [_i] * 8 + [_vp]),
     "marlin_hip_kv4_attention": (_i, [_vp] * 7 + [_i] * 5 + [_ll] * 2 + [_i] * 6 + [_f, _i, _i, _vp]),
     "marlin_hip_kv4_attention_ctx": (_i, [_vp] * 8 + [_i] * 5 + [_ll] * 2 + [_i] * 6 + [_f, _i, _i, _vp]),
     "marlin_hip_kv4_plan": (_i, [_i] * 8 + [ctypes.POINTER(_i)]),
+    "marlin_hip_rotary_angles": (_i, [_vp] * 3 + [_i] * 2 + [ctypes.c_double, _i, _vp]),
+    "marlin_hip_rotary": (_i, [_vp] * 3 + [_i] * 4 + [_ll] * 4 + [_i] * 3 + [_vp]),
+    "marlin_hip_kv4_append_rotary": (_i, [_vp] * 7 + [_i] * 5 + [_ll] * 8 + [_i] * 6 + [_vp]),
     "marlin_hip_last_error": (ctypes.c_char_p, []),
 }
 

@@ -5,6 +5,7 @@
 
 #include "kv4_device.h"
 #include "kv4_host.h"
+#include "kv4_rows.h"
 
 namespace kv4 {
 
@@ -33,6 +34,7 @@ struct TableArgs {
   int32_t* cu;
   int32_t* kv;
   int32_t* used;
+  int32_t* positions;  // of the new tokens; null: not wanted
   int requests, num_free, max_pages, log_page, tokens;
 };
 
@@ -119,12 +121,16 @@ __global__ __launch_bounds__(kTabThreads) void kv4_tables_kernel(TableArgs a) {
       }
       const long long slot = ((long long)page << lp) + (pos & ((1ll << lp) - 1));
       a.slots[t] = page < 0 || slot > 0x7FFFFFFFll ? -1 : (int32_t)slot;
+      if (a.positions) a.positions[t] = (int32_t)min(pos, 0x7FFFFFFFll);
     }
     tok_carry = tall;
     page_carry = pall;
     if (blockIdx.x != 0 && tall >= t_hi) return;  // (the first workgroup writes every request's sums)
   }
-  for (uint32_t t = max(t_lo, tok_carry) + tid; t < t_hi; t += kTabThreads) a.slots[t] = -1;
+  for (uint32_t t = max(t_lo, tok_carry) + tid; t < t_hi; t += kTabThreads) {
+    a.slots[t] = -1;
+    if (a.positions) a.positions[t] = 0;
+  }
   if (blockIdx.x == 0 && tid == 0) {
     a.cu[a.requests] = (int32_t)tok_carry;
     a.used[0] = (int32_t)page_carry;
@@ -137,39 +143,6 @@ __global__ __launch_bounds__(kTabThreads) void kv4_tables_kernel(TableArgs a) {
 // Bound by memory: 2 D bytes of fp16 and D/2 + 2 NG of codes and scales a row.
 // ---------------------------------------------------------------------------
 
-constexpr int kRowThreads = 256;
-
-struct RowArgs {
-  void* k;
-  void* v;
-  uint8_t* cache;
-  const int32_t* slots;
-  long long kt, kh, vt, vh;  // strides in elements
-  int tokens, heads, log_page, num_pages;
-};
-
-// (In fp32 with a flag for NaN, over the lanes by shuffles, and codes inserted one by one, the
-// append took 24.5 us where it now takes 20.0: it was bound by its operations.)
-// Bits of the largest |x| over the 8 dims and the G/8 lanes of a scale group: of fp16 and of
-// bf16 the bits without the sign order as the values do, and a NaN's are above infinity's.
-template <int G>
-__device__ __forceinline__ uint32_t group_max(const u32x4& raw) {
-  typedef uint16_t pair __attribute__((ext_vector_type(2)));
-  auto magnitude = [](uint32_t w) { return __builtin_bit_cast(pair, w & 0x7FFF7FFFu); };
-  const pair p = __builtin_elementwise_max(__builtin_elementwise_max(magnitude(raw.x), magnitude(raw.y)),
-                                           __builtin_elementwise_max(magnitude(raw.z), magnitude(raw.w)));
-  uint32_t m = max((uint32_t)p.x, (uint32_t)p.y);
-  auto over = [&](auto ctrl) {
-    constexpr int c = decltype(ctrl)::value;
-    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, c, 0xF, 0xF, true));
-  };
-  over(Int<0xB1>());                            // lanes 1 0 3 2 of four
-  over(Int<0x4E>());                            // 2 3 0 1
-  if constexpr (G >= 64) over(Int<0x141>());    // 7 ... 0 of eight
-  if constexpr (G >= 128) over(Int<0x140>());   // 15 ... 0 of sixteen
-  return m;
-}
-
 // Eight dims a thread: 16 bytes of a row, a word of codes.  A workgroup writes consecutive
 // tokens of one head, so that the words of a block's lines, which four tokens share in V,
 // meet in one L2 (a workgroup of one token's heads: 27.4 us where this took 24.5; read back
@@ -177,51 +150,17 @@ __device__ __forceinline__ uint32_t group_max(const u32x4& raw) {
 // a large copy reaches, read back 18.0; 24 tokens 3.1, the latency of slot, row and write.
 template <int D, int NG, int TYPE>
 __global__ __launch_bounds__(kRowThreads) void kv4_append_kernel(RowArgs a) {
-  constexpr int B = D / 8, G = D / NG;
+  constexpr int B = D / 8;
   const int token = (int)(blockIdx.x / (unsigned)a.heads * (kRowThreads / B) + threadIdx.x / B);
   const int head = (int)(blockIdx.x % (unsigned)a.heads), b = threadIdx.x % B;
   const bool is_v = blockIdx.y != 0;
   if (token >= a.tokens) return;
   const int slot = a.slots[token];
-  const int T = 1 << a.log_page;
   if (slot < 0 || (slot >> a.log_page) >= a.num_pages) return;  // (all lanes of the row)
   const uint16_t* src = static_cast<const uint16_t*>(is_v ? a.v : a.k);
   src += is_v ? token * a.vt + head * a.vh : token * a.kt + head * a.kh;
   const u32x4 raw = *reinterpret_cast<const u32x4*>(src + 8 * b);
-  float x[8];
-  unpack8<TYPE>(raw, x);
-  const uint32_t bits = group_max<G>(raw);
-  const float amax = TYPE == F16 ? (float)__builtin_bit_cast(_Float16, (uint16_t)bits) : __builtin_bit_cast(float, bits << 16);
-  // the weights' quantizer: fp16(max * 2/15), saturating (fminf would drop a NaN)
-  float scaled = amax * (2.0f / 15.0f);
-  if (scaled > kScaleMax) {  // the quotients stay finite
-    scaled = kScaleMax;
-#pragma unroll
-    for (int i = 0; i < 8; i++) x[i] = __builtin_amdgcn_fmed3f(x[i], -8.f * kScaleMax, 8.f * kScaleMax);
-  }
-  const _Float16 s16 = (_Float16)scaled;
-  const float s = (float)s16;
-  // x / s correctly rounded where that decides a code: one Newton step on x * (1 / s), within
-  // +-8 (ties such as 2.5 are exact and must stay so).  Four codes are summed in fp32, where
-  // 16 bits are exact: 8 + 8 16 + 8 16^2 + 8 16^3 is their offset.
-  const float inv = __builtin_amdgcn_rcpf(s);
-  float half[2] = {34952.f, 34952.f};
-#pragma unroll
-  for (int i = 0; i < 8; i++) {
-    const float q0 = x[i] * inv;
-    const float q = __builtin_fmaf(__builtin_fmaf(-q0, s, x[i]), inv, q0);
-    const float c = __builtin_amdgcn_fmed3f(__builtin_rintf(q), -8.f, 7.f);
-    half[i / 4] = __builtin_fmaf(c, (float)(1 << (4 * (i % 4))), half[i / 4]);
-  }
-  uint32_t word = (uint32_t)half[0] | (uint32_t)half[1] << 16;
-  if (!(s > 0.f)) word = 0x88888888u;
-  const int o = slot & (T - 1);
-  uint8_t* block = a.cache + ((size_t)(slot >> a.log_page) * a.heads + head) * block_bytes<D, NG>(T);
-  *reinterpret_cast<uint32_t*>(block + (is_v ? v_word<D>(T, o, b) : k_word<D>(o, b))) = word;
-  if (b % (G / 8) == 0) {
-    const int n = b / (G / 8);
-    *reinterpret_cast<_Float16*>(block + (is_v ? v_scale<D, NG>(T, o, n) : k_scale<D, NG>(T, o, n))) = s16;
-  }
+  write_row<D, NG, TYPE>(a, slot, head, b, is_v, raw);
 }
 
 template <int D, int NG, int TYPE>
@@ -272,9 +211,9 @@ int rows(bool append, const RowArgs& a, int head_dim, int ng, int dtype, hipStre
 
 extern "C" {
 
-int marlin_hip_kv4_tables(const void* context_lens, const void* new_lens, const void* free_pages, void* block_table,
-                          void* slots, void* cu_new, void* kv_lens, void* pages_used, int requests, int num_free,
-                          int max_pages, int page_size, int tokens, int dev, hipStream_t stream) {
+int marlin_hip_kv4_tables_pos(const void* context_lens, const void* new_lens, const void* free_pages, void* block_table,
+                              void* slots, void* cu_new, void* kv_lens, void* pages_used, void* positions, int requests,
+                              int num_free, int max_pages, int page_size, int tokens, int dev, hipStream_t stream) {
   if (requests < 0 || num_free < 0 || max_pages < 0 || tokens < 0)
     return kv4::refuse("kv4_tables takes no negative sizes");
   if (!kv4::page_ok(page_size)) return kv4::refuse("the KV cache's page_size must be 16, 32, 64, 128 or 256");
@@ -291,6 +230,7 @@ int marlin_hip_kv4_tables(const void* context_lens, const void* new_lens, const 
   a.cu = static_cast<int32_t*>(cu_new);
   a.kv = static_cast<int32_t*>(kv_lens);
   a.used = static_cast<int32_t*>(pages_used);
+  a.positions = static_cast<int32_t*>(positions);
   a.requests = requests;
   a.num_free = num_free;
   a.max_pages = max_pages;
@@ -299,6 +239,13 @@ int marlin_hip_kv4_tables(const void* context_lens, const void* new_lens, const 
   const unsigned blocks = tokens > 0 ? ((unsigned)tokens + kv4::kTabTokens - 1) / kv4::kTabTokens : 1;
   hipLaunchKernelGGL(kv4::kv4_tables_kernel, dim3(blocks), dim3(kv4::kTabThreads), 0, stream, a);
   return sm24::launch_error(hipGetLastError());
+}
+
+int marlin_hip_kv4_tables(const void* context_lens, const void* new_lens, const void* free_pages, void* block_table,
+                          void* slots, void* cu_new, void* kv_lens, void* pages_used, int requests, int num_free,
+                          int max_pages, int page_size, int tokens, int dev, hipStream_t stream) {
+  return marlin_hip_kv4_tables_pos(context_lens, new_lens, free_pages, block_table, slots, cu_new, kv_lens, pages_used,
+                                   nullptr, requests, num_free, max_pages, page_size, tokens, dev, stream);
 }
 
 int marlin_hip_kv4_append(const void* k, const void* v, void* cache, const void* slots, int tokens, int kv_heads,

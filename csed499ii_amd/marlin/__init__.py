@@ -33,6 +33,12 @@ from ._kv4 import (
     kv4_tables,
     plan_kv4_attention,
 )
+from ._rotary import (
+    kv4_append_rotary,
+    rotary,
+    rotary_angles,
+    rotary_frequencies,
+)
 from ._semi_structured_conversions import (
     mask_creator,
     sparse_semi_structured_from_dense_cutlass,
@@ -67,6 +73,10 @@ __all__ = [
     "kv4_gather",
     "kv4_attention",
     "plan_kv4_attention",
+    "rotary_frequencies",
+    "rotary_angles",
+    "rotary",
+    "kv4_append_rotary",
 ]
 
 

@@ -120,7 +120,7 @@ def kv4_cache(num_pages: int, kv_heads: int, head_dim: int, page_size: int = 16,
 
 
 def kv4_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: torch.Tensor,
-               block_table: torch.Tensor, num_tokens: int, page_size: int):
+               block_table: torch.Tensor, num_tokens: int, page_size: int, return_positions: bool = False):
     """Block tables and slot maps of a step, from the requests' lengths, in one launch.
 
     Request ``i`` holds ``context_lens[i]`` tokens and gets ``new_lens[i]`` more (int32
@@ -135,7 +135,9 @@ def kv4_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: t
     * ``kv_lens [R]``: ``context + new``, cut at the table's ``P * page_size`` (where that may
       happen :func:`kv4_attention` needs ``context_lens``, too, for the positions);
     * ``pages_used [1]``: pages wanted from ``free_pages``.  More than ``F`` means that some
-      requests have entries of -1 in the table, whose tokens :func:`kv4_attention` leaves out.
+      requests have entries of -1 in the table, whose tokens :func:`kv4_attention` leaves out;
+    * with ``return_positions`` ``positions [num_tokens]``: the new tokens' positions in their
+      requests, for :func:`rotary_angles`; 0 past the last one.
 
     ``num_tokens`` is the length of the slot map, an upper bound known on the host (a
     captured step may pass its padded size); tokens past it get no slot and no page, but count
@@ -166,15 +168,17 @@ def kv4_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: t
                                f"{block_table.size(0)}")
     if num_tokens < 0:
         raise RuntimeError("num_tokens must not be negative")
-    out = context_lens.new_empty(num_tokens + 2 * R + 2)
-    slots, cu, kv, used = out.split_with_sizes((num_tokens, R + 1, R, 1))
+    more = num_tokens if return_positions else 0
+    out = context_lens.new_empty(num_tokens + 2 * R + 2 + more)
+    slots, cu, kv, used, positions = out.split_with_sizes((num_tokens, R + 1, R, 1, more))
     at = out.data_ptr()
-    err = _lib.load().marlin_hip_kv4_tables(ctx, new, free, table, at, at + 4 * num_tokens,
-                                            at + 4 * (num_tokens + R + 1), at + 4 * (num_tokens + 2 * R + 1), R, F,
-                                            P, page_size, num_tokens, dev, _raw_stream(dev))
+    cu_at = at + 4 * num_tokens
+    err = _lib.load().marlin_hip_kv4_tables_pos(ctx, new, free, table, at, cu_at, cu_at + 4 * (R + 1),
+                                                cu_at + 4 * (2 * R + 1), cu_at + 4 * (2 * R + 2) if more else 0, R, F, P,
+                                                page_size, num_tokens, dev, _raw_stream(dev))
     if err:
         _raise(err)
-    return slots, cu, kv, used
+    return (slots, cu, kv, used, positions) if return_positions else (slots, cu, kv, used)
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor,

@@ -195,6 +195,12 @@ int marlin_hip_kv4_tables(const void* context_lens, const void* new_lens, const 
                           void* slots, void* cu_new, void* kv_lens, void* pages_used, int requests, int num_free,
                           int max_pages, int page_size, int tokens, int dev, hipStream_t stream);
 
+/* The same, with the new tokens' positions in their requests written to positions[tokens] (0 past the
+ * last one; null: not wanted). */
+int marlin_hip_kv4_tables_pos(const void* context_lens, const void* new_lens, const void* free_pages, void* block_table,
+                              void* slots, void* cu_new, void* kv_lens, void* pages_used, void* positions, int requests,
+                              int num_free, int max_pages, int page_size, int tokens, int dev, hipStream_t stream);
+
 /* Quantizes rows k, v [tokens][kv_heads][head_dim] into the cache's slots[tokens]; strides
  * in elements, multiples of 8, rows 16-byte aligned.  Slots that are negative or past the
  * last page are skipped. */
@@ -243,6 +249,34 @@ int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* b
  * stream's split-K scratch). */
 int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, int groupsize, int max_q, int max_kv,
                         int sms, int* out);
+
+/* ---- Rotary positions (no counterpart in the reference) ----
+ *
+ * Of a row's first rotary_dim dims the pairs (i, i + rotary_dim / 2), or interleaved (2 i, 2 i + 1),
+ * are turned by their token's angles: a' = a cos - b sin, b' = b cos + a sin, computed in fp64. */
+
+/* angles [tokens][pairs][2] (fp64: cos, sin, times factor) of positions[tokens] (int32) by
+ * freqs[pairs]: turns a position in units of 2^-64, modulo a turn. */
+int marlin_hip_rotary_angles(const void* positions, const void* freqs, void* angles, int tokens, int pairs,
+                             double factor, int dev, hipStream_t stream);
+
+/* Turns rows x [tokens][heads][head_dim] (dtype 0: fp16, 1: bf16; head_dim a multiple of 8, 1024 at most;
+ * strides in elements, multiples of 8, rows 16-byte aligned) by angles [tokens][rotary_dim / 2][2] into out,
+ * which is x itself, with its strides, or does not overlap it. */
+int marlin_hip_rotary(const void* x, const void* angles, void* out, int tokens, int heads, int head_dim, int rotary_dim,
+                      long long x_token_stride, long long x_head_stride, long long out_token_stride,
+                      long long out_head_stride, int interleaved, int dtype, int dev, hipStream_t stream);
+
+/* marlin_hip_rotary of q [tokens][q_heads][head_dim] into q_out (as out above; q_heads 0: none) and
+ * marlin_hip_kv4_append of k, turned and rounded to its type, and v, in one launch and to the same
+ * bits.  q_out must not overlap k or v. */
+int marlin_hip_kv4_append_rotary(const void* q, const void* k, const void* v, const void* angles, void* q_out,
+                                 void* cache, const void* slots, int tokens, int q_heads, int kv_heads, int head_dim,
+                                 int rotary_dim, long long q_token_stride, long long q_head_stride,
+                                 long long k_token_stride, long long k_head_stride, long long v_token_stride,
+                                 long long v_head_stride, long long out_token_stride, long long out_head_stride,
+                                 int page_size, int num_pages, int groupsize, int interleaved, int dtype, int dev,
+                                 hipStream_t stream);
 
 /* Message describing the last MARLIN_HIP_ERR_* of the calling thread. */
 const char* marlin_hip_last_error(void);
