@@ -46,6 +46,10 @@ SIGNATURES = {
     "marlin_hip_kv4_attention": (_i, [_vp] * 7 + [_i] * 5 + [_ll] * 2 + [_i] * 6 + [_f, _i, _i, _vp]),
     "marlin_hip_kv4_attention_ctx": (_i, [_vp] * 8 + [_i] * 5 + [_ll] * 2 + [_i] * 6 + [_f, _i, _i, _vp]),
     "marlin_hip_kv4_plan": (_i, [_i] * 8 + [ctypes.POINTER(_i)]),
+    "marlin_hip_kv4_free_pages": (_i, [_vp] * 5 + [_i] * 5 + [_vp]),
+    "marlin_hip_kv4_copy_pages": (_i, [_vp, _i, _vp, _vp] + [_i] * 7 + [_vp]),
+    "marlin_hip_kv4_fork": (_i, [_vp, _i] + [_vp] * 8 + [_i] * 10 + [_vp]),
+    "marlin_hip_kv4_compact": (_i, [_vp, _i] + [_vp] * 5 + [_i] * 8 + [_vp]),
     "marlin_hip_rotary_angles": (_i, [_vp] * 3 + [_i] * 2 + [ctypes.c_double, _i, _vp]),
     "marlin_hip_rotary": (_i, [_vp] * 3 + [_i] * 4 + [_ll] * 4 + [_i] * 3 + [_vp]),
     "marlin_hip_kv4_append_rotary": (_i, [_vp] * 7 + [_i] * 5 + [_ll] * 8 + [_i] * 6 + [_vp]),

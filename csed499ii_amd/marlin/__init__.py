@@ -33,6 +33,13 @@ from ._kv4 import (
     kv4_tables,
     plan_kv4_attention,
 )
+from ._kv4_pages import (
+    kv4_compact,
+    kv4_copy_pages,
+    kv4_fork,
+    kv4_free_pages,
+    kv4_layers,
+)
 from ._rotary import (
     kv4_append_rotary,
     rotary,
@@ -73,6 +80,11 @@ __all__ = [
     "kv4_gather",
     "kv4_attention",
     "plan_kv4_attention",
+    "kv4_layers",
+    "kv4_free_pages",
+    "kv4_copy_pages",
+    "kv4_fork",
+    "kv4_compact",
     "rotary_frequencies",
     "rotary_angles",
     "rotary",

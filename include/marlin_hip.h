@@ -250,6 +250,43 @@ int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* b
 int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, int groupsize, int max_q, int max_kv,
                         int sms, int* out);
 
+/* ---- Pages of the 4-bit KV cache (no counterpart in the reference) ----
+ *
+ * A page is held if an entry of a written token names it: block_table[i][j] [requests][max_pages] with
+ * j * page_size < kv_lens[i].  `caches` is a host array of the layers' caches, which have one
+ * geometry and num_pages pages; it is read before the call returns. */
+
+/* free_pages[num_pages]: the pages that are not held, in ascending order, then -1; count[1]: how many.
+ * workspace: num_pages bytes rounded up to 16, 16-byte aligned. */
+int marlin_hip_kv4_free_pages(const void* block_table, const void* kv_lens, void* free_pages, void* count,
+                              void* workspace, int requests, int max_pages, int page_size, int num_pages, int dev,
+                              hipStream_t stream);
+
+/* Page from[i] to page to[i] in every layer, for `pairs` pairs (one with an entry that is no page: skipped).
+ * No page may be a target twice, nor the target of one pair and the source of another. */
+int marlin_hip_kv4_copy_pages(const void* const* caches, int layers, const void* from, const void* to, int pairs,
+                              int kv_heads, int head_dim, int page_size, int num_pages, int groupsize, int dev,
+                              hipStream_t stream);
+
+/* Moves the n held pages to the numbers 0 ... n - 1 in every layer (those past them, ascending, to the free
+ * ones among them) and writes the table with the new numbers (-1 past a request's tokens and for entries that
+ * are no page), which is not block_table itself; counts[2]: n, and the pages moved.  workspace: 13 bytes a page
+ * of num_pages rounded up to 16, 16-byte aligned. */
+int marlin_hip_kv4_compact(const void* const* caches, int layers, const void* block_table, const void* kv_lens,
+                           void* new_table, void* counts, void* workspace, int requests, int max_pages, int kv_heads,
+                           int head_dim, int page_size, int num_pages, int groupsize, int dev, hipStream_t stream);
+
+/* New request i of new_requests from request parents[i] (outside [0, requests): an empty one): its entries
+ * and its length (cut at the table's width).  Full pages are shared; a last one that is not full is kept by the
+ * first new request that holds it, unless one holds it as a full page, and copied (the written tokens, in
+ * fours) for the others to the next of free_pages[num_free] in every layer (none left: -1).  pages_used[1]:
+ * pages wanted.  new_table [new_requests][max_pages] and new_lens are not the old ones.  workspace: 4 bytes a
+ * new request.  Requests may share a page at the same place of their rows only. */
+int marlin_hip_kv4_fork(const void* const* caches, int layers, const void* block_table, const void* kv_lens,
+                        const void* parents, const void* free_pages, void* new_table, void* new_lens, void* pages_used,
+                        void* workspace, int requests, int new_requests, int num_free, int max_pages, int kv_heads,
+                        int head_dim, int page_size, int num_pages, int groupsize, int dev, hipStream_t stream);
+
 /* ---- Rotary positions (no counterpart in the reference) ----
  *
  * Of a row's first rotary_dim dims the pairs (i, i + rotary_dim / 2), or interleaved (2 i, 2 i + 1),
