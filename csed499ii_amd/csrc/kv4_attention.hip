@@ -6,11 +6,9 @@
 #include <atomic>
 
 #include "kv4_host.h"
-#include "kv4_split.h"
+#include "kv4_prompt.h"
 
 namespace kv4 {
-
-hipError_t launch_prompt(const AttnArgs& a, int workgroups, int head_dim, int ng, int dtype, hipStream_t stream);
 
 // Requests of at most so many rows (new tokens times the query heads of a kv head) go to the
 // split kernel, the others to the prompt kernel, each of which passes over the other's.  The
@@ -113,6 +111,149 @@ int check(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int
   return MARLIN_HIP_OK;
 }
 
+// ---------------------------------------------------------------------------
+// The prefix that the requests of a group share: the whole pages, from the first on, that are the
+// same in their tables and lie within their contexts.  A workgroup for each group compares every
+// request's row with the first one's, all columns and requests at once; one more for the requests of
+// no group.  Once a step, for all layers.
+// ---------------------------------------------------------------------------
+
+constexpr int kSharedThreads = 1024, kSharedRound = 1024;
+
+struct SharedArgs {
+  const int32_t* table;
+  const int32_t* ctx;
+  const int32_t* cu_q;       // null: a token each
+  const int32_t* cu_groups;  // [groups + 1]
+  int32_t* lens;             // [groups] tokens of the prefix
+  int32_t* leads;            // [groups] a request that holds it
+  int32_t* cu_rows;          // [groups + 1] first token of each group
+  int32_t* start;            // [requests] tokens of the prefix, 0 for a request that does not share it
+  int requests, groups, max_pages, log_page;
+};
+
+__global__ __launch_bounds__(kSharedThreads) void kv4_shared_kernel(SharedArgs a) {
+  __shared__ int first[kSharedRound];  // column in which a request's row differs
+  __shared__ int lead, least, sharers;
+  const int tid = threadIdx.x, g = (int)blockIdx.x;
+  auto border = [&](int i) { return min(max(a.cu_groups[i], 0), a.requests); };
+  auto token = [&](int r) { return a.cu_q == nullptr ? r : max(a.cu_q[r], 0); };
+  if (g == a.groups) {
+    const int r0 = border(0), r1 = border(a.groups);
+    for (int r = tid; r < a.requests; r += kSharedThreads)
+      if (r < r0 || r >= r1) a.start[r] = 0;
+    if (tid == 0) a.cu_rows[a.groups] = token(r1);
+    return;
+  }
+  const int r0 = border(g), r1 = max(border(g + 1), r0);
+  // whole pages that may be shared: none of a request without new tokens
+  auto pages = [&](int r) {
+    if (a.cu_q != nullptr && a.cu_q[r + 1] <= a.cu_q[r]) return 0;
+    return min(max(a.ctx[r], 0) >> a.log_page, a.max_pages);
+  };
+  if (tid == 0) lead = 0x7FFFFFFF, least = 0x7FFFFFFF, sharers = 0;
+  __syncthreads();
+  for (int r = r0 + tid; r < r1; r += kSharedThreads)
+    if (pages(r) > 0) {
+      atomicMin(&lead, r);
+      break;
+    }
+  __syncthreads();
+  const int leader = lead;
+  const bool any = leader < r1;
+  const int most = any ? pages(leader) : 0;
+  const int32_t* lead_row = a.table + (size_t)(any ? leader : r0) * a.max_pages;
+  for (int from = r0; from < r1; from += kSharedRound) {
+    const int n = min(r1 - from, kSharedRound);
+    __syncthreads();  // the round before is done with LDS
+    if (tid < n) first[tid] = min(pages(from + tid), most);
+    __syncthreads();
+    for (int j0 = 0; j0 < most; j0 += kSharedThreads) {
+      // columns fill the threads as far as there are, requests the rest
+      const int width = min(most - j0, kSharedThreads), side = kSharedThreads / width;
+      const int i0 = tid / width, j = j0 + tid - i0 * width;
+      if (i0 >= side) continue;
+      const int want = lead_row[j];
+#pragma unroll 8
+      for (int i = i0; i < n; i += side)
+        if (j < first[i] && a.table[(size_t)(from + i) * a.max_pages + j] != want) atomicMin(&first[i], j);
+    }
+    __syncthreads();
+    if (tid < n) {
+      const int common = first[tid];
+      a.start[from + tid] = common;
+      if (common > 0) {
+        atomicMin(&least, common);
+        atomicAdd(&sharers, 1);
+      }
+    }
+  }
+  __syncthreads();
+  const int len = sharers > 1 ? least << a.log_page : 0;
+  for (int from = r0; from < r1; from += kSharedRound)
+    if (from + tid < r1) a.start[from + tid] = a.start[from + tid] > 0 ? len : 0;
+  if (tid == 0) {
+    a.lens[g] = len;
+    a.leads[g] = any ? leader : 0;
+    a.cu_rows[g] = token(r0);
+  }
+}
+
+struct Problem {
+  int tokens, requests, q_heads, kv_heads, head_dim, ng, max_q, max_kv, dtype, dev, cus;
+  hipStream_t stream;
+};
+
+// Every launch of a call, or of one pass of it, on the kernels that `c` names.
+template <int FORM>
+int attend(AttnArgs a, const Problem& p, const Choice& c) {
+  int err = MARLIN_HIP_OK;
+  a.max_rows = c.split ? c.few_rows : 0;
+  for (a.first = 0; a.first < p.requests; a.first += kMaxRequests) {
+    a.requests = p.requests - a.first < kMaxRequests ? p.requests - a.first : kMaxRequests;
+    if (c.prompts) {
+      const Plan plan = prompt_plan(p.tokens, a.requests, p.q_heads, p.kv_heads, p.max_q, p.max_kv, a.max_rows, p.cus);
+      if (plan.workgroups < 0) return refuse("kv4_attention: too many rows for one launch");
+      a.pieces = plan.pieces;
+      a.rest = plan.rest;
+      if (plan.split) {
+        const size_t rows = (size_t)plan.pieces * p.kv_heads * kPromptRows;
+        err = sm24::get_scratch(p.dev, p.stream, (rows * p.head_dim + 2 * rows * 2) * sizeof(float), &a.counters, &a.partial);
+        if (err != MARLIN_HIP_OK) return err;
+        if (a.partial) a.partial_ml = a.partial + rows * p.head_dim;  // (null: blocks stay whole)
+      }
+      err = sm24::launch_error(launch_prompt<FORM>(a, plan.workgroups, p.head_dim, p.ng, p.dtype, p.stream));
+      if (err != MARLIN_HIP_OK) return err;
+      a.partial = nullptr;
+    }
+    if (c.split) {
+      // (through a window a row's tokens are no more than the window's and the sinks')
+      const long long reach = FORM == WINDOW ? (long long)a.window + a.sinks + c.split_q + 2 * kStep : p.max_kv;
+      const Plan plan = kv4::plan(a.requests, p.q_heads, p.kv_heads, c.split_q, reach < p.max_kv ? (int)reach : p.max_kv, p.cus);
+      a.log_kw = plan.log_kw;
+      a.lead = plan.lead;
+      a.slots = 2 * p.cus;
+      if (plan.split) {
+        const size_t rows = (size_t)plan.workgroups * 2 * 16 * (kWaves >> plan.log_kw);
+        err = sm24::get_scratch(p.dev, p.stream, rows * (p.head_dim + 2) * sizeof(float), &a.counters, &a.partial);
+        if (err != MARLIN_HIP_OK) return err;
+        // (null while the stream is captured and has no scratch yet: tiles stay whole)
+        if (a.partial) a.partial_ml = a.partial + rows * p.head_dim;
+      }
+      err = sm24::launch_error(launch_split<FORM>(a, plan.workgroups, p.head_dim, p.ng, p.dtype, p.stream));
+      if (err != MARLIN_HIP_OK) return err;
+      a.partial = nullptr;
+    }
+    a.kv_lens += a.requests;
+    if (FORM == SHARED && a.leads != nullptr) a.leads += a.requests;
+    else a.table += (size_t)a.requests * (size_t)a.max_pages;
+    if (FORM == SHARED && a.start != nullptr) a.start += a.requests;
+    if (a.cu_q) a.cu_q += a.requests;
+    if (a.ctx) a.ctx += a.requests;
+  }
+  return MARLIN_HIP_OK;
+}
+
 }  // namespace kv4
 
 extern "C" {
@@ -143,12 +284,22 @@ int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, i
   return MARLIN_HIP_OK;
 }
 
-int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* block_table, const void* kv_lens,
-                                 const void* cu_q, const void* context_lens, void* out, void* lse, int tokens,
-                                 int requests, int q_heads, int kv_heads, int head_dim, long long q_token_stride,
-                                 long long q_head_stride, int page_size, int num_pages, int max_pages, int groupsize,
-                                 int max_q, int max_kv, float scale, int dtype, int dev, hipStream_t stream) {
-  using namespace kv4;
+}  // extern "C"
+
+namespace kv4 {
+
+// The prefix that groups of requests share (marlin_hip_kv4_shared).
+struct Prefix {
+  const int32_t *lens, *leads, *cu_rows, *start;
+  int groups;
+  float* workspace;
+};
+
+int attention(const void* q, const void* cache, const void* block_table, const void* kv_lens, const void* cu_q,
+              const void* context_lens, void* out, void* lse, int tokens, int requests, int q_heads, int kv_heads,
+              int head_dim, long long q_token_stride, long long q_head_stride, int page_size, int num_pages, int max_pages,
+              int groupsize, int max_q, int max_kv, float scale, int dtype, int dev, hipStream_t stream, int window,
+              int sinks, const Prefix* prefix) {
   // (a bound that may be far above what there is, e.g. a fixed one of all steps: the choice of
   // kernels and their grids go by rows that exist)
   if (tokens >= 0 && max_q > tokens) max_q = tokens;
@@ -186,54 +337,78 @@ int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* b
   a.group = group;
   a.max_q = max_q;
   a.c1 = scale * 1.4426950408889634f;
-  const int cus = compute_units(dev);
-  const Choice c = choose(tokens, requests, q_heads, kv_heads, head_dim, ng, max_q, cu_q != nullptr, cus);
-  a.max_rows = c.split ? c.few_rows : 0;
-  for (a.first = 0; a.first < requests; a.first += kMaxRequests) {
-    a.requests = requests - a.first < kMaxRequests ? requests - a.first : kMaxRequests;
-    if (c.prompts) {
-      const Plan p = prompt_plan(tokens, a.requests, q_heads, kv_heads, max_q, max_kv, a.max_rows, cus);
-      if (p.workgroups < 0) return refuse("kv4_attention: too many rows for one launch");
-      a.pieces = p.pieces;
-      a.rest = p.rest;
-      if (p.split) {
-        const size_t rows = (size_t)p.pieces * kv_heads * kPromptRows;
-        err = sm24::get_scratch(dev, stream, (rows * head_dim + 2 * rows * 2) * sizeof(float), &a.counters, &a.partial);
-        if (err != MARLIN_HIP_OK) return err;
-        if (a.partial) a.partial_ml = a.partial + rows * head_dim;  // (null: blocks stay whole)
-      }
-      err = sm24::launch_error(launch_prompt(a, p.workgroups, head_dim, ng, dtype, stream));
-      if (err != MARLIN_HIP_OK) return err;
-      a.partial = nullptr;
-    }
-    if (c.split) {
-      const Plan p = plan(a.requests, q_heads, kv_heads, c.split_q, max_kv, cus);
-      a.log_kw = p.log_kw;
-      a.lead = p.lead;
-      a.slots = 2 * cus;
-      if (p.split) {
-        const size_t rows = (size_t)p.workgroups * 2 * 16 * (kWaves >> p.log_kw);
-        err = sm24::get_scratch(dev, stream, rows * (head_dim + 2) * sizeof(float), &a.counters, &a.partial);
-        if (err != MARLIN_HIP_OK) return err;
-        // (null while the stream is captured and has no scratch yet: tiles stay whole)
-        if (a.partial) a.partial_ml = a.partial + rows * head_dim;
-      }
-      dispatch(head_dim, ng, [&](auto d, auto g) {
-        constexpr int D = decltype(d)::value, NG = decltype(g)::value;
-        const dim3 grid((unsigned)p.workgroups), block(64 * kWaves);
-        if (dtype == F16) hipLaunchKernelGGL((kv4_split_kernel<D, NG, F16>), grid, block, 0, stream, a);
-        else hipLaunchKernelGGL((kv4_split_kernel<D, NG, BF16>), grid, block, 0, stream, a);
-      });
-      err = sm24::launch_error(hipGetLastError());
-      if (err != MARLIN_HIP_OK) return err;
-      a.partial = nullptr;
-    }
-    a.kv_lens += a.requests;
-    a.table += (size_t)a.requests * max_pages;
-    if (a.cu_q) a.cu_q += a.requests;
-    if (a.ctx) a.ctx += a.requests;
-  }
-  return MARLIN_HIP_OK;
+  a.window = window;
+  a.sinks = sinks;
+  const Problem p{tokens, requests, q_heads, kv_heads, head_dim, ng, max_q, max_kv, dtype, dev, compute_units(dev), stream};
+  const Choice c = choose(tokens, requests, q_heads, kv_heads, head_dim, ng, max_q, cu_q != nullptr, p.cus);
+  if (window > 0) return attend<WINDOW>(a, p, c);
+  if (prefix == nullptr) return attend<PLAIN>(a, p, c);
+  a.before = prefix->workspace;
+  a.before_ml = prefix->workspace + (size_t)tokens * q_heads * head_dim;
+  // First pass: a group is a request whose tokens are the prefix and whose rows, behind it, see all of them.
+  // One kernel takes all groups, by the rows that a group has on average.
+  AttnArgs b = a;
+  b.kv_lens = b.ctx = prefix->lens;
+  b.leads = prefix->leads;
+  b.cu_q = prefix->cu_rows;
+  b.max_q = tokens;
+  Problem first = p;
+  first.requests = prefix->groups;
+  first.max_q = tokens;
+  const int average = (tokens + prefix->groups - 1) / prefix->groups;
+  Choice one{};
+  one.prompts = (long long)average * group > split_rows(prefix->groups, kv_heads, head_dim, ng, p.cus);
+  one.split = !one.prompts;
+  one.few_rows = 0x7FFFFFFF;
+  one.split_q = average;
+  err = attend<SHARED>(b, first, one);
+  if (err != MARLIN_HIP_OK) return err;
+  a.start = prefix->start;
+  return attend<SHARED>(a, p, c);
+}
+
+}  // namespace kv4
+
+extern "C" {
+
+int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* block_table, const void* kv_lens,
+                                 const void* cu_q, const void* context_lens, void* out, void* lse, int tokens,
+                                 int requests, int q_heads, int kv_heads, int head_dim, long long q_token_stride,
+                                 long long q_head_stride, int page_size, int num_pages, int max_pages, int groupsize,
+                                 int max_q, int max_kv, float scale, int dtype, int dev, hipStream_t stream) {
+  return kv4::attention(q, cache, block_table, kv_lens, cu_q, context_lens, out, lse, tokens, requests, q_heads, kv_heads,
+                        head_dim, q_token_stride, q_head_stride, page_size, num_pages, max_pages, groupsize, max_q, max_kv,
+                        scale, dtype, dev, stream, 0, 0, nullptr);
+}
+
+int marlin_hip_kv4_attention_window(const void* q, const void* cache, const void* block_table, const void* kv_lens,
+                                    const void* cu_q, const void* context_lens, void* out, void* lse, int tokens,
+                                    int requests, int q_heads, int kv_heads, int head_dim, long long q_token_stride,
+                                    long long q_head_stride, int page_size, int num_pages, int max_pages, int groupsize,
+                                    int max_q, int max_kv, float scale, int window, int sinks, int dtype, int dev,
+                                    hipStream_t stream) {
+  if (window < 1 || sinks < 0) return kv4::refuse("kv4_attention needs a window of a token at least and no negative sinks");
+  // (no position passes 2^30: as many see all)
+  if (window > 1 << 30) window = 1 << 30;
+  if (sinks > 1 << 30) sinks = 1 << 30;
+  return kv4::attention(q, cache, block_table, kv_lens, cu_q, context_lens, out, lse, tokens, requests, q_heads, kv_heads,
+                        head_dim, q_token_stride, q_head_stride, page_size, num_pages, max_pages, groupsize, max_q, max_kv,
+                        scale, dtype, dev, stream, window, sinks, nullptr);
+}
+
+int marlin_hip_kv4_attention_shared(const void* q, const void* cache, const void* block_table, const void* kv_lens,
+                                    const void* cu_q, const void* context_lens, const void* shared, void* out, void* lse,
+                                    void* workspace, int tokens, int requests, int groups, int q_heads, int kv_heads,
+                                    int head_dim, long long q_token_stride, long long q_head_stride, int page_size,
+                                    int num_pages, int max_pages, int groupsize, int max_q, int max_kv, float scale,
+                                    int dtype, int dev, hipStream_t stream) {
+  if (groups < 0) return kv4::refuse("kv4_attention takes no negative sizes");
+  const int32_t* at = static_cast<const int32_t*>(shared);
+  const kv4::Prefix prefix{at, at + groups, at + 2 * (size_t)groups, at + 3 * (size_t)groups + 1, groups,
+                           static_cast<float*>(workspace)};
+  return kv4::attention(q, cache, block_table, kv_lens, cu_q, context_lens, out, lse, tokens, requests, q_heads, kv_heads,
+                        head_dim, q_token_stride, q_head_stride, page_size, num_pages, max_pages, groupsize, max_q, max_kv,
+                        scale, dtype, dev, stream, 0, 0, groups > 0 ? &prefix : nullptr);
 }
 
 int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block_table, const void* kv_lens,
@@ -244,6 +419,24 @@ int marlin_hip_kv4_attention(const void* q, const void* cache, const void* block
   return marlin_hip_kv4_attention_ctx(q, cache, block_table, kv_lens, cu_q, nullptr, out, lse, tokens, requests,
                                       q_heads, kv_heads, head_dim, q_token_stride, q_head_stride, page_size, num_pages,
                                       max_pages, groupsize, max_q, max_kv, scale, dtype, dev, stream);
+}
+
+int marlin_hip_kv4_shared(const void* block_table, const void* context_lens, const void* cu_q, const void* cu_groups,
+                          void* shared, int requests, int groups, int max_pages, int page_size, int dev,
+                          hipStream_t stream) {
+  if (requests < 0 || groups < 0 || max_pages < 0) return kv4::refuse("kv4_shared takes no negative sizes");
+  if (!kv4::page_ok(page_size)) return kv4::refuse("the KV cache's page_size must be 16, 32, 64, 128 or 256");
+  if ((long long)max_pages * page_size > (1ll << 30)) return kv4::refuse("a block table row covers more than 2^30 tokens");
+  if (requests == 0 || groups == 0) return MARLIN_HIP_OK;
+  sm24::DeviceScope scope(dev);
+  if (!scope.ok) return MARLIN_HIP_ERR_LAUNCH;
+  int32_t* out = static_cast<int32_t*>(shared);
+  const kv4::SharedArgs a{static_cast<const int32_t*>(block_table), static_cast<const int32_t*>(context_lens),
+                          static_cast<const int32_t*>(cu_q), static_cast<const int32_t*>(cu_groups), out, out + groups,
+                          out + 2 * (size_t)groups, out + 3 * (size_t)groups + 1, requests, groups, max_pages,
+                          31 - __builtin_clz((unsigned)page_size)};
+  hipLaunchKernelGGL(kv4::kv4_shared_kernel, dim3((unsigned)groups + 1), dim3(kv4::kSharedThreads), 0, stream, a);
+  return sm24::launch_error(hipGetLastError());
 }
 
 }  // extern "C"

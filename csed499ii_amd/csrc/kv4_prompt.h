@@ -50,7 +50,7 @@ __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   return __builtin_bit_cast(uint32_t, (half2_t){(_Float16)lo, (_Float16)hi});
 }
 
-template <int D, int NG, int TYPE>
+template <int D, int NG, int TYPE, int FORM = PLAIN>
 __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnArgs a) {
   constexpr int W = kPromptWaves;
   constexpr int KU = D / 16;          // k-steps of the first product
@@ -82,9 +82,18 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   auto end_of = [&](const Request& q, int block) {
     return seen_by(q, min((block * kPromptRows + kPromptRows - 1) / G, q.n - 1));
   };
+  // (WINDOW) the tiles of tokens that some row of a block sees
+  auto reach_of = [&](const Request& q, int block) {
+    const int t0 = block * kPromptRows / G, t1 = min((block * kPromptRows + kPromptRows - 1) / G, q.n - 1);
+    return Reach(a, q, t0, t1, seen_by(q, t1), kLogTile);
+  };
+  auto tiles_in = [&](const Request& q, int block) {
+    if constexpr (FORM == WINDOW) return reach_of(q, block).steps;
+    return (end_of(q, block) + kTile - 1) / kTile;
+  };
   const int per = (a.requests + 63) / 64, r_lane = lane * per;  // a lane's requests
   int own = 0;
-  for (int r = r_lane; r < min(r_lane + per, a.requests); r++) own += blocks_of(request_of(a, r));
+  for (int r = r_lane; r < min(r_lane + per, a.requests); r++) own += blocks_of(request_of<FORM>(a, r));
   auto scan = [&](int x) {  // what the lanes before have
     int sum = x;
 #pragma unroll
@@ -116,10 +125,10 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     const int at = __builtin_ctzll(__ballot(before + own > kind));
     int i = kind - __builtin_amdgcn_readlane(before, at);
     r = at * per;
-    int n = blocks_of(request_of(a, r));
+    int n = blocks_of(request_of<FORM>(a, r));
     while (i >= n) {
       i -= n;
-      n = blocks_of(request_of(a, ++r));
+      n = blocks_of(request_of<FORM>(a, ++r));
     }
     block = n - 1 - i;
   } else {
@@ -131,12 +140,12 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         const int at = __builtin_ctzll(with);
         int i = __builtin_amdgcn_readlane(before, at);
         for (int r = at * per; r < min(at * per + per, a.requests); r++) {
-          Request q = request_of(a, r);
+          Request q = request_of<FORM>(a, r);
           set_past(a, r, q);
           const int n = blocks_of(q);
           for (int b = lane; b < n; b += 64) {
             kinds[i + b] = r * kMaxKinds + n - 1 - b;
-            kind_tiles[i + b] = max((end_of(q, n - 1 - b) + kTile - 1) / kTile, 1);
+            kind_tiles[i + b] = max(tiles_in(q, n - 1 - b), 1);
           }
           i += n;
         }
@@ -183,18 +192,26 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     const int kind = __builtin_amdgcn_readfirstlane(kinds[i]);
     r = kind / kMaxKinds, block = kind % kMaxKinds;
   }
-  Request rq = request_of(a, r);
+  Request rq = request_of<FORM>(a, r);
   set_past(a, r, rq);
   const int rows = rows_of(a, rq), row0 = block * kPromptRows;
   const int w_row0 = row0 + 32 * wave;
   // tokens that some row of the workgroup, some row of the wave and every row of it sees
   const int end = end_of(rq, block);
+  Reach reach;
+  if constexpr (FORM == WINDOW) reach = reach_of(rq, block);
+  auto token_of = [&](int tile) { return FORM == WINDOW ? reach.at(tile, kLogTile) : tile * kTile; };
+  const int tiles = FORM == WINDOW ? reach.steps : (end + kTile - 1) / kTile;
   if (most > 0) {
-    parts = max(min(most, (end + kTile - 1) / (kTile * (int)kMinShare)), 1);
+    if constexpr (FORM == WINDOW) parts = max(min(most, tiles / (int)kMinShare), 1);
+    else parts = max(min(most, (end + kTile - 1) / (kTile * (int)kMinShare)), 1);
     if (part >= parts) return;
   }
   const int w_end = w_row0 < rows ? seen_by(rq, min((w_row0 + 31) / G, rq.n - 1)) : 0;
   const int w_all = min(seen_by(rq, w_row0 / G), w_end);
+  // (WINDOW) where the wave's first window begins, and its last
+  const int w_low = FORM == WINDOW ? window_of(a, rq, w_row0 / G) : 0;
+  const int w_high = FORM == WINDOW ? window_of(a, rq, min((w_row0 + 31) / G, rq.n - 1)) : 0;
 
   typedef __attribute__((address_space(3))) uint8_t lds_u8;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_u8*)lds;
@@ -202,10 +219,14 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   // Where 64 groups of 16 tokens (16 tiles) from 64 b on begin, one a lane: the table's entries
   // as they come (a look at once would wait for them and for every load before them), then the
   // byte offset of the K codes (bit 63: no such page, which is read as the first one and masked).
-  const int tiles = (end + kTile - 1) / kTile;
   const int t0 = tiles * part / parts, t1 = tiles * (part + 1) / parts;
-  const int32_t* pages = a.table + (size_t)r * a.max_pages;
-  auto entries = [&](int b) { return pages[min((64 * b + lane) * 16, end - 1) >> a.log_page]; };
+  const int32_t* pages = pages_of<FORM>(a, r, rq);
+  // (first token of a lane's group of the block)
+  auto group_at = [&](int b) {
+    if constexpr (FORM == WINDOW) return token_of(16 * b + (lane >> 2)) + 16 * (lane & 3);
+    return (64 * b + lane) * 16;
+  };
+  auto entries = [&](int b) { return pages[min(group_at(b), end - 1) >> a.log_page]; };
   int entry0 = 0, entry1 = 0, entry = 0;  // (here, so that they and Q come together)
   if (t0 < t1) {
     entry0 = entries(t0 >> 4);
@@ -215,6 +236,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 
   // ---- Q ----
   const int seen = w_row0 + c < rows ? seen_by(rq, min((w_row0 + c) / G, rq.n - 1)) : 0;
+  const int hidden = FORM == WINDOW ? window_of(a, rq, min((w_row0 + c) / G, rq.n - 1)) : 0;  // tokens before it: sinks only
   half8_t qf[KU];
   float down = 1.f, up = 1.f;  // scores per product of the row's operands (a power of two), and back
   {
@@ -265,7 +287,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   const bool is_k = wave < KWAVES, is_v = !is_k && wave < 2 * KWAVES;
 
   auto places = [&](int b, int entry) {
-    const int tok = (64 * b + lane) * 16;
+    const int tok = group_at(b);
     const bool there = (uint32_t)entry < (uint32_t)a.num_pages;
     const uint64_t at = (uint64_t)(there ? (uint32_t)entry : 0u) * a.page_stride + (uint32_t)(tok & (T - 1)) * (D / 2);
     return there || tok >= end ? at : at | 1ull << 63;
@@ -297,7 +319,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   auto fetch_scales = [&](int tile, int block_now) {
     raw_scales = 0;
     if (s_mine) {
-      const uint32_t o = (uint32_t)(tile * kTile + 16 * s_group) & (T - 1);
+      const uint32_t o = (uint32_t)(token_of(tile) + 16 * s_group) & (T - 1);
       const uint8_t* b = place(tile, s_group, block_now) - o * (D / 2 - 2 * NG);
       if (lane < 16 * NG) raw_scales = *reinterpret_cast<const uint32_t*>(b + s_lane);
     }
@@ -371,7 +393,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     uint32_t scales_lane = buf + K_BYTES + V_BYTES + 16 * NG * h;
     uint32_t even[2] = {buf + (h * kTile + k_slot(c, h)) * 16, buf + (h * kTile + k_slot(32 + c, h)) * 16};
     uint32_t odd[2] = {buf + (h * kTile + k_slot(c, 2 + h)) * 16, buf + (h * kTile + k_slot(32 + c, 2 + h)) * 16};
-    const bool masked = (tile + 1) * kTile > w_all || hole != 0;
+    const int tok0 = token_of(tile);
+    const bool masked = tok0 + kTile > w_all || hole != 0 || (FORM == WINDOW && tok0 < w_high && tok0 + kTile > a.sinks);
     // Scores of half j, less base.
     auto scores_of = [&](int j, float (&x)[16]) {
 #pragma unroll
@@ -394,12 +417,17 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     // -infinity for what a row does not see, `least` at least for what it does (NaN stays): once
     // there is a reference so much that p is not zero, which what is not seen is told by.
     auto mask = [&](int j, float (&x)[16], float least) {
-      int left = seen - tile * kTile - 4 * h;
+      int left = seen - tok0 - 4 * h;
       asm volatile("" : "+v"(left));  // (else done for every tile)
+      int from = 0, sinks = 0;
+      if constexpr (FORM == WINDOW) {
+        from = hidden - tok0 - 4 * h, sinks = a.sinks - tok0 - 4 * h;
+        asm volatile("" : "+v"(from), "+v"(sinks));
+      }
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         const int t = 32 * j + 8 * (i / 4) + i % 4;
-        const bool in = t < left && !(hole >> (2 * j + i / 8) & 1);
+        const bool in = t < left && !(hole >> (2 * j + i / 8) & 1) && (FORM != WINDOW || t >= from || t < sinks);
         x[i] = in ? x[i] < least ? least : x[i] : -__builtin_inff();
       }
     };
@@ -470,7 +498,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       base = coarse ? base + xm : new_base;
       const float f = none ? 0.f : __builtin_amdgcn_exp2f(-less * down);
       M = none && !any ? kNone : base * down;
-      some_none = __any(M == kNone && seen > t0 * kTile);
+      some_none = __any(M == kNone && seen > token_of(t0));
       L *= f;
 #pragma unroll
       for (int i = 0; i < 16; i++) x[i] -= less;
@@ -554,7 +582,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         entry = entries(b + 2);
         missing = __ballot((int64_t)now < 0);
       }
-      if (tile * kTile < w_end)
+      if (FORM == WINDOW ? token_of(tile) < w_end && (token_of(tile) + kTile > w_low || token_of(tile) < a.sinks)
+                         : tile * kTile < w_end)
         compute(tile, (uint32_t)(missing >> ((tile & 15) * GROUPS)) & ((1u << GROUPS) - 1));
       if (tile + 1 < t1) {
         unpack(tile + 1);
@@ -628,9 +657,39 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 #pragma unroll
     for (int t = 0; t < DT; t++) O[t] = sum[t];
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;  // no token seen: zeros (a NaN stays one)
   const size_t at = (size_t)(rq.first + t_row) * a.q_heads + h_row;
   uint16_t* const dst = static_cast<uint16_t*>(a.out) + at * D;
+  float own_f = 1.f, before_f = 0.f;  // (SHARED, second pass) factors of these sums and of the first pass's
+  if constexpr (FORM == SHARED) {
+    if (a.start != nullptr && rq.start > 0 && row < rows) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.before_ml + 2 * at);
+      const float most = fmaxf(M, ml.x);
+      own_f = __builtin_amdgcn_exp2f(M - most), before_f = __builtin_amdgcn_exp2f(ml.x - most);
+      M = most, l = own_f * l + before_f * ml.y;
+    }
+  }
+  // (SHARED) the first pass leaves its sums; the second adds them
+  const bool leaves = FORM == SHARED && a.start == nullptr;
+  const float norm = l == 0.f ? 0.f : 1.f / l;  // no token seen: zeros (a NaN stays one)
+  const float inv = leaves ? 1.f : FORM == SHARED ? own_f * norm : norm;
+  if constexpr (FORM == SHARED) before_f *= norm;
+  auto finish = [&](float (&x)[8], int d) {
+    if (row >= rows) return;
+    if constexpr (FORM == SHARED) {
+      float4_t* const b = reinterpret_cast<float4_t*>(a.before + at * D + d);
+      if (leaves) {
+        b[0] = (float4_t){x[0], x[1], x[2], x[3]};
+        b[1] = (float4_t){x[4], x[5], x[6], x[7]};
+        return;
+      }
+      if (rq.start > 0) {
+        const float4_t v[2] = {b[0], b[1]};
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] = __builtin_fmaf(v[i / 4][i % 4], before_f, x[i]);
+      }
+    }
+    *reinterpret_cast<u32x4*>(dst + d) = pack8<TYPE>(x);
+  };
 #pragma unroll
   for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -647,7 +706,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
           const int m = i * BL + 8 * (k / 4);  // MFMA row less 4 out_h + k % 4
           x[i] = O[n * (BL / 4) + m / 32][m % 32 / 8 * 4 + k % 4];
         }
-        if (row < rows) *reinterpret_cast<u32x4*>(dst + 8 * (n * BL + 8 * (k / 4) + 4 * out_h + k % 4)) = pack8<TYPE>(x);
+        finish(x, 8 * (n * BL + 8 * (k / 4) + 4 * out_h + k % 4));
       }
   } else {
     // a lane has every other dim (2 e + out_h) of each of the group's four words: the lanes of a
@@ -665,11 +724,21 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
           x[2 * e] = out_h ? got : keep;
           x[2 * e + 1] = out_h ? keep : got;
         }
-        if (row < rows) *reinterpret_cast<u32x4*>(dst + 8 * (n * 4 + k + 2 * out_h)) = pack8<TYPE>(x);
+        finish(x, 8 * (n * 4 + k + 2 * out_h));
       }
+  }
+  if constexpr (FORM == SHARED) {
+    if (leaves) {
+      if (out_h == 0 && row < rows) *reinterpret_cast<float2*>(a.before_ml + 2 * at) = make_float2(M, l);
+      return;
+    }
   }
   if (a.lse != nullptr && out_h == 0 && row < rows)
     a.lse[at] = l == 0.f ? -__builtin_inff() : (M + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
 }
+
+// Launch of the kernel in one form (kv4_prompt*.hip).
+template <int FORM>
+hipError_t launch_prompt(const AttnArgs& a, int workgroups, int head_dim, int ng, int dtype, hipStream_t stream);
 
 }  // namespace kv4

@@ -68,7 +68,7 @@ constexpr int kLead = 2;
 constexpr int kWhole = 3;
 constexpr int kTilesAt = 43;       // bit of a sum of units
 constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last workgroup's read of it
-constexpr int kTile = 64;          // tokens of a tile of the prompt kernel
+constexpr int kLogTile = 6, kTile = 1 << kLogTile;  // tokens of a tile of the prompt kernel
 constexpr int kPromptWaves = 8, kPromptRows = 32 * kPromptWaves;
 constexpr int kMaxRequests = 2 * 64 * kWaves;  // of a launch that divides by the requests' lengths
 constexpr float kVTop = 7.f;       // a new reference brings the row's largest p v to 2^7
@@ -105,14 +105,32 @@ struct AttnArgs {
   int group;            // query heads of a kv head
   float c1;             // softmax scale * log2 e
   const int32_t* ctx;   // positions of the first new tokens; null: they are the last of kv_lens
+  // of SHARED
+  const int32_t* start;  // request's tokens that the pass before has attended to, whole pages (null: this is that pass)
+  const int32_t* leads;  // table row of each request (null: its own)
+  float* before;         // [token][q head][D] sums of the pass before, and its references and sums of p
+  float* before_ml;
+  // of WINDOW
+  int window, sinks;     // a token sees the last `window` positions, its own among them, and the first `sinks`
 };
+
+// What a kernel computes beside plain causal attention, none of which may cost that anything.
+//   SHARED  one of two passes over a prefix that requests share: the first takes a group of requests as
+//           one, with the prefix as its tokens, which all its rows see, and leaves its sums in fp32;
+//           the second starts each request behind the prefix and adds what the first left.
+//   WINDOW  rows see the last tokens before their own, and a few first ones.  A tile of rows goes
+//           through the steps of its first tokens, then on from the first that its window reaches.
+enum Form : int { PLAIN = 0, SHARED = 1, WINDOW = 2 };
 
 struct Request {
   int first, n, kv;  // first token, new tokens in q, tokens in all that the table covers
   int past;          // position of the first new token
+  int start;         // (SHARED) tokens passed over, which kv and past no longer count
 };
+template <int FORM = PLAIN>
 __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
   Request q;
+  q.start = 0;
   int cap = a.max_pages << a.log_page;  // (at most 2^30)
   asm volatile("" : "+s"(cap));         // (else kept in a vector register all the while)
   const int kv = max(a.kv_lens[r], 0);
@@ -129,16 +147,58 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
   }
   // positions go by the lengths as they are: what the table or q cuts off moves no token
   q.past = min(kv - n, 1 << 30);
+  if constexpr (FORM == SHARED) {
+    if (a.start != nullptr) {
+      q.start = min(max(a.start[r], 0), cap) >> a.log_page << a.log_page;
+      q.kv = max(q.kv - q.start, 0);
+      q.past -= q.start;
+    }
+  }
   return q;
 }
 // With the position that the caller gives.  (Apart, for the loads that a short call waits for:
 // loaded with the lengths it costs one of 1000 tokens 0.3 of its 11 us.)
 __device__ __forceinline__ void set_past(const AttnArgs& a, int r, Request& q) {
-  if (__builtin_expect(a.ctx != nullptr, 0)) q.past = min(max(a.ctx[r], 0), 1 << 30);
+  if (__builtin_expect(a.ctx != nullptr, 0)) q.past = min(max(a.ctx[r], 0), 1 << 30) - q.start;
 }
 
 // Tokens that new token t sees.
 __device__ __forceinline__ int seen_by(const Request& q, int t) { return max(min(q.past + t + 1, q.kv), 0); }
+
+// Where (SHARED) a request's table row lies.
+template <int FORM>
+__device__ __forceinline__ const int32_t* pages_of(const AttnArgs& a, int r, const Request& q) {
+  if constexpr (FORM == SHARED) {
+    const int row = a.leads == nullptr ? r : a.leads[r];
+    return a.table + (size_t)row * a.max_pages + (q.start >> a.log_page);
+  }
+  return a.table + (size_t)r * a.max_pages;
+}
+
+// (WINDOW) The tokens that rows first ... last of a request see, as steps of 2^log_step tokens: those with
+// sinks, then those from the first row's window on.  Step s begins at token at(s).
+struct Reach {
+  int sink_steps, gap, steps;
+  int lowest, highest;  // where the first row's window begins, and the last one's
+  __device__ __forceinline__ Reach() : sink_steps(0), gap(0), steps(0), lowest(0), highest(0) {}
+  __device__ __forceinline__ Reach(const AttnArgs& a, const Request& q, int t_first, int t_last, int end, int log_step) {
+    lowest = max(q.past + t_first + 1 - a.window, 0);
+    highest = max(q.past + t_last + 1 - a.window, 0);
+    const int up = (1 << log_step) - 1;
+    sink_steps = (min(a.sinks, end) + up) >> log_step;
+    gap = max((lowest >> log_step) - sink_steps, 0) << log_step;
+    steps = max((end - gap + up) >> log_step, sink_steps);
+  }
+  __device__ __forceinline__ int at(int s, int log_step) const { return (s << log_step) + (s >= sink_steps ? gap : 0); }
+};
+// Where the window of new token t begins.
+__device__ __forceinline__ int window_of(const AttnArgs& a, const Request& q, int t) { return max(q.past + t + 1 - a.window, 0); }
+// Steps of a tile of 16 rows at most.
+__device__ __forceinline__ int most_steps(const AttnArgs& a, const Request& q) {
+  const int more = min(q.n - 1, (14 + a.group) / a.group);  // tokens of the last row past the first row's
+  const int all = (q.kv + kStep - 1) >> kLogStep;
+  return min(all, ((min(a.sinks, q.kv) + kStep - 1) >> kLogStep) + ((a.window + more + 2 * kStep - 2) >> kLogStep));
+}
 
 // Rows of a head that are computed.
 __device__ __forceinline__ int rows_of(const AttnArgs& a, const Request& q) { return min(q.n, a.max_q) * a.group; }
@@ -271,14 +331,14 @@ __device__ __forceinline__ void v_operands(const Magic& m, const u32x4& a, const
   }
 }
 
-template <int D, int NG, int TYPE>
+template <int D, int NG, int TYPE, int FORM = PLAIN>
 __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
   using S = Shape<D, NG>;
   // the waves' rings; later 16 rows of D + 4 floats in each
   static_assert(S::RING * S::STAGE >= 16 * (D + 4) * 4 && S::RING * S::STAGE >= 16 * (kMaxSplits + 2) * 4, "");
   __shared__ __align__(16) uint8_t lds[kWaves * S::RING * S::STAGE];
   __shared__ uint32_t begins[kMaxRequests];
-  __shared__ int few_first[64], few_n[64], few_kv[64], few_past[64];
+  __shared__ int few_first[64], few_n[64], few_kv[64], few_past[64], few_start[FORM == SHARED ? 64 : 1];
   __shared__ long long wave_sum[kWaves];
   __shared__ int wave_max[kWaves];
   __shared__ uint32_t arrived;
@@ -294,14 +354,17 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
   // nothing take a unit, to write their zeros.  Without scratch, and where the units do
   // not fit 31 bits, tiles count as one and stay whole ----
   auto blocks_of = [&](const Request& q) { return rows_of(a, q) > a.max_rows ? 0 : (rows_of(a, q) + 15) / 16; };
-  auto units_of = [&](const Request& q) { return max((q.kv + kStep * KW - 1) >> (kLogStep + a.log_kw), 1) + a.lead; };
+  auto units_of = [&](const Request& q) {
+    if constexpr (FORM == WINDOW) return max((most_steps(a, q) + KW - 1) >> a.log_kw, 1) + a.lead;
+    return max((q.kv + kStep * KW - 1) >> (kLogStep + a.log_kw), 1) + a.lead;
+  };
   bool divided = a.partial != nullptr;
   uint32_t total, share;
   // Up to 64 requests are one to a lane, in every wave alike, and found by a ballot; more
   // are two to a thread and searched for.
   const bool few = a.requests <= 64;
-  Request own{0, 0, 0, 0};
-  if (few && lane < a.requests) own = request_of(a, lane);
+  Request own{0, 0, 0, 0, 0};
+  if (few && lane < a.requests) own = request_of<FORM>(a, lane);
   while (true) {
     long long mine[2] = {0, 0};
     int longest = 1;
@@ -319,7 +382,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     } else {
 #pragma unroll
       for (int u = 0; u < 2; u++)
-        if (2 * tid + u < a.requests) mine[u] = cost(request_of(a, 2 * tid + u));
+        if (2 * tid + u < a.requests) mine[u] = cost(request_of<FORM>(a, 2 * tid + u));
     }
     long long sum = mine[0] + mine[1], all, before;
     if (a.requests > 1) {
@@ -338,6 +401,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
       if (wave == 0) {
         begins[lane] = (uint32_t)before;
         few_first[lane] = own.first, few_n[lane] = own.n, few_kv[lane] = own.kv, few_past[lane] = own.past;
+        if constexpr (FORM == SHARED) few_start[lane] = own.start;
       }
       __syncthreads();
     } else {
@@ -402,14 +466,14 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     if (few) {
       const int i = lane_again();
       r = 63 - __builtin_clzll(__ballot(i < a.requests && begins[i] <= unit));
-      rq = Request{few_first[r], few_n[r], few_kv[r], few_past[r]};
+      rq = Request{few_first[r], few_n[r], few_kv[r], few_past[r], FORM == SHARED ? few_start[r] : 0};
     } else {
       for (int hi = a.requests; hi - r > 1;) {
         const int mid = (r + hi) >> 1;
         if (__builtin_amdgcn_readfirstlane(begins[mid]) <= unit) r = mid;
         else hi = mid;
       }
-      rq = request_of(a, r);
+      rq = request_of<FORM>(a, r);
     }
     r_begin = begins[r];
     r = __builtin_amdgcn_readfirstlane(r);
@@ -417,6 +481,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     rq.n = __builtin_amdgcn_readfirstlane(rq.n);
     rq.kv = __builtin_amdgcn_readfirstlane(rq.kv);
     rq.past = __builtin_amdgcn_readfirstlane(rq.past);
+    if constexpr (FORM == SHARED) rq.start = __builtin_amdgcn_readfirstlane(rq.start);
     set_past(a, r, rq);
     r_begin = __builtin_amdgcn_readfirstlane(r_begin);
     const int rows = rows_of(a, rq), row_blocks = blocks_of(rq), len = divided ? units_of(rq) : 1;
@@ -430,7 +495,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     const int t_first = one ? 0 : row0 / G, t_last = one ? 0 : min((row0 + 15) / G, rq.n - 1);
     const int end = seen_by(rq, t_last);   // tokens that some row of the tile sees
     const int all = seen_by(rq, t_first);  // ... that every row sees
-    const int steps = (end + kStep - 1) / kStep;
+    Reach reach;
+    if constexpr (FORM == WINDOW) reach = Reach(a, rq, t_first, t_last, end, kLogStep);
+    auto token_of = [&](int s) { return FORM == WINDOW ? reach.at(s, kLogStep) : s * kStep; };
+    const int steps = FORM == WINDOW ? reach.steps : (end + kStep - 1) / kStep;
     // this wave's steps: s0, s0 + KW, ... (the tile's first units are its lead)
     const uint32_t next_unit = min(tile_unit + len, last_unit), work_unit = tile_unit + (divided ? a.lead : 0);
     if (next_unit <= work_unit) break;
@@ -449,7 +517,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     half8_t qf[S::KW];
     float c1 = a.c1;
     const int row = row0 + c, t_row = one ? 0 : row / G, h_row = one ? min(row, G - 1) : row - t_row * G;
-    const int seen = row < rows ? seen_by(rq, t_row) : 0;  // tokens the row sees
+    // tokens the row sees (WINDOW: before the table's end and the window's beginning cut them)
+    const int seen = row >= rows ? (FORM == WINDOW ? -(1 << 30) : 0) : FORM == WINDOW ? rq.past + t_row + 1 : seen_by(rq, t_row);
     float x[S::KW][8];
     const uint16_t* src = static_cast<const uint16_t*>(a.q) + (long long)(rq.first + min(t_row, rq.n - 1)) * a.qt +
                           (long long)(head * G + h_row) * a.qh + 8 * g;
@@ -485,13 +554,13 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     for (int n = 0; n < NG; n++)
 #pragma unroll
       for (int i = 0; i < S::OPS; i++) O[n][i] = (float4_t){0.f, 0.f, 0.f, 0.f};
-    const int32_t* pages = a.table + (size_t)r * a.max_pages;
+    const int32_t* pages = pages_of<FORM>(a, r, rq);
     const uint8_t* const cache = a.cache + (size_t)head * block;
 
     // Places of 32 of the wave's steps from k on: lane i has half i % 2 of step k + i / 2,
     // the byte offset of its K codes (bit 63: no such page).
     auto places = [&](int k) {
-      const int tok = (s0 + (k + (lane >> 1)) * KW) * kStep + 16 * (lane & 1);
+      const int tok = token_of(s0 + (k + (lane >> 1)) * KW) + 16 * (lane & 1);
       const int id = tok < end ? pages[tok >> a.log_page] : -1;
       const bool there = (uint32_t)id < (uint32_t)a.num_pages;
       // a page that is not there is read as the first one and masked
@@ -520,7 +589,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
       }
       // scales: 8 NG lanes for K and for V of a half; they lie T D - o (D/2 - 2 NG) behind the K codes
       constexpr int L8 = 8 * NG;
-      const uint32_t tok = (uint32_t)(s0 + k * KW) * kStep;
+      const uint32_t tok = (uint32_t)token_of(s0 + k * KW);
       const uint32_t o0 = tok & (T - 1), o1 = (tok + 16) & (T - 1);
       const uint8_t* sc0 = k0 + (uint32_t)T * D - o0 * (D / 2 - 2 * NG);
       const uint8_t* sc1 = k1 + (uint32_t)T * D - o1 * (D / 2 - 2 * NG);
@@ -587,14 +656,26 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
 #pragma unroll
         for (int n = 0; n < NG; n++) vs[u][n] = S::LATE ? read_vs(from, u, n) : f.vs[u][n];
       // (wave-uniform) a step that some row does not see whole
-      const bool masked = (s + 1) * kStep > all || !there0 || !there1;
+      const int tok0 = token_of(s);
+      bool masked = tok0 + kStep > all || !there0 || !there1;
+      if constexpr (FORM == WINDOW)  // (without branches, for which the compiler makes copies of the loop)
+        masked = (tok0 + kStep > all) | !there0 | !there1 | ((tok0 < reach.highest) & (tok0 + kStep > a.sinks));
       if (masked) {
+        uint32_t bits = 0;  // (WINDOW) bit t: token t of the step, from the lane's first on, is seen
+        if constexpr (FORM == WINDOW) {
+          int mine = tok0 + 4 * g, past = seen;
+          asm volatile("" : "+v"(mine), "+v"(past));  // (else their parts are kept in registers all the while)
+          auto below = [&](int t) { return t - mine >= 32 ? ~0u : (1u << max(t - mine, 0)) - 1u; };
+          bits = below(min(past, rq.kv)) & (~below(past - a.window) | below(a.sinks));
+          if (!there0) bits &= 0xFFFF0000u;
+          if (!there1) bits &= 0x0000FFFFu;
+        }
 #pragma unroll
         for (int u = 0; u < 2; u++)
 #pragma unroll
           for (int i = 0; i < 4; i++) {
-            const int tok = s * kStep + 16 * u + 4 * g + i;
-            const bool in = tok < seen && (u ? there1 : there0);
+            const int tok = tok0 + 16 * u + 4 * g + i;
+            const bool in = FORM == WINDOW ? bits >> (16 * u + i) & 1u : tok < seen && (u ? there1 : there0);
             x[u][i] = in ? x[u][i] : -__builtin_inff();
             // (the scale of a token that the row does not see may be anything)
 #pragma unroll
@@ -763,9 +844,24 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     auto slot_row = [&](uint32_t w, int second, int row) {
       return (((size_t)w * 2 + second) * HW + hw) * 16 + row;
     };
-    auto write = [&](int row, int d0, float m, float l, const float4_t& o) {
+    auto write = [&](int row, int d0, float m, float l, const float4_t& sum) {
       const int i = row0 + row, t = one ? 0 : i / G;
       const size_t at = (size_t)(rq.first + t) * a.q_heads + head * G + i - t * G;
+      float4_t o = sum;
+      if constexpr (FORM == SHARED) {
+        if (a.start == nullptr) {
+          *reinterpret_cast<float4_t*>(a.before + at * D + d0) = o;
+          if (d0 == 0) *reinterpret_cast<float2*>(a.before_ml + 2 * at) = make_float2(m, l);
+          return;
+        }
+        if (rq.start > 0) {
+          const float2 ml = *reinterpret_cast<const float2*>(a.before_ml + 2 * at);
+          const float4_t v = *reinterpret_cast<const float4_t*>(a.before + at * D + d0);
+          const float most = fmaxf(m, ml.x), f = __builtin_amdgcn_exp2f(m - most), g = __builtin_amdgcn_exp2f(ml.x - most);
+          m = most, l = f * l + g * ml.y;
+          o = o * f + v * g;
+        }
+      }
       const float inv = l == 0.f ? 0.f : 1.f / l;  // no token seen: zeros (a NaN stays one)
       uint16_t* dst = static_cast<uint16_t*>(a.out) + at * D + d0;
       *reinterpret_cast<u32x2*>(dst) =
@@ -888,5 +984,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     unit = next_unit;
   }
 }
+
+// Launch of the kernel in one form (kv4_split_*.hip: a file each, for the compiler's sake).
+template <int FORM>
+hipError_t launch_split(const AttnArgs& a, int workgroups, int head_dim, int ng, int dtype, hipStream_t stream);
 
 }  // namespace kv4

@@ -30,6 +30,8 @@ from ._kv4 import (
     kv4_attention,
     kv4_cache,
     kv4_gather,
+    kv4_prefix,
+    kv4_shared,
     kv4_tables,
     plan_kv4_attention,
 )
@@ -78,6 +80,8 @@ __all__ = [
     "kv4_tables",
     "kv4_append",
     "kv4_gather",
+    "kv4_shared",
+    "kv4_prefix",
     "kv4_attention",
     "plan_kv4_attention",
     "kv4_layers",

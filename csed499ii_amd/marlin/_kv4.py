@@ -24,12 +24,14 @@ from __future__ import annotations
 import ctypes
 import functools
 import math
+import typing
 
 import torch
 
 from .. import _lib
 
-__all__ = ["kv4_cache", "kv4_tables", "kv4_append", "kv4_gather", "kv4_attention", "plan_kv4_attention"]
+__all__ = ["kv4_cache", "kv4_tables", "kv4_append", "kv4_gather", "kv4_shared", "kv4_prefix", "kv4_attention",
+           "plan_kv4_attention"]
 
 _DTYPES = {torch.float16: 0, torch.bfloat16: 1}
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
@@ -255,10 +257,57 @@ def kv4_gather(cache: torch.Tensor, slots: torch.Tensor, head_dim: int, groupsiz
     return k, v
 
 
+class kv4_prefix(typing.NamedTuple):
+    """What :func:`kv4_shared` found, for :func:`kv4_attention`: int32 ``[3 groups + 1 + requests]`` on the
+    GPU (tokens of each group's prefix, a request that holds it, first token of each group, tokens of the
+    prefix of each request) and the sizes it was made for."""
+    plan: torch.Tensor
+    requests: int
+    groups: int
+    pages: int
+    page_size: int
+
+    @property
+    def lens(self) -> torch.Tensor:
+        """Tokens of each group's prefix, int32 ``[groups]``; 0 where nothing is shared."""
+        return self.plan[:self.groups]
+
+
+def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups: torch.Tensor, page_size: int,
+               cu_q: torch.Tensor | None = None) -> kv4_prefix:
+    """The prefixes that groups of requests share (after :func:`kv4_fork`, say), found in the block table
+    once a step for the :func:`kv4_attention` of all layers.
+
+    Group ``g`` is the requests ``cu_groups[g]`` to ``cu_groups[g + 1] - 1`` (int32 ``[groups + 1]``, not
+    falling).  Its prefix is the leading pages that lie within ``context_lens`` and are the same in all
+    rows of the group; requests without new tokens (``cu_q``, as in the attention call) and those that share no
+    page with the group's first one are left out, and attend to all of their tokens by themselves.  So
+    whatever the groups are, the attention is right; they decide what is read once."""
+    dev = _device_of("block_table", block_table)
+    table, ctx = _ints("block_table", block_table, dev, 2), _ints("context_lens", context_lens, dev)
+    at, (R, P) = _ints("cu_groups", cu_groups, dev), block_table.shape
+    _check_page(page_size)
+    if context_lens.size(0) != R or cu_groups.size(0) < 1:
+        raise RuntimeError(f"context_lens has {context_lens.size(0)} requests, block_table {R}; cu_groups needs an entry")
+    cu = 0
+    if cu_q is not None:
+        cu = _ints("cu_q", cu_q, dev)
+        if cu_q.size(0) != R + 1:
+            raise RuntimeError(f"cu_q has {cu_q.size(0)} entries, expected {R + 1}")
+    groups = cu_groups.size(0) - 1
+    plan = block_table.new_empty(3 * groups + 1 + R)
+    err = _lib.load().marlin_hip_kv4_shared(table, ctx, cu, at, plan.data_ptr(), R, groups, P, page_size, dev,
+                                            _raw_stream(dev))
+    if err:
+        _raise(err)
+    return kv4_prefix(plan, R, groups, P, page_size)
+
+
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
                   cu_q: torch.Tensor | None = None, max_q: int | None = None, max_kv: int | None = None,
                   groupsize: int = -1, scale: float | None = None, return_lse: bool = False,
-                  out: torch.Tensor | None = None, context_lens: torch.Tensor | None = None):
+                  out: torch.Tensor | None = None, context_lens: torch.Tensor | None = None,
+                  shared: kv4_prefix | None = None, window: int | None = None, sinks: int = 0):
     """Causal attention of new tokens over the requests' cached rows, theirs included.
 
     ``q [tokens, q_heads, D]`` (fp16 or bf16; a view as in :func:`kv4_append`) holds the new
@@ -277,6 +326,12 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     the table's ``P`` pages).  ``scale`` (positive; default ``1 / sqrt(D)``) multiplies the
     scores.  Returns ``out [tokens, q_heads, D]`` in ``q``'s type, and with ``return_lse`` the
     rows' log-sum-exp, fp32 ``[tokens, q_heads]``.
+
+    With ``window`` the token at position ``p`` sees the positions ``j <= p`` of which ``j > p - window``, its
+    own and the ``window - 1`` before, and the first ``sinks`` of its request; only their pages are
+    read.  With ``shared`` (:func:`kv4_shared` of the same step; ``context_lens`` needed, too) the tokens that
+    requests of a group share are attended to once for all of them, in a pass of its own before the
+    one over each request's other tokens: the same sums in another order.  Not both.
 
     A row that sees no token gets zeros and ``-inf``.  Rows that belong to no request (before
     ``cu_q[0]``, from ``cu_q[R]`` on: a captured step's padding) and those past a request's
@@ -341,10 +396,33 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     elif N and out.data_ptr() < qp + 2 * ((N - 1) * qt + (Hq - 1) * qh + D) and qp < out.data_ptr() + 2 * N * Hq * D:
         raise RuntimeError("out must not overlap q, whose rows are read while out's are written")
     lse = torch.empty((N, Hq), dtype=torch.float32, device=q.device) if return_lse else None
-    err = _lib.load().marlin_hip_kv4_attention_ctx(
-        qp, cp, table, lens, cu, ctx, out.data_ptr(), 0 if lse is None else lse.data_ptr(), N, R, Hq, H, D, qt, qh, page,
-        pages, P, groupsize, min(max_q, N), max_kv, 1.0 / math.sqrt(D) if scale is None else scale, dtype, dev,
-        _raw_stream(dev))
+    op, lp = out.data_ptr(), 0 if lse is None else lse.data_ptr()
+    if scale is None:
+        scale = 1.0 / math.sqrt(D)
+    if shared is not None:
+        if window is not None:
+            raise RuntimeError("kv4_attention takes shared or window, not both")
+        if not isinstance(shared, kv4_prefix):
+            raise TypeError("shared must be what kv4_shared returns")
+        if (shared.requests, shared.pages, shared.page_size) != (R, P, page) or shared.plan.get_device() != dev or not ctx:
+            raise RuntimeError(f"shared is of {shared.requests} requests with {shared.pages} pages of {shared.page_size} "
+                               f"tokens and needs context_lens; the call has {R}, {P} and {page}")
+        work = torch.empty(N * Hq * (D + 2), dtype=torch.float32, device=q.device)
+        err = _lib.load().marlin_hip_kv4_attention_shared(
+            qp, cp, table, lens, cu, ctx, shared.plan.data_ptr(), op, lp, work.data_ptr(), N, R, shared.groups, Hq, H, D, qt,
+            qh, page, pages, P, groupsize, min(max_q, N), max_kv, scale, dtype, dev, _raw_stream(dev))
+    elif window is not None:
+        if window < 1 or sinks < 0:
+            raise RuntimeError(f"a window holds a token at least, and sinks are not negative (window={window}, sinks={sinks})")
+        err = _lib.load().marlin_hip_kv4_attention_window(
+            qp, cp, table, lens, cu, ctx, op, lp, N, R, Hq, H, D, qt, qh, page, pages, P, groupsize, min(max_q, N), max_kv,
+            scale, min(window, 1 << 30), min(sinks, 1 << 30), dtype, dev, _raw_stream(dev))
+    else:
+        if sinks:
+            raise RuntimeError("sinks without a window: every row sees them already")
+        err = _lib.load().marlin_hip_kv4_attention_ctx(
+            qp, cp, table, lens, cu, ctx, op, lp, N, R, Hq, H, D, qt, qh, page, pages, P, groupsize, min(max_q, N), max_kv,
+            scale, dtype, dev, _raw_stream(dev))
     if err:
         _raise(err)
     return (out, lse) if return_lse else out

@@ -241,6 +241,34 @@ int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* b
                                  long long q_head_stride, int page_size, int num_pages, int max_pages, int groupsize,
                                  int max_q, int max_kv, float scale, int dtype, int dev, hipStream_t stream);
 
+/* The same through a sliding window: the token at position p sees the positions j <= p with j > p - window
+ * (1 at least), and j < sinks.  Only their pages are read. */
+int marlin_hip_kv4_attention_window(const void* q, const void* cache, const void* block_table, const void* kv_lens,
+                                    const void* cu_q, const void* context_lens, void* out, void* lse, int tokens,
+                                    int requests, int q_heads, int kv_heads, int head_dim, long long q_token_stride,
+                                    long long q_head_stride, int page_size, int num_pages, int max_pages, int groupsize,
+                                    int max_q, int max_kv, float scale, int window, int sinks, int dtype, int dev,
+                                    hipStream_t stream);
+
+/* The prefixes that groups of requests share, once a step: group g is the requests [cu_groups[g],
+ * cu_groups[g + 1]) (`groups` + 1 entries, not falling; cut to the requests there are), its prefix the leading
+ * pages within context_lens that are the same in all its rows.  Requests without new tokens (cu_q, null: one each)
+ * and those that share no page with the group's first are left out.  shared: int32 [3 groups + 1 + requests]. */
+int marlin_hip_kv4_shared(const void* block_table, const void* context_lens, const void* cu_q, const void* cu_groups,
+                          void* shared, int requests, int groups, int max_pages, int page_size, int dev,
+                          hipStream_t stream);
+
+/* marlin_hip_kv4_attention_ctx with the prefixes of `shared` attended to once for all rows of a group, in a pass
+ * before that over each request's other tokens.  shared: from marlin_hip_kv4_shared with the same block_table,
+ * context_lens and cu_q; context_lens must be given.  workspace: fp32 [tokens][q_heads][head_dim + 2], 16-byte
+ * aligned. */
+int marlin_hip_kv4_attention_shared(const void* q, const void* cache, const void* block_table, const void* kv_lens,
+                                    const void* cu_q, const void* context_lens, const void* shared, void* out, void* lse,
+                                    void* workspace, int tokens, int requests, int groups, int q_heads, int kv_heads,
+                                    int head_dim, long long q_token_stride, long long q_head_stride, int page_size,
+                                    int num_pages, int max_pages, int groupsize, int max_q, int max_kv, float scale,
+                                    int dtype, int dev, hipStream_t stream);
+
 /* The launch plan of a marlin_hip_kv4_attention call, computed on the host without a GPU (sms
  * <= 0: 256 compute units), for `requests` requests of max_q new tokens each (cu_q null where
  * max_q is 1): out[0] 0 (kernel of few rows) or 1 (of prompts), out[1] its workgroups (of the
