@@ -118,7 +118,7 @@ int check(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int
 // no group.  Once a step, for all layers.
 // ---------------------------------------------------------------------------
 
-constexpr int kSharedThreads = 1024, kSharedRound = 1024;
+constexpr int kSharedThreads = 1024, kSharedRound = 1024, kSharedFlight = 16;
 
 struct SharedArgs {
   const int32_t* table;
@@ -174,9 +174,15 @@ __global__ __launch_bounds__(kSharedThreads) void kv4_shared_kernel(SharedArgs a
       const int i0 = tid / width, j = j0 + tid - i0 * width;
       if (i0 >= side) continue;
       const int want = lead_row[j];
-#pragma unroll 8
-      for (int i = i0; i < n; i += side)
-        if (j < first[i] && a.table[(size_t)(from + i) * a.max_pages + j] != want) atomicMin(&first[i], j);
+      const int32_t* column = a.table + (size_t)from * a.max_pages + j;
+      for (int i = i0; i < n; i += kSharedFlight * side) {
+        int page[kSharedFlight];  // (all in flight; those past the last repeat it)
+#pragma unroll
+        for (int k = 0; k < kSharedFlight; k++) page[k] = column[(size_t)min(i + k * side, n - 1) * a.max_pages];
+#pragma unroll
+        for (int k = 0; k < kSharedFlight; k++)
+          if (page[k] != want) atomicMin(&first[min(i + k * side, n - 1)], j);
+      }
     }
     __syncthreads();
     if (tid < n) {

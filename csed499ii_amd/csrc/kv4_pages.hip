@@ -56,6 +56,8 @@ __global__ __launch_bounds__(256) void kv4_mark_kernel(Tables t, uint8_t* marks)
   }
 }
 
+constexpr int kStrip = 256;  // pages that a wave looks at together
+
 // Held pages before each chunk of `step` pages (kMarkThreads chunks), in LDS, and in all.
 struct Census {
   int step, held;
@@ -63,13 +65,30 @@ struct Census {
 __device__ __forceinline__ Census census(const uint8_t* marks, int num_pages, int (&before)[kMarkThreads + 1], int (&wave_sum)[kMarkWaves]) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   Census c;
-  c.step = ((num_pages + kMarkThreads - 1) / kMarkThreads + 15) & ~15;  // (the marks end on 16 bytes)
-  const long long first = (long long)tid * c.step, last = min(first + c.step, (long long)num_pages);
-  int n = 0;
-  for (long long p = first; p < last; p += 16) {  // (bytes past the last page are 0)
-    const u32x4 w = *reinterpret_cast<const u32x4*>(&marks[p]);
-    n += __popc(w.x) + __popc(w.y) + __popc(w.z) + __popc(w.w);
+  c.step = ((num_pages + kMarkThreads - 1) / kMarkThreads + kStrip - 1) & ~(kStrip - 1);
+  // 16 bytes a lane, side by side: sixteen lanes have a strip, all strips of a chunk add up
+  before[tid] = 0;
+  __syncthreads();
+  constexpr int FLIGHT = 4;
+  const int pieces = (num_pages + 15) / 16, per_chunk = c.step / 16;  // (the marks end on 16 bytes; past the last page they are 0)
+  for (int p0 = tid; p0 < ((pieces + 63) & ~63); p0 += FLIGHT * kMarkThreads) {
+    u32x4 w[FLIGHT];
+#pragma unroll
+    for (int k = 0; k < FLIGHT; k++) {
+      const int p = p0 + k * kMarkThreads;
+      w[k] = reinterpret_cast<const u32x4*>(marks)[min(p, pieces - 1)];
+    }
+#pragma unroll
+    for (int k = 0; k < FLIGHT; k++) {
+      int n = __popc(w[k].x) + __popc(w[k].y) + __popc(w[k].z) + __popc(w[k].w);
+      if (p0 + k * kMarkThreads >= pieces) n = 0;
+#pragma unroll
+      for (int d = 1; d < 16; d <<= 1) n += __shfl_xor(n, d);
+      if ((lane & 15) == 0 && n > 0) atomicAdd(&before[(p0 + k * kMarkThreads) / per_chunk], n);
+    }
   }
+  __syncthreads();
+  const int n = before[tid];
   int sum = n;
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) {
@@ -96,15 +115,28 @@ template <class F>
 __device__ __forceinline__ void each_page(const uint8_t* marks, int num_pages, const Census& c, const int (&before)[kMarkThreads + 1],
                                           int workgroup, int workgroups, F&& f) {
   const int lane = threadIdx.x & 63;
-  for (int chunk = workgroup * kMarkWaves + (int)(threadIdx.x >> 6); chunk < kMarkThreads; chunk += workgroups * kMarkWaves) {
+  const int chunks = (num_pages + c.step - 1) / c.step;
+  for (int chunk = workgroup * kMarkWaves + (int)(threadIdx.x >> 6); chunk < chunks; chunk += workgroups * kMarkWaves) {
     const long long first = (long long)chunk * c.step, last = min(first + c.step, (long long)num_pages);
     int seen = before[chunk];
-    for (long long p = first; p < last; p += 64) {
-      const long long page = p + lane;
-      const bool held = page < last && marks[page] != 0;
-      const uint64_t all = __ballot(held);
-      if (page < last) f((int)page, held, seen + (int)__popcll(all & ((1ull << lane) - 1)));
-      seen += (int)__popcll(all);
+    for (long long p = first; p < last; p += kStrip) {
+      // a lane's four pages; held ones before them, of all lanes
+      const long long page = p + 4 * lane;
+      const uint32_t word = page < last ? *reinterpret_cast<const uint32_t*>(&marks[page]) : 0u;
+      int before_lane = 0, all = 0;
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const uint64_t m = __ballot((word >> (8 * k) & 1u) != 0);
+        before_lane += __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+        all += (int)__popcll(m);
+      }
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const bool held = (word >> (8 * k) & 1u) != 0;
+        if (page + k < last) f((int)page + k, held, seen + before_lane);
+        before_lane += held;
+      }
+      seen += all;
     }
   }
 }
@@ -176,18 +208,25 @@ __global__ __launch_bounds__(kMarkThreads) void kv4_small_page_plan_kernel(Args 
   const int tid = threadIdx.x;
   for (int i = tid; i < (t.num_pages + 15) / 16; i += kMarkThreads) reinterpret_cast<u32x4*>(marks)[i] = (u32x4){0, 0, 0, 0};
   __syncthreads();
-  // a wave a request; the lengths of its next 64 requests at once
-  const int lane = tid & 63, wave = tid >> 6;
-  for (int r0 = wave; r0 < t.requests; r0 += 64 * kMarkWaves) {
-    const int mine = r0 + lane * kMarkWaves;
-    const int len = mine < t.requests ? t.lens[mine] : 0;
-    for (int i = 0, r = r0; i < 64 && r < t.requests; i++, r += kMarkWaves) {
-      const int n = entries_of(t, __builtin_amdgcn_readlane(len, i));
-      const int32_t* row = t.table + (size_t)r * t.max_pages;
-      for (int j = lane; j < n; j += 64) {
-        const int page = row[j];
-        if ((uint32_t)page < (uint32_t)t.num_pages) marks[page] = 1;
+  // every entry, several of a thread in flight; its row and column go on without a division
+  constexpr int FLIGHT = 8;
+  const int all = t.requests * t.max_pages;  // (at most kSmallEntries)
+  if (all > 0) {
+    const int rows = kMarkThreads / t.max_pages, columns = kMarkThreads - rows * t.max_pages;
+    int row = tid / t.max_pages, column = tid - row * t.max_pages;
+    for (int e = tid; e < all; e += FLIGHT * kMarkThreads) {
+      int page[FLIGHT], len[FLIGHT], at[FLIGHT];
+#pragma unroll
+      for (int k = 0; k < FLIGHT; k++) {
+        page[k] = t.table[min(e + k * kMarkThreads, all - 1)];
+        len[k] = t.lens[min(row, t.requests - 1)];
+        at[k] = row < t.requests ? column : t.max_pages;
+        row += rows, column += columns;
+        if (column >= t.max_pages) row++, column -= t.max_pages;
       }
+#pragma unroll
+      for (int k = 0; k < FLIGHT; k++)
+        if (at[k] < entries_of(t, len[k]) && (uint32_t)page[k] < (uint32_t)t.num_pages) marks[page[k]] = 1;
     }
   }
   __syncthreads();
@@ -210,7 +249,7 @@ void plan_pages(const Args& a, const Tables& t, void* workspace, hipStream_t str
     if (across > most) across = most;
     hipLaunchKernelGGL(kv4_mark_kernel, dim3(rows, across), dim3(256), 0, stream, t, marks);
   }
-  hipLaunchKernelGGL((kv4_page_plan_kernel<Args>), dim3(32), dim3(kMarkThreads), 0, stream, a, (const uint8_t*)marks);
+  hipLaunchKernelGGL((kv4_page_plan_kernel<Args>), dim3(64), dim3(kMarkThreads), 0, stream, a, (const uint8_t*)marks);
 }
 
 // ---------------------------------------------------------------------------
@@ -281,7 +320,7 @@ struct ForkArgs {
   int32_t* table;
   int32_t* lens;
   int32_t* used;
-  int32_t* copies;  // [new request]: 1 if it gets a copy
+  int32_t* copies;  // [new request]: the page that it gets a copy of, or -1
   int rows, num_free;
 };
 
@@ -317,29 +356,35 @@ __global__ __launch_bounds__(256) void kv4_fork_table_kernel(ForkArgs a) {
   __syncthreads();
   if (tid == 0) {
     a.lens[i] = len;
-    a.copies[i] = shared;
+    a.copies[i] = shared ? page : -1;
   }
 }
 
 constexpr int kForkRound = 1024;
 
-// A wave copies one head's part of a page in one layer.
 __global__ __launch_bounds__(kCopyThreads) void kv4_fork_copy_kernel(Layers layers, ForkArgs a, int heads, int head_dim, int ng) {
-  __shared__ int rows[kForkRound];
+  __shared__ int sources[kForkRound], targets[kForkRound], fours_of[kForkRound];
   __shared__ int wave_sum[kCopyWaves];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lp = a.old.log_page, T = 1 << lp;
-  const uint32_t block = (uint32_t)(T * (head_dim + 4 * ng));
+  const uint32_t blocks = (uint32_t)layers.count * heads;  // (below 2^22: the heads are checked on the host)
+  const uint32_t block = (uint32_t)(T * (head_dim + 4 * ng)), page_bytes = block * heads;
+  constexpr int FLIGHT = 4;
+  const uint32_t half_lane = lane & 31;
+  const uint32_t per_four = head_dim / 8, codes_of_page = (T / 4) * per_four;  // 16-byte runs of K's codes, or of V's
+  const uint32_t code_at = lane < 32 ? 0 : (uint32_t)(T * head_dim / 2);
+  const uint32_t scale_at = (uint32_t)(T * head_dim) + (lane < 32 ? 0 : 2 * T * ng);
   int taken = 0;  // pages that the rounds before took
   for (int r0 = 0; r0 < a.rows; r0 += kForkRound) {
     // the round's requests that get a copy, in order
     constexpr int PER = kForkRound / kCopyThreads;
-    int own[PER], n = 0;
+    int own[PER], len[PER], n = 0;
 #pragma unroll
     for (int u = 0; u < PER; u++) {
       const int r = r0 + PER * tid + u;
-      own[u] = r < a.rows ? a.copies[r] : 0;
-      n += own[u];
+      own[u] = r < a.rows ? a.copies[r] : -1;
+      len[u] = r < a.rows ? a.lens[r] : 0;
+      n += own[u] >= 0;
     }
     int sum = n;
 #pragma unroll
@@ -358,39 +403,59 @@ __global__ __launch_bounds__(kCopyThreads) void kv4_fork_copy_kernel(Layers laye
     }
 #pragma unroll
     for (int u = 0; u < PER; u++) {
-      if (own[u]) {
-        const int r = r0 + PER * tid + u;
-        if (blockIdx.x == 0) {
-          const int rank = taken + at, fresh = rank < a.num_free ? a.free_pages[rank] : -1;
-          a.table[(size_t)r * a.old.max_pages + (a.lens[r] >> lp)] = (uint32_t)fresh < (uint32_t)a.old.num_pages ? fresh : -1;
-        }
-        rows[at++] = r;
+      if (own[u] >= 0) {
+        const int r = r0 + PER * tid + u, rank = taken + at;
+        const int fresh = rank < a.num_free ? a.free_pages[rank] : -1;
+        const bool there = (uint32_t)fresh < (uint32_t)a.old.num_pages;
+        if (blockIdx.x == 0) a.table[(size_t)r * a.old.max_pages + (len[u] >> lp)] = there ? fresh : -1;
+        sources[at] = own[u];
+        targets[at] = fresh;
+        fours_of[at] = there ? ((len[u] & (T - 1)) + 3) >> 2 : 0;  // (no page: nothing to copy)
+        at++;
       }
     }
     __syncthreads();
-    const long long total = (long long)all * layers.count * heads;
-    for (long long i = (long long)blockIdx.x * kCopyWaves + wave; i < total; i += (long long)gridDim.x * kCopyWaves) {
-      const long long pair = i / heads;
-      const int head = (int)(i - pair * heads), layer = (int)(pair % layers.count), k = (int)(pair / layers.count);
-      const int rank = taken + k, to = rank < a.num_free ? a.free_pages[rank] : -1;
-      if ((uint32_t)to >= (uint32_t)a.old.num_pages) continue;
-      const int r = rows[k], len = a.lens[r];
-      const int from = a.old.table[(size_t)a.parents[r] * a.old.max_pages + (len >> lp)];
-      const int fours = ((len & (T - 1)) + 3) >> 2;
-      const uint8_t* src = layers.at[layer] + ((size_t)from * heads + head) * block;
-      uint8_t* dst = layers.at[layer] + ((size_t)to * heads + head) * block;
-      // four runs of 16 (scales: 8) bytes: K and V codes, K and V scales
-      const int codes = fours * (2 * head_dim / 16), scales = fours * ng;
-      const uint32_t v_at = (uint32_t)(T * head_dim / 2), s_at = (uint32_t)(T * head_dim), sv_at = s_at + 2 * T * ng;
-      for (int c = lane; c < codes; c += 64) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(src + 16 * c), y = *reinterpret_cast<const u32x4*>(src + v_at + 16 * c);
-        *reinterpret_cast<u32x4*>(dst + 16 * c) = x;
-        *reinterpret_cast<u32x4*>(dst + v_at + 16 * c) = y;
-      }
-      for (int c = lane; c < scales; c += 64) {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(src + s_at + 8 * c), y = *reinterpret_cast<const u32x2*>(src + sv_at + 8 * c);
-        *reinterpret_cast<u32x2*>(dst + s_at + 8 * c) = x;
-        *reinterpret_cast<u32x2*>(dst + sv_at + 8 * c) = y;
+    // A wave takes one head of one layer and a run of the copies, and keeps what it has read for those
+    // of the same page (samples of one prompt).  Lanes 0 to 31 have K's codes and scales, the others V's.
+    if (all > 0) {
+      const uint32_t waves = gridDim.x * kCopyWaves, id = blockIdx.x * kCopyWaves + wave;
+      const uint32_t runs = min(max(waves / blocks, 1u), (uint32_t)all);
+      const uint32_t most = ((uint32_t)all + runs - 1) / runs;
+      for (uint32_t item = id; item < blocks * runs; item += waves) {
+        const uint32_t b = item / runs, k0 = (item - b * runs) * most, k1 = min(k0 + most, (uint32_t)all);
+        const uint32_t layer = b / (uint32_t)heads, head = b - layer * (uint32_t)heads;
+        uint8_t* const base = layers.at[layer] + (size_t)head * block;
+        for (uint32_t c0 = 0; c0 < codes_of_page; c0 += 32 * FLIGHT) {
+          u32x4 v[FLIGHT];
+          u32x2 s[FLIGHT];
+          int held = -1, held_fours = 0;  // what v and s hold
+          bool more = false;              // some copy goes on past this part
+          for (uint32_t k = k0; k < k1; k++) {
+            const int source = __builtin_amdgcn_readfirstlane(sources[k]), target = __builtin_amdgcn_readfirstlane(targets[k]);
+            const int fours = __builtin_amdgcn_readfirstlane(fours_of[k]);
+            const uint32_t codes = (uint32_t)fours * per_four, scales = (uint32_t)fours * ng;
+            if (codes <= c0) continue;
+            more |= codes > c0 + 32 * FLIGHT;
+            if (source != held || fours > held_fours) {
+              const uint8_t* src = base + (size_t)(uint32_t)source * page_bytes;
+#pragma unroll
+              for (int u = 0; u < FLIGHT; u++) {
+                const uint32_t c = c0 + 32 * u + half_lane;
+                if (c < codes) v[u] = *reinterpret_cast<const u32x4*>(src + code_at + 16 * c);
+                if (c < scales) s[u] = *reinterpret_cast<const u32x2*>(src + scale_at + 8 * c);
+              }
+              held = source, held_fours = fours;
+            }
+            uint8_t* dst = base + (size_t)(uint32_t)target * page_bytes;
+#pragma unroll
+            for (int u = 0; u < FLIGHT; u++) {
+              const uint32_t c = c0 + 32 * u + half_lane;
+              if (c < codes) *reinterpret_cast<u32x4*>(dst + code_at + 16 * c) = v[u];
+              if (c < scales) *reinterpret_cast<u32x2*>(dst + scale_at + 8 * c) = s[u];
+            }
+          }
+          if (!more) break;
+        }
       }
     }
     taken += all;
@@ -508,6 +573,7 @@ int marlin_hip_kv4_fork(const void* const* caches, int layers, const void* block
   if (err == MARLIN_HIP_OK) err = check_tables(requests, max_pages, page_size, num_pages);
   if (err != MARLIN_HIP_OK) return err;
   if (new_requests < 0 || num_free < 0) return refuse("kv4_fork takes no negative sizes");
+  if (kv_heads > 32767) return refuse("kv4_fork takes at most 32767 heads");
   sm24::DeviceScope scope(dev);
   if (!scope.ok) return MARLIN_HIP_ERR_LAUNCH;
   const Tables t{static_cast<const int32_t*>(block_table), static_cast<const int32_t*>(kv_lens), requests, max_pages,

@@ -609,6 +609,51 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     constexpr int kPart = DT * 16 * 64;  // floats of a wave's part
     const uint32_t stride = (uint32_t)a.kv_heads * W;  // from a part's waves to the next one's
     const uint32_t first = (slot - (uint32_t)(part * a.kv_heads)) * W + wave, mine = first + part * stride;
+    if constexpr (FORM != PLAIN) {
+      // By pairs: of two neighbouring sums the first to arrive leaves its own and ends, the other adds
+      // it, the earlier part's first, and goes on with the pair's.  (One wave for all parts reads them one
+      // after the other: 16 parts of 512 rows on 8 heads, 8192 tokens, 58 us where this takes 36.)
+      uint32_t low = part;  // of the parts that O sums
+      for (uint32_t width = 1; width < (uint32_t)parts; width *= 2) {
+        const uint32_t other = low ^ width;
+        if (other >= (uint32_t)parts) continue;
+        uint32_t* const met = a.counters + first + max(low, other) * stride;
+        uint32_t there = 0;
+        if (out_lane == 0) there = __hip_atomic_load(met, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (__builtin_amdgcn_readfirstlane(there) == 0) {
+          float* const o_low = a.partial + (size_t)(first + low * stride) * kPart + 4 * out_lane;
+#pragma unroll
+          for (int t = 0; t < DT; t++)
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+              *reinterpret_cast<float4_t*>(o_low + (4 * t + i) * 256) =
+                  (float4_t){O[t][4 * i], O[t][4 * i + 1], O[t][4 * i + 2], O[t][4 * i + 3]};
+          *reinterpret_cast<float2*>(a.partial_ml + (size_t)(first + low * stride) * 128 + 2 * out_lane) = make_float2(M, l);
+          __atomic_signal_fence(__ATOMIC_SEQ_CST);
+          __builtin_amdgcn_s_waitcnt(0);
+          __atomic_signal_fence(__ATOMIC_SEQ_CST);
+          if (out_lane == 0) there = __hip_atomic_fetch_add(met, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+          if (__builtin_amdgcn_readfirstlane(there) == 0) return;
+        }
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        if (out_lane == 0) __hip_atomic_store(met, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        const float2 x = *reinterpret_cast<const float2*>(a.partial_ml + (size_t)(first + other * stride) * 128 + 2 * out_lane);
+        const float* const o = a.partial + (size_t)(first + other * stride) * kPart + 4 * out_lane;
+        float4_t v[DT * 4];
+#pragma unroll
+        for (int i = 0; i < DT * 4; i++) v[i] = *reinterpret_cast<const float4_t*>(o + i * 256);
+        const float most = fmaxf(M, x.x), f = __builtin_amdgcn_exp2f(M - most), g = __builtin_amdgcn_exp2f(x.x - most);
+        const bool after = other < low;
+        l = after ? __builtin_fmaf(x.y, g, l * f) : __builtin_fmaf(l, f, x.y * g);
+        M = most;
+#pragma unroll
+        for (int i = 0; i < DT * 16; i++) {
+          const float mine_i = O[i / 16][i % 16], v_i = v[i / 4][i % 4];
+          O[i / 16][i % 16] = after ? __builtin_fmaf(v_i, g, mine_i * f) : __builtin_fmaf(mine_i, f, v_i * g);
+        }
+        low = min(low, other);
+      }
+    } else {
     float* const o_mine = a.partial + (size_t)mine * kPart + 4 * out_lane;
 #pragma unroll
     for (int t = 0; t < DT; t++)
@@ -656,6 +701,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     M = most;
 #pragma unroll
     for (int t = 0; t < DT; t++) O[t] = sum[t];
+    }
   }
   const size_t at = (size_t)(rq.first + t_row) * a.q_heads + h_row;
   uint16_t* const dst = static_cast<uint16_t*>(a.out) + at * D;

@@ -170,17 +170,16 @@ def kv4_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: t
                                f"{block_table.size(0)}")
     if num_tokens < 0:
         raise RuntimeError("num_tokens must not be negative")
-    more = num_tokens if return_positions else 0
-    out = context_lens.new_empty(num_tokens + 2 * R + 2 + more)
-    slots, cu, kv, used, positions = out.split_with_sizes((num_tokens, R + 1, R, 1, more))
+    sizes = (num_tokens, R + 1, R, 1, num_tokens) if return_positions else (num_tokens, R + 1, R, 1)
+    out = context_lens.new_empty(sum(sizes))
     at = out.data_ptr()
-    cu_at = at + 4 * num_tokens
-    err = _lib.load().marlin_hip_kv4_tables_pos(ctx, new, free, table, at, cu_at, cu_at + 4 * (R + 1),
-                                                cu_at + 4 * (2 * R + 1), cu_at + 4 * (2 * R + 2) if more else 0, R, F, P,
+    err = _lib.load().marlin_hip_kv4_tables_pos(ctx, new, free, table, at, at + 4 * num_tokens,
+                                                at + 4 * (num_tokens + R + 1), at + 4 * (num_tokens + 2 * R + 1),
+                                                at + 4 * (num_tokens + 2 * R + 2) if return_positions else 0, R, F, P,
                                                 page_size, num_tokens, dev, _raw_stream(dev))
     if err:
         _raise(err)
-    return (slots, cu, kv, used, positions) if return_positions else (slots, cu, kv, used)
+    return out.split_with_sizes(sizes)
 
 
 def kv4_append(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor,

@@ -56,15 +56,23 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scale: float = 1.
 def rotary_angles(positions: torch.Tensor, freqs: torch.Tensor, factor: float = 1.0) -> torch.Tensor:
     """Cosine and sine, times ``factor``, of the angles of ``positions`` (int32 ``[tokens]``, of any
     size and sign): float64 ``[tokens, pairs, 2]``.  Positions of the other sign turn rows back."""
-    dev = _device_of("positions", positions)
-    at = _ints("positions", positions, dev)
-    if not isinstance(freqs, torch.Tensor):
-        raise TypeError("freqs must be a torch.Tensor")
-    if freqs.dtype != torch.int64 or freqs.dim() != 1 or freqs.get_device() != dev or not freqs.is_contiguous():
-        raise RuntimeError(f"freqs must be a contiguous 1-dimensional int64 tensor on cuda:{dev}, as rotary_frequencies "
-                           f"makes it")
-    tokens, pairs = positions.size(0), freqs.size(0)
-    out = torch.empty((tokens, pairs, 2), dtype=torch.float64, device=positions.device)
+    try:  # (as in kv4_append)
+        (tokens,), (pairs,) = positions.shape, freqs.shape
+        dev, at = positions.get_device(), positions.data_ptr()
+        fits = (dev >= 0 and positions.dtype is torch.int32 and positions.is_contiguous() and freqs.dtype is torch.int64
+                and freqs.get_device() == dev and freqs.is_contiguous())
+    except (AttributeError, TypeError, ValueError):
+        fits = False
+    if not fits:
+        dev = _device_of("positions", positions)
+        at = _ints("positions", positions, dev)
+        if not isinstance(freqs, torch.Tensor):
+            raise TypeError("freqs must be a torch.Tensor")
+        if freqs.dtype != torch.int64 or freqs.dim() != 1 or freqs.get_device() != dev or not freqs.is_contiguous():
+            raise RuntimeError(f"freqs must be a contiguous 1-dimensional int64 tensor on cuda:{dev}, as "
+                               f"rotary_frequencies makes it")
+        tokens, pairs = positions.size(0), freqs.size(0)
+    out = freqs.new_empty((tokens, pairs, 2), dtype=torch.float64)
     err = _lib.load().marlin_hip_rotary_angles(at, freqs.data_ptr(), out.data_ptr(), tokens, pairs, factor, dev,
                                                _raw_stream(dev))
     if err:
@@ -114,9 +122,7 @@ def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
 
 
 def _out_for(x: torch.Tensor, out, dev: int, *others):
-    """``out``, made or checked: x itself or a tensor of its shape apart from it and from the others."""
-    if out is None:
-        return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+    """``out``, checked: x itself or a tensor of its shape apart from it and from the others."""
     if not isinstance(out, torch.Tensor):
         raise TypeError("out must be a torch.Tensor")
     if out.shape != x.shape or out.dtype != x.dtype or out.get_device() != dev:
@@ -142,16 +148,32 @@ def rotary(x: torch.Tensor, angles: torch.Tensor, interleaved: bool = False, out
     bits, rounded once to ``x``'s type (by way of fp32, as torch does).  Returns ``out``, which may be
     ``x`` itself; its rows may have strides as ``x``'s may.  No gradient flows through the call; turning
     by the angles of the negative positions is its transpose."""
-    dev = _device_of("x", x)
-    xt, xh = _rows("x", x, dev)
-    N, H, D = x.shape
-    if D % 8 or not 8 <= D <= 1024:
-        raise RuntimeError(f"rotary takes heads of a multiple of 8 dims, 1024 at most, got {D}")
-    r = _angles(angles, N, D, dev)
-    out = _out_for(x, out, dev)
-    yt, yh = _strides(out)
-    err = _lib.load().marlin_hip_rotary(x.data_ptr(), angles.data_ptr(), out.data_ptr(), N, H, D, r, xt, xh, yt, yh,
-                                        int(interleaved), _DTYPES[x.dtype], dev, _raw_stream(dev))
+    try:  # (as in kv4_append)
+        N, H, D = x.shape
+        xt, xh, xd = x.stride()
+        dev, dtype, xp, ap = x.get_device(), _DTYPES.get(x.dtype), x.data_ptr(), angles.data_ptr()
+        r = 2 * angles.shape[1]
+        fits = (dtype is not None and dev >= 0 and out is None and xd == 1 and not (xt | xh | D) & 7 and not (xp | ap) & 15
+                and angles.dtype is torch.float64 and angles.get_device() == dev and angles.is_contiguous()
+                and angles.shape == (N, r // 2, 2) and 2 <= r <= D <= 1024)
+    except (AttributeError, TypeError, ValueError, IndexError):
+        fits = False
+    if not fits:
+        dev = _device_of("x", x)
+        xt, xh = _rows("x", x, dev)
+        N, H, D = x.shape
+        if D % 8 or not 8 <= D <= 1024:
+            raise RuntimeError(f"rotary takes heads of a multiple of 8 dims, 1024 at most, got {D}")
+        r = _angles(angles, N, D, dev)
+        xp, ap, dtype = x.data_ptr(), angles.data_ptr(), _DTYPES[x.dtype]
+    if out is None:
+        out = torch.empty_like(x) if x.is_contiguous() else x.new_empty((N, H, D))
+        yt, yh = H * D, D
+    else:
+        out = _out_for(x, out, dev)
+        yt, yh = _strides(out)
+    err = _lib.load().marlin_hip_rotary(xp, ap, out.data_ptr(), N, H, D, r, xt, xh, yt, yh, int(interleaved), dtype, dev,
+                                        _raw_stream(dev))
     if err:
         _raise(err)
     return out
