@@ -419,16 +419,35 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     auto mask = [&](int j, float (&x)[16], float least) {
       int left = seen - tok0 - 4 * h;
       asm volatile("" : "+v"(left));  // (else done for every tile)
-      int from = 0, sinks = 0;
-      if constexpr (FORM == WINDOW) {
-        from = hidden - tok0 - 4 * h, sinks = a.sinks - tok0 - 4 * h;
-        asm volatile("" : "+v"(from), "+v"(sinks));
-      }
 #pragma unroll
       for (int i = 0; i < 16; i++) {
         const int t = 32 * j + 8 * (i / 4) + i % 4;
-        const bool in = t < left && !(hole >> (2 * j + i / 8) & 1) && (FORM != WINDOW || t >= from || t < sinks);
+        const bool in = t < left && !(hole >> (2 * j + i / 8) & 1);
         x[i] = in ? x[i] < least ? least : x[i] : -__builtin_inff();
+      }
+    };
+    // The same in the other forms, by a bit for each token of a half tile, from 4 h on, that the lane's row sees:
+    // two operations a score and two a pair of p v, where comparisons take twelve.  (Through a window nine
+    // tiles of a block of rows are masked in some wave: 8000 tokens on 32 heads, a window of 1024.)
+    uint32_t bits[2] = {0, 0};
+    if (FORM != PLAIN && masked) {
+      int mine = tok0 + 4 * h;
+      asm volatile("" : "+v"(mine));
+#pragma unroll
+      for (int j = 0; j < 2; j++) {
+        auto below = [&](int t) { return t - mine - 32 * j >= 32 ? ~0u : (1u << max(t - mine - 32 * j, 0)) - 1u; };
+        bits[j] = below(seen);
+        if constexpr (FORM == WINDOW) bits[j] &= ~below(hidden) | below(a.sinks);
+        if (hole >> (2 * j) & 1) bits[j] &= 0xFFFF0000u;
+        if (hole >> (2 * j + 1) & 1) bits[j] &= 0x0000FFFFu;
+      }
+    }
+    auto sees = [&](int j, int i) { return (uint32_t)__builtin_amdgcn_sbfe((int)bits[j], 8 * (i / 4) + i % 4, 1); };  // all ones or none
+    auto hide = [&](int j, float (&x)[16]) {
+#pragma unroll
+      for (int i = 0; i < 16; i++) {
+        const uint32_t s = sees(j, i);
+        x[i] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x[i]) & s) | (0xFF800000u & ~s));
       }
     };
     // p and p v (fp16 pairs) of half j; sum of p, the largest p v.
@@ -456,7 +475,9 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       if (masked) {  // what a row does not see is zero, whatever its scale
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
-          const uint32_t keep = (x[i] == 0.f ? 0u : 0xFFFFu) | (x[i + 1] == 0.f ? 0u : 0xFFFF0000u);
+          uint32_t keep;
+          if constexpr (FORM == PLAIN) keep = (x[i] == 0.f ? 0u : 0xFFFFu) | (x[i + 1] == 0.f ? 0u : 0xFFFF0000u);
+          else keep = (sees(j, i) & 0xFFFFu) | (sees(j, i + 1) & 0xFFFF0000u);
 #pragma unroll
           for (int n = 0; n < NG; n++) P[n][i / 8][i % 8 / 2] &= keep;
         }
@@ -517,7 +538,10 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       for (int jj = 0; jj < HALVES; jj++) scores_of(j0 + jj, x[jj]);
       if (masked) {
 #pragma unroll
-        for (int jj = 0; jj < HALVES; jj++) mask(j0 + jj, x[jj], some_none ? -__builtin_inff() : least);
+        for (int jj = 0; jj < HALVES; jj++) {
+          if constexpr (FORM == PLAIN) mask(j0 + jj, x[jj], some_none ? -__builtin_inff() : least);
+          else hide(j0 + jj, x[jj]);
+        }
       }
 #pragma unroll
       for (int jj = 0; jj < HALVES; jj++) {
@@ -530,7 +554,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 #pragma unroll
             for (int i = 0; i < 16; i++) x[HALVES - 1][i] -= less;
           }
-          if (masked) {
+          if (FORM == PLAIN && masked) {
 #pragma unroll
             for (int k = jj; k < HALVES; k++) mask(j0 + k, x[k], least);
           }
@@ -544,7 +568,10 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
           if (!first) {
             asm volatile("" : "+v"(even[j]), "+v"(odd[j]), "+v"(scales_lane)::"memory");
             scores_of(j, x[jj]);
-            if (masked) mask(j, x[jj], -__builtin_inff());
+            if (masked) {
+              if constexpr (FORM == PLAIN) mask(j, x[jj], -__builtin_inff());
+              else hide(j, x[jj]);
+            }
           }
           refer_to();
           weigh(j, x[jj], P, sum, most);
