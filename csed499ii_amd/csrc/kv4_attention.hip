@@ -46,13 +46,13 @@ struct Plan {
 // 4096: 61, 65, 66).  From two blocks a workgroup on, a workgroup goes through many short
 // ones instead, and two waves take a block (64 requests of 4096 tokens on 32 heads: 220 us
 // with eight, 215 with four, 210 with two; 200 of 1000: 208, 187, 177).
-Plan plan(int requests, int q_heads, int kv_heads, int max_q, int max_kv, int cus) {
+Plan plan(int requests, int q_heads, int kv_heads, int max_q, int max_kv, int cus, bool behind = false) {
   Plan p{};
   const long long row_blocks = ((long long)max_q * (q_heads / kv_heads) + 15) / 16;
   const long long steps = ((long long)max_kv + kStep - 1) / kStep;
   const long long most = 2ll * cus;
   const long long blocks = requests * row_blocks * kv_heads;
-  p.log_kw = blocks <= 2 * most ? kLogWaves : 1;
+  p.log_kw = behind ? (blocks <= most ? 3 : blocks <= 2 * most ? 2 : 1) : blocks <= 2 * most ? kLogWaves : 1;
   const int hw = kWaves >> p.log_kw;
   const long long units = steps < 1 ? 1 : (steps + (1 << p.log_kw) - 1) >> p.log_kw;
   const long long w = requests * ((row_blocks * kv_heads + hw - 1) / hw) * units;
@@ -114,11 +114,11 @@ int check(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int
 // ---------------------------------------------------------------------------
 // The prefix that the requests of a group share: the whole pages, from the first on, that are the
 // same in their tables and lie within their contexts.  A workgroup for each group compares every
-// request's row with the first one's, all columns and requests at once; one more for the requests of
+// request's row with the first one's; one more for the requests of
 // no group.  Once a step, for all layers.
 // ---------------------------------------------------------------------------
 
-constexpr int kSharedThreads = 1024, kSharedRound = 1024, kSharedFlight = 16;
+constexpr int kSharedThreads = 1024, kSharedRound = 1024, kSharedWaves = kSharedThreads / 64, kSharedRows = 4;
 
 struct SharedArgs {
   const int32_t* table;
@@ -135,7 +135,7 @@ struct SharedArgs {
 __global__ __launch_bounds__(kSharedThreads) void kv4_shared_kernel(SharedArgs a) {
   __shared__ int first[kSharedRound];  // column in which a request's row differs
   __shared__ int lead, least, sharers;
-  const int tid = threadIdx.x, g = (int)blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = (int)blockIdx.x;
   auto border = [&](int i) { return min(max(a.cu_groups[i], 0), a.requests); };
   auto token = [&](int r) { return a.cu_q == nullptr ? r : max(a.cu_q[r], 0); };
   if (g == a.groups) {
@@ -153,36 +153,53 @@ __global__ __launch_bounds__(kSharedThreads) void kv4_shared_kernel(SharedArgs a
   };
   if (tid == 0) lead = 0x7FFFFFFF, least = 0x7FFFFFFF, sharers = 0;
   __syncthreads();
-  for (int r = r0 + tid; r < r1; r += kSharedThreads)
-    if (pages(r) > 0) {
-      atomicMin(&lead, r);
-      break;
+  const bool one_round = r1 - r0 <= kSharedRound;  // (what `first` holds then serves below)
+  for (int from = r0; from < r1; from += kSharedRound)
+    if (from + tid < r1) {
+      const int n = first[tid] = pages(from + tid);
+      if (n > 0) atomicMin(&lead, from + tid);
     }
   __syncthreads();
   const int leader = lead;
   const bool any = leader < r1;
-  const int most = any ? pages(leader) : 0;
+  const int most = !any ? 0 : one_round ? first[leader - r0] : pages(leader);
   const int32_t* lead_row = a.table + (size_t)(any ? leader : r0) * a.max_pages;
   for (int from = r0; from < r1; from += kSharedRound) {
     const int n = min(r1 - from, kSharedRound);
     __syncthreads();  // the round before is done with LDS
-    if (tid < n) first[tid] = min(pages(from + tid), most);
-    __syncthreads();
-    for (int j0 = 0; j0 < most; j0 += kSharedThreads) {
-      // columns fill the threads as far as there are, requests the rest
-      const int width = min(most - j0, kSharedThreads), side = kSharedThreads / width;
-      const int i0 = tid / width, j = j0 + tid - i0 * width;
-      if (i0 >= side) continue;
-      const int want = lead_row[j];
-      const int32_t* column = a.table + (size_t)from * a.max_pages + j;
-      for (int i = i0; i < n; i += kSharedFlight * side) {
-        int page[kSharedFlight];  // (all in flight; those past the last repeat it)
+    if (!one_round) {
+      if (tid < n) first[tid] = pages(from + tid);
+      __syncthreads();
+    }
+    // A wave takes four rows, 256 columns of each in flight.
+    for (int i0 = kSharedRows * wave; i0 < n; i0 += kSharedRows * kSharedWaves) {
+      int common[kSharedRows];
 #pragma unroll
-        for (int k = 0; k < kSharedFlight; k++) page[k] = column[(size_t)min(i + k * side, n - 1) * a.max_pages];
+      for (int k = 0; k < kSharedRows; k++) common[k] = most;
+      for (int j0 = 0; j0 < most; j0 += 256) {
+        int want[4], page[kSharedRows][4];
 #pragma unroll
-        for (int k = 0; k < kSharedFlight; k++)
-          if (page[k] != want) atomicMin(&first[min(i + k * side, n - 1)], j);
+        for (int u = 0; u < 4; u++) {  // (those past the last repeat it)
+          const int j = min(j0 + 64 * u + lane, most - 1);
+          want[u] = lead_row[j];
+#pragma unroll
+          for (int k = 0; k < kSharedRows; k++) page[k][u] = a.table[(size_t)(from + min(i0 + k, n - 1)) * a.max_pages + j];
+        }
+        bool more = false;
+#pragma unroll
+        for (int k = 0; k < kSharedRows; k++) {
+#pragma unroll
+          for (int u = 3; u >= 0; u--) {
+            const uint64_t differ = __ballot(page[k][u] != want[u]);
+            if (differ != 0) common[k] = min(common[k], j0 + 64 * u + __builtin_ctzll(differ));
+          }
+          more |= common[k] >= j0 + 256;
+        }
+        if (!more) break;
       }
+#pragma unroll
+      for (int k = 0; k < kSharedRows; k++)
+        if (lane == 0 && i0 + k < n) first[i0 + k] = min(first[i0 + k], common[k]);
     }
     __syncthreads();
     if (tid < n) {
@@ -235,7 +252,8 @@ int attend(AttnArgs a, const Problem& p, const Choice& c) {
     if (c.split) {
       // (through a window a row's tokens are no more than the window's and the sinks')
       const long long reach = FORM == WINDOW ? (long long)a.window + a.sinks + c.split_q + 2 * kStep : p.max_kv;
-      const Plan plan = kv4::plan(a.requests, p.q_heads, p.kv_heads, c.split_q, reach < p.max_kv ? (int)reach : p.max_kv, p.cus);
+      const Plan plan = kv4::plan(a.requests, p.q_heads, p.kv_heads, c.split_q, reach < p.max_kv ? (int)reach : p.max_kv, p.cus,
+                                  FORM == SHARED && a.start != nullptr);
       a.log_kw = plan.log_kw;
       a.lead = plan.lead;
       a.slots = 2 * p.cus;
@@ -299,6 +317,7 @@ struct Prefix {
   const int32_t *lens, *leads, *cu_rows, *start;
   int groups;
   float* workspace;
+  long long bytes;
 };
 
 int attention(const void* q, const void* cache, const void* block_table, const void* kv_lens, const void* cu_q,
@@ -349,8 +368,11 @@ int attention(const void* q, const void* cache, const void* block_table, const v
   const Choice c = choose(tokens, requests, q_heads, kv_heads, head_dim, ng, max_q, cu_q != nullptr, p.cus);
   if (window > 0) return attend<WINDOW>(a, p, c);
   if (prefix == nullptr) return attend<PLAIN>(a, p, c);
+  const size_t rows = (size_t)tokens * q_heads;
+  if (prefix->bytes < (long long)(rows * (head_dim + 2) * sizeof(float)))
+    return refuse("kv4_attention of a shared prefix needs a workspace of head_dim + 2 floats a row");
   a.before = prefix->workspace;
-  a.before_ml = prefix->workspace + (size_t)tokens * q_heads * head_dim;
+  a.before_ml = a.before + rows * head_dim;
   // First pass: a group is a request whose tokens are the prefix and whose rows, behind it, see all of them.
   // One kernel takes all groups, by the rows that a group has on average.
   AttnArgs b = a;
@@ -367,6 +389,19 @@ int attention(const void* q, const void* cache, const void* block_table, const v
   one.split = !one.prompts;
   one.few_rows = 0x7FFFFFFF;
   one.split_q = average;
+  // Blocks of rows that the prompt kernel divides leave their parts where the second pass, if it runs on the
+  // split kernel alone, adds them as it writes: they would meet through memory that is not cached.
+  // (One launch of the first pass: a second would write over its parts.  And one block a workgroup of the
+  // second: 128 requests on 32 heads of 8192 shared tokens, 47 and 106 us so, 52 and 84 joined.)
+  const size_t place = ((size_t)p.cus / kv_heads) * kv_heads * kPromptRows;
+  const size_t parts_at = (rows * (head_dim + 4) + 3) & ~(size_t)3;
+  const long long blocks = (long long)requests * ((c.split_q * group + 15) / 16) * kv_heads;
+  if (one.prompts && !c.prompts && blocks <= 2 * p.cus && prefix->groups <= kMaxRequests && place <= 0x7FFFFFFF &&
+      prefix->bytes >= (long long)((parts_at + place * (head_dim + 2)) * sizeof(float))) {
+    a.where = b.where = reinterpret_cast<int2*>(a.before_ml + 2 * rows);
+    a.parts = b.parts = prefix->workspace + parts_at;
+    a.parts_ml = b.parts_ml = a.parts + place * head_dim;
+  }
   err = attend<SHARED>(b, first, one);
   if (err != MARLIN_HIP_OK) return err;
   a.start = prefix->start;
@@ -407,11 +442,11 @@ int marlin_hip_kv4_attention_shared(const void* q, const void* cache, const void
                                     void* workspace, int tokens, int requests, int groups, int q_heads, int kv_heads,
                                     int head_dim, long long q_token_stride, long long q_head_stride, int page_size,
                                     int num_pages, int max_pages, int groupsize, int max_q, int max_kv, float scale,
-                                    int dtype, int dev, hipStream_t stream) {
+                                    int dtype, long long workspace_bytes, int dev, hipStream_t stream) {
   if (groups < 0) return kv4::refuse("kv4_attention takes no negative sizes");
   const int32_t* at = static_cast<const int32_t*>(shared);
   const kv4::Prefix prefix{at, at + groups, at + 2 * (size_t)groups, at + 3 * (size_t)groups + 1, groups,
-                           static_cast<float*>(workspace)};
+                           static_cast<float*>(workspace), workspace_bytes};
   return kv4::attention(q, cache, block_table, kv_lens, cu_q, context_lens, out, lse, tokens, requests, q_heads, kv_heads,
                         head_dim, q_token_stride, q_head_stride, page_size, num_pages, max_pages, groupsize, max_q, max_kv,
                         scale, dtype, dev, stream, 0, 0, groups > 0 ? &prefix : nullptr);

@@ -166,7 +166,11 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       longest = fmaxf(longest, __shfl_xor(longest, d));
     }
     const float lo = fmaxf(fmaxf(sum / (float)a.pieces, kMinShare), longest / (float)kMaxParts), hi = fmaxf(lo, longest);
-    const float per_tile = 1.f / (lo + (hi - lo) * ((float)(lane + 1) / 64.f));
+    // (in the other forms from the shortest itself on, in equal ratios: of 128 tiles in two blocks and 32 workgroups
+    // 16 parts of 8 where steps of hi / 64 make 13 of 10)
+    const float per_tile = FORM == PLAIN
+        ? 1.f / (lo + (hi - lo) * ((float)(lane + 1) / 64.f))
+        : __builtin_amdgcn_exp2f(__builtin_amdgcn_logf(hi / lo) * ((float)lane / -63.f)) / lo;
     auto parts_of = [&](int tiles, float f) { return max((int)ceilf((float)tiles * f - 0.001f), 1); };
     int n = 0;
     for (int i = 0; i < all; i += 4) {
@@ -426,11 +430,11 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         x[i] = in ? x[i] < least ? least : x[i] : -__builtin_inff();
       }
     };
-    // The same in the other forms, by a bit for each token of a half tile, from 4 h on, that the lane's row sees:
+    // The same through a window, by a bit for each token of a half tile, from 4 h on, that the lane's row sees:
     // two operations a score and two a pair of p v, where comparisons take twelve.  (Through a window nine
     // tiles of a block of rows are masked in some wave: 8000 tokens on 32 heads, a window of 1024.)
     uint32_t bits[2] = {0, 0};
-    if (FORM != PLAIN && masked) {
+    if (FORM == WINDOW && masked) {
       int mine = tok0 + 4 * h;
       asm volatile("" : "+v"(mine));
 #pragma unroll
@@ -476,7 +480,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 #pragma unroll
         for (int i = 0; i < 16; i += 2) {
           uint32_t keep;
-          if constexpr (FORM == PLAIN) keep = (x[i] == 0.f ? 0u : 0xFFFFu) | (x[i + 1] == 0.f ? 0u : 0xFFFF0000u);
+          if constexpr (FORM != WINDOW) keep = (x[i] == 0.f ? 0u : 0xFFFFu) | (x[i + 1] == 0.f ? 0u : 0xFFFF0000u);
           else keep = (sees(j, i) & 0xFFFFu) | (sees(j, i + 1) & 0xFFFF0000u);
 #pragma unroll
           for (int n = 0; n < NG; n++) P[n][i / 8][i % 8 / 2] &= keep;
@@ -539,7 +543,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       if (masked) {
 #pragma unroll
         for (int jj = 0; jj < HALVES; jj++) {
-          if constexpr (FORM == PLAIN) mask(j0 + jj, x[jj], some_none ? -__builtin_inff() : least);
+          if constexpr (FORM != WINDOW) mask(j0 + jj, x[jj], some_none ? -__builtin_inff() : least);
           else hide(j0 + jj, x[jj]);
         }
       }
@@ -554,7 +558,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
 #pragma unroll
             for (int i = 0; i < 16; i++) x[HALVES - 1][i] -= less;
           }
-          if (FORM == PLAIN && masked) {
+          if (FORM != WINDOW && masked) {
 #pragma unroll
             for (int k = jj; k < HALVES; k++) mask(j0 + k, x[k], least);
           }
@@ -569,7 +573,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
             asm volatile("" : "+v"(even[j]), "+v"(odd[j]), "+v"(scales_lane)::"memory");
             scores_of(j, x[jj]);
             if (masked) {
-              if constexpr (FORM == PLAIN) mask(j, x[jj], -__builtin_inff());
+              if constexpr (FORM != WINDOW) mask(j, x[jj], -__builtin_inff());
               else hide(j, x[jj]);
             }
           }
@@ -636,10 +640,12 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     constexpr int kPart = DT * 16 * 64;  // floats of a wave's part
     const uint32_t stride = (uint32_t)a.kv_heads * W;  // from a part's waves to the next one's
     const uint32_t first = (slot - (uint32_t)(part * a.kv_heads)) * W + wave, mine = first + part * stride;
-    if constexpr (FORM != PLAIN) {
+    if (FORM == SHARED && a.parts != nullptr) {
+      // left for the second pass (below)
+    } else if constexpr (FORM != PLAIN) {
       // By pairs: of two neighbouring sums the first to arrive leaves its own and ends, the other adds
       // it, the earlier part's first, and goes on with the pair's.  (One wave for all parts reads them one
-      // after the other: 16 parts of 512 rows on 8 heads, 8192 tokens, 58 us where this takes 36.)
+      // after the other: 13 parts of 512 rows on 8 heads, 8192 tokens, 58 us where this takes 55.)
       uint32_t low = part;  // of the parts that O sums
       for (uint32_t width = 1; width < (uint32_t)parts; width *= 2) {
         const uint32_t other = low ^ width;
@@ -730,32 +736,42 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
     for (int t = 0; t < DT; t++) O[t] = sum[t];
     }
   }
+  // (the passes' addresses from the kernel's arguments anew: not kept in registers through the loop either)
+  typedef const __attribute__((address_space(4))) AttnArgs* Late;
+  Late late = (Late)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(late));
   const size_t at = (size_t)(rq.first + t_row) * a.q_heads + h_row;
   uint16_t* const dst = static_cast<uint16_t*>(a.out) + at * D;
   float own_f = 1.f, before_f = 0.f;  // (SHARED, second pass) factors of these sums and of the first pass's
+  size_t left_at = at;  // where a first pass leaves its sums
+  float* left = nullptr;
   if constexpr (FORM == SHARED) {
-    if (a.start != nullptr && rq.start > 0 && row < rows) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.before_ml + 2 * at);
+    left = late->before;
+    if (late->parts != nullptr && late->start == nullptr) {
+      if (parts > 1) {
+        // (a slot's rows are the block's; the parts of a block are kv_heads slots apart)
+        left = late->parts;
+        left_at = (size_t)slot * kPromptRows + 32 * wave + out_c;
+      }
+      if (part == 0 && out_h == 0 && row < rows) late->where[at] = make_int2((int)left_at, parts > 1 ? parts : 0);
+    }
+    if (late->start != nullptr && rq.start > 0 && row < rows) {
+      const float2 ml = *reinterpret_cast<const float2*>(late->before_ml + 2 * at);
       const float most = fmaxf(M, ml.x);
       own_f = __builtin_amdgcn_exp2f(M - most), before_f = __builtin_amdgcn_exp2f(ml.x - most);
       M = most, l = own_f * l + before_f * ml.y;
     }
   }
   // (SHARED) the first pass leaves its sums; the second adds them
-  const bool leaves = FORM == SHARED && a.start == nullptr;
+  const bool leaves = FORM == SHARED && late->start == nullptr;
   const float norm = l == 0.f ? 0.f : 1.f / l;  // no token seen: zeros (a NaN stays one)
   const float inv = leaves ? 1.f : FORM == SHARED ? own_f * norm : norm;
   if constexpr (FORM == SHARED) before_f *= norm;
   auto finish = [&](float (&x)[8], int d) {
     if (row >= rows) return;
     if constexpr (FORM == SHARED) {
-      float4_t* const b = reinterpret_cast<float4_t*>(a.before + at * D + d);
-      if (leaves) {
-        b[0] = (float4_t){x[0], x[1], x[2], x[3]};
-        b[1] = (float4_t){x[4], x[5], x[6], x[7]};
-        return;
-      }
       if (rq.start > 0) {
+        const float4_t* const b = reinterpret_cast<const float4_t*>(late->before + at * D + d);
         const float4_t v[2] = {b[0], b[1]};
 #pragma unroll
         for (int i = 0; i < 8; i++) x[i] = __builtin_fmaf(v[i / 4][i % 4], before_f, x[i]);
@@ -767,6 +783,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   for (int t = 0; t < DT; t++)
 #pragma unroll
     for (int i = 0; i < 16; i++) O[t][i] *= inv;
+  // f(eight dims, the first one's place) of the lane's row
+  auto words = [&](auto f) {
   if constexpr (BL >= 8) {
     // all eight dims of a word: row v_row(blk, i) of the group
 #pragma unroll
@@ -779,7 +797,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
           const int m = i * BL + 8 * (k / 4);  // MFMA row less 4 out_h + k % 4
           x[i] = O[n * (BL / 4) + m / 32][m % 32 / 8 * 4 + k % 4];
         }
-        finish(x, 8 * (n * BL + 8 * (k / 4) + 4 * out_h + k % 4));
+        f(x, 8 * (n * BL + 8 * (k / 4) + 4 * out_h + k % 4));
       }
   } else {
     // a lane has every other dim (2 e + out_h) of each of the group's four words: the lanes of a
@@ -797,12 +815,53 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
           x[2 * e] = out_h ? got : keep;
           x[2 * e + 1] = out_h ? keep : got;
         }
-        finish(x, 8 * (n * 4 + k + 2 * out_h));
+        f(x, 8 * (n * 4 + k + 2 * out_h));
       }
+  }
+  };
+  if constexpr (FORM == SHARED) {
+    if (leaves) {
+      // Through LDS, which the tiles no longer need: a wave's rows, 16 at a time, come out side by side.  (Each
+      // lane's eight dims straight to memory: 43 us where this takes 34.)
+      constexpr int RP = 16 * (D + 4) * 4 * W <= 2 * BUF ? D + 4 : D;
+      static_assert(16 * RP * 4 * W <= 2 * BUF, "");
+      float* const mine = reinterpret_cast<float*>(lds) + wave * (16 * RP);
+#pragma unroll 1
+      for (int half = 0; half < 2; half++) {
+        words([&](float (&x)[8], int d) {
+          if (out_c >> 4 != half) return;
+          float4_t* const to = reinterpret_cast<float4_t*>(mine + (out_c & 15) * RP + d);
+          to[0] = (float4_t){x[0], x[1], x[2], x[3]};
+          to[1] = (float4_t){x[4], x[5], x[6], x[7]};
+        });
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        constexpr int ITEMS = 16 * D / 4 / 64;  // of four dims
+        float4_t v[ITEMS];
+        uint32_t lo[ITEMS], hi[ITEMS];
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+          const int item = out_lane + 64 * i, r = item / (D / 4), d = item % (D / 4) * 4;
+          v[i] = *reinterpret_cast<const float4_t*>(mine + r * RP + d);
+          lo[i] = __shfl((int)(uint32_t)left_at, 16 * half + r), hi[i] = __shfl((int)(uint32_t)(left_at >> 32), 16 * half + r);
+        }
+#pragma unroll
+        for (int i = 0; i < ITEMS; i++) {
+          const int item = out_lane + 64 * i, r = item / (D / 4), d = item % (D / 4) * 4;
+          if (w_row0 + 16 * half + r < rows)
+            *reinterpret_cast<float4_t*>(left + ((size_t)hi[i] << 32 | lo[i]) * D + d) = v[i];
+        }
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      }
+    } else {
+      words(finish);
+    }
+  } else {
+    words(finish);
   }
   if constexpr (FORM == SHARED) {
     if (leaves) {
-      if (out_h == 0 && row < rows) *reinterpret_cast<float2*>(a.before_ml + 2 * at) = make_float2(M, l);
+      float* const ml = left == late->before ? late->before_ml : late->parts_ml;
+      if (out_h == 0 && row < rows) *reinterpret_cast<float2*>(ml + 2 * left_at) = make_float2(M, l);
       return;
     }
   }

@@ -110,6 +110,9 @@ struct AttnArgs {
   const int32_t* leads;  // table row of each request (null: its own)
   float* before;         // [token][q head][D] sums of the pass before, and its references and sums of p
   float* before_ml;
+  int2* where;           // [token][q head] a row's first place among the parts of divided blocks, and their number
+  float* parts;          // [part][row of 256][D] sums of parts that the second pass adds (null: they meet in the first)
+  float* parts_ml;
   // of WINDOW
   int window, sinks;     // a token sees the last `window` positions, its own among them, and the first `sinks`
 };
@@ -854,7 +857,41 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
           if (d0 == 0) *reinterpret_cast<float2*>(a.before_ml + 2 * at) = make_float2(m, l);
           return;
         }
-        if (rq.start > 0) {
+        const int2 left = a.where != nullptr && rq.start > 0 ? a.where[at] : make_int2(0, 0);
+        if (left.y > 0) {
+          // the parts in order, after this row's own
+          const size_t stride = (size_t)a.kv_heads * kPromptRows;
+          const float* const ml = a.parts_ml + 2 * (size_t)left.x;
+          const float* const v = a.parts + (size_t)left.x * D + d0;
+          constexpr int FLIGHT = 8;
+          float most = m;
+          for (int p = 0; p < left.y; p += FLIGHT) {
+            float x[FLIGHT];  // (those past the last repeat it)
+#pragma unroll
+            for (int k = 0; k < FLIGHT; k++) x[k] = ml[2 * stride * min(p + k, left.y - 1)];
+#pragma unroll
+            for (int k = 0; k < FLIGHT; k++) most = fmaxf(most, x[k]);
+          }
+          const float f = __builtin_amdgcn_exp2f(m - most);
+          m = most, l *= f, o *= f;
+          for (int p = 0; p < left.y; p += FLIGHT) {
+            float2 x[FLIGHT];
+            float4_t y[FLIGHT];
+#pragma unroll
+            for (int k = 0; k < FLIGHT; k++) {
+              const size_t i = stride * min(p + k, left.y - 1);
+              x[k] = *reinterpret_cast<const float2*>(ml + 2 * i);
+              y[k] = *reinterpret_cast<const float4_t*>(v + i * D);
+            }
+#pragma unroll
+            for (int k = 0; k < FLIGHT; k++) {
+              if (p + k >= left.y) break;
+              const float g = __builtin_amdgcn_exp2f(x[k].x - most);
+              l = __builtin_fmaf(g, x[k].y, l);
+              o += y[k] * g;
+            }
+          }
+        } else if (rq.start > 0) {
           const float2 ml = *reinterpret_cast<const float2*>(a.before_ml + 2 * at);
           const float4_t v = *reinterpret_cast<const float4_t*>(a.before + at * D + d0);
           const float most = fmaxf(m, ml.x), f = __builtin_amdgcn_exp2f(m - most), g = __builtin_amdgcn_exp2f(ml.x - most);

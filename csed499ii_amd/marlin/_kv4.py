@@ -406,10 +406,14 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
         if (shared.requests, shared.pages, shared.page_size) != (R, P, page) or shared.plan.get_device() != dev or not ctx:
             raise RuntimeError(f"shared is of {shared.requests} requests with {shared.pages} pages of {shared.page_size} "
                                f"tokens and needs context_lens; the call has {R}, {P} and {page}")
-        work = torch.empty(N * Hq * (D + 2), dtype=torch.float32, device=q.device)
+        # (beside the rows of the first pass its parts, where it has more than a few rows a group: 256 of each compute unit)
+        size = N * Hq * (D + 4) + 4
+        if N * Hq > 64 * H * shared.groups:
+            size += 65536 * (D + 2)
+        work = torch.empty(size, dtype=torch.float32, device=q.device)
         err = _lib.load().marlin_hip_kv4_attention_shared(
             qp, cp, table, lens, cu, ctx, shared.plan.data_ptr(), op, lp, work.data_ptr(), N, R, shared.groups, Hq, H, D, qt,
-            qh, page, pages, P, groupsize, min(max_q, N), max_kv, scale, dtype, dev, _raw_stream(dev))
+            qh, page, pages, P, groupsize, min(max_q, N), max_kv, scale, dtype, 4 * size, dev, _raw_stream(dev))
     elif window is not None:
         if window < 1 or sinks < 0:
             raise RuntimeError(f"a window holds a token at least, and sinks are not negative (window={window}, sinks={sinks})")
