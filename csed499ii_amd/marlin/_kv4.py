@@ -282,12 +282,24 @@ def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups:
     rows of the group; requests without new tokens (``cu_q``, as in the attention call) and those that share no
     page with the group's first one are left out, and attend to all of their tokens by themselves.  So
     whatever the groups are, the attention is right; they decide what is read once."""
-    dev = _device_of("block_table", block_table)
-    table, ctx = _ints("block_table", block_table, dev, 2), _ints("context_lens", context_lens, dev)
-    at, (R, P) = _ints("cu_groups", cu_groups, dev), block_table.shape
-    _check_page(page_size)
-    if context_lens.size(0) != R or cu_groups.size(0) < 1:
-        raise RuntimeError(f"context_lens has {context_lens.size(0)} requests, block_table {R}; cu_groups needs an entry")
+    try:  # (as in kv4_append)
+        R, P = block_table.shape
+        dev, table, ctx, at = block_table.get_device(), block_table.data_ptr(), context_lens.data_ptr(), cu_groups.data_ptr()
+        kind = torch.int32
+        fits = (dev >= 0 and context_lens.shape == (R,) and cu_groups.dim() == 1 and cu_groups.size(0) > 0
+                and block_table.dtype is context_lens.dtype is cu_groups.dtype is kind
+                and context_lens.get_device() == cu_groups.get_device() == dev and block_table.is_contiguous()
+                and context_lens.is_contiguous() and cu_groups.is_contiguous()
+                and page_size in (16, 32, 64, 128, 256))
+    except (AttributeError, TypeError, ValueError):
+        fits = False
+    if not fits:
+        dev = _device_of("block_table", block_table)
+        table, ctx = _ints("block_table", block_table, dev, 2), _ints("context_lens", context_lens, dev)
+        at, (R, P) = _ints("cu_groups", cu_groups, dev), block_table.shape
+        _check_page(page_size)
+        if context_lens.size(0) != R or cu_groups.size(0) < 1:
+            raise RuntimeError(f"context_lens has {context_lens.size(0)} requests, block_table {R}; cu_groups needs an entry")
     cu = 0
     if cu_q is not None:
         cu = _ints("cu_q", cu_q, dev)

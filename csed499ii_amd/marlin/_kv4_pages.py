@@ -47,7 +47,7 @@ class kv4_layers:
         if len(set(at)) != len(at):
             raise RuntimeError("kv4_layers got one cache twice")
         self.num_pages, self.kv_heads = shape[0], shape[1]
-        self.head_dim, self.groupsize = head_dim, groupsize
+        self.head_dim, self.groupsize, self.count = head_dim, groupsize, len(at)
         self._at = (ctypes.c_void_p * len(at))(*at)
 
     def __len__(self):
@@ -55,6 +55,14 @@ class kv4_layers:
 
 
 def _table(block_table, kv_lens):
+    try:  # (what fits passes in one look; anything else is checked step by step, for the message)
+        R, P = block_table.shape
+        dev, kind = block_table.get_device(), torch.int32
+        if dev >= 0 and kv_lens.shape == (R,) and block_table.dtype is kind and kv_lens.dtype is kind \
+                and kv_lens.get_device() == dev and block_table.is_contiguous() and kv_lens.is_contiguous():
+            return dev, block_table.data_ptr(), kv_lens.data_ptr(), R, P
+    except (AttributeError, TypeError, ValueError):
+        pass
     dev = _device_of("block_table", block_table)
     table, lens = _ints("block_table", block_table, dev, 2), _ints("kv_lens", kv_lens, dev)
     R, P = block_table.shape
@@ -78,14 +86,15 @@ def kv4_free_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, num_pages: 
     _check_page(page_size)
     if num_pages < 1 or num_pages * page_size > 2**31 - 1:
         raise RuntimeError("the KV cache holds a page at least and 2^31 - 1 tokens at most")
-    out = block_table.new_empty(num_pages + 1 + (num_pages + 15) // 16 * 4 + 4)
-    free, count, marks = out.split_with_sizes((num_pages, 1, out.numel() - num_pages - 1))
-    at = (marks.data_ptr() + 15) // 16 * 16
-    err = _lib.load().marlin_hip_kv4_free_pages(table, lens, free.data_ptr(), count.data_ptr(), at, R, P, page_size,
+    # (the marks behind the results, from a multiple of 16 bytes on)
+    marks = (num_pages + 1 + 3) // 4 * 4
+    out = block_table.new_empty(marks + (num_pages + 15) // 16 * 4)
+    at = out.data_ptr()
+    err = _lib.load().marlin_hip_kv4_free_pages(table, lens, at, at + 4 * num_pages, at + 4 * marks, R, P, page_size,
                                                 num_pages, dev, _raw_stream(dev))
     if err:
         _raise(err)
-    return free, count
+    return out.split_with_sizes((num_pages, 1, out.numel() - num_pages - 1))[:2]
 
 
 def kv4_copy_pages(layers: kv4_layers, source: torch.Tensor, target: torch.Tensor) -> None:
@@ -97,7 +106,7 @@ def kv4_copy_pages(layers: kv4_layers, source: torch.Tensor, target: torch.Tenso
     src, dst = _ints("source", source, layers.device), _ints("target", target, layers.device)
     if source.size(0) != target.size(0):
         raise RuntimeError(f"source has {source.size(0)} pages, target {target.size(0)}")
-    err = _lib.load().marlin_hip_kv4_copy_pages(layers._at, len(layers), src, dst, source.size(0), layers.kv_heads,
+    err = _lib.load().marlin_hip_kv4_copy_pages(layers._at, layers.count, src, dst, source.size(0), layers.kv_heads,
                                                 layers.head_dim, layers.page_size, layers.num_pages, layers.groupsize,
                                                 layers.device, _raw_stream(layers.device))
     if err:
@@ -124,16 +133,16 @@ def kv4_fork(layers: kv4_layers, block_table: torch.Tensor, kv_lens: torch.Tenso
     dev, table, lens, R, P = _table(block_table, kv_lens)
     _of_layers(layers, dev)
     par, free = _ints("parents", parents, dev), _ints("free_pages", free_pages, dev)
-    N = parents.size(0)
-    out = block_table.new_empty(N * P + 2 * N + 1)
-    new_table, new_lens, used, copies = out.split_with_sizes((N * P, N, 1, N))
-    err = _lib.load().marlin_hip_kv4_fork(layers._at, len(layers), table, lens, par, free, new_table.data_ptr(),
-                                          new_lens.data_ptr(), used.data_ptr(), copies.data_ptr(), R, N,
-                                          free_pages.size(0), P, layers.kv_heads, layers.head_dim, layers.page_size,
-                                          layers.num_pages, layers.groupsize, dev, _raw_stream(dev))
+    (N,), (F,) = parents.shape, free_pages.shape
+    new_table, out = block_table.new_empty((N, P)), block_table.new_empty(2 * N + 1)
+    at = out.data_ptr()
+    err = _lib.load().marlin_hip_kv4_fork(layers._at, layers.count, table, lens, par, free, new_table.data_ptr(), at,
+                                          at + 4 * N, at + 4 * (N + 1), R, N, F, P, layers.kv_heads, layers.head_dim,
+                                          layers.page_size, layers.num_pages, layers.groupsize, dev, _raw_stream(dev))
     if err:
         _raise(err)
-    return new_table.view(N, P), new_lens, used
+    new_lens, used, _ = out.split_with_sizes((N, 1, N))
+    return new_table, new_lens, used
 
 
 def kv4_compact(layers: kv4_layers, block_table: torch.Tensor, kv_lens: torch.Tensor):
@@ -148,7 +157,7 @@ def kv4_compact(layers: kv4_layers, block_table: torch.Tensor, kv_lens: torch.Te
     new_table = block_table.new_empty((R, P))
     work = block_table.new_empty(3 * pages + pages // 4 + 2 + 4)
     counts, lists = work[:2], (work.data_ptr() + 8 + 15) // 16 * 16
-    err = _lib.load().marlin_hip_kv4_compact(layers._at, len(layers), table, lens, new_table.data_ptr(),
+    err = _lib.load().marlin_hip_kv4_compact(layers._at, layers.count, table, lens, new_table.data_ptr(),
                                              counts.data_ptr(), lists, R, P, layers.kv_heads, layers.head_dim,
                                              layers.page_size, layers.num_pages, layers.groupsize, dev, _raw_stream(dev))
     if err:
