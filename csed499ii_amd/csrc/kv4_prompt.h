@@ -513,7 +513,9 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       e = fmaxf(pe.a, pe.b);
       const bool none = M == kNone, any = xm > -__builtin_inff();
       // (2^24: below the least v; where all v so far are zero the next may be any)
-      const float rel = fmaxf(e - kVTop, none ? -(kVTop + 24.f) : -kMostShift);
+      // (WINDOW: few sinks, the first tile, say little of what is to come)
+      const float top = FORM == WINDOW && tok0 < a.sinks ? kVTop - 6.f : kVTop;
+      const float rel = fmaxf(e - top, none ? -(top + 24.f) : -kMostShift);
       const bool rises = any && (none || __builtin_fmaf(xm, down, rel) > 0.f);
       const float new_base = rises ? base + __builtin_fmaf(rel, up, xm) : base;
       float less = new_base - base;
