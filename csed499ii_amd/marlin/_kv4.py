@@ -265,6 +265,7 @@ class kv4_prefix(typing.NamedTuple):
     groups: int
     pages: int
     page_size: int
+    one: bool  # made without cu_q: a token each
 
     @property
     def lens(self) -> torch.Tensor:
@@ -311,7 +312,7 @@ def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups:
                                             _raw_stream(dev))
     if err:
         _raise(err)
-    return kv4_prefix(plan, R, groups, P, page_size)
+    return kv4_prefix(plan, R, groups, P, page_size, cu_q is None)
 
 
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -342,7 +343,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     own and the ``window - 1`` before, and the first ``sinks`` of its request; only their pages are
     read.  With ``shared`` (:func:`kv4_shared` of the same step; ``context_lens`` needed, too) the tokens that
     requests of a group share are attended to once for all of them, in a pass of its own before the
-    one over each request's other tokens: the same sums in another order.  Not both.
+    one over each request's other tokens: the same sums in another order.  Not both.  ``shared`` is made from the
+    ``block_table``, ``context_lens`` and ``cu_q`` of this call: with others the result is wrong.
 
     A row that sees no token gets zeros and ``-inf``.  Rows that belong to no request (before
     ``cu_q[0]``, from ``cu_q[R]`` on: a captured step's padding) and those past a request's
@@ -415,9 +417,11 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
             raise RuntimeError("kv4_attention takes shared or window, not both")
         if not isinstance(shared, kv4_prefix):
             raise TypeError("shared must be what kv4_shared returns")
-        if (shared.requests, shared.pages, shared.page_size) != (R, P, page) or shared.plan.get_device() != dev or not ctx:
+        if (shared.requests, shared.pages, shared.page_size) != (R, P, page) or shared.plan.get_device() != dev or not ctx \
+                or shared.one != (cu_q is None):
             raise RuntimeError(f"shared is of {shared.requests} requests with {shared.pages} pages of {shared.page_size} "
-                               f"tokens and needs context_lens; the call has {R}, {P} and {page}")
+                               f"tokens, {'without' if shared.one else 'with'} cu_q, and needs context_lens; the call has "
+                               f"{R}, {P} and {page}")
         # (beside the rows of the first pass its parts, where it has more than a few rows a group: 256 of each compute unit)
         size = N * Hq * (D + 4) + 4
         if N * Hq > 64 * H * shared.groups:

@@ -81,7 +81,8 @@ def _of_layers(layers, dev):
 def kv4_free_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, num_pages: int, page_size: int):
     """The pages of a cache of ``num_pages`` that no request holds: ``(free [num_pages], count [1])``,
     int32, the free ones in ascending order and -1 behind them; ``free`` goes to :func:`kv4_tables` and
-    :func:`kv4_fork` as it is.  Entries that are no page are passed over."""
+    :func:`kv4_fork` as it is (where they want more than ``count`` pages, the tables get -1 as if the list had ended
+    there).  Entries that are no page are passed over."""
     dev, table, lens, R, P = _table(block_table, kv_lens)
     _check_page(page_size)
     if num_pages < 1 or num_pages * page_size > 2**31 - 1:
