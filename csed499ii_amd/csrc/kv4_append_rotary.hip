@@ -70,6 +70,7 @@ extern "C" int marlin_hip_kv4_append_rotary(
   const int err = check_geometry(kv_heads, head_dim, groupsize, page_size, num_pages, dtype);
   if (err != MARLIN_HIP_OK) return err;
   if (tokens < 0 || q_heads < 0) return refuse("kv4_append_rotary takes no negative sizes");
+  if (tokens > (1 << 30)) return refuse("more rows than one launch of the KV cache takes");
   if (rotary_dim < 2 || rotary_dim % 2 != 0 || rotary_dim > head_dim)
     return refuse("kv4_append_rotary turns an even number of dims, 2 at least and head_dim at most");
   if ((q_token_stride | q_head_stride | k_token_stride | k_head_stride | v_token_stride | v_head_stride |

@@ -401,6 +401,7 @@ int attention(const void* q, const void* cache, const void* block_table, const v
     a.where = b.where = reinterpret_cast<int2*>(a.before_ml + 2 * rows);
     a.parts = b.parts = prefix->workspace + parts_at;
     a.parts_ml = b.parts_ml = a.parts + place * head_dim;
+    a.places = b.places = (int)place;
   }
   err = attend<SHARED>(b, first, one);
   if (err != MARLIN_HIP_OK) return err;
@@ -468,6 +469,7 @@ int marlin_hip_kv4_shared(const void* block_table, const void* context_lens, con
   if (requests < 0 || groups < 0 || max_pages < 0) return kv4::refuse("kv4_shared takes no negative sizes");
   if (!kv4::page_ok(page_size)) return kv4::refuse("the KV cache's page_size must be 16, 32, 64, 128 or 256");
   if ((long long)max_pages * page_size > (1ll << 30)) return kv4::refuse("a block table row covers more than 2^30 tokens");
+  if (groups > (1 << 20)) return kv4::refuse("kv4_shared takes at most 2^20 groups");
   if (requests == 0 || groups == 0) return MARLIN_HIP_OK;
   sm24::DeviceScope scope(dev);
   if (!scope.ok) return MARLIN_HIP_ERR_LAUNCH;

@@ -576,6 +576,8 @@ int marlin_hip_kv4_fork(const void* const* caches, int layers, const void* block
   if (err != MARLIN_HIP_OK) return err;
   if (new_requests < 0 || num_free < 0) return refuse("kv4_fork takes no negative sizes");
   if (kv_heads > 32767) return refuse("kv4_fork takes at most 32767 heads");
+  // (each looks at the others' entries of one column)
+  if (new_requests > 65536) return refuse("kv4_fork makes at most 65536 requests");
   sm24::DeviceScope scope(dev);
   if (!scope.ok) return MARLIN_HIP_ERR_LAUNCH;
   const Tables t{static_cast<const int32_t*>(block_table), static_cast<const int32_t*>(kv_lens), requests, max_pages,

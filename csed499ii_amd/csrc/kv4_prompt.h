@@ -33,7 +33,7 @@
 namespace kv4 {
 
 constexpr int kMaxKinds = 256;     // row blocks of a launch whose tokens are divided
-constexpr int kMaxParts = 32;      // of a row block's tokens
+constexpr int kMaxParts = kMaxPartsLeft;  // of a row block's tokens
 constexpr float kMinShare = 4.f;   // tiles: a part costs its write and its read
 
 typedef float float16_t __attribute__((ext_vector_type(16)));

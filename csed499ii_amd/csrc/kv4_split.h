@@ -69,6 +69,7 @@ constexpr int kWhole = 3;
 constexpr int kTilesAt = 43;       // bit of a sum of units
 constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last workgroup's read of it
 constexpr int kLogTile = 6, kTile = 1 << kLogTile;  // tokens of a tile of the prompt kernel
+constexpr int kMaxPartsLeft = 32;  // of a block of rows of the prompt kernel
 constexpr int kPromptWaves = 8, kPromptRows = 32 * kPromptWaves;
 constexpr int kMaxRequests = 2 * 64 * kWaves;  // of a launch that divides by the requests' lengths
 constexpr float kVTop = 7.f;       // a new reference brings the row's largest p v to 2^7
@@ -113,6 +114,7 @@ struct AttnArgs {
   int2* where;           // [token][q head] a row's first place among the parts of divided blocks, and their number
   float* parts;          // [part][row of 256][D] sums of parts that the second pass adds (null: they meet in the first)
   float* parts_ml;
+  int places;            // rows that parts holds
   // of WINDOW
   int window, sinks;     // a token sees the last `window` positions, its own among them, and the first `sinks`
 };
@@ -857,7 +859,9 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
           if (d0 == 0) *reinterpret_cast<float2*>(a.before_ml + 2 * at) = make_float2(m, l);
           return;
         }
-        const int2 left = a.where != nullptr && rq.start > 0 ? a.where[at] : make_int2(0, 0);
+        int2 left = a.where != nullptr && rq.start > 0 ? a.where[at] : make_int2(0, 0);
+        // (a row that the first pass did not take, of a plan for other requests, has nothing sensible there)
+        if (left.x < 0 || left.y > kMaxPartsLeft || left.x + (long long)(left.y - 1) * a.kv_heads * kPromptRows >= a.places) left.y = 0;
         if (left.y > 0) {
           // the parts in order, after this row's own
           const size_t stride = (size_t)a.kv_heads * kPromptRows;

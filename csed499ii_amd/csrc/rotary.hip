@@ -39,7 +39,7 @@ int marlin_hip_rotary_angles(const void* positions, const void* freqs, void* ang
                              double factor, int dev, hipStream_t stream) {
   if (tokens < 0 || pairs < 0) return kv4::refuse("rotary_angles takes no negative sizes");
   const long long total = (long long)tokens * pairs;
-  if (total > 0x7FFFFFFFll * 64) return kv4::refuse("rotary_angles: too many angles for one launch");
+  if (total > 0xFFFFFF00ll) return kv4::refuse("rotary_angles: too many angles for one launch");
   if (total == 0) return MARLIN_HIP_OK;
   sm24::DeviceScope scope(dev);
   if (!scope.ok) return MARLIN_HIP_ERR_LAUNCH;
@@ -63,15 +63,16 @@ int marlin_hip_rotary(const void* x, const void* angles, void* out, int tokens, 
     return MARLIN_HIP_ERR_KERN_SHAPE;
   }
   if (tokens == 0 || heads == 0) return MARLIN_HIP_OK;
+  const int pairs = rotary_dim / 2;
+  const rotary::Shape s = rotary::shape_of(head_dim, pairs, interleaved != 0, heads);
+  const unsigned tiles = ((unsigned)tokens + s.tokens - 1) / s.tokens;
+  if (tiles > 0xFFFFFF) return kv4::refuse("rotary: more tokens than one launch takes");
   sm24::DeviceScope scope(dev);
   if (!scope.ok) return MARLIN_HIP_ERR_LAUNCH;
-  const int pairs = rotary_dim / 2;
   const rotary::Rows a{static_cast<const uint16_t*>(x), static_cast<uint16_t*>(out),
                        static_cast<const rotary::double2_t*>(angles), x_token_stride, x_head_stride, out_token_stride,
                        out_head_stride, tokens, heads, head_dim, pairs};
-  const rotary::Shape s = rotary::shape_of(head_dim, pairs, interleaved != 0, heads);
   // Few tokens: a workgroup for each round of heads; many: a thread keeps its angles for all of them.
-  const unsigned tiles = ((unsigned)tokens + s.tokens - 1) / s.tokens;
   const int rounds = (heads + s.heads - 1) / s.heads;
   int per = tiles < 512 ? 1 : rounds;
   if ((rounds + per - 1) / per > 65535) per = (rounds + 65534) / 65535;

@@ -282,7 +282,13 @@ def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups:
     falling).  Its prefix is the leading pages that lie within ``context_lens`` and are the same in all
     rows of the group; requests without new tokens (``cu_q``, as in the attention call) and those that share no
     page with the group's first one are left out, and attend to all of their tokens by themselves.  So
-    whatever the groups are, the attention is right; they decide what is read once."""
+    whatever the groups are, the attention is right; they decide what is read once.
+
+    The attention then takes two passes, which pays where reads that fall away cost more than a second launch
+    and the sums between them: (requests - groups) x kv heads x shared tokens from about a million on
+    (32 samples of 4096 shared tokens on 32 kv heads, 4.1 million: 47 us where 98 without; 8 samples of 8192 tokens on
+    8 kv heads, half a million: 37 to 41 where 30), with several tokens and query heads to a kv head from two
+    million (32 samples of 4 tokens on 64 and 8 heads, 4096 shared tokens, a million: 62 where 56)."""
     try:  # (as in kv4_append)
         R, P = block_table.shape
         dev, table, ctx, at = block_table.get_device(), block_table.data_ptr(), context_lens.data_ptr(), cu_groups.data_ptr()

@@ -25,12 +25,22 @@ def calls(lib, layers=1, requests=1, new=1, pairs=1, free=1, width=4, H=2, D=128
     ({"pages": 2 ** 28}, "free copy compact fork", _lib.ERR_PROB_SHAPE), ({"pages": 0}, "free compact fork", _lib.ERR_PROB_SHAPE),
     ({"layers": -1}, "copy compact fork", _lib.ERR_PROB_SHAPE), ({"pairs": -1}, "copy", _lib.ERR_PROB_SHAPE),
     ({"new": -1}, "fork", _lib.ERR_PROB_SHAPE), ({"free": -1}, "fork", _lib.ERR_PROB_SHAPE), ({"H": 0}, "copy compact fork", _lib.ERR_PROB_SHAPE),
+    ({"H": 32768}, "fork", _lib.ERR_PROB_SHAPE), ({"new": 65537}, "fork", _lib.ERR_PROB_SHAPE),
     ({"H": 2 ** 20, "page": 256}, "copy compact fork", _lib.ERR_PROB_SHAPE), ({"D": 96}, "copy compact fork", _lib.ERR_KERN_SHAPE),
     ({"g": 16}, "copy compact fork", _lib.ERR_KERN_SHAPE), ({"pairs": 0}, "copy", _lib.OK), ({"layers": 0}, "copy", _lib.OK),
 ])
 def test_codes(built_lib, change, who, code):
     for name in who.split():
         assert calls(built_lib, **change)[name]() == code, name
+
+
+def test_shared_codes(built_lib):
+    def call(requests=4, groups=2, width=4, page=16):
+        return built_lib.marlin_hip_kv4_shared(*[NULL] * 5, requests, groups, width, page, 0, NULL)
+
+    assert call(requests=0) == call(groups=0) == _lib.OK
+    for change in ({"requests": -1}, {"groups": -1}, {"width": -1}, {"width": 2 ** 27}, {"page": 24}, {"groups": 2 ** 20 + 1}):
+        assert call(**change) == _lib.ERR_PROB_SHAPE, change
 
 
 def test_wrappers_refuse(built_lib):

@@ -37,7 +37,7 @@ def rows(lib, tokens=2, heads=2, D=128, r=64, s=128, dtype=0):
 @pytest.mark.parametrize("change,code", [
     ({"tokens": 0}, _lib.OK), ({"heads": 0}, _lib.OK), ({"tokens": -1}, _lib.ERR_PROB_SHAPE), ({"D": 12, "r": 2}, _lib.ERR_PROB_SHAPE),
     ({"D": 1032}, _lib.ERR_PROB_SHAPE), ({"r": 130}, _lib.ERR_PROB_SHAPE), ({"r": 7}, _lib.ERR_PROB_SHAPE), ({"r": 0}, _lib.ERR_PROB_SHAPE),
-    ({"s": 129}, _lib.ERR_PROB_SHAPE), ({"dtype": 2}, _lib.ERR_KERN_SHAPE),
+    ({"s": 129}, _lib.ERR_PROB_SHAPE), ({"tokens": 2 ** 31 - 1, "heads": 64}, _lib.ERR_PROB_SHAPE), ({"dtype": 2}, _lib.ERR_KERN_SHAPE),
 ])
 def test_row_codes(built_lib, change, code):
     assert rows(built_lib, **change) == code
@@ -48,7 +48,7 @@ def append(lib, tokens=2, Hq=4, H=2, D=128, r=64, s=128, page=16, g=-1, dtype=0)
 
 
 @pytest.mark.parametrize("change,code", [
-    ({"tokens": 0}, _lib.OK), ({"tokens": -1}, _lib.ERR_PROB_SHAPE), ({"Hq": -1}, _lib.ERR_PROB_SHAPE), ({"H": 0}, _lib.ERR_PROB_SHAPE),
+    ({"tokens": 0}, _lib.OK), ({"tokens": -1}, _lib.ERR_PROB_SHAPE), ({"Hq": -1}, _lib.ERR_PROB_SHAPE), ({"tokens": 2 ** 31 - 1}, _lib.ERR_PROB_SHAPE), ({"H": 0}, _lib.ERR_PROB_SHAPE),
     ({"r": 130}, _lib.ERR_PROB_SHAPE), ({"r": 5}, _lib.ERR_PROB_SHAPE), ({"s": 4}, _lib.ERR_PROB_SHAPE), ({"page": 17}, _lib.ERR_PROB_SHAPE),
     ({"D": 96}, _lib.ERR_KERN_SHAPE), ({"g": 8}, _lib.ERR_KERN_SHAPE), ({"dtype": 3}, _lib.ERR_KERN_SHAPE),
 ])
@@ -58,7 +58,7 @@ def test_append_codes(built_lib, change, code):
 
 def test_angle_codes(built_lib):
     call = lambda n, p: built_lib.marlin_hip_rotary_angles(NULL, NULL, NULL, n, p, 1.0, 0, NULL)  # noqa: E731
-    assert call(0, 4) == call(4, 0) == _lib.OK and call(-1, 4) == call(4, -1) == _lib.ERR_PROB_SHAPE
+    assert call(0, 4) == call(4, 0) == _lib.OK and call(-1, 4) == call(4, -1) == call(2 ** 26, 64) == _lib.ERR_PROB_SHAPE
 
 
 def test_wrappers_refuse_cpu_tensors(built_lib):
