@@ -204,7 +204,7 @@ __global__ __launch_bounds__(kSharedThreads) void kv4_shared_kernel(SharedArgs a
     __syncthreads();
     if (tid < n) {
       const int common = first[tid];
-      a.start[from + tid] = common;
+      if (!one_round) a.start[from + tid] = common;
       if (common > 0) {
         atomicMin(&least, common);
         atomicAdd(&sharers, 1);
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(kSharedThreads) void kv4_shared_kernel(SharedArgs a
   __syncthreads();
   const int len = sharers > 1 ? least << a.log_page : 0;
   for (int from = r0; from < r1; from += kSharedRound)
-    if (from + tid < r1) a.start[from + tid] = a.start[from + tid] > 0 ? len : 0;
+    if (from + tid < r1) a.start[from + tid] = (one_round ? first[tid] : a.start[from + tid]) > 0 ? len : 0;
   if (tid == 0) {
     a.lens[g] = len;
     a.leads[g] = any ? leader : 0;
