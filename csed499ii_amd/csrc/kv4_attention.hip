@@ -114,8 +114,8 @@ int check(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int
 // ---------------------------------------------------------------------------
 // The prefix that the requests of a group share: the whole pages, from the first on, that are the
 // same in their tables and lie within their contexts.  A workgroup for each group compares every
-// request's row with the first one's; one more for the requests of
-// no group.  Once a step, for all layers.
+// request's row with the first one's; one more for the requests of no group.  Once a step, for all
+// layers.  64 rows of 512 entries in one group take 10 us, what one compute unit reads at; 4 groups of 8 rows 4.6.
 // ---------------------------------------------------------------------------
 
 constexpr int kSharedThreads = 1024, kSharedRound = 1024, kSharedWaves = kSharedThreads / 64, kSharedRows = 4;
@@ -318,7 +318,24 @@ struct Prefix {
   int groups;
   float* workspace;
   long long bytes;
+  bool always;
 };
+
+// Whether two passes can pay: what falls away, in steps of 16 rows and 32 tokens, if the prefix were all of max_kv.
+// A block of 256 rows of the prompt kernel counts as eight.  (With the second launch and the sums between
+// them the passes cost 15 to 20 us, an undivided pass 0.5 ns a step.  In graphs: 16 requests on 64 and 8 heads behind
+// 8192 tokens, 17000 steps fewer, 44.5 us where 42 in one pass; four groups of 8 on 32 heads behind 1500,
+// 47000 fewer, 42 where 53; 32 on 32 heads behind 4096, 130000 fewer, 47 where 98.  The worst that was found: 32
+// requests of 4 tokens on 64 and 8 heads behind 4096, 43000 fewer, 62 where 56.  Prompts, which the second
+// pass takes through the same kernel, from four times as many on.)
+bool shares(const Prefix& f, int tokens, int requests, int group, int kv_heads, int max_kv, bool first_prompts, bool prompts) {
+  auto blocks = [&](int n, bool big) {
+    const long long rows = ((long long)tokens + n - 1) / n * group;
+    return n * (big ? (rows + kPromptRows - 1) / kPromptRows * 8 : (rows + 15) / 16);
+  };
+  const long long fewer = blocks(requests, prompts) - blocks(f.groups, first_prompts);
+  return fewer * kv_heads * (max_kv / kStep) >= (prompts ? 4 : 1) * 20480ll;
+}
 
 int attention(const void* q, const void* cache, const void* block_table, const void* kv_lens, const void* cu_q,
               const void* context_lens, void* out, void* lse, int tokens, int requests, int q_heads, int kv_heads,
@@ -368,6 +385,10 @@ int attention(const void* q, const void* cache, const void* block_table, const v
   const Choice c = choose(tokens, requests, q_heads, kv_heads, head_dim, ng, max_q, cu_q != nullptr, p.cus);
   if (window > 0) return attend<WINDOW>(a, p, c);
   if (prefix == nullptr) return attend<PLAIN>(a, p, c);
+  const int average = (tokens + prefix->groups - 1) / prefix->groups;  // tokens that a group has
+  const bool big = (long long)average * group > split_rows(prefix->groups, kv_heads, head_dim, ng, p.cus);
+  if (!prefix->always && !shares(*prefix, tokens, requests, group, kv_heads, max_kv, big, c.prompts))
+    return attend<PLAIN>(a, p, c);
   const size_t rows = (size_t)tokens * q_heads;
   if (prefix->bytes < (long long)(rows * (head_dim + 2) * sizeof(float)))
     return refuse("kv4_attention of a shared prefix needs a workspace of head_dim + 2 floats a row");
@@ -383,9 +404,8 @@ int attention(const void* q, const void* cache, const void* block_table, const v
   Problem first = p;
   first.requests = prefix->groups;
   first.max_q = tokens;
-  const int average = (tokens + prefix->groups - 1) / prefix->groups;
   Choice one{};
-  one.prompts = (long long)average * group > split_rows(prefix->groups, kv_heads, head_dim, ng, p.cus);
+  one.prompts = big;
   one.split = !one.prompts;
   one.few_rows = 0x7FFFFFFF;
   one.split_q = average;
@@ -443,11 +463,11 @@ int marlin_hip_kv4_attention_shared(const void* q, const void* cache, const void
                                     void* workspace, int tokens, int requests, int groups, int q_heads, int kv_heads,
                                     int head_dim, long long q_token_stride, long long q_head_stride, int page_size,
                                     int num_pages, int max_pages, int groupsize, int max_q, int max_kv, float scale,
-                                    int dtype, long long workspace_bytes, int dev, hipStream_t stream) {
+                                    int dtype, long long workspace_bytes, int always, int dev, hipStream_t stream) {
   if (groups < 0) return kv4::refuse("kv4_attention takes no negative sizes");
   const int32_t* at = static_cast<const int32_t*>(shared);
   const kv4::Prefix prefix{at, at + groups, at + 2 * (size_t)groups, at + 3 * (size_t)groups + 1, groups,
-                           static_cast<float*>(workspace), workspace_bytes};
+                           static_cast<float*>(workspace), workspace_bytes, always != 0};
   return kv4::attention(q, cache, block_table, kv_lens, cu_q, context_lens, out, lse, tokens, requests, q_heads, kv_heads,
                         head_dim, q_token_stride, q_head_stride, page_size, num_pages, max_pages, groupsize, max_q, max_kv,
                         scale, dtype, dev, stream, 0, 0, groups > 0 ? &prefix : nullptr);

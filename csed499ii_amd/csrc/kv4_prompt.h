@@ -27,6 +27,11 @@
 // workgroup; the waves of the same rows meet in the uncached scratch, and the last to arrive
 // adds the parts in order.  A 512-token chunk on 64 and 8 heads with 4096 in all: 134 us
 // whole, 87 in two parts, whose write and read take 6.
+//
+// SHARED, first pass: 64 requests on 64 and 8 heads that share 8192 tokens are 512 rows a head, 16
+// blocks in 16 parts of 8 tiles: 37 us, 460 TFLOP/s, of which beginnings, the write of the parts (34 MB)
+// and 8 tiles' worth of filling take half.  WINDOW: 8000 tokens on 32 heads through 1024 and a few first
+// ones, 230 us where 126 GFLOP are seen: 16 tiles are whole and nine masked of a block's.
 #pragma once
 #include "kv4_split.h"
 
@@ -431,8 +436,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       }
     };
     // The same through a window, by a bit for each token of a half tile, from 4 h on, that the lane's row sees:
-    // two operations a score and two a pair of p v, where comparisons take twelve.  (Through a window nine
-    // tiles of a block of rows are masked in some wave: 8000 tokens on 32 heads, a window of 1024.)
+    // two operations a score and two a pair of p v, where comparisons take twelve.  (Through a window of 1024 nine
+    // tiles of a block of rows are masked in some wave: 8000 tokens on 32 heads, 291 us so and 260 by bits.)
     uint32_t bits[2] = {0, 0};
     if (FORM == WINDOW && masked) {
       int mine = tok0 + 4 * h;
@@ -824,7 +829,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   if constexpr (FORM == SHARED) {
     if (leaves) {
       // Through LDS, which the tiles no longer need: a wave's rows, 16 at a time, come out side by side.  (Each
-      // lane's eight dims straight to memory: 43 us where this takes 34.)
+      // lane's eight dims straight to memory: 42.9 us where this takes 38.5, 64 requests on 64 and 8 heads that
+      // share 8192 tokens.)
       constexpr int RP = 16 * (D + 4) * 4 * W <= 2 * BUF ? D + 4 : D;
       static_assert(16 * RP * 4 * W <= 2 * BUF, "");
       float* const mine = reinterpret_cast<float*>(lds) + wave * (16 * RP);

@@ -266,6 +266,7 @@ class kv4_prefix(typing.NamedTuple):
     pages: int
     page_size: int
     one: bool  # made without cu_q: a token each
+    always: bool = False  # two passes, whatever the sizes
 
     @property
     def lens(self) -> torch.Tensor:
@@ -274,7 +275,7 @@ class kv4_prefix(typing.NamedTuple):
 
 
 def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups: torch.Tensor, page_size: int,
-               cu_q: torch.Tensor | None = None) -> kv4_prefix:
+               cu_q: torch.Tensor | None = None, always: bool = False) -> kv4_prefix:
     """The prefixes that groups of requests share (after :func:`kv4_fork`, say), found in the block table
     once a step for the :func:`kv4_attention` of all layers.
 
@@ -284,11 +285,11 @@ def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups:
     page with the group's first one are left out, and attend to all of their tokens by themselves.  So
     whatever the groups are, the attention is right; they decide what is read once.
 
-    The attention then takes two passes, which pays where reads that fall away cost more than a second launch
-    and the sums between them: (requests - groups) x kv heads x shared tokens from about a million on
-    (32 samples of 4096 shared tokens on 32 kv heads, 4.1 million: 47 us where 98 without; 8 samples of 8192 tokens on
-    8 kv heads, half a million: 37 to 41 where 30), with several tokens and query heads to a kv head from two
-    million (32 samples of 4 tokens on 64 and 8 heads, 4096 shared tokens, a million: 62 where 56)."""
+    The attention then takes two passes, where the sizes say that they pay: by the blocks of rows, with ``max_kv``
+    for the prefix, whose reads fall away (32 samples of 4096 shared tokens on 32 kv heads 47 us where 98; but 8
+    samples on 8 kv heads, whose blocks of rows then fall from eight to four, 37 to 41 where 30, so one pass).
+    ``always`` makes it two whatever the sizes.
+    """
     try:  # (as in kv4_append)
         R, P = block_table.shape
         dev, table, ctx, at = block_table.get_device(), block_table.data_ptr(), context_lens.data_ptr(), cu_groups.data_ptr()
@@ -318,7 +319,7 @@ def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups:
                                             _raw_stream(dev))
     if err:
         _raise(err)
-    return kv4_prefix(plan, R, groups, P, page_size, cu_q is None)
+    return kv4_prefix(plan, R, groups, P, page_size, cu_q is None, always)
 
 
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
@@ -349,7 +350,7 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     own and the ``window - 1`` before, and the first ``sinks`` of its request; only their pages are
     read.  With ``shared`` (:func:`kv4_shared` of the same step; ``context_lens`` needed, too) the tokens that
     requests of a group share are attended to once for all of them, in a pass of its own before the
-    one over each request's other tokens: the same sums in another order.  Not both.  ``shared`` is made from the
+    one over each request's other tokens, where that pays: the same sums in another order.  Not both.  ``shared`` is made from the
     ``block_table``, ``context_lens`` and ``cu_q`` of this call: with others the result is wrong.
 
     A row that sees no token gets zeros and ``-inf``.  Rows that belong to no request (before
@@ -435,7 +436,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
         work = torch.empty(size, dtype=torch.float32, device=q.device)
         err = _lib.load().marlin_hip_kv4_attention_shared(
             qp, cp, table, lens, cu, ctx, shared.plan.data_ptr(), op, lp, work.data_ptr(), N, R, shared.groups, Hq, H, D, qt,
-            qh, page, pages, P, groupsize, min(max_q, N), max_kv, scale, dtype, 4 * size, dev, _raw_stream(dev))
+            qh, page, pages, P, groupsize, min(max_q, N), max_kv, scale, dtype, 4 * size, shared.always, dev,
+            _raw_stream(dev))
     elif window is not None:
         if window < 1 or sinks < 0:
             raise RuntimeError(f"a window holds a token at least, and sinks are not negative (window={window}, sinks={sinks})")

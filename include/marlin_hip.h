@@ -262,13 +262,14 @@ int marlin_hip_kv4_shared(const void* block_table, const void* context_lens, con
  * before that over each request's other tokens.  shared: from marlin_hip_kv4_shared with the same block_table,
  * context_lens and cu_q; context_lens must be given.  workspace: 16-byte aligned, workspace_bytes at least
  * 4 (head_dim + 2) for each row of q; with 4 (head_dim + 4) + 16 and 1024 (head_dim + 2) for each compute unit
- * the parts of a divided prefix meet as the rows are written, which is faster. */
+ * the parts of a divided prefix meet as the rows are written, which is faster.  always 0: in one pass, as
+ * marlin_hip_kv4_attention_ctx, where the sizes (max_kv for the prefix) say that two do not pay. */
 int marlin_hip_kv4_attention_shared(const void* q, const void* cache, const void* block_table, const void* kv_lens,
                                     const void* cu_q, const void* context_lens, const void* shared, void* out, void* lse,
                                     void* workspace, int tokens, int requests, int groups, int q_heads, int kv_heads,
                                     int head_dim, long long q_token_stride, long long q_head_stride, int page_size,
                                     int num_pages, int max_pages, int groupsize, int max_q, int max_kv, float scale,
-                                    int dtype, long long workspace_bytes, int dev, hipStream_t stream);
+                                    int dtype, long long workspace_bytes, int always, int dev, hipStream_t stream);
 
 /* The launch plan of a marlin_hip_kv4_attention call, computed on the host without a GPU (sms
  * <= 0: 256 compute units), for `requests` requests of max_q new tokens each (cu_q null where

@@ -191,7 +191,7 @@ def _shared(p, cu_groups, g, T, one=False, ctx=None, **kw):
     ctx = ints(kv - np.diff(cu) if ctx is None else ctx)
     cu = None if one else ints(cu)
     table, kv_ = ints(table), ints(kv)
-    s = marlin.kv4_shared(table, ctx, ints(cu_groups), T, cu)
+    s = marlin.kv4_shared(table, ctx, ints(cu_groups), T, cu, always=True)  # (two passes of the smallest, too)
     kw.setdefault("max_q", int(max(np.diff(p[4]), default=1)))
     kw.setdefault("max_kv", int(kv.max(initial=0)))
     return s, marlin.kv4_attention(q.to(DEV), torch.from_numpy(cache).to(DEV), table, kv_, cu, groupsize=g, return_lse=True,
@@ -268,6 +268,25 @@ def test_shared_what_is_shared():
     assert find([0]).lens.numel() == 0
 
 
+def test_shared_in_one_pass_where_two_do_not_pay():
+    """Few samples: the bits of a call without the prefix.  Many: two passes, other sums of the same."""
+    D, T = 128, 16
+    for R, H, same in ((4, 2, True), (64, 32, False)):
+        p, cu_groups = _forked([(80, R)], [1 + i % 30 for i in range(R)], [1] * R, H, H, D, -1, T, torch.float16, seed=8)
+        q, cache, table, kv = p[0].to(DEV), torch.from_numpy(p[1]).to(DEV), ints(p[2]), ints(p[3])
+        kw = dict(max_kv=int(p[3].max()), context_lens=kv - 1, return_lse=True)
+        plain = marlin.kv4_attention(q, cache, table, kv, **kw)
+        s = marlin.kv4_shared(table, kv - 1, ints(cu_groups), T)
+        assert s.lens.tolist() == [1280]
+        got = marlin.kv4_attention(q, cache, table, kv, shared=s, **kw)
+        assert all(torch.equal(a, b) for a, b in zip(plain, got)) == same
+        always = marlin.kv4_attention(q, cache, table, kv, shared=s._replace(always=True), **kw)
+        assert same or all(torch.equal(a, b) for a, b in zip(always, got))
+        want = attention(p[0].double().numpy(), *p[1:5], D, 1, T)
+        for out, lse in (got, always):
+            _check(out, lse, want, torch.float16, f"{R} requests")
+
+
 def test_shared_prefix_of_many_requests():
     """Several rounds of requests of one group, and more groups than a launch of attention takes."""
     T, D, R = 16, 64, 2300
@@ -304,7 +323,7 @@ def test_shared_missing_pages_padding_and_nan(one):
         wide = torch.cat([p[0], p[0][:3]]).to(DEV)  # three rows behind the last request
         out = torch.full(wide.shape, 7.0, dtype=torch.float16, device=DEV)
         table, kv, cu, ctx = ints(p[2]), ints(p[3]), ints(p[4]), ints(ctx)
-        s = marlin.kv4_shared(table, ctx, ints(cu_groups), T, cu)
+        s = marlin.kv4_shared(table, ctx, ints(cu_groups), T, cu, always=True)
         marlin.kv4_attention(wide, torch.from_numpy(p[1]).to(DEV), table, kv, cu, max_q=4, context_lens=ctx, shared=s, out=out)
         assert (out[-3:] == 7.0).all()
 
@@ -327,7 +346,7 @@ def test_shared_and_window_in_graphs_and_refusals():
     ctx, groups = kv - 1, ints(cu_groups)
 
     def step():
-        s = marlin.kv4_shared(table, ctx, groups, T)
+        s = marlin.kv4_shared(table, ctx, groups, T, always=True)
         return (marlin.kv4_attention(q, cache, table, kv, context_lens=ctx, shared=s, max_kv=700),
                 marlin.kv4_attention(q, cache, table, kv, context_lens=ctx, window=70, sinks=4, max_kv=700))
 

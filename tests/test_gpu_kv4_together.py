@@ -61,7 +61,7 @@ def test_forked_samples_are_the_requests_they_would_be(D, g, page, prompt):
         q0, _, n0 = write(y, caches[0], alone, alone_lens, [1] * S, pages)
         q1, _, n1 = write(y, caches[1], table, lens, [1] * S, pages)
         assert torch.equal(q0, q1) and torch.equal(n0, n1)
-        shared = marlin.kv4_shared(table, lens, groups, page)
+        shared = marlin.kv4_shared(table, lens, groups, page, always=i % 2 == 0)
         assert shared.lens.item() == prompt // page * page
         a = marlin.kv4_attention(q0, caches[0], alone, n0, max_kv=prompt + steps, groupsize=g)
         b = marlin.kv4_attention(q1, caches[1], table, n1, max_kv=prompt + steps, groupsize=g, context_lens=lens, shared=shared)
