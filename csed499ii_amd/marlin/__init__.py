@@ -13,8 +13,11 @@ Extensions that the reference keeps in side experiments:
 * ``mul_2_4_w3`` / ``pack_w3``: 3-bit nonzero values (no reference implementation).
 
 Beside the linear layers, what a decoder needs between qkv and o (no reference
-counterpart): ``kv4_cache``, ``kv4_tables``, ``kv4_append``, ``kv4_gather`` and
-``kv4_attention``, a paged KV cache held in 4 bits (``_kv4.py``).
+counterpart): ``kv4_cache``, ``kv4_tables``, ``kv4_append``, ``kv4_gather``, ``kv4_shared`` and
+``kv4_attention``, a paged KV cache held in 4 bits (``_kv4.py``); ``rotary_frequencies``,
+``rotary_angles``, ``rotary`` and ``kv4_append_rotary``, rotary positions (``_rotary.py``);
+``kv4_layers``, ``kv4_free_pages``, ``kv4_copy_pages``, ``kv4_fork`` and ``kv4_compact``, the cache's
+pages (``_kv4_pages.py``).
 """
 from __future__ import annotations
 

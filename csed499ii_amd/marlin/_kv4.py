@@ -420,12 +420,12 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     if scale is None:
         scale = 1.0 / math.sqrt(D)
     if shared is not None:
-        if window is not None:
-            raise RuntimeError("kv4_attention takes shared or window, not both")
+        if window is not None or sinks:
+            raise RuntimeError("kv4_attention takes shared or window and sinks, not both")
         if not isinstance(shared, kv4_prefix):
             raise TypeError("shared must be what kv4_shared returns")
-        if (shared.requests, shared.pages, shared.page_size) != (R, P, page) or shared.plan.get_device() != dev or not ctx \
-                or shared.one != (cu_q is None):
+        if (shared.requests, shared.pages, shared.page_size) != (R, P, page) or shared.plan.get_device() != dev \
+                or context_lens is None or shared.one != (cu_q is None):
             raise RuntimeError(f"shared is of {shared.requests} requests with {shared.pages} pages of {shared.page_size} "
                                f"tokens, {'without' if shared.one else 'with'} cu_q, and needs context_lens; the call has "
                                f"{R}, {P} and {page}")

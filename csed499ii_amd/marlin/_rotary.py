@@ -45,11 +45,14 @@ def rotary_frequencies(rotary_dim: int, base: float = 10000.0, scale: float = 1.
     if original is not None and not (0 < original < math.inf and -math.inf < slow < fast < math.inf):
         raise RuntimeError("rotary_frequencies by parts needs a positive original length and slow < fast")
     out = []
-    for i in range(rotary_dim // 2):
-        f = base ** (-2 * i / rotary_dim)
-        m = 0.0 if original is None else min(max((original * f / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0)
-        turns = int(f * (m + (1.0 - m) / scale) / (2 * math.pi) * 2.0 ** 64) % 2 ** 64
-        out.append(turns - 2 ** 64 if turns >= 2 ** 63 else turns)
+    try:
+        for i in range(rotary_dim // 2):
+            f = base ** (-2 * i / rotary_dim)
+            m = 0.0 if original is None else min(max((original * f / (2 * math.pi) - slow) / (fast - slow), 0.0), 1.0)
+            turns = int(f * (m + (1.0 - m) / scale) / (2 * math.pi) * 2.0 ** 64) % 2 ** 64
+            out.append(turns - 2 ** 64 if turns >= 2 ** 63 else turns)
+    except OverflowError:
+        raise RuntimeError(f"base {base} and scale {scale} make frequencies that are not finite") from None
     return torch.tensor(out, dtype=torch.int64).to(device)
 
 

@@ -1,5 +1,7 @@
 """Helpers of the GPU parity tests: oracle references for packed operands and
 column slices of the packed layouts."""
+import ctypes
+
 import numpy as np
 import torch
 
@@ -7,6 +9,15 @@ from oracle import sm24_oracle as o
 
 REL_MAE = 1e-3   # mean|C - ref| / mean|ref|
 MAX_REL = 2e-2   # max|C - ref| / max|ref|
+
+
+def new_stream(device="cuda:0"):
+    """A stream of its own, kept for good: torch hands out a pool's in turn, and other tests count
+    on getting one that no call has used."""
+    hip, handle = ctypes.CDLL("libamdhip64.so"), ctypes.c_void_p()
+    with torch.cuda.device(device):
+        assert hip.hipStreamCreateWithFlags(ctypes.byref(handle), 1) == 0  # (does not wait for the null stream)
+    return torch.cuda.ExternalStream(handle.value, device=device)
 
 
 def slice_cols(t: dict, c0: int, nc: int) -> dict:

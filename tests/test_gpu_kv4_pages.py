@@ -7,6 +7,7 @@ import torch
 from csed499ii_amd import marlin
 from tests import kv4_pages_ref as pages
 from tests import kv4_ref as ref
+from tests.gpu_util import new_stream
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -251,7 +252,7 @@ def test_graph():
         c, counts = marlin.kv4_compact(on, t, kv)
         return t, n, used, count, slots, kv, c, counts
 
-    side = torch.cuda.Stream()
+    side = new_stream()
     side.wait_stream(torch.cuda.current_stream())
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.stream(side):

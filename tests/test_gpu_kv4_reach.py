@@ -12,6 +12,7 @@ import torch
 
 from csed499ii_amd import marlin
 from tests import kv4_ref as ref
+from tests.gpu_util import new_stream
 from tests.test_gpu_kv4 import GEOMETRIES, _check, _problem
 
 pytestmark = pytest.mark.gpu
@@ -268,6 +269,14 @@ def test_shared_what_is_shared():
     assert find([0]).lens.numel() == 0
 
 
+def test_shared_of_nothing():
+    cache = marlin.kv4_cache(4, 2, 128, device=DEV)
+    table, none, q = torch.zeros((0, 3), dtype=torch.int32, device=DEV), ints([]), torch.zeros((0, 4, 128), dtype=torch.float16, device=DEV)
+    for cu_groups in ([0], [0, 0]):
+        s = marlin.kv4_shared(table, none, ints(cu_groups), 16, always=True)
+        assert marlin.kv4_attention(q, cache, table, none, context_lens=none, shared=s).shape == q.shape
+
+
 def test_shared_in_one_pass_where_two_do_not_pay():
     """Few samples: the bits of a call without the prefix.  Many: two passes, other sums of the same."""
     D, T = 128, 16
@@ -350,7 +359,7 @@ def test_shared_and_window_in_graphs_and_refusals():
         return (marlin.kv4_attention(q, cache, table, kv, context_lens=ctx, shared=s, max_kv=700),
                 marlin.kv4_attention(q, cache, table, kv, context_lens=ctx, window=70, sinks=4, max_kv=700))
 
-    side = torch.cuda.Stream()
+    side = new_stream()
     side.wait_stream(torch.cuda.current_stream())
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.stream(side):
@@ -370,7 +379,7 @@ def test_shared_and_window_in_graphs_and_refusals():
         assert all(torch.equal(a, b) for a, b in zip(got, again))
     s = marlin.kv4_shared(table, ctx, groups, T)
     call = lambda **kw: marlin.kv4_attention(q, cache, table, kv, **kw)  # noqa: E731
-    for kw, what in (({"shared": s}, "context_lens"), ({"shared": s, "context_lens": ctx, "window": 5}, "not both"), ({"window": 0}, "window"),
+    for kw, what in (({"shared": s}, "context_lens"), ({"shared": s, "context_lens": ctx, "window": 5}, "not both"), ({"shared": s, "context_lens": ctx, "sinks": 2}, "not both"), ({"window": 0}, "window"),
                      ({"window": 4, "sinks": -1}, "sinks"), ({"sinks": 4}, "sinks")):
         with pytest.raises(RuntimeError, match=what):
             call(**kw)

@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from csed499ii_amd import marlin
+from tests.gpu_util import new_stream
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -177,7 +178,7 @@ def test_graph_and_other_stream():
     def step():
         return marlin.kv4_append_rotary(q, k, v, cache, slots, marlin.rotary_angles(pos, f))
 
-    side = torch.cuda.Stream()
+    side = new_stream()
     side.wait_stream(torch.cuda.current_stream())
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.stream(side):

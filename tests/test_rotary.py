@@ -23,7 +23,8 @@ def test_frequencies_are_turns():
 
 
 @pytest.mark.parametrize("kw", [{"rotary_dim": 3}, {"rotary_dim": 0}, {"rotary_dim": 8, "base": 0.0}, {"rotary_dim": 8, "scale": -1.0},
-                                {"rotary_dim": 8, "scale": float("nan")}, {"rotary_dim": 8, "original": 0},
+                                {"rotary_dim": 8, "scale": float("nan")},
+                                {"rotary_dim": 256, "base": 1e-300}, {"rotary_dim": 8, "scale": 1e-308}, {"rotary_dim": 8, "original": 0},
                                 {"rotary_dim": 8, "original": 4096, "slow": 4.0, "fast": 4.0}])
 def test_frequencies_refuse(kw):
     with pytest.raises(RuntimeError):
