@@ -68,6 +68,9 @@ constexpr int kLead = 2;
 // 23.3 us divided, 16.6 whole; 16 of 1000 on 8 heads 14.3 and 14.2; one of 1000 on 32 heads,
 // which stays divided, 11.0 and 12.7.
 constexpr int kWhole = 3;
+// The same of a prefix, whose blocks have more rows, all of which meet: four groups of 8 requests of 4 tokens behind 1000
+// to 2000, 32 heads, 36.7 us with 3, 25.3 with 8, 25.6 with 14; one group behind 4096 (16 units) 26.0, 26.3 and 31.8.
+constexpr int kWholePrefix = 8;
 constexpr int kTilesAt = 43;       // bit of a sum of units
 constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last workgroup's read of it
 constexpr int kLogTile = 6, kTile = 1 << kLogTile;  // tokens of a tile of the prompt kernel
@@ -432,7 +435,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
       const long long tiles = all >> kTilesAt, units = all & ((1ll << kTilesAt) - 1);
       // tiles stay whole, one a workgroup, where none takes much more than an even share
       const bool whole = tiles <= gridDim.x &&
-                         (longest - a.lead - kWhole) * (long long)a.slots <= units - tiles * a.lead;
+                         (longest - a.lead - (FORM == SHARED && a.start == nullptr ? kWholePrefix : kWhole)) * (long long)a.slots <= units - tiles * a.lead;
       if (__builtin_amdgcn_readfirstlane((int)(whole || units > 0x7FFFFFFFll))) {
         divided = false;
         continue;
