@@ -17,9 +17,11 @@ namespace kv4 {
 // us beside 72 to 73; with groups of 32, 128, 144 and 160 rows, 104, 123 and 133 beside 108,
 // 125 and 125.
 // Few tiles leave the prompt kernel's large parts waiting: one request of 8192 tokens, 24 us
-// beside 34 at 64 rows, 41 beside 57 at 256.
-int split_rows(int requests, int kv_heads, int head_dim, int ng, int cus) {
-  if ((long long)requests * kv_heads <= cus / 16) return 256;
+// beside 34 at 64 rows, 41 beside 57 at 256.  (Of a prefix, whose parts need not meet, only tiles that
+// kMaxParts leaves compute units without one, `few` = cus / 64: 32 requests on 64 and 8 heads behind 8192 tokens in one
+// and two groups 63 and 82 us in the split kernel, 58 and 64 here; 64 on 16 and 4 heads 45 and 49.)
+int split_rows(int requests, int kv_heads, int head_dim, int ng, int few) {
+  if ((long long)requests * kv_heads <= few) return 256;
   return head_dim == 128 && ng == 4 ? 144 : 80;
 }
 
@@ -89,7 +91,7 @@ struct Choice {
 Choice choose(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int ng, int max_q, bool cu, int cus) {
   Choice c;
   const int group = q_heads / kv_heads;
-  c.few_rows = split_rows(requests, kv_heads, head_dim, ng, cus);
+  c.few_rows = split_rows(requests, kv_heads, head_dim, ng, cus / 16);
   c.prompts = (long long)max_q * group > c.few_rows;
   c.split_q = c.prompts ? c.few_rows / group : max_q;
   // (where the tokens say that no request can be short, the prompt kernel takes all)
@@ -326,7 +328,8 @@ struct Prefix {
 // them the passes cost 15 to 20 us, an undivided pass 0.5 ns a step.  In graphs: 16 requests on 64 and 8 heads behind
 // 8192 tokens, 17000 steps fewer, 44.5 us where 42 in one pass; four groups of 8 on 32 heads behind 1500,
 // 47000 fewer, 42 where 53; 32 on 32 heads behind 4096, 130000 fewer, 47 where 98.  The worst that was found: 32
-// requests of 4 tokens on 64 and 8 heads behind 4096, 43000 fewer, 62 where 56.  Prompts, which the second
+// requests of 4 tokens on 64 and 8 heads behind 4096, 43000 fewer, 62 where 56.  A prefix in the prompt kernel from half
+// as many more on: 64 on 64 and 8 heads behind 2000 in two groups, 25000 fewer, 46 where 33.  Prompts, which the second
 // pass takes through the same kernel, from four times as many on.)
 bool shares(const Prefix& f, int tokens, int requests, int group, int kv_heads, int max_kv, bool first_prompts, bool prompts) {
   auto blocks = [&](int n, bool big) {
@@ -334,7 +337,7 @@ bool shares(const Prefix& f, int tokens, int requests, int group, int kv_heads, 
     return n * (big ? (rows + kPromptRows - 1) / kPromptRows * 8 : (rows + 15) / 16);
   };
   const long long fewer = blocks(requests, prompts) - blocks(f.groups, first_prompts);
-  return fewer * kv_heads * (max_kv / kStep) >= (prompts ? 4 : 1) * 20480ll;
+  return fewer * kv_heads * (max_kv / kStep) >= (prompts ? 81920 : first_prompts ? 32768 : 20480);
 }
 
 int attention(const void* q, const void* cache, const void* block_table, const void* kv_lens, const void* cu_q,
@@ -386,7 +389,7 @@ int attention(const void* q, const void* cache, const void* block_table, const v
   if (window > 0) return attend<WINDOW>(a, p, c);
   if (prefix == nullptr) return attend<PLAIN>(a, p, c);
   const int average = (tokens + prefix->groups - 1) / prefix->groups;  // tokens that a group has
-  const bool big = (long long)average * group > split_rows(prefix->groups, kv_heads, head_dim, ng, p.cus);
+  const bool big = (long long)average * group > split_rows(prefix->groups, kv_heads, head_dim, ng, p.cus / 64);
   if (!prefix->always && !shares(*prefix, tokens, requests, group, kv_heads, max_kv, big, c.prompts))
     return attend<PLAIN>(a, p, c);
   const size_t rows = (size_t)tokens * q_heads;

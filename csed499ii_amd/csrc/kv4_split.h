@@ -873,18 +873,8 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
           const float* const ml = a.parts_ml + 2 * (size_t)left.x;
           const float* const v = a.parts + (size_t)left.x * D + d0;
           constexpr int FLIGHT = 8;
-          float most = m;
           for (int p = 0; p < left.y; p += FLIGHT) {
-            float x[FLIGHT];  // (those past the last repeat it)
-#pragma unroll
-            for (int k = 0; k < FLIGHT; k++) x[k] = ml[2 * stride * min(p + k, left.y - 1)];
-#pragma unroll
-            for (int k = 0; k < FLIGHT; k++) most = fmaxf(most, x[k]);
-          }
-          const float f = __builtin_amdgcn_exp2f(m - most);
-          m = most, l *= f, o *= f;
-          for (int p = 0; p < left.y; p += FLIGHT) {
-            float2 x[FLIGHT];
+            float2 x[FLIGHT];  // (those past the last repeat it)
             float4_t y[FLIGHT];
 #pragma unroll
             for (int k = 0; k < FLIGHT; k++) {
@@ -892,6 +882,11 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
               x[k] = *reinterpret_cast<const float2*>(ml + 2 * i);
               y[k] = *reinterpret_cast<const float4_t*>(v + i * D);
             }
+            float most = m;
+#pragma unroll
+            for (int k = 0; k < FLIGHT; k++) most = fmaxf(most, x[k].x);
+            const float f = __builtin_amdgcn_exp2f(m - most);
+            m = most, l *= f, o *= f;
 #pragma unroll
             for (int k = 0; k < FLIGHT; k++) {
               if (p + k >= left.y) break;
