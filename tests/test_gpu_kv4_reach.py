@@ -269,6 +269,55 @@ def test_shared_what_is_shared():
     assert find([0]).lens.numel() == 0
 
 
+@pytest.mark.parametrize("n", [1, 3, 30])
+def test_far_pages(n):
+    """Pages whose byte offset passes 32 bits, through a window and behind a prefix, turned as they are written."""
+    D, T, H, G, R = 128, 256, 8, 2, 4
+    pages = 17000  # 4.6 GB
+    cache = torch.zeros((pages, H, T * (D + 4)), dtype=torch.uint8, device=DEV)
+    assert cache.numel() > 2 ** 32
+    gen = torch.Generator().manual_seed(n)
+    k, v = (torch.randn((7 * T, H, D), generator=gen).half().to(DEV) for _ in range(2))
+    angles = marlin.rotary_angles(torch.arange(7 * T, dtype=torch.int32, device=DEV), marlin.rotary_frequencies(D, device=DEV))
+    marlin.kv4_append_rotary(None, k, v, cache, ints(np.arange(7 * T) + (pages - 7) * T), angles)
+    small = cache[-7:].cpu().numpy()
+    want_small = marlin.kv4_cache(7, H, D, T, device=DEV)
+    marlin.kv4_append(marlin.rotary(k, angles), v, want_small, ints(np.arange(7 * T)))
+    assert torch.equal(cache[-7:], want_small)
+    table = np.array([[0, 1, 2, 3 + r] for r in range(R)])  # three pages shared, the last one each request's own
+    kv, cu = np.array([3 * T + 9 + 60 * r + n for r in range(R)]), np.arange(R + 1) * n
+    q = torch.randn((R * n, G * H, D), generator=gen).half()
+    far = ints(table + pages - 7)
+    kw = dict(cu_q=ints(cu), max_q=n, max_kv=int(kv.max()), return_lse=True, context_lens=ints(kv - n))
+    want = attention(q.double().numpy(), small, table, kv, cu, D, 1, T)
+    s = marlin.kv4_shared(far, ints(kv - n), ints([0, R]), T, ints(cu), always=True)
+    assert s.lens.tolist() == [3 * T]
+    _check(*marlin.kv4_attention(q.to(DEV), cache, far, ints(kv), shared=s, **kw), want, torch.float16, f"{n} tokens, shared")
+    want = attention(q.double().numpy(), small, table, kv, cu, D, 1, T, 100, 5)
+    _check(*marlin.kv4_attention(q.to(DEV), cache, far, ints(kv), window=100, sinks=5, **kw), want, torch.float16, f"{n} tokens, window")
+
+
+@pytest.mark.parametrize("form", ["shared", "window"])
+@pytest.mark.parametrize("n", [4, 40])
+def test_strided_rows_and_tokens_past_max_q(form, n):
+    """q a slice of wider rows, out given; a request's tokens past max_q keep what out held."""
+    D, T, R, Hq, H = 128, 16, 12, 8, 2
+    p, cu_groups = _forked([(20, R)], [n + 3 + i for i in range(R)], [n] * R, Hq, H, D, -1, T, torch.float16, seed=n)
+    q, cache, table, kv, cu = p[0].to(DEV), torch.from_numpy(p[1]).to(DEV), ints(p[2]), ints(p[3]), ints(p[4])
+    wide = torch.randn((R * n, Hq + 5, D + 8), device=DEV).half()
+    wide[:, 2:2 + Hq, :D] = q
+    reach = {"window": 50, "sinks": 3} if form == "window" else {"shared": marlin.kv4_shared(table, kv - n, ints(cu_groups), T, cu, always=True)}
+    want = attention(p[0].double().numpy(), *p[1:5], D, 1, T, *((50, 3) if form == "window" else ()))
+    out = torch.full((R * n, Hq, D), 7.0, dtype=torch.float16, device=DEV)
+    most = n - 1
+    got, lse = marlin.kv4_attention(wide[:, 2:2 + Hq, :D], cache, table, kv, cu, max_q=most, max_kv=int(p[3].max()), out=out,
+                                    return_lse=True, context_lens=kv - n, **reach)
+    assert got.data_ptr() == out.data_ptr()
+    rows = torch.tensor([t % n < most for t in range(R * n)])
+    assert (out[~rows] == 7.0).all()
+    _check(got[rows], lse[rows], [x[rows.numpy()] for x in want], torch.float16, f"{form}, {n} tokens")
+
+
 def test_shared_of_nothing():
     cache = marlin.kv4_cache(4, 2, 128, device=DEV)
     table, none, q = torch.zeros((0, 3), dtype=torch.int32, device=DEV), ints([]), torch.zeros((0, 4, 128), dtype=torch.float16, device=DEV)
