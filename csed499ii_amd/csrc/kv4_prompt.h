@@ -31,7 +31,7 @@
 // SHARED, first pass: 64 requests on 64 and 8 heads that share 8192 tokens are 512 rows a head, 16
 // blocks in 16 parts of 8 tiles: 37 us, 460 TFLOP/s, of which beginnings, the write of the parts (34 MB)
 // and 8 tiles' worth of filling take half.  WINDOW: 8000 tokens on 32 heads through 1024 and a few first
-// ones, 230 us where 126 GFLOP are seen: 16 tiles are whole and nine masked of a block's.
+// ones, 230 us where 126 GFLOP are seen: of a block's 21 tiles twelve are whole.
 #pragma once
 #include "kv4_split.h"
 

@@ -44,9 +44,9 @@
 // 5.1 that a large copy reaches.  From two blocks on, by the unpacking, which every block
 // repeats (12 requests of five tokens, 40 rows, 4096 in all: 47 us, 36 at 24 rows).  Short ones
 // by latencies one after the other (lengths, table, codes, the meeting): one request of 1000
-// tokens on 32 heads, 11.0 us.  Through a window 24 requests on 8 heads have 130 steps a row block,
-// six a wave: 33 us, 2.9 TB/s of what they see.  Behind a prefix (SHARED) 64 requests of 100 to 200 tokens on
-// 64 and 8 heads take 22 us, 28 where they add 16 parts of a row.
+// tokens on 32 heads, 11.0 us.  Through a window of 4096 tokens 24 requests on 8 heads have 192 tiles, which
+// stay whole, 17 steps a wave: 33 us, 3.0 TB/s of what they see.  Behind a prefix (SHARED) 64 requests of 100 to 200 tokens
+// on 64 and 8 heads take 21 us, 1 to 1000 tokens 27, with the 16 parts of each row that they add.
 //
 // The waves meet in LDS; the partial sums of a divided tile go through the uncached
 // scratch, and the last of its workgroups to arrive on its counter adds them in order: one
