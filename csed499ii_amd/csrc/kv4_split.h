@@ -68,12 +68,12 @@ constexpr int kLead = 2;
 // 23.3 us divided, 16.6 whole; 16 of 1000 on 8 heads 14.3 and 14.2; one of 1000 on 32 heads,
 // which stays divided, 11.0 and 12.7.
 constexpr int kWhole = 3;
-// The same of a prefix, whose blocks have more rows, all of which meet: four groups of 8 requests of 4 tokens behind 1000
-// to 2000, 32 heads, 36.7 us with 3, 25.3 with 8, 25.6 with 14; one group behind 4096 (16 units) 26.0, 26.3 and 31.8.
-constexpr int kWholePrefix = 8;
-// And through a window, where the tiles are alike: 24 requests on 8 heads, 1024 tokens (5 units), 20.6 us divided, 15.0 whole;
-// 8 on 32 heads, 4096 (17 units, an even share of 8.5), 38.6 and 33.5; 3 on 32 heads (a share of 3), 23.3 and 31.0.
-constexpr int kWholeWindow = 11;
+// In the other forms, whose tiles are many, the meeting costs as much as the share besides: so much
+// traffic to uncached memory.  Units beyond twice an even share (lead counted):
+// through a window 192 tiles of 5 units (a share of 2.6) 20.6 us divided, 15.0 whole, 256 of 17 (9.5) 38.6 and 33.5, 96 of
+// 17 (3.6) 23.3 and 31.0, 58 of 9 and less (0.7) 15.6 and 22.3; of a prefix 256 of 4 to 8 (4) 36.7 and 25.3, 64 of 16 (2.3)
+// 26.0 and 31.8.
+constexpr int kWholeTwice = 4;
 constexpr int kTilesAt = 43;       // bit of a sum of units
 constexpr int kMaxSplits = 32;     // pieces of one tile: each costs its last workgroup's read of it
 constexpr int kLogTile = 6, kTile = 1 << kLogTile;  // tokens of a tile of the prompt kernel
@@ -437,9 +437,10 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     if (divided) {
       const long long tiles = all >> kTilesAt, units = all & ((1ll << kTilesAt) - 1);
       // tiles stay whole, one a workgroup, where none takes much more than an even share
-      const int whole_beyond = FORM == WINDOW ? kWholeWindow : FORM == SHARED && a.start == nullptr ? kWholePrefix : kWhole;
+      const bool twice = FORM == WINDOW || (FORM == SHARED && a.start == nullptr);
       const bool whole = tiles <= gridDim.x &&
-                         (longest - a.lead - whole_beyond) * (long long)a.slots <= units - tiles * a.lead;
+                         (twice ? (longest - a.lead - kWholeTwice) * (long long)a.slots <= 2 * units
+                                : (longest - a.lead - kWhole) * (long long)a.slots <= units - tiles * a.lead);
       if (__builtin_amdgcn_readfirstlane((int)(whole || units > 0x7FFFFFFFll))) {
         divided = false;
         continue;
