@@ -816,8 +816,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
         float x[8];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float keep = out_h ? O[n][4 * e + k + 2] : O[n][4 * e + k];
-          const float give = out_h ? O[n][4 * e + k] : O[n][4 * e + k + 2];
+          const float low = O[n][4 * e + k], high = O[n][4 * e + k + 2];  // (by value: a choice of elements becomes an index)
+          const float keep = out_h ? high : low, give = out_h ? low : high;
           const float got = __shfl_xor(give, 32);
           x[2 * e] = out_h ? got : keep;
           x[2 * e + 1] = out_h ? keep : got;
