@@ -286,10 +286,9 @@ def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups:
     whatever the groups are, the attention is right; they decide what is read once.
 
     The attention then takes two passes, where the sizes say that they pay: by the blocks of rows, with ``max_kv``
-    for the prefix, whose reads fall away (32 samples of 4096 shared tokens on 32 kv heads 47 us where 98; but 8
-    samples on 8 kv heads, whose blocks of rows then fall from eight to four, 37 to 41 where 30, so one pass).
-    ``always`` makes it two whatever the sizes.
-    """
+    for the prefix, whose reads fall away (32 samples of 4096 shared tokens on 32 heads 47 us where 98; but 8 samples
+    of 8192 on 64 and 8 heads, whose blocks of 16 rows fall from eight to four a head, 37 to 41 where 30, so one pass).
+    ``always`` makes it two whatever the sizes."""
     try:  # (as in kv4_append)
         R, P = block_table.shape
         dev, table, ctx, at = block_table.get_device(), block_table.data_ptr(), context_lens.data_ptr(), cu_groups.data_ptr()
