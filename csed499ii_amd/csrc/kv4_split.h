@@ -162,8 +162,10 @@ __device__ __forceinline__ Request request_of(const AttnArgs& a, int r) {
   q.past = min(kv - n, 1 << 30);
   if constexpr (FORM == SHARED) {
     if (a.start != nullptr) {
-      q.start = min(max(a.start[r], 0), cap) >> a.log_page << a.log_page;
-      q.kv = max(q.kv - q.start, 0);
+      // (a request whose tokens end inside the prefix attends by itself: the pass before has summed all of it)
+      const int start = min(max(a.start[r], 0), cap) >> a.log_page << a.log_page;
+      q.start = start <= q.kv ? start : 0;
+      q.kv -= q.start;
       q.past -= q.start;
     }
   }

@@ -349,7 +349,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     own and the ``window - 1`` before, and the first ``sinks`` of its request; only their pages are
     read.  With ``shared`` (:func:`kv4_shared` of the same step; ``context_lens`` needed, too) the tokens that
     requests of a group share are attended to once for all of them, in a pass of its own before the
-    one over each request's other tokens, where that pays: the same sums in another order.  Not both.  ``shared`` is made from the
+    one over each request's other tokens, where that pays: the same sums in another order (a request whose ``kv_lens``
+    end inside the prefix attends by itself).  Not both.  ``shared`` is made from the
     ``block_table``, ``context_lens`` and ``cu_q`` of this call: with others the result is wrong.
 
     A row that sees no token gets zeros and ``-inf``.  Rows that belong to no request (before

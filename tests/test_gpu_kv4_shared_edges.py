@@ -1,0 +1,29 @@
+"""Attention behind shared prefixes where lengths do not fit each other, or there is nothing to share."""
+import numpy as np
+import pytest
+import torch
+
+from csed499ii_amd import marlin
+from tests.test_gpu_kv4 import DEV, _check, ints
+from tests.test_gpu_kv4_reach import _forked, _shared, attention
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("q,R,Hq,Hkv", [(1, 6, 4, 2), (1, 40, 8, 1), (5, 6, 4, 2), (90, 6, 6, 2)])
+@pytest.mark.parametrize("D,g", [(128, -1), (64, 32)])
+def test_lengths_that_end_inside_the_prefix(q, R, Hq, Hkv, D, g):
+    """Requests whose kv_lens end within what their contexts say that they share (one that has finished, whose
+    context is out of date, has none at all): a row sees the tokens up to kv_lens, as without the prefix."""
+    T, pages = 16, 20
+    p, cu_groups = _forked([(pages, R)], [q + i for i in range(R)], [q] * R, Hq, Hkv, D, g, T, torch.float16, seed=q + D)
+    ctx = p[3] - q
+    p[3][[0, 2, 3, 4, 5]] = 0, 33, pages * T - 1, pages * T, pages * T + 1
+    want = attention(p[0].double().numpy(), *p[1:5], D, p[5], T, ctx=ctx)
+    assert np.isneginf(want[1][:q]).all() and np.isfinite(want[1][q:]).all()
+    s, (out, lse) = _shared(p, cu_groups, g, T, one=q == 1, ctx=ctx, max_kv=pages * T + 200)
+    assert s.lens.tolist() == [pages * T]
+    _check(out, lse, want, torch.float16, f"{q} tokens")
+    plain = marlin.kv4_attention(p[0].to(DEV), torch.from_numpy(p[1]).to(DEV), ints(p[2]), ints(p[3]), ints(p[4]), groupsize=g,
+                                 max_q=q, max_kv=pages * T + 200, context_lens=ints(ctx), return_lse=True)
+    _check(*plain, want, torch.float16, f"{q} tokens, without the prefix")
