@@ -381,7 +381,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   // M as in kv4_split.h; the scores, in units of `down`, are taken less `base`, which is M, or
   // 0 before there is one
   float M = kNone, base = 0.f, L = 0.f;
-  bool some_none = true;  // some row of the wave that has tokens here has no M
+  bool some_none = true;  // some row of the wave that has tokens here has no M, or is bare
+  bool bare = false;      // the row has seen no v but zeros
 #pragma unroll
   for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -517,11 +518,15 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       const Pair pe = across32(e);
       e = fmaxf(pe.a, pe.b);
       const bool none = M == kNone, any = xm > -__builtin_inff();
-      // (2^24: below the least v; where all v so far are zero the next may be any)
       // (WINDOW: few sinks, the first tile, say little of what is to come)
       const float top = FORM == WINDOW && tok0 < a.sinks ? kVTop - 6.f : kVTop;
-      const float rel = fmaxf(e - top, none ? -(top + 24.f) : -kMostShift);
-      const bool rises = any && (none || __builtin_fmaf(xm, down, rel) > 0.f);
+      // While all v of a row are zero its sums are, and its reference says nothing: the first v bring their own,
+      // which may be lower (the largest p, 2^kNoV so far, stays below 2^kMostShift).
+      const bool has_v = e > -__builtin_inff(), brings = bare && has_v;
+      float rel = fmaxf(e - top, (none || bare) && !has_v ? -kNoV : -kMostShift);
+      if (brings) rel = fmaxf(rel, __builtin_fmaf(-xm, down, kNoV - kMostShift));
+      const bool rises = any && (none || brings || __builtin_fmaf(xm, down, rel) > 0.f);
+      bare = (bare || (none && any)) && !has_v;
       const float new_base = rises ? base + __builtin_fmaf(rel, up, xm) : base;
       float less = new_base - base;
       // (scores so large that base's rounding moves it by more than the slack: p = 1 for the largest)
@@ -530,7 +535,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       base = coarse ? base + xm : new_base;
       const float f = none ? 0.f : __builtin_amdgcn_exp2f(-less * down);
       M = none && !any ? kNone : base * down;
-      some_none = __any(M == kNone && seen > token_of(t0));
+      some_none = __any((M == kNone && seen > token_of(t0)) || bare);
       L *= f;
 #pragma unroll
       for (int i = 0; i < 16; i++) x[i] -= less;
