@@ -31,7 +31,7 @@
 // SHARED, first pass: 64 requests on 64 and 8 heads that share 8192 tokens are 512 rows a head, 16
 // blocks in 16 parts of 8 tiles: 37 us, 460 TFLOP/s, of which beginnings, the write of the parts (34 MB)
 // and 8 tiles' worth of filling take half.  WINDOW: 8000 tokens on 32 heads through 1024 and a few first
-// ones, 230 us where 126 GFLOP are seen: of a block's 21 tiles twelve are whole.
+// ones, 234 us where 126 GFLOP are seen: of a block's 21 tiles twelve are whole.
 #pragma once
 #include "kv4_split.h"
 
@@ -518,12 +518,10 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       const Pair pe = across32(e);
       e = fmaxf(pe.a, pe.b);
       const bool none = M == kNone, any = xm > -__builtin_inff();
-      // (WINDOW: few sinks, the first tile, say little of what is to come)
-      const float top = FORM == WINDOW && tok0 < a.sinks ? kVTop - 6.f : kVTop;
       // While all v of a row are zero its sums are, and its reference says nothing: the first v bring their own,
       // which may be lower (the largest p, 2^kNoV so far, stays below 2^kMostShift).
       const bool has_v = e > -__builtin_inff(), brings = bare && has_v;
-      float rel = fmaxf(e - top, (none || bare) && !has_v ? -kNoV : -kMostShift);
+      float rel = fmaxf(e - kVTop, (none || bare) && !has_v ? -kNoV : -kMostShift);
       if (brings) rel = fmaxf(rel, __builtin_fmaf(-xm, down, kNoV - kMostShift));
       const bool rises = any && (none || brings || __builtin_fmaf(xm, down, rel) > 0.f);
       bare = (bare || (none && any)) && !has_v;
