@@ -313,7 +313,7 @@ def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups:
         if cu_q.size(0) != R + 1:
             raise RuntimeError(f"cu_q has {cu_q.size(0)} entries, expected {R + 1}")
     groups = cu_groups.size(0) - 1
-    plan = block_table.new_empty(3 * groups + 1 + R)
+    plan = (block_table.new_empty if R and groups else block_table.new_zeros)(3 * groups + 1 + R)  # (nothing: not launched)
     err = _lib.load().marlin_hip_kv4_shared(table, ctx, cu, at, plan.data_ptr(), R, groups, P, page_size, dev,
                                             _raw_stream(dev))
     if err:

@@ -253,7 +253,8 @@ int marlin_hip_kv4_attention_window(const void* q, const void* cache, const void
 /* The prefixes that groups of requests share, once a step: group g is the requests [cu_groups[g],
  * cu_groups[g + 1]) (`groups` + 1 entries, not falling; cut to the requests there are), its prefix the leading
  * pages within context_lens that are the same in all its rows.  Requests without new tokens (cu_q, null: one each)
- * and those that share no page with the group's first are left out.  shared: int32 [3 groups + 1 + requests]. */
+ * and those that share no page with the group's first are left out.  shared: int32 [3 groups + 1 + requests],
+ * not written where there are no requests or no groups. */
 int marlin_hip_kv4_shared(const void* block_table, const void* context_lens, const void* cu_q, const void* cu_groups,
                           void* shared, int requests, int groups, int max_pages, int page_size, int dev,
                           hipStream_t stream);

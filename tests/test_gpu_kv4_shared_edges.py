@@ -27,3 +27,16 @@ def test_lengths_that_end_inside_the_prefix(q, R, Hq, Hkv, D, g):
     plain = marlin.kv4_attention(p[0].to(DEV), torch.from_numpy(p[1]).to(DEV), ints(p[2]), ints(p[3]), ints(p[4]), groupsize=g,
                                  max_q=q, max_kv=pages * T + 200, context_lens=ints(ctx), return_lse=True)
     _check(*plain, want, torch.float16, f"{q} tokens, without the prefix")
+
+
+@pytest.mark.parametrize("R,groups", [(0, 2), (0, 0), (3, 0)])
+@pytest.mark.parametrize("one", [True, False])
+def test_plan_of_nothing_to_share(R, groups, one):
+    """No requests, or no groups: prefixes of no tokens, whatever the memory held."""
+    n = 3 * groups + 1 + R
+    for fill in (7, -9):
+        junk = [torch.full((n,), fill, dtype=torch.int32, device=DEV) for _ in range(8)]
+        del junk
+        s = marlin.kv4_shared(ints(np.arange(2 * R).reshape(R, 2)), ints([20] * R), ints([0] * (groups + 1)), 16,
+                              None if one else ints(range(R + 1)))
+        assert s.plan.shape == (n,) and (s.plan == 0).all() and s.lens.tolist() == [0] * groups
