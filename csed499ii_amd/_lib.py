@@ -48,6 +48,7 @@ SIGNATURES = {
     "marlin_hip_kv4_attention_window": (_i, [_vp] * 8 + [_i] * 5 + [_ll] * 2 + [_i] * 6 + [_f] + [_i] * 4 + [_vp]),
     "marlin_hip_kv4_shared": (_i, [_vp] * 5 + [_i] * 5 + [_vp]),
     "marlin_hip_kv4_attention_shared": (_i, [_vp] * 10 + [_i] * 6 + [_ll] * 2 + [_i] * 6 + [_f, _i, _ll, _i, _i, _vp]),
+    "marlin_hip_kv4_shared_plan": (_i, [_i] * 12 + [ctypes.POINTER(_ll)]),
     "marlin_hip_kv4_plan": (_i, [_i] * 8 + [ctypes.POINTER(_i)]),
     "marlin_hip_kv4_free_pages": (_i, [_vp] * 5 + [_i] * 5 + [_vp]),
     "marlin_hip_kv4_copy_pages": (_i, [_vp, _i, _vp, _vp] + [_i] * 7 + [_vp]),

@@ -120,6 +120,7 @@ int check(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int
 // layers.  64 rows of 512 entries in one group take 10 us, what one compute unit reads at; 4 groups of 8 rows 4.6.
 // ---------------------------------------------------------------------------
 
+constexpr int kMaxGroups = 1 << 20;
 constexpr int kSharedThreads = 1024, kSharedRound = 1024, kSharedWaves = kSharedThreads / 64, kSharedRows = 4;
 
 struct SharedArgs {
@@ -331,13 +332,46 @@ struct Prefix {
 // requests of 4 tokens on 64 and 8 heads behind 4096, 43000 fewer, 62 where 56.  A prefix in the prompt kernel from half
 // as many more on: 64 on 64 and 8 heads behind 2000 in two groups, 25000 fewer, 46 where 33.  Prompts, which the second
 // pass takes through the same kernel, from four times as many on.)
-bool shares(const Prefix& f, int tokens, int requests, int group, int kv_heads, int max_kv, bool first_prompts, bool prompts) {
+bool shares(int groups, const Problem& p, int group, bool first_prompts, bool prompts) {
   auto blocks = [&](int n, bool big) {
-    const long long rows = ((long long)tokens + n - 1) / n * group;
+    const long long rows = ((long long)p.tokens + n - 1) / n * group;
     return n * (big ? (rows + kPromptRows - 1) / kPromptRows * 8 : (rows + 15) / 16);
   };
-  const long long fewer = blocks(requests, prompts) - blocks(f.groups, first_prompts);
-  return fewer * kv_heads * (max_kv / kStep) >= (prompts ? 81920 : first_prompts ? 32768 : 20480);
+  const long long fewer = blocks(p.requests, prompts) - blocks(groups, first_prompts);
+  return fewer * p.kv_heads * (p.max_kv / kStep) >= (prompts ? 81920 : first_prompts ? 32768 : 20480);
+}
+
+// How a call with a prefix runs, the same for the call and for the query of its workspace.
+struct SharedPlan {
+  bool two;                 // passes
+  Choice first;             // of the first one
+  bool parts;               // its divided blocks leave their parts to the second one
+  size_t parts_at, places;  // floats before the parts, rows that they hold
+  size_t least, bytes;      // of workspace: what two passes need, and what serves them best
+};
+SharedPlan plan_shared(const Problem& p, const Choice& c, int groups, bool always) {
+  SharedPlan s{};
+  const int group = p.q_heads / p.kv_heads, average = (p.tokens + groups - 1) / groups;  // tokens that a group has
+  const bool big = (long long)average * group > split_rows(groups, p.kv_heads, p.head_dim, p.ng, p.cus / 64);
+  s.two = always || shares(groups, p, group, big, c.prompts);
+  if (!s.two) return s;
+  // One kernel takes all groups, by the rows that a group has on average.
+  s.first.prompts = big;
+  s.first.split = !big;
+  s.first.few_rows = 0x7FFFFFFF;
+  s.first.split_q = average;
+  // Blocks of rows that the prompt kernel divides leave their parts where the second pass, if it runs on the
+  // split kernel alone, adds them as it writes: they would meet through memory that is not cached.
+  // (One launch of the first pass: a second would write over its parts.  And one block a workgroup of the
+  // second: 128 requests on 32 heads of 8192 shared tokens, 47 and 106 us so, 52 and 84 joined.)
+  const size_t rows = (size_t)p.tokens * p.q_heads;
+  s.places = ((size_t)p.cus / p.kv_heads) * p.kv_heads * kPromptRows;
+  s.parts_at = (rows * (p.head_dim + 4) + 3) & ~(size_t)3;
+  const long long blocks = (long long)p.requests * ((c.split_q * group + 15) / 16) * p.kv_heads;
+  s.parts = big && !c.prompts && blocks <= 2 * p.cus && groups <= kMaxRequests && s.places <= 0x7FFFFFFF;
+  s.least = rows * (p.head_dim + 2) * sizeof(float);
+  s.bytes = s.parts ? (s.parts_at + s.places * (p.head_dim + 2)) * sizeof(float) : s.least;
+  return s;
 }
 
 int attention(const void* q, const void* cache, const void* block_table, const void* kv_lens, const void* cu_q,
@@ -388,17 +422,14 @@ int attention(const void* q, const void* cache, const void* block_table, const v
   const Choice c = choose(tokens, requests, q_heads, kv_heads, head_dim, ng, max_q, cu_q != nullptr, p.cus);
   if (window > 0) return attend<WINDOW>(a, p, c);
   if (prefix == nullptr) return attend<PLAIN>(a, p, c);
-  const int average = (tokens + prefix->groups - 1) / prefix->groups;  // tokens that a group has
-  const bool big = (long long)average * group > split_rows(prefix->groups, kv_heads, head_dim, ng, p.cus / 64);
-  if (!prefix->always && !shares(*prefix, tokens, requests, group, kv_heads, max_kv, big, c.prompts))
-    return attend<PLAIN>(a, p, c);
+  const SharedPlan s = plan_shared(p, c, prefix->groups, prefix->always);
+  if (!s.two) return attend<PLAIN>(a, p, c);
   const size_t rows = (size_t)tokens * q_heads;
-  if (prefix->bytes < (long long)(rows * (head_dim + 2) * sizeof(float)))
+  if (prefix->bytes < (long long)s.least)
     return refuse("kv4_attention of a shared prefix needs a workspace of head_dim + 2 floats a row");
   a.before = prefix->workspace;
   a.before_ml = a.before + rows * head_dim;
   // First pass: a group is a request whose tokens are the prefix and whose rows, behind it, see all of them.
-  // One kernel takes all groups, by the rows that a group has on average.
   AttnArgs b = a;
   b.kv_lens = b.ctx = prefix->lens;
   b.leads = prefix->leads;
@@ -407,26 +438,13 @@ int attention(const void* q, const void* cache, const void* block_table, const v
   Problem first = p;
   first.requests = prefix->groups;
   first.max_q = tokens;
-  Choice one{};
-  one.prompts = big;
-  one.split = !one.prompts;
-  one.few_rows = 0x7FFFFFFF;
-  one.split_q = average;
-  // Blocks of rows that the prompt kernel divides leave their parts where the second pass, if it runs on the
-  // split kernel alone, adds them as it writes: they would meet through memory that is not cached.
-  // (One launch of the first pass: a second would write over its parts.  And one block a workgroup of the
-  // second: 128 requests on 32 heads of 8192 shared tokens, 47 and 106 us so, 52 and 84 joined.)
-  const size_t place = ((size_t)p.cus / kv_heads) * kv_heads * kPromptRows;
-  const size_t parts_at = (rows * (head_dim + 4) + 3) & ~(size_t)3;
-  const long long blocks = (long long)requests * ((c.split_q * group + 15) / 16) * kv_heads;
-  if (one.prompts && !c.prompts && blocks <= 2 * p.cus && prefix->groups <= kMaxRequests && place <= 0x7FFFFFFF &&
-      prefix->bytes >= (long long)((parts_at + place * (head_dim + 2)) * sizeof(float))) {
+  if (s.parts && prefix->bytes >= (long long)s.bytes) {
     a.where = b.where = reinterpret_cast<int2*>(a.before_ml + 2 * rows);
-    a.parts = b.parts = prefix->workspace + parts_at;
-    a.parts_ml = b.parts_ml = a.parts + place * head_dim;
-    a.places = b.places = (int)place;
+    a.parts = b.parts = prefix->workspace + s.parts_at;
+    a.parts_ml = b.parts_ml = a.parts + s.places * head_dim;
+    a.places = b.places = (int)s.places;
   }
-  err = attend<SHARED>(b, first, one);
+  err = attend<SHARED>(b, first, s.first);
   if (err != MARLIN_HIP_OK) return err;
   a.start = prefix->start;
   return attend<SHARED>(a, p, c);
@@ -435,6 +453,25 @@ int attention(const void* q, const void* cache, const void* block_table, const v
 }  // namespace kv4
 
 extern "C" {
+
+int marlin_hip_kv4_shared_plan(int tokens, int requests, int groups, int q_heads, int kv_heads, int head_dim,
+                               int groupsize, int max_q, int max_kv, int cu_q, int always, int dev, long long* out) {
+  using namespace kv4;
+  if (tokens >= 0 && max_q > tokens) max_q = tokens;
+  const int err = check(tokens, requests, q_heads, kv_heads, head_dim, 16, 1, 0, groupsize, max_q, max_kv, 1.f, 0);
+  if (err != MARLIN_HIP_OK) return err;
+  if (groups < 0 || groups > kMaxGroups) return refuse("kv4_attention takes prefixes of 2^20 groups at most");
+  out[0] = out[1] = out[2] = 0;
+  if (tokens == 0 || requests == 0 || max_q == 0 || groups == 0) return MARLIN_HIP_OK;
+  const Problem p{tokens, requests, q_heads, kv_heads, head_dim, kv4::groups(head_dim, groupsize), max_q, max_kv, 0, dev,
+                  dev < 0 ? 256 : compute_units(dev), nullptr};
+  const SharedPlan s = plan_shared(p, choose(tokens, requests, q_heads, kv_heads, head_dim, p.ng, max_q, cu_q != 0, p.cus),
+                                   groups, always != 0);
+  out[0] = (long long)s.bytes;
+  out[1] = s.first.prompts;
+  out[2] = s.parts;
+  return MARLIN_HIP_OK;
+}
 
 int marlin_hip_kv4_attention_ctx(const void* q, const void* cache, const void* block_table, const void* kv_lens,
                                  const void* cu_q, const void* context_lens, void* out, void* lse, int tokens,
@@ -467,7 +504,7 @@ int marlin_hip_kv4_attention_shared(const void* q, const void* cache, const void
                                     int head_dim, long long q_token_stride, long long q_head_stride, int page_size,
                                     int num_pages, int max_pages, int groupsize, int max_q, int max_kv, float scale,
                                     int dtype, long long workspace_bytes, int always, int dev, hipStream_t stream) {
-  if (groups < 0) return kv4::refuse("kv4_attention takes no negative sizes");
+  if (groups < 0 || groups > kv4::kMaxGroups) return kv4::refuse("kv4_attention takes prefixes of 2^20 groups at most");
   const int32_t* at = static_cast<const int32_t*>(shared);
   const kv4::Prefix prefix{at, at + groups, at + 2 * (size_t)groups, at + 3 * (size_t)groups + 1, groups,
                            static_cast<float*>(workspace), workspace_bytes, always != 0};
@@ -492,7 +529,7 @@ int marlin_hip_kv4_shared(const void* block_table, const void* context_lens, con
   if (requests < 0 || groups < 0 || max_pages < 0) return kv4::refuse("kv4_shared takes no negative sizes");
   if (!kv4::page_ok(page_size)) return kv4::refuse("the KV cache's page_size must be 16, 32, 64, 128 or 256");
   if ((long long)max_pages * page_size > (1ll << 30)) return kv4::refuse("a block table row covers more than 2^30 tokens");
-  if (groups > (1 << 20)) return kv4::refuse("kv4_shared takes at most 2^20 groups");
+  if (groups > kv4::kMaxGroups) return kv4::refuse("kv4_shared takes at most 2^20 groups");
   if (requests == 0 || groups == 0) return MARLIN_HIP_OK;
   sm24::DeviceScope scope(dev);
   if (!scope.ok) return MARLIN_HIP_ERR_LAUNCH;

@@ -321,6 +321,17 @@ def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups:
     return kv4_prefix(plan, R, groups, P, page_size, cu_q is None, always)
 
 
+@functools.lru_cache(maxsize=4096)
+def _shared_bytes(tokens, requests, groups, q_heads, kv_heads, head_dim, groupsize, max_q, max_kv, cu_q, always, dev) -> int:
+    """Workspace of an attention call with a prefix (0: the sizes send it through one pass).  A step asks for all layers."""
+    out = (ctypes.c_longlong * 3)()
+    err = _lib.load().marlin_hip_kv4_shared_plan(tokens, requests, groups, q_heads, kv_heads, head_dim, groupsize, max_q,
+                                                 max_kv, cu_q, always, dev, out)
+    if err:
+        _raise(err)
+    return out[0]
+
+
 def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tensor, kv_lens: torch.Tensor,
                   cu_q: torch.Tensor | None = None, max_q: int | None = None, max_kv: int | None = None,
                   groupsize: int = -1, scale: float | None = None, return_lse: bool = False,
@@ -429,14 +440,11 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
             raise RuntimeError(f"shared is of {shared.requests} requests with {shared.pages} pages of {shared.page_size} "
                                f"tokens, {'without' if shared.one else 'with'} cu_q, and needs context_lens; the call has "
                                f"{R}, {P} and {page}")
-        # (beside the rows of the first pass its parts, where it has more than a few rows a group: 256 of each compute unit)
-        size = N * Hq * (D + 4) + 4
-        if N * Hq > 64 * H * shared.groups:
-            size += 65536 * (D + 2)
-        work = torch.empty(size, dtype=torch.float32, device=q.device)
+        size = _shared_bytes(N, R, shared.groups, Hq, H, D, groupsize, min(max_q, N), max_kv, cu != 0, shared.always, dev)
+        work = torch.empty(size // 4, dtype=torch.float32, device=q.device) if size else None
         err = _lib.load().marlin_hip_kv4_attention_shared(
-            qp, cp, table, lens, cu, ctx, shared.plan.data_ptr(), op, lp, work.data_ptr(), N, R, shared.groups, Hq, H, D, qt,
-            qh, page, pages, P, groupsize, min(max_q, N), max_kv, scale, dtype, 4 * size, shared.always, dev,
+            qp, cp, table, lens, cu, ctx, shared.plan.data_ptr(), op, lp, work.data_ptr() if size else 0, N, R, shared.groups,
+            Hq, H, D, qt, qh, page, pages, P, groupsize, min(max_q, N), max_kv, scale, dtype, size, shared.always, dev,
             _raw_stream(dev))
     elif window is not None:
         if window < 1 or sinks < 0:

@@ -261,16 +261,24 @@ int marlin_hip_kv4_shared(const void* block_table, const void* context_lens, con
 
 /* marlin_hip_kv4_attention_ctx with the prefixes of `shared` attended to once for all rows of a group, in a pass
  * before that over each request's other tokens.  shared: from marlin_hip_kv4_shared with the same block_table,
- * context_lens and cu_q; context_lens must be given.  workspace: 16-byte aligned, workspace_bytes at least
- * 4 (head_dim + 2) for each row of q; with 4 (head_dim + 4) + 16 and 1024 (head_dim + 2) for each compute unit
- * the parts of a divided prefix meet as the rows are written, which is faster.  always 0: in one pass, as
- * marlin_hip_kv4_attention_ctx, where the sizes (max_kv for the prefix) say that two do not pay. */
+ * context_lens and cu_q; context_lens must be given.  workspace: 16-byte aligned, workspace_bytes as
+ * marlin_hip_kv4_shared_plan says, or at least 4 (head_dim + 2) for each row of q where it takes two passes: the
+ * parts of a divided prefix then meet in the first one, which is slower.  always 0: in one pass, as
+ * marlin_hip_kv4_attention_ctx, where the sizes (max_kv for the prefix, which may be far less) say that two do
+ * not pay. */
 int marlin_hip_kv4_attention_shared(const void* q, const void* cache, const void* block_table, const void* kv_lens,
                                     const void* cu_q, const void* context_lens, const void* shared, void* out, void* lse,
                                     void* workspace, int tokens, int requests, int groups, int q_heads, int kv_heads,
                                     int head_dim, long long q_token_stride, long long q_head_stride, int page_size,
                                     int num_pages, int max_pages, int groupsize, int max_q, int max_kv, float scale,
                                     int dtype, long long workspace_bytes, int always, int dev, hipStream_t stream);
+
+/* How marlin_hip_kv4_attention_shared runs a call of these sizes on device dev (below zero: with 256 compute units),
+ * computed on the host: out[0] the bytes of workspace that serve it best, 0 where it takes one pass; of two passes
+ * out[1] the kernel of the first (0: of few rows, 1: of prompts) and out[2] whether the parts of its divided blocks
+ * are left to the second.  cu_q: whether the call gives it. */
+int marlin_hip_kv4_shared_plan(int tokens, int requests, int groups, int q_heads, int kv_heads, int head_dim,
+                               int groupsize, int max_q, int max_kv, int cu_q, int always, int dev, long long* out);
 
 /* The launch plan of a marlin_hip_kv4_attention call, computed on the host without a GPU (sms
  * <= 0: 256 compute units), for `requests` requests of max_q new tokens each (cu_q null where

@@ -40,3 +40,22 @@ def test_plan_of_nothing_to_share(R, groups, one):
         s = marlin.kv4_shared(ints(np.arange(2 * R).reshape(R, 2)), ints([20] * R), ints([0] * (groups + 1)), 16,
                               None if one else ints(range(R + 1)))
         assert s.plan.shape == (n,) and (s.plan == 0).all() and s.lens.tolist() == [0] * groups
+
+
+@pytest.mark.parametrize("cu_groups", [[0, 16], [0]])
+@pytest.mark.parametrize("n", [1, 40])
+def test_one_pass_takes_no_workspace(n, cu_groups):
+    """A call that the sizes send through one pass allocates nothing (out is given)."""
+    D, T, R, Hq, H = 128, 16, 16, 64, 8
+    p, _ = _forked([(2, R)], [n + 3] * R, [n] * R, Hq, H, D, -1, T, torch.float16, seed=n)
+    q, cache, table, kv, cu = p[0].to(DEV), torch.from_numpy(p[1]).to(DEV), ints(p[2]), ints(p[3]), ints(p[4])
+    ctx, out = kv - n, torch.empty((R * n, Hq, D), dtype=torch.float16, device=DEV)
+    kw = dict(max_q=n, max_kv=int(p[3].max()), context_lens=ctx)
+    s = marlin.kv4_shared(table, ctx, ints(cu_groups), T, cu)
+    plain = marlin.kv4_attention(q, cache, table, kv, cu, **kw)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    marlin.kv4_attention(q, cache, table, kv, cu, shared=s, out=out, **kw)
+    assert torch.cuda.max_memory_allocated() == before
+    assert torch.equal(out, plain)
