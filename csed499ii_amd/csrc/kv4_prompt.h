@@ -31,7 +31,7 @@
 // SHARED, first pass: 64 requests on 64 and 8 heads that share 8192 tokens are 512 rows a head, 16
 // blocks in 16 parts of 8 tiles: 37 us, 460 TFLOP/s, of which beginnings, the write of the parts (34 MB)
 // and 8 tiles' worth of filling take half.  WINDOW: 8000 tokens on 32 heads through 1024 and a few first
-// ones, 234 us where 126 GFLOP are seen: of a block's 21 tiles twelve are whole.
+// ones, 231 us where 126 GFLOP are seen: of a block's 21 tiles twelve are whole.
 #pragma once
 #include "kv4_split.h"
 
@@ -381,8 +381,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
   // M as in kv4_split.h; the scores, in units of `down`, are taken less `base`, which is M, or
   // 0 before there is one
   float M = kNone, base = 0.f, L = 0.f;
-  bool some_none = true;  // some row of the wave that has tokens here has no M, or is bare
-  bool bare = false;      // the row has seen no v but zeros
+  bool some_none = true;  // some row of the wave that has tokens here has no M
 #pragma unroll
   for (int t = 0; t < DT; t++)
 #pragma unroll
@@ -518,13 +517,8 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       const Pair pe = across32(e);
       e = fmaxf(pe.a, pe.b);
       const bool none = M == kNone, any = xm > -__builtin_inff();
-      // While all v of a row are zero its sums are, and its reference says nothing: the first v bring their own,
-      // which may be lower (the largest p, 2^kNoV so far, stays below 2^kMostShift).
-      const bool has_v = e > -__builtin_inff(), brings = bare && has_v;
-      float rel = fmaxf(e - kVTop, (none || bare) && !has_v ? -kNoV : -kMostShift);
-      if (brings) rel = fmaxf(rel, __builtin_fmaf(-xm, down, kNoV - kMostShift));
-      const bool rises = any && (none || brings || __builtin_fmaf(xm, down, rel) > 0.f);
-      bare = (bare || (none && any)) && !has_v;
+      const float rel = fmaxf(e - kVTop, none && !(e > -__builtin_inff()) ? -kNoV : -kMostShift);
+      const bool rises = any && (none || __builtin_fmaf(xm, down, rel) > 0.f);
       const float new_base = rises ? base + __builtin_fmaf(rel, up, xm) : base;
       float less = new_base - base;
       // (scores so large that base's rounding moves it by more than the slack: p = 1 for the largest)
@@ -533,7 +527,7 @@ __global__ __launch_bounds__(64 * kPromptWaves, 2) void kv4_prompt_kernel(AttnAr
       base = coarse ? base + xm : new_base;
       const float f = none ? 0.f : __builtin_amdgcn_exp2f(-less * down);
       M = none && !any ? kNone : base * down;
-      some_none = __any((M == kNone && seen > token_of(t0)) || bare);
+      some_none = __any(M == kNone && seen > token_of(t0));
       L *= f;
 #pragma unroll
       for (int i = 0; i < 16; i++) x[i] -= less;

@@ -29,10 +29,10 @@
 // M is not the running maximum but a reference that is only changed, by a wave-uniform branch,
 // when a row's p v, which is rounded to fp16 for the matrix cores, would pass 2^15 (or its sum
 // of p 2^100): rare after the first step.  The branch brings the row's largest p v so far to 2^7,
-// however large the v of tokens of little weight (a row whose v so far are all zero has none, and
-// takes the branch until it has).  So p v has fp16's 11 bits where it is not
-// below 2^-14, and is off by 2^-25 at most there: an output by 2^-11 sum_j w_j |v_j| (w: the
-// softmax) and 2^-32 a token of the largest w_j s_j of the row, all its scale groups alike, which
+// however large the v of tokens of little weight, and p to 2^90 at most (2^80 while all v are
+// zero).  So p v has fp16's 11 bits where it is not below 2^-14, and is off by 2^-25 at most
+// there: an output by 2^-11 sum_j w_j |v_j| (w: the softmax) and 2^-32 a token of the largest
+// w_j s_j of the row (s_j: its v's scale), all its scale groups alike, which
 // share M.  With the largest v in M's place, however small its weight, values 2^21 below it lost
 // bits, and all of them 2^31 below.  Sums are fp32.
 //
@@ -86,7 +86,7 @@ constexpr float kMostPV = 1 << 15; // ... which later ones may pass by 2^8 (6550
 constexpr float kSlack = 8.f;      // of a reference that is rounded, in log2 units
 constexpr float kMostL = 0x1p100f; // of a row's sum of p, before it gets a new reference
 constexpr float kMostShift = 90.f; // p <= 2^90 at a new reference, however small its v
-constexpr float kNoV = kVTop + 24.f;  // the largest p, 2^31, while all v so far are zero: the next may be any
+constexpr float kNoV = 80.f;       // ... 2^80 where the row's v are all zero (2^20 such p make 2^100)
 constexpr float kBig = 1 << 20;    // of a row's largest score, in log2 units
 constexpr float kNone = -1.0e30f;  // reference of a row that has seen nothing
 
@@ -567,7 +567,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
     // ---- the loop ----
     float4_t O[NG][S::OPS];
     bool big = false, some_big = false;  // the row, some row
-    bool fresh = true;                   // (wave-uniform) no step yet, or a row has seen no v but zeros
+    bool fresh = true;                   // (wave-uniform) no step yet
     float M = kNone, L = 0.f, shift = 0.f, x_top = 0.f;  // M = x_top c1 - shift, x_top a score
 #pragma unroll
     for (int n = 0; n < NG; n++)
@@ -735,16 +735,13 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
                            __builtin_amdgcn_logf((float)vt[i / 4][i % 4]));
         }
         e = column_max(e);
-        // (where all v so far are zero the sums are, and the shift says nothing: `fresh` below)
-        const float e_old = none || shift == kNoV ? e : kVTop - shift + drop;
-        const float e_all = fmaxf(e, e_old);
+        const float e_all = none ? e : fmaxf(e, kVTop - shift + drop);
         const float new_shift = e_all > -__builtin_inff() ? fminf(kVTop - e_all, kMostShift) : kNoV;
         const float new_M = new_max <= kNone ? kNone : new_max - new_shift;
         const float f = none ? 0.f : __builtin_amdgcn_exp2f(big ? drop + (new_shift - shift) : M - new_M);
         M = new_M;
         shift = new_shift;
         some_big = __any(big);
-        fresh = __any(M != kNone && shift == kNoV);
         L *= f;
 #pragma unroll
         for (int n = 0; n < NG; n++)
@@ -784,6 +781,7 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
       // (a row without a reference has p = 2^(10^30) of what it sees)
       if (fresh || __any(!(L + sum < kMostL) || most > kMostPV)) {
         refer();
+        fresh = false;
         weigh();
       }
       L += sum;
