@@ -25,6 +25,11 @@ int split_rows(int requests, int kv_heads, int head_dim, int ng, int few) {
   return head_dim == 128 && ng == 4 ? 144 : 80;
 }
 
+// Compute units that launches are planned for: the stream's arrival counters, one a workgroup of the split kernel
+// (two of which fill a unit) and one a wave of a part of the prompt kernel (one of which does), are enough for so many.
+constexpr int kMostUnits = (int)(sm24::kCounterBytes / sizeof(uint32_t)) / kPromptWaves;
+static_assert(kPromptWaves >= 2, "");
+
 // (the query takes the host 0.2 us of each call, so its answer is kept)
 int compute_units(int dev) {
   static std::atomic<int> known[64];
@@ -32,6 +37,7 @@ int compute_units(int dev) {
     return known[dev].load(std::memory_order_relaxed);
   int n = 0;
   if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) return 256;
+  if (n > kMostUnits) n = kMostUnits;
   if (dev >= 0 && dev < 64) known[dev].store(n, std::memory_order_relaxed);
   return n;
 }
@@ -292,7 +298,7 @@ int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, i
   out[0] = out[1] = out[2] = 0;
   if (requests == 0 || max_q == 0) return MARLIN_HIP_OK;
   using namespace kv4;
-  const int cus = sms > 0 ? sms : 256, ng = groups(head_dim, groupsize), most = (1 << 30) / (q_heads / kv_heads);
+  const int cus = sms <= 0 ? 256 : sms < kMostUnits ? sms : kMostUnits, ng = groups(head_dim, groupsize), most = (1 << 30) / (q_heads / kv_heads);
   const int tokens = (long long)requests * max_q < most ? requests * max_q : most;
   const Choice c = choose(tokens, requests, q_heads, kv_heads, head_dim, ng, max_q, max_q > 1, cus);
   if (requests > kMaxRequests) requests = kMaxRequests;  // (of the first launch)

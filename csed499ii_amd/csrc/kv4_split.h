@@ -100,7 +100,7 @@ struct AttnArgs {
   float* lse;           // null: not wanted
   float* partial;       // [workgroup][first, last][row][D] (prompt kernel: [part][wave][..]); null: no tile is divided
   float* partial_ml;    // as many pairs of a reference and a sum
-  uint32_t* counters;   // [workgroup] (prompt kernel: [block of rows][wave]), zero between launches
+  uint32_t* counters;   // [workgroup] (prompt kernel: [part][wave]), zero between launches
   long long qt, qh;     // strides of q in elements
   int tokens, requests, q_heads, kv_heads;
   uint32_t page_stride; // bytes of a page, all heads
