@@ -533,6 +533,7 @@ int marlin_hip_kv4_shared(const void* block_table, const void* context_lens, con
                           void* shared, int requests, int groups, int max_pages, int page_size, int dev,
                           hipStream_t stream) {
   if (requests < 0 || groups < 0 || max_pages < 0) return kv4::refuse("kv4_shared takes no negative sizes");
+  if (requests > (1 << 30)) return kv4::refuse("kv4_shared takes at most 2^30 requests");  // (as of pages)
   if (!kv4::page_ok(page_size)) return kv4::refuse("the KV cache's page_size must be 16, 32, 64, 128 or 256");
   if ((long long)max_pages * page_size > (1ll << 30)) return kv4::refuse("a block table row covers more than 2^30 tokens");
   if (groups > kv4::kMaxGroups) return kv4::refuse("kv4_shared takes at most 2^20 groups");

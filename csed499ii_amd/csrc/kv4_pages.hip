@@ -481,6 +481,8 @@ void each_layers(const void* const* caches, int count, F&& f) {
 
 int check_tables(int requests, int max_pages, int page_size, int num_pages) {
   if (requests < 0 || max_pages < 0) return refuse("the KV cache's pages take no negative sizes");
+  // (the kernels go through them in steps that must not pass 31 bits)
+  if (requests > (1 << 30)) return refuse("the KV cache's pages take tables of at most 2^30 requests");
   if (!page_ok(page_size)) return refuse("the KV cache's page_size must be 16, 32, 64, 128 or 256");
   if (num_pages < 1 || (long long)num_pages * page_size > 0x7FFFFFFFll)
     return refuse("the KV cache holds a page at least and 2^31 - 1 tokens at most");

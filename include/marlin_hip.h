@@ -254,7 +254,7 @@ int marlin_hip_kv4_attention_window(const void* q, const void* cache, const void
  * cu_groups[g + 1]) (`groups` + 1 entries, not falling; cut to the requests there are), its prefix the leading
  * pages within context_lens that are the same in all its rows.  Requests without new tokens (cu_q, null: one each)
  * and those that share no page with the group's first are left out.  shared: int32 [3 groups + 1 + requests],
- * not written where there are no requests or no groups. */
+ * not written where there are no requests or no groups (at most 2^30 and 2^20). */
 int marlin_hip_kv4_shared(const void* block_table, const void* context_lens, const void* cu_q, const void* cu_groups,
                           void* shared, int requests, int groups, int max_pages, int page_size, int dev,
                           hipStream_t stream);
@@ -292,8 +292,8 @@ int marlin_hip_kv4_plan(int requests, int q_heads, int kv_heads, int head_dim, i
 /* ---- Pages of the 4-bit KV cache (no counterpart in the reference) ----
  *
  * A page is held if an entry of a written token names it: block_table[i][j] [requests][max_pages] with
- * j * page_size < kv_lens[i].  `caches` is a host array of the layers' caches, which have one
- * geometry and num_pages pages; it is read before the call returns. */
+ * j * page_size < kv_lens[i]; tables have at most 2^30 requests.  `caches` is a host array of the layers' caches, which
+ * have one geometry and num_pages pages and no memory in common; it is read before the call returns. */
 
 /* free_pages[num_pages]: the pages that are not held, in ascending order, then -1; count[1]: how many.
  * workspace: num_pages bytes rounded up to 16, 16-byte aligned. */
