@@ -46,6 +46,9 @@ class kv4_layers:
         at = [c.data_ptr() for c in self.caches]
         if len(set(at)) != len(at):
             raise RuntimeError("kv4_layers got one cache twice")
+        order = sorted(at)
+        if any(b - a < self.caches[0].numel() for a, b in zip(order, order[1:])):
+            raise RuntimeError("the caches of layers must not overlap one another")
         self.num_pages, self.kv_heads = shape[0], shape[1]
         self.head_dim, self.groupsize, self.count = head_dim, groupsize, len(at)
         self._at = (ctypes.c_void_p * len(at))(*at)

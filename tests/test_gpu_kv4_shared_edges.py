@@ -59,3 +59,12 @@ def test_one_pass_takes_no_workspace(n, cu_groups):
     marlin.kv4_attention(q, cache, table, kv, cu, shared=s, out=out, **kw)
     assert torch.cuda.max_memory_allocated() == before
     assert torch.equal(out, plain)
+
+
+def test_layers_that_overlap_are_refused():
+    """Caches of two layers that have memory in common: pages of one would be written over by those of the other."""
+    pool = marlin.kv4_cache(9, 2, 128, device=DEV)
+    for caches in ((pool[:4], pool[3:7]), (pool[4:8], pool[:4], pool[5:]), (pool, pool)):
+        with pytest.raises(RuntimeError, match="overlap|twice"):
+            marlin.kv4_layers(caches, 128)
+    assert len(marlin.kv4_layers((pool[4:8], pool[:4]), 128)) == 2
