@@ -267,6 +267,7 @@ class kv4_prefix(typing.NamedTuple):
     page_size: int
     one: bool  # made without cu_q: a token each
     always: bool = False  # two passes, whatever the sizes
+    most: int | None = None  # a bound on the prefixes' tokens (None: the attention's max_kv)
 
     @property
     def lens(self) -> torch.Tensor:
@@ -275,7 +276,7 @@ class kv4_prefix(typing.NamedTuple):
 
 
 def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups: torch.Tensor, page_size: int,
-               cu_q: torch.Tensor | None = None, always: bool = False) -> kv4_prefix:
+               cu_q: torch.Tensor | None = None, always: bool = False, max_prefix: int | None = None) -> kv4_prefix:
     """The prefixes that groups of requests share (after :func:`kv4_fork`, say), found in the block table
     once a step for the :func:`kv4_attention` of all layers.
 
@@ -285,9 +286,11 @@ def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups:
     page with the group's first one are left out, and attend to all of their tokens by themselves.  So
     whatever the groups are, the attention is right; they decide what is read once.
 
-    The attention then takes two passes, where the sizes say that they pay: by the blocks of rows, with ``max_kv``
-    for the prefix, whose reads fall away (32 samples of 4096 shared tokens on 32 heads 47 us where 98; but 8 samples
-    of 8192 on 64 and 8 heads, whose blocks of 16 rows fall from eight to four a head, 37 to 41 where 30, so one pass).
+    The attention then takes two passes, where the sizes say that they pay: by the blocks of rows and, for the tokens
+    that are shared, ``max_prefix`` (a bound known on the host; default: the call's ``max_kv``), whose reads fall away
+    (32 samples of 4096 shared tokens on 32 heads 47 us where 98; but 8 samples of 8192 on 64 and 8 heads, whose blocks
+    of 16 rows fall from eight to four a head, 37 to 41 where 30, so one pass).  The lengths themselves are on the GPU:
+    with a bound far above them two passes are taken where one would do, and cost 8 to 23 us more.
     ``always`` makes it two whatever the sizes."""
     try:  # (as in kv4_append)
         R, P = block_table.shape
@@ -312,13 +315,15 @@ def kv4_shared(block_table: torch.Tensor, context_lens: torch.Tensor, cu_groups:
         cu = _ints("cu_q", cu_q, dev)
         if cu_q.size(0) != R + 1:
             raise RuntimeError(f"cu_q has {cu_q.size(0)} entries, expected {R + 1}")
+    if max_prefix is not None and max_prefix < 0:
+        raise RuntimeError(f"max_prefix must not be negative, got {max_prefix}")
     groups = cu_groups.size(0) - 1
     plan = (block_table.new_empty if R and groups else block_table.new_zeros)(3 * groups + 1 + R)  # (nothing: not launched)
     err = _lib.load().marlin_hip_kv4_shared(table, ctx, cu, at, plan.data_ptr(), R, groups, P, page_size, dev,
                                             _raw_stream(dev))
     if err:
         _raise(err)
-    return kv4_prefix(plan, R, groups, P, page_size, cu_q is None, always)
+    return kv4_prefix(plan, R, groups, P, page_size, cu_q is None, always, max_prefix)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -351,8 +356,8 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
 
     ``max_q`` is the most new tokens of a request (a longer one's later tokens are not
     computed; default: 1 without ``cu_q``, else all tokens) and ``max_kv`` a bound on
-    ``kv_lens`` that the split of long caches is planned for (any value is correct; default:
-    the table's ``P`` pages).  ``scale`` (positive; default ``1 / sqrt(D)``) multiplies the
+    ``kv_lens`` that the split of long caches, and with ``shared`` one pass or two, is planned for
+    (any value is correct; default: the table's ``P`` pages).  ``scale`` (positive; default ``1 / sqrt(D)``) multiplies the
     scores.  Returns ``out [tokens, q_heads, D]`` in ``q``'s type, and with ``return_lse`` the
     rows' log-sum-exp, fp32 ``[tokens, q_heads]``.
 
@@ -430,6 +435,7 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
     op, lp = out.data_ptr(), 0 if lse is None else lse.data_ptr()
     if scale is None:
         scale = 1.0 / math.sqrt(D)
+    size = 0  # of the workspace for two passes
     if shared is not None:
         if window is not None or sinks:
             raise RuntimeError("kv4_attention takes shared or window and sinks, not both")
@@ -440,12 +446,13 @@ def kv4_attention(q: torch.Tensor, cache: torch.Tensor, block_table: torch.Tenso
             raise RuntimeError(f"shared is of {shared.requests} requests with {shared.pages} pages of {shared.page_size} "
                                f"tokens, {'without' if shared.one else 'with'} cu_q, and needs context_lens; the call has "
                                f"{R}, {P} and {page}")
-        size = _shared_bytes(N, R, shared.groups, Hq, H, D, groupsize, min(max_q, N), max_kv, cu != 0, shared.always, dev)
-        work = torch.empty(size // 4, dtype=torch.float32, device=q.device) if size else None
+        size = _shared_bytes(N, R, shared.groups, Hq, H, D, groupsize, min(max_q, N),
+                             max_kv if shared.most is None else min(max_kv, shared.most), cu != 0, shared.always, dev)
+    if size:
+        work = torch.empty(size // 4, dtype=torch.float32, device=q.device)
         err = _lib.load().marlin_hip_kv4_attention_shared(
-            qp, cp, table, lens, cu, ctx, shared.plan.data_ptr(), op, lp, work.data_ptr() if size else 0, N, R, shared.groups,
-            Hq, H, D, qt, qh, page, pages, P, groupsize, min(max_q, N), max_kv, scale, dtype, size, shared.always, dev,
-            _raw_stream(dev))
+            qp, cp, table, lens, cu, ctx, shared.plan.data_ptr(), op, lp, work.data_ptr(), N, R, shared.groups, Hq, H, D, qt,
+            qh, page, pages, P, groupsize, min(max_q, N), max_kv, scale, dtype, size, 1, dev, _raw_stream(dev))
     elif window is not None:
         if window < 1 or sinks < 0:
             raise RuntimeError(f"a window holds a token at least, and sinks are not negative (window={window}, sinks={sinks})")

@@ -78,7 +78,7 @@ class Decoder:
                        for i in range(layers)]
         self.caches = marlin.kv4_layers([layer.cache for layer in self.layers], head_dim, groupsize)
         self.freqs = marlin.rotary_frequencies(head_dim, device=device)
-        self.groups = None  # of requests that share a prompt
+        self.groups, self.prompt = None, 0  # of requests that share a prompt, and the longest one's tokens
 
     def free(self):
         return marlin.kv4_free_pages(self.table, self.kv_lens, self.pages, self.page)[0]
@@ -88,6 +88,7 @@ class Decoder:
         parents = torch.arange(len(self.lens), dtype=torch.int32).repeat_interleave(samples).to(self.device)
         self.table, self.kv_lens, _ = marlin.kv4_fork(self.caches, self.table, self.kv_lens, parents, self.free())
         self.groups = torch.arange(0, len(parents) + 1, samples, dtype=torch.int32).to(self.device)
+        self.prompt = max(self.lens)
         self.lens = [n for n in self.lens for _ in range(samples)]
 
     def step(self, x, new):
@@ -104,7 +105,7 @@ class Decoder:
         if self.window:
             reach = {"window": self.window, "sinks": self.sinks}
         elif self.groups is not None:
-            reach = {"shared": marlin.kv4_shared(self.table, context_lens, self.groups, self.page, one)}
+            reach = {"shared": marlin.kv4_shared(self.table, context_lens, self.groups, self.page, one, max_prefix=self.prompt)}
         for layer in self.layers:
             x = layer(x, slots, angles, self.table, kv_lens, one, max(new), max(self.lens), context_lens, **reach)
         return x, cu

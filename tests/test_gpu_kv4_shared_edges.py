@@ -68,3 +68,25 @@ def test_layers_that_overlap_are_refused():
         with pytest.raises(RuntimeError, match="overlap|twice"):
             marlin.kv4_layers(caches, 128)
     assert len(marlin.kv4_layers((pool[4:8], pool[:4]), 128)) == 2
+
+
+def test_a_bound_on_the_prefix_decides_the_passes():
+    """Short prefixes under a max_kv far above them: with the bound one pass, which needs no workspace and gives the
+    bits of a call without the prefix; without it the sizes speak for two."""
+    D, T, R, H = 128, 16, 32, 32
+    p, cu_groups = _forked([(2, R)], [1 + i for i in range(R)], [1] * R, H, H, D, -1, T, torch.float16, seed=3)
+    q, cache, table, kv = p[0].to(DEV), torch.from_numpy(p[1]).to(DEV), ints(p[2]), ints(p[3])
+    kw = dict(max_kv=16384, context_lens=kv - 1)
+    plain = marlin.kv4_attention(q, cache, table, kv, **kw)
+    want = attention(p[0].double().numpy(), *p[1:5], D, 1, T)
+    for bound, always, one in ((32, False, True), (0, False, True), (32, True, False), (None, False, False), (20000, False, False)):
+        s, out = marlin.kv4_shared(table, kv - 1, ints(cu_groups), T, always=always, max_prefix=bound), torch.empty_like(q)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        marlin.kv4_attention(q, cache, table, kv, shared=s, out=out, **kw)
+        assert (torch.cuda.max_memory_allocated() == before) == one, (bound, always)
+        assert torch.equal(out, plain) or not one
+        _check(out, None, want, torch.float16, f"bound {bound}")
+    with pytest.raises(RuntimeError, match="max_prefix"):
+        marlin.kv4_shared(table, kv - 1, ints(cu_groups), T, max_prefix=-1)
