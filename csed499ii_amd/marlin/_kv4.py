@@ -136,8 +136,9 @@ def kv4_tables(context_lens: torch.Tensor, new_lens: torch.Tensor, free_pages: t
     * ``cu_new [R + 1]``: the first new token of each request, and their number;
     * ``kv_lens [R]``: ``context + new``, cut at the table's ``P * page_size`` (where that may
       happen :func:`kv4_attention` needs ``context_lens``, too, for the positions);
-    * ``pages_used [1]``: pages wanted from ``free_pages``.  More than ``F`` means that some
-      requests have entries of -1 in the table, whose tokens :func:`kv4_attention` leaves out;
+    * ``pages_used [1]``: pages wanted from ``free_pages``.  More than there are in it (``F``, or
+      the ``count`` of :func:`kv4_free_pages`) means that some requests have entries of -1 in the
+      table, whose tokens :func:`kv4_attention` leaves out;
     * with ``return_positions`` ``positions [num_tokens]``: the new tokens' positions in their
       requests, for :func:`rotary_angles`; 0 past the last one.
 

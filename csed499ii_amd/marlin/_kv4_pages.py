@@ -4,8 +4,10 @@ counterpart.
 
 The block table with the lengths is the only state.  A page is *held* if an entry of a written token
 (``block_table[i][j]`` with ``j * page_size < kv_lens[i]``) names it, however many requests do; a
-request is finished by a length of zero and shortened by a smaller one.  A decoding step with
-samples that share their prompt's pages::
+request is finished by a length of zero and shortened by a smaller one.  (One that may share pages goes
+through :func:`kv4_fork` before it gets tokens again: others may hold the page in which it was cut, and
+its next tokens would be written over theirs.)  A decoding step with samples that share their prompt's
+pages::
 
     layers = kv4_layers(caches, head_dim, groupsize)             # once
     free, count = kv4_free_pages(table, lens, num_pages, T)
@@ -84,8 +86,8 @@ def _of_layers(layers, dev):
 def kv4_free_pages(block_table: torch.Tensor, kv_lens: torch.Tensor, num_pages: int, page_size: int):
     """The pages of a cache of ``num_pages`` that no request holds: ``(free [num_pages], count [1])``,
     int32, the free ones in ascending order and -1 behind them; ``free`` goes to :func:`kv4_tables` and
-    :func:`kv4_fork` as it is (where they want more than ``count`` pages, the tables get -1 as if the list had ended
-    there).  Entries that are no page are passed over."""
+    :func:`kv4_fork` as it is (where their ``pages_used`` passes ``count``, the tables get -1 as if the list had
+    ended there).  Entries that are no page are passed over."""
     dev, table, lens, R, P = _table(block_table, kv_lens)
     _check_page(page_size)
     if num_pages < 1 or num_pages * page_size > 2**31 - 1:
@@ -130,8 +132,9 @@ def kv4_fork(layers: kv4_layers, block_table: torch.Tensor, kv_lens: torch.Tenso
 
     * ``block_table [new requests, P]``: entries past a request's tokens and entries that were no page are -1;
     * ``kv_lens [new requests]``: the parents' lengths, cut at the table's width;
-    * ``pages_used [1]``: pages wanted from ``free_pages``.  More than ``F`` means that some requests have -1
-      for their last page, whose tokens :func:`kv4_attention` leaves out.
+    * ``pages_used [1]``: pages wanted from ``free_pages``.  More than there are in it (``F``, or the ``count`` of
+      :func:`kv4_free_pages`, whose list has -1 behind them) means that some requests have -1 for their last
+      page, whose tokens :func:`kv4_attention` leaves out.
 
     Requests may share a page at the same place of their tables only, as forks do."""
     dev, table, lens, R, P = _table(block_table, kv_lens)

@@ -90,3 +90,41 @@ def test_a_bound_on_the_prefix_decides_the_passes():
         _check(out, None, want, torch.float16, f"bound {bound}")
     with pytest.raises(RuntimeError, match="max_prefix"):
         marlin.kv4_shared(table, kv - 1, ints(cu_groups), T, max_prefix=-1)
+
+
+@pytest.mark.parametrize("cut", [1, 16, 25, 32, 40])
+def test_a_request_cut_into_shared_pages_goes_on_after_a_fork(cut):
+    """Two samples of one prompt of 40 tokens; the first is cut back and goes on otherwise: forked in between, no
+    token of the second is written over, and the first holds what it was cut to and its new tokens."""
+    D, T, H, pages = 64, 16, 2, 12
+    gen = torch.Generator().manual_seed(cut)
+    rows = lambda n: torch.randn((n, 2, H, D), generator=gen).half().to(DEV).unbind(1)  # noqa: E731
+    cache, table = marlin.kv4_cache(pages, H, D, T, device=DEV), torch.full((1, 4), -1, dtype=torch.int32, device=DEV)
+    layers = marlin.kv4_layers(cache, D)
+
+    def append(k, v, lens, new, table):
+        free, _ = marlin.kv4_free_pages(table, lens, pages, T)
+        slots, _, kv, _ = marlin.kv4_tables(lens, ints(new), free, table, k.size(0), T)
+        marlin.kv4_append(k, v, cache, slots)
+        return kv
+
+    def read(table, i, n):
+        pos = torch.arange(n, device=DEV)
+        return marlin.kv4_gather(cache, (table[i].long()[pos // T] * T + pos % T).int(), D)
+
+    lens = append(*rows(40), ints([0]), [40], table)
+    free, _ = marlin.kv4_free_pages(table, lens, pages, T)
+    table, lens, _ = marlin.kv4_fork(layers, table, lens, ints([0, 0]), free)
+    first, second = (read(table, i, 40) for i in range(2))
+    assert all(torch.equal(a, b) for a, b in zip(first, second))
+    lens = ints([cut, 40])
+    free, _ = marlin.kv4_free_pages(table, lens, pages, T)
+    table, lens, _ = marlin.kv4_fork(layers, table, lens, ints([0, 1]), free)
+    k, v = rows(14)
+    want = marlin.kv4_cache(1, H, D, T, device=DEV)
+    marlin.kv4_append(k, v, want, ints(range(14)))
+    lens = append(k, v, lens, [14, 0], table)
+    assert lens.tolist() == [cut + 14, 40]
+    assert all(torch.equal(a, b) for a, b in zip(read(table, 1, 40), second))
+    for got, old, new in zip(read(table, 0, cut + 14), first, marlin.kv4_gather(want, ints(range(14)), D)):
+        assert torch.equal(got[:cut], old[:cut]) and torch.equal(got[cut:], new)
