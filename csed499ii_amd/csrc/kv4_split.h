@@ -87,7 +87,7 @@ constexpr float kSlack = 8.f;      // of a reference that is rounded, in log2 un
 constexpr float kMostL = 0x1p100f; // of a row's sum of p, before it gets a new reference
 constexpr float kMostShift = 90.f; // p <= 2^90 at a new reference, however small its v
 constexpr float kNoV = 80.f;       // ... 2^80 where the row's v are all zero (2^20 such p make 2^100)
-constexpr float kBig = 1 << 20;    // of a row's largest score, in log2 units
+constexpr float kBig = 1 << 20;    // of a row's largest score, in log2 units (the prompt kernel's have fp32's rounding there)
 constexpr float kNone = -1.0e30f;  // reference of a row that has seen nothing
 
 struct AttnArgs {
@@ -919,6 +919,15 @@ __global__ __launch_bounds__(64 * kWaves, 4) void kv4_split_kernel(AttnArgs a) {
       if (a.lse != nullptr && d0 == 0)
         a.lse[at] = l == 0.f ? -__builtin_inff() : (m + __builtin_amdgcn_logf(l)) * 0.6931471805599453f;
     };
+    if (some_big) {  // M's rounding would show where sums meet: they are brought to the largest score itself
+      const float f = big ? __builtin_amdgcn_exp2f(-shift) : 1.f;
+      M = big ? x_top * c1 : M;
+      L *= f;
+#pragma unroll
+      for (int n = 0; n < NG; n++)
+#pragma unroll
+        for (int i = 0; i < S::OPS; i++) O[n][i] *= f;
+    }
     __syncthreads();  // the rings are done with
     L = column_sum(L);
     float* mine = reinterpret_cast<float*>(ring);

@@ -115,6 +115,28 @@ def test_values_over_many_orders_of_magnitude(case, form, D, g, n, Hq, Hkv):
     assert np.abs(lse.double().cpu().numpy() - ref_lse).max() <= 2.0 ** -16 * 100
 
 
+@pytest.mark.parametrize("n,Hq,Hkv,gain", [(3, 4, 2, x) for x in (1.0, 1e4, 1e6, 1e7, 1e9, 1e20)] + [(50, 34, 17, x) for x in (1.0, 1e3)])
+@pytest.mark.parametrize("D,g", [(128, -1), (128, 32), (64, 32)])
+@pytest.mark.parametrize("form", ["plain", "window", "shared"])
+def test_equal_scores_of_any_size(form, D, g, n, Hq, Hkv, gain):
+    """Keys that are all alike, values of many sizes: every token that a row sees has the same weight, wherever its
+    sums meet, however large the score (in the prompt kernel while fp32 has its fraction: past 10^4 a score's
+    rounding shows)."""
+    T, kv = 32, 600
+    p = _two(n, kv, 10, Hq, Hkv, D, g, T, torch.bfloat16, 3, poison=False)
+    k, _, k_at, v_at = ref.places(T, D, p[5])
+    rng = np.random.default_rng(0)
+    for page in np.unique(p[2][p[2] >= 0]):
+        codes, halves = p[1][page], p[1][page].view(np.float16)
+        nibbles = np.unique(k // 2)
+        codes[:, nibbles] = 0x99  # both codes 1
+        for o in range(T):
+            halves[:, k_at[o]] = 1.0
+            halves[:, v_at[o]] *= np.float16(2.0 ** rng.integers(-6, 6))
+    p[0] = (p[0].double() * gain).to(torch.bfloat16)
+    _check(*_run(p, g, T, form, 333, 5), _want(p, D, T, form, 333, 5), torch.bfloat16, f"gain {gain}", x_max=100.0 * gain)
+
+
 @pytest.mark.parametrize("n,Hq,Hkv", KERNELS)
 @pytest.mark.parametrize("D,g", [(128, -1), (128, 32), (64, 32)])
 @pytest.mark.parametrize("form,pos", [("window", 2), ("window", 85), ("window", 200), ("window", 397), ("shared", 100), ("shared", 397)])
