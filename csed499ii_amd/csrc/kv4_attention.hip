@@ -123,7 +123,7 @@ int check(int tokens, int requests, int q_heads, int kv_heads, int head_dim, int
 // The prefix that the requests of a group share: the whole pages, from the first on, that are the
 // same in their tables and lie within their contexts.  A workgroup for each group compares every
 // request's row with the first one's; one more for the requests of no group.  Once a step, for all
-// layers.  64 rows of 512 entries in one group take 10 us, what one compute unit reads at; 4 groups of 8 rows 4.6.
+// layers.  64 rows of 512 entries in one group take 10 us, what one compute unit reads at; 4 groups of 8 rows 4.1.
 // ---------------------------------------------------------------------------
 
 constexpr int kMaxGroups = 1 << 20;

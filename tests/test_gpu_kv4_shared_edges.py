@@ -1,9 +1,12 @@
 """Attention behind shared prefixes where lengths do not fit each other, or there is nothing to share."""
+import threading
+
 import numpy as np
 import pytest
 import torch
 
 from csed499ii_amd import marlin
+from tests.gpu_util import new_stream
 from tests.test_gpu_kv4 import DEV, _check, ints
 from tests.test_gpu_kv4_reach import _forked, _shared, attention
 
@@ -128,3 +131,44 @@ def test_a_request_cut_into_shared_pages_goes_on_after_a_fork(cut):
     assert all(torch.equal(a, b) for a, b in zip(read(table, 1, 40), second))
     for got, old, new in zip(read(table, 0, cut + 14), first, marlin.kv4_gather(want, ints(range(14)), D)):
         assert torch.equal(got[:cut], old[:cut]) and torch.equal(got[cut:], new)
+
+
+@pytest.mark.parametrize("streams", [1, 2])
+def test_windows_and_prefixes_of_two_host_threads(streams):
+    """Windows and shared prefixes whose tokens are divided, in either kernel, issued by two host threads at once, on
+    one stream and on one each: the bits of a call by itself."""
+    D, T, calls = 128, 16, []
+    for seed, (q, R, Hq, H, pages) in enumerate(((1, 40, 64, 8, 60), (4, 8, 8, 2, 120), (60, 4, 20, 20, 40))):
+        p, cu_groups = _forked([(pages, R)], [q + 9 + i for i in range(R)], [q] * R, Hq, H, D, -1, T, torch.float16, seed=seed)
+        dev = [x.to(DEV) for x in (p[0], torch.from_numpy(p[1]))] + [ints(x) for x in p[2:5]]
+        ctx, kw = dev[3] - q, dict(max_q=q, max_kv=int(p[3].max()), return_lse=True)
+
+        def shared(dev=dev, ctx=ctx, groups=ints(cu_groups), kw=kw):
+            s = marlin.kv4_shared(dev[2], ctx, groups, T, dev[4], always=True)
+            return marlin.kv4_attention(*dev, context_lens=ctx, shared=s, **kw)
+
+        def window(dev=dev, kw=kw):
+            return marlin.kv4_attention(*dev, window=500, sinks=4, **kw)
+
+        calls += [(f, f()) for f in (shared, window)]
+    torch.cuda.synchronize()
+    own, got, errors = [new_stream() for _ in range(streams)], [[], []], []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(own[i % streams]):
+                for k in range(30):
+                    f, want = calls[(5 * k + 2 * i) % 6]
+                    got[i].append((f(), want))
+        except Exception as e:  # noqa: BLE001 (shown by the test's own thread)
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors and len(got[0]) == len(got[1]) == 30
+    for result, want in got[0] + got[1]:
+        assert all(torch.equal(a, b) for a, b in zip(result, want))
